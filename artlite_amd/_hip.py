@@ -35,6 +35,14 @@ class Desc(ctypes.Structure):
                                                     ("shared_down_type", ctypes.c_int32)]
 
 
+class Ffn(ctypes.Structure):
+    """``artlite_ffn``."""
+
+    _fields_ = [("gate", ctypes.c_void_p), ("up", ctypes.c_void_p), ("down", ctypes.c_void_p), ("act", ctypes.c_int32)]
+
+
+_P, _I, _I64, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
+
 # every exported function: (restype, argtypes)
 SIGNATURES = {
     "artlite_last_error": (ctypes.c_size_t, [ctypes.c_char_p, ctypes.c_size_t]),
@@ -66,6 +74,21 @@ SIGNATURES = {
                                               c_i32p]),
     "artlite_moe_kernel_names": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_char_p, ctypes.c_size_t]),
     "artlite_hbm_copy": (ctypes.c_int, [ctypes.c_size_t, ctypes.c_int, c_f64p]),
+    "artlite_matrix_supported": (_I, [_I]),
+    "artlite_matrix_create": (_I, [_I, _I64, _I64, ctypes.POINTER(_P)]),
+    "artlite_matrix_destroy": (_I, [_P]),
+    "artlite_matrix_upload": (_I, [_P, _P, _Z]),
+    "artlite_matrix_upload_bias": (_I, [_P, _P, _Z]),
+    "artlite_workspace_create": (_I, [_Z, ctypes.POINTER(_P)]),
+    "artlite_workspace_destroy": (_I, [_P]),
+    "artlite_linear_workspace": (_I, [_P, _I, _I64, _I, ctypes.POINTER(_Z)]),
+    "artlite_linear": (_I, [_P, _P, _I, _I64, _I64, _P, _I64, _P, _P]),
+    "artlite_ffn_workspace": (_I, [ctypes.POINTER(Ffn), _I, _I64, _I, ctypes.POINTER(_Z)]),
+    "artlite_ffn_forward": (_I, [ctypes.POINTER(Ffn), _P, _I, _I64, _I64, _P, _I64, _P, _P]),
+    "artlite_ffn_backward": (_I, [ctypes.POINTER(Ffn), _P, _I64, _P, _I64, _I, _I64, _P, _I64, _P, _P, _P, _P, _P]),
+    "artlite_device_alloc": (_I, [_Z, ctypes.POINTER(_P), ctypes.POINTER(_I)]),
+    "artlite_device_free": (_I, [_P]),
+    "artlite_device_copy": (_I, [_P, _P, _Z, _I]),
 }
 
 _lib: ctypes.CDLL | None = None

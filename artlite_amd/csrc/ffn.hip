@@ -1,0 +1,593 @@
+// The dense operators' calls: one matrix's product and the gated feed-forward block, forward and backward, on device memory
+// (the C entry points artlite_linear*, artlite_ffn*), and the passes over activations that the large tiles need.
+//
+// Up to FEW_ROWS rows go through k_few (linear.hip), straight from the blocks. More rows go through the large tiles
+// (hgemm.hip), over fp16 operands made for the call in its workspace:
+//   x, dy: each row times the power of two that brings its largest value into [2^14, 2^15): bf16 values convert exactly
+//     (those above 2^-29 of their row's largest; smaller ones keep 2^-39 of it), fp32 ones as two planes (hi + lo, 2^-22);
+//   weights: each value times the matrix's power of two, rounded once to fp16 (2^-11; fp32 calls: two planes, 2^-22), an
+//     eighth of the rounding of a bf16 output;
+//   h, dg, du: in fp32 from the sums, then fp16 (fp32 calls: two planes) scaled by a row's power of two from bounds:
+//     |g| <= |x| max |gate row| in the 2-norm, |act(g)| <= |g|, |act'| < 2, |dh| <= |dy| max |down| sqrt(H); typical values lie
+//     some 2^14 below their bound, fp16 holds 2^29 below it in full.
+// Products of two planes are three sums (hi hi + hi lo + lo hi). The weights' gradients sum over rows, so their operands are
+// turned and take one power of two for all rows (the largest; a value keeps 2^-39 of the largest).
+#include "hgemm.h"
+#include "matrix.h"
+
+#include <cmath>
+#include <initializer_list>
+
+namespace artlite {
+
+namespace {
+
+// x (a row a workgroup) -> fp16 planes of Kp values times 2^-xe, xe and the exponent of its 2-norm
+template <bool BF16>
+__global__ __launch_bounds__(256) void k_rows16(const void* __restrict__ x, int64_t K, int64_t stride, int vec,
+                                                uint16_t* __restrict__ out, int64_t Kp, int64_t plane, int planes,
+                                                int32_t* __restrict__ xe, int32_t* __restrict__ ne) {
+  __shared__ float red[4];
+  const int64_t m = blockIdx.x;
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  auto load = [&](int64_t k, float(&v)[8]) {
+    if constexpr (BF16) {
+      const uint16_t* p = static_cast<const uint16_t*>(x) + m * stride + k;
+      uint16_t b[8];
+      if (vec)
+        __builtin_memcpy(b, __builtin_assume_aligned(p, 16), 16);
+      else
+        for (int i = 0; i < 8; i++) b[i] = p[i];
+      for (int i = 0; i < 8; i++) v[i] = bf16_to_f32(b[i]);
+    } else {
+      const float* p = static_cast<const float*>(x) + m * stride + k;
+      if (vec)
+        __builtin_memcpy(v, __builtin_assume_aligned(p, 16), 32);
+      else
+        for (int i = 0; i < 8; i++) v[i] = p[i];
+    }
+  };
+  auto all = [&](float v, bool add) {
+    for (int o = 32; o; o >>= 1) {
+      const float u = __shfl_xor(v, o);
+      v = add ? v + u : fmaxf(v, u);
+    }
+    __syncthreads();
+    if (lane == 0) red[wv] = v;
+    __syncthreads();
+    return add ? red[0] + red[1] + red[2] + red[3] : fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  };
+  float mx = 0.0f;
+  for (int64_t k = threadIdx.x * 8; k < K; k += 2048) {
+    float v[8];
+    load(k, v);
+    for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(v[i]));
+  }
+  mx = all(mx, false);
+  const int e = exp_above(mx);
+  float ss = 0.0f;
+  for (int64_t k = threadIdx.x * 8; k < Kp; k += 2048) {
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (k < K) load(k, v);
+    uint16_t a[8], b[8];
+    for (int i = 0; i < 8; i++) {
+      const float r = ldexpf(v[i], -e), s = ldexpf(r, 15);
+      ss = __builtin_fmaf(r, r, ss);
+      const _Float16 hi = _Float16(s);
+      a[i] = __builtin_bit_cast(uint16_t, hi);
+      // (an infinite value is its first plane)
+      b[i] = __builtin_bit_cast(uint16_t, _Float16(__builtin_isinf(s) ? 0.0f : s - float(hi)));
+    }
+    __builtin_memcpy(__builtin_assume_aligned(out + m * Kp + k, 16), a, 16);
+    if (planes == 2) __builtin_memcpy(__builtin_assume_aligned(out + plane + m * Kp + k, 16), b, 16);
+  }
+  ss = all(ss, true);
+  if (threadIdx.x == 0) {
+    xe[m] = e - 15;
+    // (|x| < 2^e sqrt(ss); ss is at most K and its fp32 sum off by less than the step to the next exponent)
+    if (ne) ne[m] = e + (exp_above(sqrtf(ss) * 1.01f));
+  }
+}
+
+// the rows' scales of h and of dg, du, from the exponents of the rows' norms
+__global__ void k_exps(int64_t M, const int32_t* __restrict__ nx, const int32_t* __restrict__ ny, int lh, int ld,
+                       int32_t* __restrict__ he, int32_t* __restrict__ de) {
+  const int64_t m = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (m >= M) return;
+  he[m] = 2 * nx[m] + lh - 15;
+  if (de) de[m] = ny[m] + nx[m] + ld - 15;
+}
+
+// the largest of each of up to 4 arrays
+struct MaxE {
+  const int32_t* a[4];
+};
+__global__ __launch_bounds__(256) void k_max_e(const MaxE in, int64_t M, int32_t* __restrict__ out) {
+  __shared__ int red[4];
+  const int32_t* a = in.a[blockIdx.x];
+  int v = INT32_MIN;
+  for (int64_t m = threadIdx.x; m < M; m += 256) v = max(v, a[m]);
+  for (int o = 32; o; o >>= 1) v = max(v, __shfl_xor(v, o));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) out[blockIdx.x] = max(max(red[0], red[1]), max(red[2], red[3]));
+}
+
+// rows of C fp16 values (ld apart, row t worth 2^e[t]) turned: C rows of Tp values worth 2^*top, zeros past T
+__global__ __launch_bounds__(256) void k_turn(const uint16_t* __restrict__ in, int64_t ld, int64_t T, int64_t C,
+                                              const int32_t* __restrict__ e, const int32_t* __restrict__ top,
+                                              uint16_t* __restrict__ out, int64_t Tp) {
+  __shared__ __attribute__((aligned(16))) uint16_t t[64][72];
+  const int64_t c0 = int64_t(blockIdx.x) * 64, t0 = int64_t(blockIdx.y) * 64;
+  const int E = *top;
+  for (int i = threadIdx.x; i < 64 * 8; i += 256) {
+    const int r = i >> 3, c = 8 * (i & 7);
+    uint16_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (t0 + r < T && c0 + c < ld) {  // (ld is a multiple of 64: the row's padding is read at most)
+      __builtin_memcpy(v, __builtin_assume_aligned(in + (t0 + r) * ld + c0 + c, 16), 16);
+      const int sh = e[t0 + r] - E;
+      for (int k = 0; k < 8; k++)
+        v[k] = __builtin_bit_cast(uint16_t, _Float16(ldexpf(float(__builtin_bit_cast(_Float16, v[k])), sh)));
+    }
+    for (int k = 0; k < 8; k++) t[c + k][r] = v[k];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 64 * 8; i += 256) {
+    const int c = i >> 3, r = 8 * (i & 7);
+    if (c0 + c < C) *reinterpret_cast<uint4*>(out + (c0 + c) * Tp + t0 + r) = *reinterpret_cast<const uint4*>(&t[c][r]);
+  }
+}
+
+__global__ __launch_bounds__(256) void k_zero(uint16_t* p, int64_t n) {
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) p[i] = 0;
+}
+
+int rows16(const void* x, int dtype, int64_t M, int64_t K, int64_t stride, uint16_t* out, int64_t Kp, int planes,
+           int32_t* xe, int32_t* ne, hipStream_t s) {
+  const bool b = dtype == ARTLITE_X_BF16;
+  const int vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (stride * (b ? 2 : 4)) % 16 == 0;
+  if (b)
+    k_rows16<true><<<unsigned(M), 256, 0, s>>>(x, K, stride, vec, out, Kp, M * Kp, planes, xe, ne);
+  else
+    k_rows16<false><<<unsigned(M), 256, 0, s>>>(x, K, stride, vec, out, Kp, M * Kp, planes, xe, ne);
+  ART_HIP(hipGetLastError());
+  return ARTLITE_OK;
+}
+
+int turn(const uint16_t* in, int64_t ld, int64_t T, int64_t C, int planes, const int32_t* e, const int32_t* top,
+         uint16_t* out, int64_t Tp, hipStream_t s) {
+  for (int p = 0; p < planes; p++)
+    k_turn<<<dim3(unsigned((C + 63) / 64), unsigned(Tp / 64)), 256, 0, s>>>(in + p * T * ld, ld, T, C, e, top,
+                                                                            out + p * C * Tp, Tp);
+  ART_HIP(hipGetLastError());
+  return ARTLITE_OK;
+}
+
+// Products' operand pairs as segments: of one plane each, or of two lo hi + hi lo, then hi hi: the small sums first, so that
+// only the last ones' additions are rounded at the result's size.
+struct Pair {
+  const uint16_t* a;
+  int64_t ap;  // (values from a plane to the next)
+  const uint16_t* b;
+  int64_t bp;
+  const uint16_t* b2 = nullptr;
+};
+void segments(HGemm& g, std::initializer_list<Pair> pairs, int planes) {
+  const auto add = [&](const Pair& p, int pa, int pb) {
+    g.a[g.segs] = p.a + pa * p.ap;
+    g.b[g.segs] = p.b + pb * p.bp;
+    g.b2[g.segs] = p.b2 ? p.b2 + pb * p.bp : nullptr;
+    g.segs++;
+  };
+  if (planes == 2)
+    for (const Pair& p : pairs) add(p, 1, 0), add(p, 0, 1);
+  for (const Pair& p : pairs) add(p, 0, 0);
+}
+
+// the most rows of a call of the large tiles (their launches' grids and a workspace's sizes stay in range)
+constexpr int64_t MOST_ROWS = int64_t(1) << 22;
+
+bool aligned_rows(const void* x, int dtype, int64_t n, int64_t stride) {
+  return dtype == ARTLITE_X_BF16 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (n <= 1 || stride % 8 == 0);
+}
+
+// ---- one matrix's product
+
+struct LinearPlan {
+  bool few;
+  uint16_t* planes = nullptr;                 // few rows: x as planes, where it is not read as it is
+  uint16_t *x16 = nullptr, *w16 = nullptr;    // else
+  int32_t* xe = nullptr;
+};
+LinearPlan linear_plan(Carve& c, const artlite_matrix* w, int dtype, int64_t n, bool direct) {
+  LinearPlan p;
+  p.few = n <= FEW_ROWS;
+  if (p.few) {
+    if (!direct) p.planes = c.take<uint16_t>(size_t(dtype == ARTLITE_X_BF16 ? 1 : 3) * n * w->K);
+  } else {
+    const int pl = dtype == ARTLITE_X_BF16 ? 1 : 2;
+    const int64_t Kp = pad64(w->K);
+    p.x16 = c.take<uint16_t>(size_t(pl) * n * Kp);
+    p.w16 = c.take<uint16_t>(size_t(pl) * w->N * Kp);
+    p.xe = c.take<int32_t>(n);
+  }
+  return p;
+}
+
+int check_matrix(const artlite_matrix* m, const char* what) {
+  if (!m) return fail(ARTLITE_EINVAL, "%s: null matrix", what);
+  if (!m->have) return fail(ARTLITE_EINVAL, "%s: matrix not uploaded", what);
+  return ARTLITE_OK;
+}
+int check_dtype(int dtype, const char* what) {
+  if (dtype != ARTLITE_X_F32 && dtype != ARTLITE_X_BF16) return fail(ARTLITE_EINVAL, "%s: dtype %d", what, dtype);
+  return ARTLITE_OK;
+}
+int check_rows(int64_t n, const char* what) {
+  if (n < 0 || n > MOST_ROWS) return fail(ARTLITE_EINVAL, "%s: %lld rows", what, (long long)n);
+  return ARTLITE_OK;
+}
+// rows of `cols` values that a call reads (stride at least 0) or writes (at least cols)
+int check_array(const void* p, int64_t n, int64_t cols, int64_t stride, bool written, int dtype, int device,
+                const char* what) {
+  if (n > 1 && (stride < (written ? cols : 0) || stride > (int64_t(1) << 40)))
+    return fail(ARTLITE_EINVAL, "%s: rows of %lld values %lld apart", what, (long long)cols, (long long)stride);
+  if (reinterpret_cast<uintptr_t>(p) % (dtype == ARTLITE_X_BF16 ? 2 : 4))
+    return fail(ARTLITE_EINVAL, "%s: address not aligned to its values", what);
+  return check_device(p, device, what);
+}
+
+int linear(const artlite_matrix* w, const void* x, int dtype, int64_t n, int64_t x_stride, void* y, int64_t y_stride,
+           char* base, hipStream_t s) {
+  Carve c(base);
+  const bool direct = aligned_rows(x, dtype, n, x_stride);
+  const LinearPlan p = linear_plan(c, w, dtype, n, direct);
+  if (p.few) {
+    FewArgs a{};
+    a.w = w;
+    a.planes = dtype == ARTLITE_X_BF16 ? 1 : 3;
+    a.x = static_cast<const uint16_t*>(x), a.x_stride = x_stride;
+    if (!direct) {
+      ART_TRY(launch_planes(x, dtype, n, w->K, x_stride, p.planes, w->K, n * w->K, a.planes, s));
+      a.x = p.planes, a.x_stride = w->K, a.x_plane = n * w->K;
+    }
+    a.M = n;
+    a.y = y, a.y_stride = y_stride, a.dtype = dtype;
+    return launch_few(a, s);
+  }
+  const int pl = dtype == ARTLITE_X_BF16 ? 1 : 2, e = wexp16(w);
+  const int64_t Kp = pad64(w->K);
+  ART_TRY(rows16(x, dtype, n, w->K, x_stride, p.x16, Kp, pl, p.xe, nullptr, s));
+  ART_TRY(launch_unpack(w, false, e, p.w16, Kp, w->N * Kp, pl, s));
+  HGemm g{};
+  segments(g, {{p.x16, n * Kp, p.w16, w->N * Kp}}, pl);
+  g.lda = g.ldb = g.K = Kp;
+  g.M = n, g.N = w->N;
+  g.row_e = p.xe, g.e = e;
+  g.bias = w->has_bias ? w->bias.as<float>() : nullptr;
+  g.y = y, g.y_stride = y_stride, g.dtype = dtype;
+  return launch_hgemm(g, s);
+}
+
+// ---- the gated block
+
+struct Ffn {
+  const artlite_matrix *gate, *up, *down;
+  int act;
+  int64_t H, F, Hp, Fp;
+};
+int check_ffn(const artlite_ffn* f, Ffn& o, const char* what) {
+  if (!f) return fail(ARTLITE_EINVAL, "%s: null", what);
+  for (const artlite_matrix* m : {f->gate, f->up, f->down}) {
+    ART_TRY(check_matrix(m, what));
+    if (m->has_bias) return fail(ARTLITE_EINVAL, "%s: a matrix with a bias", what);
+    if (m->device != f->gate->device) return fail(ARTLITE_EINVAL, "%s: matrices of devices %d and %d", what, m->device, f->gate->device);
+  }
+  if (f->act != ARTLITE_ACT_SILU && f->act != ARTLITE_ACT_GELU_TANH)
+    return fail(ARTLITE_EINVAL, "%s: activation %d", what, f->act);
+  const artlite_matrix *g = f->gate, *u = f->up, *d = f->down;
+  if (g->N != u->N || g->K != u->K || g->t != u->t || d->N != g->K || d->K != g->N)
+    return fail(ARTLITE_EINVAL, "%s: gate %lld x %lld (%s), up %lld x %lld (%s), down %lld x %lld", what, (long long)g->N,
+                (long long)g->K, g->t->name, (long long)u->N, (long long)u->K, u->t->name, (long long)d->N, (long long)d->K);
+  o = Ffn{g, u, d, f->act, g->K, g->N, pad64(g->K), pad64(g->N)};
+  return ARTLITE_OK;
+}
+
+struct FfnPlan {
+  bool few;
+  uint16_t *planes = nullptr, *hp = nullptr;  // few rows: x as planes (where it is not read as it is), h as planes
+  uint16_t *x16, *w16, *u16, *d16, *h16;      // else: x, the unpacked matrices, h
+  int32_t *xe, *nx, *he;
+};
+FfnPlan ffn_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool direct) {
+  FfnPlan p{};
+  p.few = n <= FEW_ROWS;
+  const bool b = dtype == ARTLITE_X_BF16;
+  if (p.few) {
+    if (!direct) p.planes = c.take<uint16_t>(size_t(b ? 1 : 3) * n * f.H);
+    p.hp = c.take<uint16_t>(size_t(b ? 2 : 3) * n * f.F);
+    return p;
+  }
+  const size_t pl = b ? 1 : 2;
+  p.x16 = c.take<uint16_t>(pl * n * f.Hp);
+  p.w16 = c.take<uint16_t>(pl * f.F * f.Hp);
+  p.u16 = c.take<uint16_t>(pl * f.F * f.Hp);
+  p.d16 = c.take<uint16_t>(pl * f.H * f.Fp);
+  p.h16 = c.take<uint16_t>(pl * n * f.Fp);
+  p.xe = c.take<int32_t>(n);
+  p.nx = c.take<int32_t>(n);
+  p.he = c.take<int32_t>(n);
+  return p;
+}
+
+int ffn_forward(const Ffn& f, const void* x, int dtype, int64_t n, int64_t x_stride, void* y, int64_t y_stride, char* base,
+                hipStream_t s) {
+  Carve c(base);
+  const bool direct = aligned_rows(x, dtype, n, x_stride), b = dtype == ARTLITE_X_BF16;
+  const FfnPlan p = ffn_plan(c, f, dtype, n, direct);
+  if (p.few) {
+    FewArgs a{};
+    a.w = f.gate, a.up = f.up, a.act = f.act;
+    a.planes = b ? 1 : 3;
+    a.x = static_cast<const uint16_t*>(x), a.x_stride = x_stride;
+    if (!direct) {
+      ART_TRY(launch_planes(x, dtype, n, f.H, x_stride, p.planes, f.H, n * f.H, a.planes, s));
+      a.x = p.planes, a.x_stride = f.H, a.x_plane = n * f.H;
+    }
+    a.M = n;
+    a.h = p.hp, a.h_stride = f.F, a.h_plane = n * f.F, a.h_planes = b ? 2 : 3;
+    ART_TRY(launch_few(a, s));
+    FewArgs d{};
+    d.w = f.down;
+    d.planes = a.h_planes;
+    d.x = p.hp, d.x_stride = f.F, d.x_plane = n * f.F;
+    d.M = n;
+    d.y = y, d.y_stride = y_stride, d.dtype = dtype;
+    return launch_few(d, s);
+  }
+  const int pl = b ? 1 : 2;
+  ART_TRY(rows16(x, dtype, n, f.H, x_stride, p.x16, f.Hp, pl, p.xe, p.nx, s));
+  k_exps<<<unsigned((n + 255) / 256), 256, 0, s>>>(n, p.nx, nullptr, f.gate->row_exp + f.up->row_exp, 0, p.he, nullptr);
+  ART_TRY(launch_unpack(f.gate, false, wexp16(f.gate), p.w16, f.Hp, f.F * f.Hp, pl, s));
+  ART_TRY(launch_unpack(f.up, false, wexp16(f.up), p.u16, f.Hp, f.F * f.Hp, pl, s));
+  ART_TRY(launch_unpack(f.down, false, wexp16(f.down), p.d16, f.Fp, f.H * f.Fp, pl, s));
+  HGemm g{};
+  segments(g, {{p.x16, n * f.Hp, p.w16, f.F * f.Hp, p.u16}}, pl);
+  g.lda = g.ldb = g.K = f.Hp;
+  g.M = n, g.N = f.F;
+  g.epilogue = H_GLU;
+  g.row_e = p.xe, g.e = wexp16(f.gate), g.e2 = wexp16(f.up);
+  g.act = f.act;
+  g.out_e = p.he, g.h = p.h16, g.h_stride = f.Fp, g.h_plane = n * f.Fp, g.planes = pl;
+  ART_TRY(launch_hgemm(g, s));
+  HGemm d{};
+  segments(d, {{p.h16, n * f.Fp, p.d16, f.H * f.Fp}}, pl);
+  d.lda = d.ldb = d.K = f.Fp;
+  d.M = n, d.N = f.H;
+  d.row_e = p.he, d.e = wexp16(f.down);
+  d.y = y, d.y_stride = y_stride, d.dtype = dtype;
+  return launch_hgemm(d, s);
+}
+
+struct GradPlan {
+  uint16_t *x16, *dy16, *a16, *b16, *c16;        // x, dy; gate and up, later their transposes; down's transpose
+  uint16_t *h16, *dg16, *du16;
+  uint16_t *xt, *dyt, *ht, *dgt, *dut;           // (weights' gradients) turned
+  float* dh;
+  int32_t *xe, *nx, *ye, *ny, *he, *de, *top;
+};
+GradPlan grad_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool weights) {
+  GradPlan p{};
+  const size_t pl = dtype == ARTLITE_X_BF16 ? 1 : 2;
+  const size_t w = pl * size_t(f.F * f.Hp > f.H * f.Fp ? f.F * f.Hp : f.H * f.Fp);
+  p.x16 = c.take<uint16_t>(pl * n * f.Hp);
+  p.dy16 = c.take<uint16_t>(pl * n * f.Hp);
+  p.a16 = c.take<uint16_t>(w);
+  p.b16 = c.take<uint16_t>(w);
+  p.c16 = c.take<uint16_t>(pl * f.F * f.Hp);
+  p.dg16 = c.take<uint16_t>(pl * n * f.Fp);
+  p.du16 = c.take<uint16_t>(pl * n * f.Fp);
+  p.dh = c.take<float>(n * f.Fp);
+  p.xe = c.take<int32_t>(n);
+  p.nx = c.take<int32_t>(n);
+  p.ye = c.take<int32_t>(n);
+  p.ny = c.take<int32_t>(n);
+  p.he = c.take<int32_t>(n);
+  p.de = c.take<int32_t>(n);
+  if (weights) {
+    const int64_t Tp = pad64(n);
+    p.h16 = c.take<uint16_t>(pl * n * f.Fp);
+    p.xt = c.take<uint16_t>(pl * f.H * Tp);
+    p.dyt = c.take<uint16_t>(pl * f.H * Tp);
+    p.ht = c.take<uint16_t>(pl * f.F * Tp);
+    p.dgt = c.take<uint16_t>(pl * f.F * Tp);
+    p.dut = c.take<uint16_t>(pl * f.F * Tp);
+    p.top = c.take<int32_t>(4);
+  }
+  return p;
+}
+
+int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, int dtype, int64_t n,
+                 void* dx, int64_t dx_stride, void* dgate, void* dup, void* ddown, char* base, hipStream_t s) {
+  const bool weights = dgate || dup || ddown;
+  Carve c(base);
+  const GradPlan p = grad_plan(c, f, dtype, n, weights);
+  const int pl = dtype == ARTLITE_X_BF16 ? 1 : 2;
+  ART_TRY(rows16(x, dtype, n, f.H, x_stride, p.x16, f.Hp, pl, p.xe, p.nx, s));
+  ART_TRY(rows16(dy, dtype, n, f.H, dy_stride, p.dy16, f.Hp, pl, p.ye, p.ny, s));
+  const int lg = f.gate->row_exp, lu = f.up->row_exp;
+  const int ld = f.down->max_exp + int(std::ceil(0.5 * std::log2(double(f.H)))) + (lg > lu ? lg : lu) + 1;
+  k_exps<<<unsigned((n + 255) / 256), 256, 0, s>>>(n, p.nx, p.ny, lg + lu, ld, p.he, p.de);
+  // (gate and up share a scale: dx sums over both)
+  const int e = wexp16(f.gate) > wexp16(f.up) ? wexp16(f.gate) : wexp16(f.up), ed = wexp16(f.down);
+  ART_TRY(launch_unpack(f.gate, false, e, p.a16, f.Hp, f.F * f.Hp, pl, s));
+  ART_TRY(launch_unpack(f.up, false, e, p.b16, f.Hp, f.F * f.Hp, pl, s));
+  ART_TRY(launch_unpack(f.down, true, ed, p.c16, f.Hp, f.F * f.Hp, pl, s));
+  HGemm d{};
+  segments(d, {{p.dy16, n * f.Hp, p.c16, f.F * f.Hp}}, pl);
+  d.lda = d.ldb = d.K = f.Hp;
+  d.M = n, d.N = f.F;
+  d.row_e = p.ye, d.e = ed;
+  d.y = p.dh, d.y_stride = f.Fp, d.dtype = ARTLITE_X_F32;
+  ART_TRY(launch_hgemm(d, s));
+  HGemm g{};
+  segments(g, {{p.x16, n * f.Hp, p.a16, f.F * f.Hp, p.b16}}, pl);
+  g.lda = g.ldb = g.K = f.Hp;
+  g.M = n, g.N = f.F;
+  g.epilogue = H_DGLU;
+  g.row_e = p.xe, g.e = g.e2 = e;
+  g.act = f.act;
+  g.dh = p.dh;
+  g.out_e = p.de, g.h_e = p.he;
+  g.dg = p.dg16, g.du = p.du16, g.h = p.h16;
+  g.h_stride = f.Fp, g.h_plane = n * f.Fp, g.planes = pl;
+  ART_TRY(launch_hgemm(g, s));
+  if (dx) {
+    ART_TRY(launch_unpack(f.gate, true, e, p.a16, f.Fp, f.H * f.Fp, pl, s));
+    ART_TRY(launch_unpack(f.up, true, e, p.b16, f.Fp, f.H * f.Fp, pl, s));
+    HGemm x2{};
+    segments(x2, {{p.dg16, n * f.Fp, p.a16, f.H * f.Fp}, {p.du16, n * f.Fp, p.b16, f.H * f.Fp}}, pl);
+    x2.lda = x2.ldb = x2.K = f.Fp;
+    x2.M = n, x2.N = f.H;
+    x2.row_e = p.de, x2.e = e;
+    x2.y = dx, x2.y_stride = dx_stride, x2.dtype = dtype;
+    ART_TRY(launch_hgemm(x2, s));
+  }
+  if (!weights) return ARTLITE_OK;
+  const int64_t Tp = pad64(n);
+  k_max_e<<<4, 256, 0, s>>>(MaxE{{p.xe, p.ye, p.he, p.de}}, n, p.top);
+  if (dgate || dup) ART_TRY(turn(p.x16, f.Hp, n, f.H, pl, p.xe, p.top, p.xt, Tp, s));
+  if (dgate) ART_TRY(turn(p.dg16, f.Fp, n, f.F, pl, p.de, p.top + 3, p.dgt, Tp, s));
+  if (dup) ART_TRY(turn(p.du16, f.Fp, n, f.F, pl, p.de, p.top + 3, p.dut, Tp, s));
+  if (ddown) {
+    ART_TRY(turn(p.dy16, f.Hp, n, f.H, pl, p.ye, p.top + 1, p.dyt, Tp, s));
+    ART_TRY(turn(p.h16, f.Fp, n, f.F, pl, p.he, p.top + 2, p.ht, Tp, s));
+  }
+  const auto grad = [&](const uint16_t* a, int64_t M, const int32_t* ea, const uint16_t* b, int64_t N, const int32_t* eb,
+                        void* out) {
+    HGemm w{};
+    segments(w, {{a, M * Tp, b, N * Tp}}, pl);
+    w.lda = w.ldb = w.K = Tp;
+    w.M = M, w.N = N;
+    w.e0 = ea, w.e1 = eb;
+    w.y = out, w.y_stride = N, w.dtype = dtype;
+    return launch_hgemm(w, s);
+  };
+  if (dgate) ART_TRY(grad(p.dgt, f.F, p.top + 3, p.xt, f.H, p.top, dgate));
+  if (dup) ART_TRY(grad(p.dut, f.F, p.top + 3, p.xt, f.H, p.top, dup));
+  if (ddown) ART_TRY(grad(p.dyt, f.H, p.top + 1, p.ht, f.F, p.top + 2, ddown));
+  return ARTLITE_OK;
+}
+
+}  // namespace
+
+}  // namespace artlite
+
+using namespace artlite;
+
+extern "C" int artlite_linear_workspace(const artlite_matrix* w, int dtype, int64_t n, int aligned, size_t* nbytes) {
+  if (!w || !nbytes) return fail(ARTLITE_EINVAL, "linear: null");
+  ART_TRY(check_dtype(dtype, "linear"));
+  ART_TRY(check_rows(n, "linear"));
+  Carve c(nullptr);
+  if (n) (void)linear_plan(c, w, dtype, n, aligned && dtype == ARTLITE_X_BF16);
+  *nbytes = c.at;
+  return ARTLITE_OK;
+}
+
+extern "C" int artlite_linear(const artlite_matrix* w, const void* x, int dtype, int64_t n, int64_t x_stride, void* y,
+                              int64_t y_stride, artlite_workspace* work, void* stream) {
+  ART_TRY(check_matrix(w, "linear"));
+  ART_TRY(check_dtype(dtype, "linear"));
+  ART_TRY(check_rows(n, "linear"));
+  if (n == 0) return ARTLITE_OK;
+  ART_TRY(check_array(x, n, w->K, x_stride, false, dtype, w->device, "linear: x"));
+  ART_TRY(check_array(y, n, w->N, y_stride, true, dtype, w->device, "linear: y"));
+  Carve c(nullptr);
+  (void)linear_plan(c, w, dtype, n, aligned_rows(x, dtype, n, x_stride));
+  if (c.at && work && work->w.device != w->device)
+    return fail(ARTLITE_EINVAL, "linear: a workspace of device %d, not %d", work->w.device, w->device);
+  OnDevice on;
+  ART_TRY(on.set(w->device));
+  WorkScope ws;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  ART_TRY(ws.begin(work ? &work->w : nullptr, c.at, s, "linear"));
+  return linear(w, x, dtype, n, x_stride, y, y_stride, work ? work->w.p : nullptr, s);
+}
+
+extern "C" int artlite_ffn_workspace(const artlite_ffn* d, int dtype, int64_t n, int backward, size_t* nbytes) {
+  Ffn f;
+  ART_TRY(check_ffn(d, f, "ffn"));
+  if (!nbytes) return fail(ARTLITE_EINVAL, "ffn: null");
+  ART_TRY(check_dtype(dtype, "ffn"));
+  ART_TRY(check_rows(n, "ffn"));
+  Carve c(nullptr);
+  if (n && backward) {
+    (void)grad_plan(c, f, dtype, n, backward == 2);
+  } else if (n) {
+    (void)ffn_plan(c, f, dtype, n, false);
+    // (calls of fewer rows need less on either side of the few, but not across it)
+    if (n > FEW_ROWS) {
+      Carve few(nullptr);
+      (void)ffn_plan(few, f, dtype, FEW_ROWS, false);
+      if (few.at > c.at) c.at = few.at;
+    }
+  }
+  *nbytes = c.at;
+  return ARTLITE_OK;
+}
+
+extern "C" int artlite_ffn_forward(const artlite_ffn* d, const void* x, int dtype, int64_t n, int64_t x_stride, void* y,
+                                   int64_t y_stride, artlite_workspace* work, void* stream) {
+  Ffn f;
+  ART_TRY(check_ffn(d, f, "ffn"));
+  ART_TRY(check_dtype(dtype, "ffn"));
+  ART_TRY(check_rows(n, "ffn"));
+  if (n == 0) return ARTLITE_OK;
+  const int dev = f.gate->device;
+  ART_TRY(check_array(x, n, f.H, x_stride, false, dtype, dev, "ffn: x"));
+  ART_TRY(check_array(y, n, f.H, y_stride, true, dtype, dev, "ffn: y"));
+  Carve c(nullptr);
+  (void)ffn_plan(c, f, dtype, n, aligned_rows(x, dtype, n, x_stride));
+  if (work && work->w.device != dev) return fail(ARTLITE_EINVAL, "ffn: a workspace of device %d, not %d", work->w.device, dev);
+  OnDevice on;
+  ART_TRY(on.set(dev));
+  WorkScope ws;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  ART_TRY(ws.begin(work ? &work->w : nullptr, c.at, s, "ffn"));
+  return ffn_forward(f, x, dtype, n, x_stride, y, y_stride, work->w.p, s);
+}
+
+extern "C" int artlite_ffn_backward(const artlite_ffn* d, const void* x, int64_t x_stride, const void* dy,
+                                    int64_t dy_stride, int dtype, int64_t n, void* dx, int64_t dx_stride, void* dgate,
+                                    void* dup, void* ddown, artlite_workspace* work, void* stream) {
+  Ffn f;
+  ART_TRY(check_ffn(d, f, "ffn backward"));
+  ART_TRY(check_dtype(dtype, "ffn backward"));
+  ART_TRY(check_rows(n, "ffn backward"));
+  const int dev = f.gate->device;
+  const bool weights = dgate || dup || ddown;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  for (void* p : {dgate, dup, ddown})
+    if (p) ART_TRY(check_array(p, 1, 0, 0, true, dtype, dev, "ffn backward: a weight's gradient"));
+  OnDevice on;
+  if (n == 0) {  // (sums of nothing)
+    ART_TRY(on.set(dev));
+    for (void* p : {dgate, dup, ddown})
+      if (p) k_zero<<<1024, 256, 0, s>>>(static_cast<uint16_t*>(p), f.F * f.H * (dtype == ARTLITE_X_BF16 ? 1 : 2));
+    ART_HIP(hipGetLastError());
+    return ARTLITE_OK;
+  }
+  ART_TRY(check_array(x, n, f.H, x_stride, false, dtype, dev, "ffn backward: x"));
+  ART_TRY(check_array(dy, n, f.H, dy_stride, false, dtype, dev, "ffn backward: dy"));
+  if (dx) ART_TRY(check_array(dx, n, f.H, dx_stride, true, dtype, dev, "ffn backward: dx"));
+  if (!dx && !weights) return ARTLITE_OK;
+  Carve c(nullptr);
+  (void)grad_plan(c, f, dtype, n, weights);
+  if (work && work->w.device != dev)
+    return fail(ARTLITE_EINVAL, "ffn backward: a workspace of device %d, not %d", work->w.device, dev);
+  ART_TRY(on.set(dev));
+  WorkScope ws;
+  ART_TRY(ws.begin(work ? &work->w : nullptr, c.at, s, "ffn backward"));
+  return ffn_backward(f, x, x_stride, dy, dy_stride, dtype, n, dx, dx_stride, dgate, dup, ddown, work->w.p, s);
+}

@@ -1,0 +1,241 @@
+// A matrix of 4-bit GGUF blocks in HBM (matrix.hip) and what the dense operators share: its tile layout and the decode of
+// it, workspaces, the checks of device arguments, the launches of the dense products.
+#pragma once
+
+#include <mutex>
+
+#include "codes.h"
+#include "common.h"
+
+// The tile layout. A matrix of N rows of K values is cut into tiles of 16 rows and units of 256 values (rows and values past
+// its end are zeros: scales of 0). A unit of a tile is 2048 bytes of codes, then 16 headers of HB bytes, one a row:
+//   codes: half h (128 values), lane l = 16 lg + lr: 16 bytes at 1024 h + 16 l, dword j those of row lr's values
+//     32 (4 h + j) + 8 lg .. + 8, value 2 p in nibble p and value 2 p + 1 in nibble p + 4 (p < 4), so that
+//     (dword >> 4 p) & 0x000F000F are the codes of values 2 p and 2 p + 1: one 16-bit operand dword of the MFMA;
+//   header: Q4_0, IQ4_NL: the 8 groups' fp16 scales; Q4_1: their (scale, min) pairs; Q4_K: the block's 16 bytes before its
+//     codes (d, dmin, the 6-bit scales and mins); IQ4_XS: its 8 (d and the 6-bit scales).
+// The bytes are the file's (but for the padding), in the order in which a wave reads them: 1 KiB of codes a load, contiguous.
+namespace artlite {
+
+constexpr int UNIT = 256;   // values of a unit
+constexpr int TROWS = 16;   // rows of a tile
+
+template <int QT>
+constexpr int hdr_bytes() {
+  return QT == ARTLITE_Q4_1 ? 32 : QT == ARTLITE_IQ4_XS ? 8 : 16;
+}
+template <int QT>
+constexpr int unit_bytes() {
+  return 2048 + TROWS * hdr_bytes<QT>();
+}
+
+// whether a format has the tile layout, and its bytes a unit (0: none)
+int tile_unit_bytes(int qtype);
+
+// a switch over the formats of the tile layout
+#define ART_TILE_QTYPES(qtype, X)            \
+  switch (qtype) {                           \
+    case ARTLITE_Q4_0: X(ARTLITE_Q4_0);      \
+    case ARTLITE_Q4_1: X(ARTLITE_Q4_1);      \
+    case ARTLITE_Q4_K: X(ARTLITE_Q4_K);      \
+    case ARTLITE_IQ4_NL: X(ARTLITE_IQ4_NL);  \
+    default: X(ARTLITE_IQ4_XS);              \
+  }
+
+// A row's header of a unit in registers, and the scale s and offset o of group g (of 8) from it: a value is s c - o with c
+// the code (Q4_1, Q4_K), c - 8 (Q4_0) or IQ4[c] (o = 0), exact in fp32 but for that last product and difference.
+template <int QT>
+struct TileHdr {
+  static constexpr int DW = hdr_bytes<QT>() / 4;
+  uint32_t h[DW];
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    if constexpr (DW == 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      h[0] = v.x, h[1] = v.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < DW; i += 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p + 4 * i);
+        h[i] = v.x, h[i + 1] = v.y, h[i + 2] = v.z, h[i + 3] = v.w;
+      }
+    }
+  }
+  __device__ __forceinline__ float scale(int g) const {
+    if constexpr (QT == ARTLITE_Q4_0 || QT == ARTLITE_IQ4_NL) {
+      return h2f((h[g >> 1] >> (16 * (g & 1))) & 0xFFFFu);
+    } else if constexpr (QT == ARTLITE_Q4_1) {
+      return h2f(h[g] & 0xFFFFu);
+    } else if constexpr (QT == ARTLITE_Q4_K) {
+      const int sh = 8 * (g & 3);
+      const uint32_t q = g < 4 ? (h[1] >> sh) & 63 : ((h[3] >> sh) & 15) | (((h[1] >> (sh + 6)) & 3) << 4);
+      return __fmul_rn(h2f(h[0] & 0xFFFFu), float(q));
+    } else {
+      const int ls = int((h[1] >> (4 * g)) & 15) | (int((h[0] >> (16 + 2 * g)) & 3) << 4);
+      return __fmul_rn(h2f(h[0] & 0xFFFFu), float(ls - 32));
+    }
+  }
+  __device__ __forceinline__ float offset(int g) const {
+    if constexpr (QT == ARTLITE_Q4_1) {
+      return -h2f(h[g] >> 16);
+    } else if constexpr (QT == ARTLITE_Q4_K) {
+      const int sh = 8 * (g & 3);
+      const uint32_t m = g < 4 ? (h[2] >> sh) & 63 : ((h[3] >> (sh + 4)) & 15) | (((h[2] >> (sh + 6)) & 3) << 4);
+      return __fmul_rn(h2f(h[0] >> 16), float(m));
+    } else {
+      return 0.0f;
+    }
+  }
+};
+
+template <int QT>
+constexpr bool has_offset = QT == ARTLITE_Q4_1 || QT == ARTLITE_Q4_K;
+template <int QT>
+constexpr bool iq4 = QT == ARTLITE_IQ4_NL || QT == ARTLITE_IQ4_XS;
+
+// the 8 values of a code dword as fp32, in order (dequantized as the file's: rows of artlite_dequant_rows)
+template <int QT>
+__device__ __forceinline__ void tile_values(uint32_t w, float s, float o, float (&v)[8]) {
+#pragma unroll
+  for (int p = 0; p < 4; p++) {
+    const uint32_t c = (w >> (4 * p)) & 0x000F000Fu;
+    float a, b;
+    if constexpr (iq4<QT>) {
+      const uint32_t t = iq4_int8((c | (c >> 8)) & 0x0F0Fu);
+      a = float(int8_t(t & 0xFFu)), b = float(int8_t((t >> 8) & 0xFFu));
+    } else {
+      a = float(c & 0xFFFFu), b = float(c >> 16);
+      if constexpr (QT == ARTLITE_Q4_0) a -= 8.0f, b -= 8.0f;
+    }
+    v[2 * p] = has_offset<QT> ? __fsub_rn(__fmul_rn(s, a), o) : __fmul_rn(s, a);
+    v[2 * p + 1] = has_offset<QT> ? __fsub_rn(__fmul_rn(s, b), o) : __fmul_rn(s, b);
+  }
+}
+
+// the gated block's activation and its derivative (artlite_act), fp32
+__device__ __forceinline__ float gate_act(int act, float g) {
+  if (act == ARTLITE_ACT_SILU) return g / (1.0f + expf(-g));
+  const float z = 0.7978845608028654f * (g + 0.044715f * g * g * g);
+  return 0.5f * g * (1.0f + tanhf(z));
+}
+__device__ __forceinline__ float gate_act_grad(int act, float g) {
+  if (act == ARTLITE_ACT_SILU) {
+    const float s = 1.0f / (1.0f + expf(-g));
+    return s * (1.0f + g * (1.0f - s));
+  }
+  const float z = 0.7978845608028654f * (g + 0.044715f * g * g * g), t = tanhf(z);
+  const float d = 1.0f - t * t;  // (0 where z is large: nothing times a large g stays nothing)
+  return 0.5f * (1.0f + t) + (d > 0.0f ? 0.5f * g * d * 0.7978845608028654f * (1.0f + 3.0f * 0.044715f * g * g) : 0.0f);
+}
+
+// the least e with |v| < 2^e of a finite v (0 and what is no number: a very small one)
+__host__ __device__ __forceinline__ int exp_above(float v) {
+  if (!(v > 0.0f)) return -200;
+  if (v > 3.0e38f) return 129;
+  int e;
+  (void)frexpf(v, &e);
+  return e;
+}
+
+// A workspace: device memory that calls carve their scratch from. Calls on one stream follow each other; a call on another
+// stream than the last one's waits for that one's end.
+struct Work {
+  int device = -1;
+  char* p = nullptr;
+  size_t n = 0;
+  std::mutex mu;
+  hipEvent_t done = nullptr;
+  hipStream_t last = nullptr;
+  bool used = false;
+};
+// Around the launches of a call that uses a workspace: `begin` locks it, checks its size and orders the call behind the last
+// one; the destructor notes where the call ends. (Inside a stream capture nothing is ordered: a graph's replays and other
+// calls on its workspace follow each other by the caller's streams.)
+struct WorkScope {
+  Work* w = nullptr;
+  hipStream_t s = nullptr;
+  bool note = false;
+  int begin(Work* work, size_t need, hipStream_t stream, const char* what);
+  ~WorkScope();
+};
+// bytes carved from a workspace in turn, 256-aligned; with a null base it only counts
+struct Carve {
+  char* base;
+  size_t at = 0;
+  explicit Carve(void* b) : base(static_cast<char*>(b)) {}
+  template <class T>
+  T* take(size_t count) {
+    const size_t a = at;
+    at = (a + count * sizeof(T) + 255) / 256 * 256;
+    return base ? reinterpret_cast<T*>(base + a) : nullptr;
+  }
+};
+
+// the device of a call's handles made current for its duration
+struct OnDevice {
+  int was = -1;
+  int set(int device);
+  ~OnDevice() {
+    if (was >= 0) (void)hipSetDevice(was);
+  }
+};
+// p: device memory of `device`
+int check_device(const void* p, int device, const char* what);
+
+}  // namespace artlite
+
+struct artlite_workspace {
+  artlite::Work w;
+};
+
+struct artlite_matrix {
+  int device = -1;
+  const artlite::QType* t = nullptr;
+  int64_t N = 0, K = 0;
+  int64_t tiles = 0;
+  int units = 0;
+  int ub = 0;              // bytes a unit of a tile
+  bool have = false, has_bias = false;
+  artlite::DevBuf w, bias;
+  int max_exp = 0;         // every |value| < 2^max_exp
+  int row_exp = 0;         // every row's 2-norm < 2^row_exp
+};
+
+namespace artlite {
+
+// ---- the dense products over few rows (linear.hip)
+
+// One launch: out[m][n] = sum_k x[m][k] W[n][k] (+ bias[n]) for M rows of A given as P planes of bf16 (x = the sum of its
+// planes), or with `up` set the gated products act(x W^T) (x U^T), written as planes of bf16 for the launch after.
+struct FewArgs {
+  const artlite_matrix *w, *up;
+  int act;                  // (gated) artlite_act
+  const uint16_t* x;        // plane p of row m at x + p x_plane + m x_stride, 16-byte aligned rows
+  int64_t x_stride, x_plane;
+  int planes;               // 1, 2 or 3
+  int64_t M;
+  void* y;                  // plain: bf16 or fp32 rows, y_stride values apart
+  int64_t y_stride;
+  int dtype;
+  uint16_t* h;              // gated: h_planes planes of M rows of h_stride values
+  int64_t h_stride, h_plane;
+  int h_planes;
+};
+int launch_few(const FewArgs& a, hipStream_t s);
+// rows past which the dense products go by way of 16-bit weights and the large tiles
+constexpr int FEW_ROWS = 64;
+// x (M rows of K values of dtype, stride apart) as planes of bf16 (1: bf16 as it is; 3: fp32), rows of Kp values (zeros past K)
+int launch_planes(const void* x, int dtype, int64_t M, int64_t K, int64_t stride, uint16_t* out, int64_t Kp, int64_t plane,
+                  int planes, hipStream_t s);
+
+// ---- 16-bit operands of the large tiles (matrix.hip)
+
+// W (or its transpose) as fp16 rows of ld values, times 2^-e (e: `wexp16`): plane 0, with planes 2 also what its rounding
+// left (at out + plane). Values past the matrix's columns (transposed: rows) up to ld are zeros.
+int launch_unpack(const artlite_matrix* m, bool transposed, int e, uint16_t* out, int64_t ld, int64_t plane, int planes,
+                  hipStream_t s);
+// the scale that brings a matrix's largest value into [2^14, 2^15)
+inline int wexp16(const artlite_matrix* m) { return m->max_exp - 15; }
+
+inline int64_t pad64(int64_t v) { return (v + 63) / 64 * 64; }
+
+}  // namespace artlite

@@ -1,0 +1,412 @@
+// Matrices of 4-bit GGUF blocks in the tile layout (matrix.h): upload, the bounds that scale their 16-bit forms, those forms
+// (unpacked into a workspace for the large tiles); workspaces; the C entry points of both and of device arrays.
+//
+// What bounds the kernels here: memory. k_unpack reads 0.56 bytes a value and writes 2: 4096 x 11008 in about 18 us. Uploads
+// happen once a matrix and are not tuned.
+#include "matrix.h"
+
+#include <cmath>
+#include <new>
+
+namespace artlite {
+
+int tile_unit_bytes(int qtype) {
+  switch (qtype) {
+    case ARTLITE_Q4_0: return unit_bytes<ARTLITE_Q4_0>();
+    case ARTLITE_Q4_1: return unit_bytes<ARTLITE_Q4_1>();
+    case ARTLITE_Q4_K: return unit_bytes<ARTLITE_Q4_K>();
+    case ARTLITE_IQ4_NL: return unit_bytes<ARTLITE_IQ4_NL>();
+    case ARTLITE_IQ4_XS: return unit_bytes<ARTLITE_IQ4_XS>();
+    default: return 0;
+  }
+}
+
+namespace {
+
+// code v (of 32) of group g of the file's block at b (a block of 32 values has one group)
+template <int QT>
+__device__ __forceinline__ uint32_t file_code(const uint8_t* b, int g, int v) {
+  if constexpr (QT == ARTLITE_Q4_K) {
+    const uint32_t c = b[16 + 32 * (g >> 1) + v];
+    return g & 1 ? c >> 4 : c & 15u;
+  } else {
+    const uint8_t* q = b + (QT == ARTLITE_Q4_1 ? 4 : QT == ARTLITE_IQ4_XS ? 8 + 16 * g : 2);
+    return v < 16 ? q[v] & 15u : uint32_t(q[v - 16]) >> 4;
+  }
+}
+
+// the file's rows -> the tile layout: a workgroup per unit of a tile, thread 64 h + l the 16 code bytes of half h, lane l;
+// then a header's halves-words each
+template <int QT, int PER, int BYTES>
+__global__ __launch_bounds__(128) void k_tile(const uint8_t* __restrict__ raw, int64_t N, int64_t K, int units,
+                                              uint8_t* __restrict__ out) {
+  const int64_t tile = int64_t(blockIdx.x) / units;
+  const int u = int(int64_t(blockIdx.x) % units);
+  uint8_t* o = out + int64_t(blockIdx.x) * unit_bytes<QT>();
+  const int h = threadIdx.x >> 6, l = threadIdx.x & 63, lg = l >> 4, lr = l & 15;
+  const int64_t n = tile * TROWS + lr, row_bytes = K / PER * BYTES;
+  const uint8_t* row = raw + n * row_bytes;
+  uint4 v;
+  uint32_t* d = reinterpret_cast<uint32_t*>(&v);
+  for (int j = 0; j < 4; j++) {
+    const int g = 4 * h + j;
+    const int64_t k = int64_t(u) * UNIT + 32 * g;
+    d[j] = 0;
+    if (n < N && k < K) {
+      const uint8_t* b = row + k / PER * BYTES;
+      for (int p = 0; p < 4; p++) {
+        d[j] |= file_code<QT>(b, int(k % PER) / 32, 8 * lg + 2 * p) << (4 * p);
+        d[j] |= file_code<QT>(b, int(k % PER) / 32, 8 * lg + 2 * p + 1) << (4 * p + 16);
+      }
+    }
+  }
+  *reinterpret_cast<uint4*>(o + 1024 * h + 16 * l) = v;
+  constexpr int HW = hdr_bytes<QT>() / 2;  // (16-bit words of a header)
+  for (int i = threadIdx.x; i < TROWS * HW; i += 128) {
+    const int r = i / HW, w = i % HW;
+    const int64_t nr = tile * TROWS + r;
+    uint16_t x = 0;
+    if (nr < N) {
+      const uint8_t* rr = raw + nr * row_bytes;
+      if constexpr (PER == UNIT) {
+        if (int64_t(u) * UNIT < K) {
+          const uint8_t* b = rr + int64_t(u) * BYTES + 2 * w;
+          x = uint16_t(b[0] | b[1] << 8);
+        }
+      } else {
+        constexpr int F = HW / 8;  // (the fp16 fields of a block)
+        const int64_t k = int64_t(u) * UNIT + 32 * (w / F);
+        if (k < K) {
+          const uint8_t* b = rr + k / 32 * BYTES + 2 * (w % F);
+          x = uint16_t(b[0] | b[1] << 8);
+        }
+      }
+    }
+    *reinterpret_cast<uint16_t*>(o + 2048 + hdr_bytes<QT>() * r + 2 * w) = x;
+  }
+}
+
+// a lane's 32 values of half h of a unit: groups 4 h + j, values 8 lg .. + 8 of each
+template <int QT, class F>
+__device__ __forceinline__ void tile_half(const uint8_t* ub, int h, int lane, F&& f) {
+  TileHdr<QT> hd;
+  hd.load(ub + 2048 + hdr_bytes<QT>() * (lane & 15));
+  const uint4 c = *reinterpret_cast<const uint4*>(ub + 1024 * h + 16 * lane);
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    float v[8];
+    tile_values<QT>(w[j], hd.scale(4 * h + j), has_offset<QT> ? hd.offset(4 * h + j) : 0.0f, v);
+    f(j, v);
+  }
+}
+
+// out[0] = max |value|, out[1] = the largest 2-norm of a row, as bits (finite values; atomic maxima of floats that are not
+// negative): a workgroup of 4 waves per tile
+template <int QT>
+__global__ __launch_bounds__(256) void k_bounds(const uint8_t* __restrict__ w, int units, int64_t K, uint32_t* out) {
+  __shared__ float red[4][TROWS];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const uint8_t* t = w + int64_t(blockIdx.x) * units * unit_bytes<QT>();
+  float mx = 0.0f, ss = 0.0f;
+  for (int i = wv; i < 2 * units; i += 4)
+    tile_half<QT>(t + int64_t(i >> 1) * unit_bytes<QT>(), i & 1, lane, [&](int j, const float(&v)[8]) {
+      if (int64_t(i >> 1) * UNIT + 128 * (i & 1) + 32 * j >= K) return;
+#pragma unroll
+      for (int p = 0; p < 8; p++) {
+        mx = fmaxf(mx, fabsf(v[p]));
+        ss = __builtin_fmaf(v[p], v[p], ss);
+      }
+    });
+  for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+  ss += __shfl_xor(ss, 16);
+  ss += __shfl_xor(ss, 32);
+  if (lane < TROWS) red[wv][lane] = ss;
+  if (lane == 0) atomicMax(out, __float_as_uint(mx));
+  __syncthreads();
+  if (threadIdx.x < TROWS) {
+    const float s = red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane];
+    if (s < __builtin_inff()) atomicMax(out + 1, __float_as_uint(sqrtf(s) * 1.001f));
+  }
+}
+
+// W as fp16 rows of ld values: a wave per half unit of a tile; plane 1 (where there is one) what plane 0's rounding left
+template <int QT>
+__global__ __launch_bounds__(256) void k_unpack(const uint8_t* __restrict__ w, int units, int64_t N, int64_t K, int e,
+                                                uint16_t* __restrict__ out, int64_t ld, int64_t plane, int planes) {
+  const int64_t i = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6), tile = i / (2 * units);
+  const int r = int(i % (2 * units)), lane = threadIdx.x & 63;
+  const int64_t n = tile * TROWS + (lane & 15);
+  if (n >= N) return;
+  const int64_t k0 = int64_t(r >> 1) * UNIT + 128 * (r & 1) + 8 * (lane >> 4);
+  uint16_t* o = out + n * ld + k0;
+  tile_half<QT>(w + (tile * units + (r >> 1)) * unit_bytes<QT>(), r & 1, lane, [&](int j, const float(&v)[8]) {
+    const int64_t k = k0 + 32 * j;
+    if (k >= ld) return;
+    uint16_t a[8], b[8];
+#pragma unroll
+    for (int p = 0; p < 8; p++) {
+      const float x = k < K ? ldexpf(v[p], -e) : 0.0f;
+      const _Float16 hi = _Float16(x);
+      a[p] = __builtin_bit_cast(uint16_t, hi);
+      b[p] = __builtin_bit_cast(uint16_t, _Float16(x - float(hi)));
+    }
+    __builtin_memcpy(__builtin_assume_aligned(o + 32 * j, 16), a, 16);
+    if (planes == 2) __builtin_memcpy(__builtin_assume_aligned(o + plane + 32 * j, 16), b, 16);
+  });
+}
+
+// W's transpose as fp16 rows of ld values: a workgroup per half unit of 4 tiles (64 rows of W), turned in LDS
+template <int QT>
+__global__ __launch_bounds__(256) void k_unpack_t(const uint8_t* __restrict__ w, int units, int64_t tiles, int64_t N,
+                                                  int64_t K, int e, uint16_t* __restrict__ out, int64_t ld, int64_t plane,
+                                                  int planes) {
+  constexpr int LD = 72;  // (a row's 64 values and 8 more: 16-byte rows, their banks spread)
+  __shared__ __attribute__((aligned(16))) uint16_t t[2][128][LD];
+  const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, lg = lane >> 4, lr = lane & 15;
+  const int64_t g4 = int64_t(blockIdx.x) / (2 * units), tile = 4 * g4 + wv;
+  const int r = int(int64_t(blockIdx.x) % (2 * units));
+  const int64_t k0 = int64_t(r >> 1) * UNIT + 128 * (r & 1);
+  const bool live = tile < tiles && tile * TROWS + lr < N;
+  const uint8_t* ub = w + ((tile < tiles ? tile : 0) * units + (r >> 1)) * unit_bytes<QT>();
+  tile_half<QT>(ub, r & 1, lane, [&](int j, const float(&v)[8]) {
+#pragma unroll
+    for (int p = 0; p < 8; p++) {
+      const float x = live ? ldexpf(v[p], -e) : 0.0f;
+      const _Float16 hi = _Float16(x);
+      t[0][32 * j + 8 * lg + p][16 * wv + lr] = __builtin_bit_cast(uint16_t, hi);
+      if (planes == 2) t[1][32 * j + 8 * lg + p][16 * wv + lr] = __builtin_bit_cast(uint16_t, _Float16(x - float(hi)));
+    }
+  });
+  __syncthreads();
+  for (int i = threadIdx.x; i < 128 * 8; i += 256) {
+    const int row = i >> 3, c = i & 7;
+    const int64_t k = k0 + row, n = 64 * g4 + 8 * c;
+    if (k >= K || n >= ld) continue;
+    for (int pl = 0; pl < planes; pl++)
+      *reinterpret_cast<uint4*>(out + pl * plane + k * ld + n) = *reinterpret_cast<const uint4*>(&t[pl][row][8 * c]);
+  }
+}
+
+}  // namespace
+
+int launch_unpack(const artlite_matrix* m, bool transposed, int e, uint16_t* out, int64_t ld, int64_t plane, int planes,
+                  hipStream_t s) {
+  const uint8_t* w = m->w.as<uint8_t>();
+  const int64_t rows = transposed ? (m->tiles + 3) / 4 : m->tiles;
+  const unsigned grid = unsigned(transposed ? rows * 2 * m->units : (rows * 2 * m->units + 3) / 4);
+#define ART_U(QT)                                                                                          \
+  if (transposed)                                                                                          \
+    k_unpack_t<QT><<<grid, 256, 0, s>>>(w, m->units, m->tiles, m->N, m->K, e, out, ld, plane, planes);     \
+  else                                                                                                     \
+    k_unpack<QT><<<grid, 256, 0, s>>>(w, m->units, m->N, m->K, e, out, ld, plane, planes);                 \
+  break
+  ART_TILE_QTYPES(m->t->id, ART_U)
+#undef ART_U
+  ART_HIP(hipGetLastError());
+  return ARTLITE_OK;
+}
+
+int OnDevice::set(int device) {
+  int cur = -1;
+  ART_HIP(hipGetDevice(&cur));
+  if (cur == device) return ARTLITE_OK;
+  ART_HIP(hipSetDevice(device));
+  was = cur;
+  return ARTLITE_OK;
+}
+
+int check_device(const void* p, int device, const char* what) {
+  hipPointerAttribute_t a;
+  if (!p) return fail(ARTLITE_EINVAL, "%s: null", what);
+  if (hipPointerGetAttributes(&a, p) != hipSuccess) {
+    (void)hipGetLastError();
+    return fail(ARTLITE_EINVAL, "%s: not device memory", what);
+  }
+  if (a.type != hipMemoryTypeDevice) return fail(ARTLITE_EINVAL, "%s: not device memory", what);
+  if (a.device != device) return fail(ARTLITE_EINVAL, "%s: memory of device %d, not %d", what, a.device, device);
+  return ARTLITE_OK;
+}
+
+int WorkScope::begin(Work* work, size_t need, hipStream_t stream, const char* what) {
+  if (need == 0) return ARTLITE_OK;
+  if (!work) return fail(ARTLITE_EINVAL, "%s: needs a workspace of %zu bytes", what, need);
+  if (work->n < need) return fail(ARTLITE_EINVAL, "%s: a workspace of %zu bytes, not %zu", what, work->n, need);
+  work->mu.lock();
+  w = work;
+  s = stream;
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  ART_HIP(hipStreamIsCapturing(stream, &st));
+  if (st != hipStreamCaptureStatusNone) return ARTLITE_OK;
+  if (w->used && w->last != stream) ART_HIP(hipStreamWaitEvent(stream, w->done, 0));
+  note = true;
+  return ARTLITE_OK;
+}
+
+WorkScope::~WorkScope() {
+  if (!w) return;
+  if (note && hipEventRecord(w->done, s) == hipSuccess) {
+    w->used = true;
+    w->last = s;
+  }
+  w->mu.unlock();
+}
+
+namespace {
+int matrix_upload(artlite_matrix* m, const void* data) {
+  HostCtx* c;
+  ART_TRY(host_ctx(&c));
+  const size_t nb = size_t(m->N) * size_t(m->K / m->t->per) * m->t->bytes;
+  DevBuf raw;
+  ART_TRY(raw.reserve(nb));
+  ART_TRY(c->flag.reserve(256));
+  ART_TRY(m->w.reserve(size_t(m->tiles) * m->units * m->ub + WEIGHT_TAIL));
+  uint32_t b[2] = {0, 0};
+  ART_HIP(hipMemcpyAsync(raw.p, data, nb, hipMemcpyHostToDevice, c->stream));
+  ART_HIP(hipMemcpyAsync(c->flag.p, b, 8, hipMemcpyHostToDevice, c->stream));
+  const unsigned grid = unsigned(m->tiles * m->units);
+#define ART_T(QT)                                                                                                   \
+  k_tile<QT, QT == ARTLITE_Q4_K || QT == ARTLITE_IQ4_XS ? 256 : 32,                                                 \
+         QT == ARTLITE_Q4_K ? 144 : QT == ARTLITE_IQ4_XS ? 136 : QT == ARTLITE_Q4_1 ? 20 : 18>                      \
+      <<<grid, 128, 0, c->stream>>>(raw.as<uint8_t>(), m->N, m->K, m->units, m->w.as<uint8_t>());                   \
+  k_bounds<QT><<<unsigned(m->tiles), 256, 0, c->stream>>>(m->w.as<uint8_t>(), m->units, m->K, c->flag.as<uint32_t>()); \
+  break
+  ART_TILE_QTYPES(m->t->id, ART_T)
+#undef ART_T
+  ART_HIP(hipGetLastError());
+  ART_HIP(hipMemcpyAsync(b, c->flag.p, 8, hipMemcpyDeviceToHost, c->stream));
+  ART_HIP(hipStreamSynchronize(c->stream));
+  float f[2];
+  std::memcpy(f, b, 8);
+  // (a matrix of zeros, or with scales that are no numbers: any bound will do)
+  m->max_exp = f[0] > 0.0f ? exp_above(f[0]) : 0;
+  m->row_exp = f[1] > 0.0f ? exp_above(f[1]) : 0;
+  m->have = true;
+  return ARTLITE_OK;
+}
+}  // namespace
+
+}  // namespace artlite
+
+using namespace artlite;
+
+extern "C" int artlite_matrix_supported(int qtype) { return tile_unit_bytes(qtype) != 0; }
+
+extern "C" int artlite_matrix_create(int qtype, int64_t rows, int64_t cols, artlite_matrix** out) {
+  if (!out) return fail(ARTLITE_EINVAL, "matrix: null");
+  *out = nullptr;
+  const QType* t = qtype_by_id(qtype);
+  const int ub = tile_unit_bytes(qtype);
+  if (!t || !ub)
+    return fail(ARTLITE_EINVAL, "matrix: weight type %d (%s) is not one of Q4_0, Q4_1, Q4_K, IQ4_NL, IQ4_XS", qtype,
+                t ? t->name : "unknown");
+  // (sizes whose tiles and rows every launch's grid reaches)
+  if (rows < 1 || cols < 1 || rows > (int64_t(1) << 24) || cols > (int64_t(1) << 20) || cols % t->per)
+    return fail(ARTLITE_EINVAL, "matrix: %lld rows of %lld values in blocks of %d", (long long)rows, (long long)cols, t->per);
+  const int64_t tiles = (rows + TROWS - 1) / TROWS, units = (cols + UNIT - 1) / UNIT;
+  if (tiles * units > (int64_t(1) << 30))
+    return fail(ARTLITE_EINVAL, "matrix: %lld rows of %lld values", (long long)rows, (long long)cols);
+  HostCtx* c;
+  ART_TRY(host_ctx(&c, false));
+  artlite_matrix* m = new (std::nothrow) artlite_matrix;
+  if (!m) return fail(ARTLITE_ENOMEM, "matrix: no memory");
+  m->device = c->device;
+  m->t = t;
+  m->N = rows, m->K = cols;
+  m->tiles = tiles, m->units = int(units), m->ub = ub;
+  *out = m;
+  return ARTLITE_OK;
+}
+
+extern "C" int artlite_matrix_destroy(artlite_matrix* m) {
+  if (!m) return ARTLITE_OK;
+  OnDevice on;
+  const int rc = on.set(m->device);
+  delete m;
+  return rc;
+}
+
+extern "C" int artlite_matrix_upload(artlite_matrix* m, const void* data, size_t nbytes) {
+  if (!m || !data) return fail(ARTLITE_EINVAL, "matrix upload: null argument");
+  const size_t want = size_t(m->N) * size_t(m->K / m->t->per) * m->t->bytes;
+  if (nbytes != want) return fail(ARTLITE_EINVAL, "matrix upload: %zu bytes, not %zu", nbytes, want);
+  OnDevice on;
+  ART_TRY(on.set(m->device));
+  // (calls that read the bytes of an earlier upload come to their end first)
+  if (m->have) ART_HIP(hipDeviceSynchronize());
+  m->have = false;
+  return matrix_upload(m, data);
+}
+
+extern "C" int artlite_matrix_upload_bias(artlite_matrix* m, const float* data, size_t n) {
+  if (!m) return fail(ARTLITE_EINVAL, "matrix bias: null argument");
+  if (n && (!data || int64_t(n) != m->N))
+    return fail(ARTLITE_EINVAL, "matrix bias: %zu values for %lld rows", n, (long long)m->N);
+  OnDevice on;
+  ART_TRY(on.set(m->device));
+  if (m->has_bias) ART_HIP(hipDeviceSynchronize());
+  m->has_bias = false;
+  if (!n) return ARTLITE_OK;
+  ART_TRY(m->bias.reserve(n * 4));
+  ART_HIP(hipMemcpy(m->bias.p, data, n * 4, hipMemcpyHostToDevice));
+  m->has_bias = true;
+  return ARTLITE_OK;
+}
+
+extern "C" int artlite_workspace_create(size_t nbytes, artlite_workspace** out) {
+  if (!out) return fail(ARTLITE_EINVAL, "workspace: null");
+  *out = nullptr;
+  HostCtx* c;
+  ART_TRY(host_ctx(&c, false));
+  artlite_workspace* w = new (std::nothrow) artlite_workspace;
+  if (!w) return fail(ARTLITE_ENOMEM, "workspace: no memory");
+  w->w.device = c->device;
+  w->w.n = nbytes;
+  hipError_t e = hipMalloc(reinterpret_cast<void**>(&w->w.p), nbytes ? nbytes : 256);
+  if (e == hipSuccess) e = hipEventCreateWithFlags(&w->w.done, hipEventDisableTiming);
+  if (e != hipSuccess) {
+    (void)hipGetLastError();
+    if (w->w.p) (void)hipFree(w->w.p);
+    delete w;
+    return fail(ARTLITE_ENOMEM, "workspace of %zu bytes: %s", nbytes, hipGetErrorString(e));
+  }
+  *out = w;
+  return ARTLITE_OK;
+}
+
+extern "C" int artlite_workspace_destroy(artlite_workspace* w) {
+  if (!w) return ARTLITE_OK;
+  OnDevice on;
+  const int rc = on.set(w->w.device);
+  if (w->w.done) (void)hipEventDestroy(w->w.done);
+  if (w->w.p) (void)hipFree(w->w.p);  // (waits for the device)
+  delete w;
+  return rc;
+}
+
+extern "C" int artlite_device_alloc(size_t nbytes, void** out, int* device) {
+  if (!out || !device) return fail(ARTLITE_EINVAL, "device memory: null");
+  *out = nullptr;
+  HostCtx* c;
+  ART_TRY(host_ctx(&c, false));
+  if (hipMalloc(out, nbytes ? nbytes : 1) != hipSuccess) {
+    (void)hipGetLastError();
+    return fail(ARTLITE_ENOMEM, "device memory: %zu bytes", nbytes);
+  }
+  *device = c->device;
+  return ARTLITE_OK;
+}
+
+extern "C" int artlite_device_free(void* p) {
+  if (p) ART_HIP(hipFree(p));
+  return ARTLITE_OK;
+}
+
+extern "C" int artlite_device_copy(void* dst, const void* src, size_t nbytes, int to_host) {
+  if (!nbytes) return ARTLITE_OK;
+  if (!dst || !src) return fail(ARTLITE_EINVAL, "device copy: null");
+  // (behind everything queued on the device, whichever streams it is on)
+  ART_HIP(hipDeviceSynchronize());
+  ART_HIP(hipMemcpy(dst, src, nbytes, to_host ? hipMemcpyDeviceToHost : hipMemcpyHostToDevice));
+  return ARTLITE_OK;
+}

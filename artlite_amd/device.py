@@ -1,0 +1,163 @@
+"""Arrays in GPU memory for the dense operators (``linear``, ``ffn``), and their workspaces. No torch: an operator takes
+
+- a ``DeviceArray`` (this module's own, for programs without an allocator),
+- any object that describes device memory: with ``data_ptr()``, ``shape``, ``stride()`` and ``dtype`` (a torch tensor), or
+  with ``__cuda_array_interface__``
+  (a program that uses torch imports it before this package's library loads, so that both share torch's HIP runtime: memory
+  of another runtime is refused),
+- or a host numpy array: copied to the GPU, computed there, and its result copied back before the call returns.
+
+Arrays are (rows, values) of fp32 or bf16 (numpy has no bf16: uint16 bit patterns), each row's values consecutive."""
+
+import ctypes
+import threading
+
+import numpy as np
+
+from . import _hip
+
+F32, BF16 = 0, 1  # artlite_dtype
+_CODES: dict[object, int] = {}  # a dtype object seen before -> its code
+_NAMES = {"float32": F32, "torch.float32": F32, "<f4": F32, "bfloat16": BF16, "torch.bfloat16": BF16, "uint16": BF16,
+          "torch.uint16": BF16, "<u2": BF16}
+
+
+def _code(dtype: object) -> int:
+    try:
+        return _CODES[dtype]
+    except KeyError:
+        code = _NAMES.get(str(dtype))
+        if code is None:
+            raise _hip.Error(f"device arrays are float32 or bfloat16 (uint16 bits), not {dtype}") from None
+        _CODES[dtype] = code
+        return code
+
+
+class DeviceArray:
+    """(rows, values) in GPU memory, on the device that is current when it is made. dtype: ``float32``, or ``uint16`` for
+    bf16 bits."""
+
+    def __init__(self, shape: tuple[int, int], dtype: object = np.float32):
+        self.dtype = np.dtype(dtype)
+        _code(self.dtype)
+        self.shape = (int(shape[0]), int(shape[1]))
+        p, dev = ctypes.c_void_p(), ctypes.c_int(0)
+        _hip.check(_hip.lib().artlite_device_alloc(self.nbytes, ctypes.byref(p), ctypes.byref(dev)))
+        self._p, self.device = p, dev.value
+
+    @classmethod
+    def of(cls, a: np.ndarray) -> "DeviceArray":
+        """A host array's copy."""
+        d = cls(a.shape, a.dtype)
+        d.copy_from(a)
+        return d
+
+    @property
+    def nbytes(self) -> int:
+        return self.shape[0] * self.shape[1] * self.dtype.itemsize
+
+    def data_ptr(self) -> int:
+        if self._p is None:
+            raise _hip.Error("DeviceArray: closed")
+        return self._p.value or 0
+
+    def stride(self) -> tuple[int, int]:
+        return self.shape[1], 1
+
+    def copy_from(self, a: np.ndarray) -> None:
+        a = np.ascontiguousarray(a)
+        if a.shape != self.shape or a.dtype != self.dtype:
+            raise _hip.Error(f"DeviceArray: {a.dtype} {a.shape} into {self.dtype} {self.shape}")
+        _hip.check(_hip.lib().artlite_device_copy(self.data_ptr(), a.ctypes.data, a.nbytes, 0))
+
+    def numpy(self) -> np.ndarray:
+        """A host copy, behind everything queued on the device."""
+        a = np.empty(self.shape, self.dtype)
+        _hip.check(_hip.lib().artlite_device_copy(a.ctypes.data, self.data_ptr(), a.nbytes, 1))
+        return a
+
+    def close(self) -> None:
+        if getattr(self, "_p", None) is not None:
+            _hip.lib().artlite_device_free(self._p)
+            self._p = None
+
+    def __del__(self) -> None:
+        self.close()
+
+
+class Workspace:
+    """Scratch memory of the operators' calls, of a fixed size, on the device that is current when it is made. Calls outside
+    a stream capture order themselves on it; graphs that run beside each other, or beside calls, take one each."""
+
+    def __init__(self, nbytes: int):
+        h = ctypes.c_void_p()
+        _hip.check(_hip.lib().artlite_workspace_create(nbytes, ctypes.byref(h)))
+        self._h, self.nbytes = h, nbytes
+
+    @property
+    def handle(self) -> ctypes.c_void_p:
+        if self._h is None:
+            raise _hip.Error("Workspace: closed")
+        return self._h
+
+    def close(self) -> None:
+        if getattr(self, "_h", None) is not None:
+            _hip.lib().artlite_workspace_destroy(self._h)
+            self._h = None
+
+    def __del__(self) -> None:
+        self.close()
+
+
+class Scratch:
+    """An operator's own workspace, grown as its calls need more. A workspace that it outgrows is kept: a graph captured on
+    it may be replayed yet (each is at least twice the one before, so that all take at most twice the last)."""
+
+    def __init__(self) -> None:
+        self._all: list[Workspace] = []
+        self._lock = threading.Lock()
+
+    def get(self, nbytes: int) -> Workspace:
+        with self._lock:
+            if not self._all or self._all[-1].nbytes < nbytes:
+                self._all.append(Workspace(max(nbytes, 2 * self._all[-1].nbytes if self._all else 0)))
+            return self._all[-1]
+
+    def close(self) -> None:
+        for w in self._all:
+            w.close()
+        self._all = []
+
+
+class View:
+    """An argument as a call takes it: address, dtype code, rows, values a row, row stride in values."""
+
+    __slots__ = ("at", "code", "rows", "cols", "row")
+
+    def __init__(self, a: object, what: str):
+        if hasattr(a, "data_ptr"):
+            shape, strides, self.code = a.shape, a.stride(), _code(a.dtype)
+            if len(shape) != 2:
+                raise _hip.Error(f"{what}: {tuple(shape)}, not (rows, values)")
+            self.at = a.data_ptr()
+        elif hasattr(a, "__cuda_array_interface__"):
+            d = a.__cuda_array_interface__
+            shape, self.at, self.code = d["shape"], d["data"][0], _code(d["typestr"])
+            if len(shape) != 2:
+                raise _hip.Error(f"{what}: {tuple(shape)}, not (rows, values)")
+            size = 4 if self.code == F32 else 2
+            strides = [s // size for s in d["strides"]] if d.get("strides") else (shape[1], 1)
+        else:
+            raise _hip.Error(f"{what}: {type(a).__name__} is no array of device memory")
+        self.rows, self.cols = shape
+        self.row = strides[0]
+        if strides[1] != 1 and self.cols > 1:
+            raise _hip.Error(f"{what}: a row's values are {strides[1]} apart")
+
+
+def overlap(a: View, b: View) -> bool:
+    """Whether the memory that two views span meets."""
+    def end(v: View) -> int:
+        return v.at + ((v.rows - 1) * v.row + v.cols) * (4 if v.code == F32 else 2)
+
+    return bool(a.rows and b.rows) and a.at < end(b) and b.at < end(a)

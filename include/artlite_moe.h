@@ -164,6 +164,65 @@ int artlite_moe_kernel_names(artlite_moe_layer* layer, int64_t T, char* buf, siz
 /* Bytes copied per ms by a plain device copy of nbytes (HBM calibration of the profile counters). */
 int artlite_hbm_copy(size_t nbytes, int iters, double* ms_per_copy);
 
+/* ---- dense products over 4-bit blocks: no counterpart in the reference's native module (its models run them as NPU
+ * programs). A matrix of a GGUF file (rows = output features, cols = K) in HBM, in the format's own bytes re-ordered for the
+ * kernels; Q4_0, Q4_1, Q4_K, IQ4_NL or IQ4_XS; cols a multiple of the format's block, at most 2^20; at most 2^24 rows.
+ * Created on the calling thread's current device, which its calls then use whichever device is current.
+ *
+ * x, y and the gradients below are DEVICE memory of that device (anything else is refused), bf16 or fp32 (artlite_dtype; y
+ * and gradients in x's type), rows of consecutive values `stride` values apart: x's at least 0 (0: one row for all), those
+ * of what is written at least the row's values. Calls are enqueued on `stream` (a hipStream_t; null: the null stream) and
+ * return at once; 0 rows write nothing. They may be captured into a graph: its replays use the workspace that was given, and
+ * whatever else uses that workspace has to be ordered with them by the caller's streams (a workspace for each graph that
+ * runs beside others). Outside captures, calls on one workspace order themselves, whichever streams and threads they come
+ * from. */
+typedef struct artlite_matrix artlite_matrix;
+int artlite_matrix_supported(int qtype);
+int artlite_matrix_create(int qtype, int64_t rows, int64_t cols, artlite_matrix** out);
+int artlite_matrix_destroy(artlite_matrix* m); /* its calls have come to their end */
+/* The rows' raw blocks (host, exactly their size); replaces earlier ones. */
+int artlite_matrix_upload(artlite_matrix* m, const void* data, size_t nbytes);
+/* n = rows fp32 values added to every output row of artlite_linear; n = 0: none. */
+int artlite_matrix_upload_bias(artlite_matrix* m, const float* data, size_t n);
+
+/* Scratch memory of calls, of a fixed size. */
+typedef struct artlite_workspace artlite_workspace;
+int artlite_workspace_create(size_t nbytes, artlite_workspace** out);
+int artlite_workspace_destroy(artlite_workspace* work); /* its calls have come to their end */
+
+/* y (n x rows) = x (n x cols) W^T (+ bias). x's products with the blocks' values are summed in fp32 and rounded once to y's
+ * type (up to 64 rows without rounding a weight; past that weights are fp16 of 11 bits for bf16 x, of 22 for fp32 x).
+ * artlite_linear_workspace: the bytes of workspace that such a call of n rows needs (aligned: x's rows start on 16 bytes and
+ * cols are a multiple of 32 anyhow; 0: they may not); work may be null where that is 0. */
+int artlite_linear_workspace(const artlite_matrix* w, int dtype, int64_t n, int aligned, size_t* nbytes);
+int artlite_linear(const artlite_matrix* w, const void* x, int dtype, int64_t n, int64_t x_stride, void* y,
+                   int64_t y_stride, artlite_workspace* work, void* stream);
+
+/* ---- the gated feed-forward block (a model's dense blocks: ffn_gate, ffn_up F x H, ffn_down H x F):
+ * y = (act(x gate^T) (x up^T)) down^T, and its backward pass from x and dy (n x H):
+ * dx = dg gate + du up, dgate = dg^T x, dup = du^T x, ddown = dy^T h, where g = x gate^T, u = x up^T, h = act(g) u,
+ * dh = dy down, dg = dh u act'(g), du = dh act(g); dgate, dup (F x H) and ddown (H x F) are the gradients of the blocks'
+ * values. The forward keeps nothing; the backward computes g and u again. Outputs that are null are not computed (dx too);
+ * dgate, dup, ddown: rows without gaps. */
+enum artlite_act { ARTLITE_ACT_SILU = 0, ARTLITE_ACT_GELU_TANH = 1 };
+typedef struct artlite_ffn {
+  const artlite_matrix *gate, *up, *down;
+  int32_t act; /* artlite_act */
+} artlite_ffn;
+/* the most that forward calls of at most n rows (backward = 0), or backward ones (1: dx alone, 2: weights' gradients) need */
+int artlite_ffn_workspace(const artlite_ffn* f, int dtype, int64_t n, int backward, size_t* nbytes);
+int artlite_ffn_forward(const artlite_ffn* f, const void* x, int dtype, int64_t n, int64_t x_stride, void* y,
+                        int64_t y_stride, artlite_workspace* work, void* stream);
+int artlite_ffn_backward(const artlite_ffn* f, const void* x, int64_t x_stride, const void* dy, int64_t dy_stride,
+                         int dtype, int64_t n, void* dx, int64_t dx_stride, void* dgate, void* dup, void* ddown,
+                         artlite_workspace* work, void* stream);
+
+/* Device memory for callers that have no allocator of their own: allocated on the current device (*device), and copied to
+ * (to_host 0) or from the host behind everything queued on the current device. */
+int artlite_device_alloc(size_t nbytes, void** out, int* device);
+int artlite_device_free(void* p);
+int artlite_device_copy(void* dst, const void* src, size_t nbytes, int to_host);
+
 #ifdef __cplusplus
 }
 #endif

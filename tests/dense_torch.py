@@ -1,0 +1,129 @@
+"""The dense operators on torch tensors, streams and graphs: a program of its own, since torch has to be imported before the
+library loads (both then share torch's HIP runtime). Run by test_dense_torch_gpu.py.
+
+TOL: a bf16 output's half step (2^-8) and the inner roundings' eighths of it (at most 8)."""
+
+import sys
+from pathlib import Path
+
+import numpy as np
+import torch
+
+sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
+
+from artlite_amd.device import Workspace  # noqa: E402
+from artlite_amd.ffn import GatedFFN  # noqa: E402
+from artlite_amd.linear import QLinear  # noqa: E402
+from oracle import dense  # noqa: E402
+
+TOL = 2.0 ** -8 + 8 * 2.0 ** -11
+
+
+def linear_streams_and_graphs() -> None:
+    """Torch tensors: calls that alternate between streams on one object's workspace; captured calls replayed with other
+    inputs, beside eager ones on workspaces of their own."""
+    N, K = 200, 512
+    lin = QLinear("Q4_1", N, K)
+    raw, w = dense.matrix("Q4_1", N, K, 8)
+    lin.upload(raw)
+    w = torch.from_numpy(w)
+
+    def ref(x: object) -> object:
+        return x.cpu().double() @ w.T
+
+    def near(y: object, x: object) -> None:
+        want = ref(x)
+        assert (y.cpu().double() - want).norm() <= 2.0 ** -7 * want.norm()
+
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    xs = [torch.randn(100 + i, K, device="cuda").bfloat16() for i in range(12)]
+    ys = [torch.empty(x.shape[0], N, device="cuda", dtype=torch.bfloat16) for x in xs]
+    torch.cuda.synchronize()
+    for i, (x, y) in enumerate(zip(xs, ys)):
+        lin(x, y, stream=streams[i % 3].cuda_stream)
+    torch.cuda.synchronize()
+    for x, y in zip(xs, ys):
+        near(y, x)
+    graphs = []
+    for M in (1, 100):
+        x = torch.randn(M, K, device="cuda").bfloat16()
+        y = torch.empty(M, N, device="cuda", dtype=torch.bfloat16)
+        work = Workspace(max(1, lin.workspace_bytes(M, "bf16")))
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            lin(x, y, stream=torch.cuda.current_stream().cuda_stream, work=work)
+        graphs.append((g, x, y, work))
+    for _ in range(3):
+        for g, x, y, _ in graphs:
+            x.copy_(torch.randn_like(x))
+            y.zero_()
+            g.replay()
+        lin(xs[0], ys[0])
+        torch.cuda.synchronize()
+        for _, x, y, _ in graphs:
+            near(y, x)
+        near(ys[0], xs[0])
+
+
+def ffn_streams_and_graphs() -> None:
+    """Torch tensors on several streams over one workspace; forward and backward captured and replayed with other inputs,
+    beside eager calls on other workspaces."""
+    H, F = 256, 512
+    f, w = GatedFFN(hidden=H, ffn=F, gate_type="Q4_K", down_type="Q4_K"), []
+    for i, (name, r, c) in enumerate((("gate", F, H), ("up", F, H), ("down", H, F))):
+        raw, v = dense.matrix("Q4_K", r, c, i)
+        f.upload("ffn_" + name, raw)
+        w.append(v)
+
+    def near(got: object, want: np.ndarray, tol: float) -> None:
+        assert np.linalg.norm(got.double().cpu().numpy() - want) <= tol * np.linalg.norm(want)
+
+    def host(t: object) -> np.ndarray:
+        return t.double().cpu().numpy()
+
+    def rand(n: int) -> object:
+        return torch.randn(n, H, device="cuda").bfloat16()
+
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    xs = [rand(n) for n in (5, 100, 64, 70, 1, 33)]
+    ys = [torch.empty_like(x) for x in xs]
+    torch.cuda.synchronize()
+    for i, (x, y) in enumerate(zip(xs, ys)):
+        f(x, y, stream=streams[i % 3].cuda_stream)
+    torch.cuda.synchronize()
+    for x, y in zip(xs, ys):
+        near(y, dense.ffn("silu", host(x), *w), TOL)
+    graphs = []
+    for n in (4, 90):
+        x, dy = rand(n), rand(n)
+        out = {"y": torch.empty_like(x), "dx": torch.empty_like(x),
+               "dgate": torch.empty(F, H, device="cuda", dtype=torch.bfloat16)}
+        work = Workspace(max(f.workspace_bytes(n), f.workspace_bytes(n, weights=True)))
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            s = torch.cuda.current_stream().cuda_stream
+            f(x, out["y"], stream=s, work=work)
+            f.backward(x, dy, dx=out["dx"], dgate=out["dgate"], stream=s, work=work)
+        graphs.append((g, x, dy, out, work))
+    for _ in range(3):
+        for g, x, dy, out, _ in graphs:
+            x.copy_(torch.randn_like(x))
+            dy.copy_(torch.randn_like(dy))
+            for t in out.values():
+                t.zero_()
+            g.replay()
+        f(xs[1], ys[1])
+        torch.cuda.synchronize()
+        near(ys[1], dense.ffn("silu", host(xs[1]), *w), TOL)
+        for _, x, dy, out, _ in graphs:
+            want = {"y": dense.ffn("silu", host(x), *w), **dense.ffn_grad("silu", host(x), host(dy), *w)}
+            for k, t in out.items():
+                near(t, want[k], TOL)
+
+
+if __name__ == "__main__":
+    for case in (linear_streams_and_graphs, ffn_streams_and_graphs):
+        case()
+        print(case.__name__, "passed", flush=True)

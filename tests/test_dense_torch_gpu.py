@@ -1,0 +1,16 @@
+"""The dense operators on torch tensors, in a process that imports torch first."""
+
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def test_torch_tensors_streams_and_graphs() -> None:
+    pytest.importorskip("torch")
+    r = subprocess.run([sys.executable, "-u", str(Path(__file__).with_name("dense_torch.py"))], capture_output=True, text=True,
+                       timeout=110)
+    assert r.returncode == 0 and r.stdout.count("passed") == 2, r.stdout + r.stderr
