@@ -15,6 +15,7 @@
 #include "hgemm.h"
 #include "matrix.h"
 
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
 
@@ -71,7 +72,7 @@ __global__ __launch_bounds__(256) void k_rows16(const void* __restrict__ x, int6
     if (k < K) load(k, v);
     uint16_t a[8], b[8];
     for (int i = 0; i < 8; i++) {
-      const float r = ldexpf(v[i], -e), s = ldexpf(r, 15);
+      const float r = __builtin_amdgcn_ldexpf(v[i], -e), s = __builtin_amdgcn_ldexpf(r, 15);
       ss = __builtin_fmaf(r, r, ss);
       const _Float16 hi = _Float16(s);
       a[i] = __builtin_bit_cast(uint16_t, hi);
@@ -89,13 +90,17 @@ __global__ __launch_bounds__(256) void k_rows16(const void* __restrict__ x, int6
   }
 }
 
-// the rows' scales of h and of dg, du, from the exponents of the rows' norms
-__global__ void k_exps(int64_t M, const int32_t* __restrict__ nx, const int32_t* __restrict__ ny, int lh, int ld,
-                       int32_t* __restrict__ he, int32_t* __restrict__ de) {
+// the rows' scales of h, dh and dg, du, from the exponents of the rows' norms and of the matrices' bounds (lh: gate's and up's
+// together, ld: down's, lw: the larger of gate's and up's and 1 for the derivative)
+__global__ void k_exps(int64_t M, const int32_t* __restrict__ nx, const int32_t* __restrict__ ny, int lh, int ld, int lw,
+                       int32_t* __restrict__ he, int32_t* __restrict__ dhe, int32_t* __restrict__ de) {
   const int64_t m = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (m >= M) return;
   he[m] = 2 * nx[m] + lh - 15;
-  if (de) de[m] = ny[m] + nx[m] + ld - 15;
+  if (ny) {
+    dhe[m] = ny[m] + ld - 15;
+    de[m] = ny[m] + ld + nx[m] + lw - 15;
+  }
 }
 
 // the largest of each of up to 4 arrays
@@ -127,7 +132,7 @@ __global__ __launch_bounds__(256) void k_turn(const uint16_t* __restrict__ in, i
       __builtin_memcpy(v, __builtin_assume_aligned(in + (t0 + r) * ld + c0 + c, 16), 16);
       const int sh = e[t0 + r] - E;
       for (int k = 0; k < 8; k++)
-        v[k] = __builtin_bit_cast(uint16_t, _Float16(ldexpf(float(__builtin_bit_cast(_Float16, v[k])), sh)));
+        v[k] = __builtin_bit_cast(uint16_t, _Float16(__builtin_amdgcn_ldexpf(float(__builtin_bit_cast(_Float16, v[k])), sh)));
     }
     for (int k = 0; k < 8; k++) t[c + k][r] = v[k];
   }
@@ -198,6 +203,7 @@ struct LinearPlan {
   uint16_t* planes = nullptr;                 // few rows: x as planes, where it is not read as it is
   uint16_t *x16 = nullptr, *w16 = nullptr;    // else
   int32_t* xe = nullptr;
+  float* parts = nullptr;
 };
 LinearPlan linear_plan(Carve& c, const artlite_matrix* w, int dtype, int64_t n, bool direct) {
   LinearPlan p;
@@ -210,6 +216,7 @@ LinearPlan linear_plan(Carve& c, const artlite_matrix* w, int dtype, int64_t n, 
     p.x16 = c.take<uint16_t>(size_t(pl) * n * Kp);
     p.w16 = c.take<uint16_t>(size_t(pl) * w->N * Kp);
     p.xe = c.take<int32_t>(n);
+    p.parts = c.take<float>(hgemm_parts_bytes(n, w->N, Kp, pl == 2 ? 3 : 1, false) / 4);
   }
   return p;
 }
@@ -266,6 +273,7 @@ int linear(const artlite_matrix* w, const void* x, int dtype, int64_t n, int64_t
   g.row_e = p.xe, g.e = e;
   g.bias = w->has_bias ? w->bias.as<float>() : nullptr;
   g.y = y, g.y_stride = y_stride, g.dtype = dtype;
+  g.parts = p.parts;
   return launch_hgemm(g, s);
 }
 
@@ -298,6 +306,7 @@ struct FfnPlan {
   uint16_t *planes = nullptr, *hp = nullptr;  // few rows: x as planes (where it is not read as it is), h as planes
   uint16_t *x16, *w16, *u16, *d16, *h16;      // else: x, the unpacked matrices, h
   int32_t *xe, *nx, *he;
+  float* parts;
 };
 FfnPlan ffn_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool direct) {
   FfnPlan p{};
@@ -317,6 +326,8 @@ FfnPlan ffn_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool direct) {
   p.xe = c.take<int32_t>(n);
   p.nx = c.take<int32_t>(n);
   p.he = c.take<int32_t>(n);
+  const int sg = b ? 1 : 3;
+  p.parts = c.take<float>(std::max(hgemm_parts_bytes(n, f.F, f.Hp, sg, true), hgemm_parts_bytes(n, f.H, f.Fp, sg, false)) / 4);
   return p;
 }
 
@@ -347,7 +358,8 @@ int ffn_forward(const Ffn& f, const void* x, int dtype, int64_t n, int64_t x_str
   }
   const int pl = b ? 1 : 2;
   ART_TRY(rows16(x, dtype, n, f.H, x_stride, p.x16, f.Hp, pl, p.xe, p.nx, s));
-  k_exps<<<unsigned((n + 255) / 256), 256, 0, s>>>(n, p.nx, nullptr, f.gate->row_exp + f.up->row_exp, 0, p.he, nullptr);
+  k_exps<<<unsigned((n + 255) / 256), 256, 0, s>>>(n, p.nx, nullptr, f.gate->row_exp + f.up->row_exp, 0, 0, p.he, nullptr,
+                                                   nullptr);
   ART_TRY(launch_unpack(f.gate, false, wexp16(f.gate), p.w16, f.Hp, f.F * f.Hp, pl, s));
   ART_TRY(launch_unpack(f.up, false, wexp16(f.up), p.u16, f.Hp, f.F * f.Hp, pl, s));
   ART_TRY(launch_unpack(f.down, false, wexp16(f.down), p.d16, f.Fp, f.H * f.Fp, pl, s));
@@ -359,6 +371,7 @@ int ffn_forward(const Ffn& f, const void* x, int dtype, int64_t n, int64_t x_str
   g.row_e = p.xe, g.e = wexp16(f.gate), g.e2 = wexp16(f.up);
   g.act = f.act;
   g.out_e = p.he, g.h = p.h16, g.h_stride = f.Fp, g.h_plane = n * f.Fp, g.planes = pl;
+  g.parts = p.parts;
   ART_TRY(launch_hgemm(g, s));
   HGemm d{};
   segments(d, {{p.h16, n * f.Fp, p.d16, f.H * f.Fp}}, pl);
@@ -366,15 +379,16 @@ int ffn_forward(const Ffn& f, const void* x, int dtype, int64_t n, int64_t x_str
   d.M = n, d.N = f.H;
   d.row_e = p.he, d.e = wexp16(f.down);
   d.y = y, d.y_stride = y_stride, d.dtype = dtype;
+  d.parts = p.parts;
   return launch_hgemm(d, s);
 }
 
 struct GradPlan {
   uint16_t *x16, *dy16, *a16, *b16, *c16;        // x, dy; gate and up, later their transposes; down's transpose
-  uint16_t *h16, *dg16, *du16;
+  uint16_t *h16, *dh16, *dg16, *du16;
   uint16_t *xt, *dyt, *ht, *dgt, *dut;           // (weights' gradients) turned
-  float* dh;
-  int32_t *xe, *nx, *ye, *ny, *he, *de, *top;
+  int32_t *xe, *nx, *ye, *ny, *he, *dhe, *de, *top;
+  float* parts;
 };
 GradPlan grad_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool weights) {
   GradPlan p{};
@@ -387,12 +401,13 @@ GradPlan grad_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool weights) {
   p.c16 = c.take<uint16_t>(pl * f.F * f.Hp);
   p.dg16 = c.take<uint16_t>(pl * n * f.Fp);
   p.du16 = c.take<uint16_t>(pl * n * f.Fp);
-  p.dh = c.take<float>(n * f.Fp);
+  p.dh16 = c.take<uint16_t>(pl * n * f.Fp);
   p.xe = c.take<int32_t>(n);
   p.nx = c.take<int32_t>(n);
   p.ye = c.take<int32_t>(n);
   p.ny = c.take<int32_t>(n);
   p.he = c.take<int32_t>(n);
+  p.dhe = c.take<int32_t>(n);
   p.de = c.take<int32_t>(n);
   if (weights) {
     const int64_t Tp = pad64(n);
@@ -404,6 +419,12 @@ GradPlan grad_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool weights) {
     p.dut = c.take<uint16_t>(pl * f.F * Tp);
     p.top = c.take<int32_t>(4);
   }
+  const int sg = pl == 2 ? 3 : 1;
+  size_t parts = std::max({hgemm_parts_bytes(n, f.F, f.Hp, sg, false), hgemm_parts_bytes(n, f.F, f.Hp, sg, true),
+                           hgemm_parts_bytes(n, f.H, f.Fp, 2 * sg, false)});
+  if (weights)
+    parts = std::max({parts, hgemm_parts_bytes(f.F, f.H, pad64(n), sg, false), hgemm_parts_bytes(f.H, f.F, pad64(n), sg, false)});
+  p.parts = c.take<float>(parts / 4);
   return p;
 }
 
@@ -416,8 +437,8 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
   ART_TRY(rows16(x, dtype, n, f.H, x_stride, p.x16, f.Hp, pl, p.xe, p.nx, s));
   ART_TRY(rows16(dy, dtype, n, f.H, dy_stride, p.dy16, f.Hp, pl, p.ye, p.ny, s));
   const int lg = f.gate->row_exp, lu = f.up->row_exp;
-  const int ld = f.down->max_exp + int(std::ceil(0.5 * std::log2(double(f.H)))) + (lg > lu ? lg : lu) + 1;
-  k_exps<<<unsigned((n + 255) / 256), 256, 0, s>>>(n, p.nx, p.ny, lg + lu, ld, p.he, p.de);
+  const int ld = f.down->max_exp + int(std::ceil(0.5 * std::log2(double(f.H))));
+  k_exps<<<unsigned((n + 255) / 256), 256, 0, s>>>(n, p.nx, p.ny, lg + lu, ld, (lg > lu ? lg : lu) + 1, p.he, p.dhe, p.de);
   // (gate and up share a scale: dx sums over both)
   const int e = wexp16(f.gate) > wexp16(f.up) ? wexp16(f.gate) : wexp16(f.up), ed = wexp16(f.down);
   ART_TRY(launch_unpack(f.gate, false, e, p.a16, f.Hp, f.F * f.Hp, pl, s));
@@ -427,8 +448,10 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
   segments(d, {{p.dy16, n * f.Hp, p.c16, f.F * f.Hp}}, pl);
   d.lda = d.ldb = d.K = f.Hp;
   d.M = n, d.N = f.F;
+  d.epilogue = H_ROWS;
   d.row_e = p.ye, d.e = ed;
-  d.y = p.dh, d.y_stride = f.Fp, d.dtype = ARTLITE_X_F32;
+  d.out_e = p.dhe, d.h = p.dh16, d.h_stride = f.Fp, d.h_plane = n * f.Fp, d.planes = pl;
+  d.parts = p.parts;
   ART_TRY(launch_hgemm(d, s));
   HGemm g{};
   segments(g, {{p.x16, n * f.Hp, p.a16, f.F * f.Hp, p.b16}}, pl);
@@ -437,10 +460,11 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
   g.epilogue = H_DGLU;
   g.row_e = p.xe, g.e = g.e2 = e;
   g.act = f.act;
-  g.dh = p.dh;
+  g.dh = p.dh16, g.dh_e = p.dhe;
   g.out_e = p.de, g.h_e = p.he;
   g.dg = p.dg16, g.du = p.du16, g.h = p.h16;
   g.h_stride = f.Fp, g.h_plane = n * f.Fp, g.planes = pl;
+  g.parts = p.parts;
   ART_TRY(launch_hgemm(g, s));
   if (dx) {
     ART_TRY(launch_unpack(f.gate, true, e, p.a16, f.Fp, f.H * f.Fp, pl, s));
@@ -451,6 +475,7 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
     x2.M = n, x2.N = f.H;
     x2.row_e = p.de, x2.e = e;
     x2.y = dx, x2.y_stride = dx_stride, x2.dtype = dtype;
+    x2.parts = p.parts;
     ART_TRY(launch_hgemm(x2, s));
   }
   if (!weights) return ARTLITE_OK;
@@ -471,6 +496,7 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
     w.M = M, w.N = N;
     w.e0 = ea, w.e1 = eb;
     w.y = out, w.y_stride = N, w.dtype = dtype;
+    w.parts = p.parts;
     return launch_hgemm(w, s);
   };
   if (dgate) ART_TRY(grad(p.dgt, f.F, p.top + 3, p.xt, f.H, p.top, dgate));
@@ -526,12 +552,6 @@ extern "C" int artlite_ffn_workspace(const artlite_ffn* d, int dtype, int64_t n,
     (void)grad_plan(c, f, dtype, n, backward == 2);
   } else if (n) {
     (void)ffn_plan(c, f, dtype, n, false);
-    // (calls of fewer rows need less on either side of the few, but not across it)
-    if (n > FEW_ROWS) {
-      Carve few(nullptr);
-      (void)ffn_plan(few, f, dtype, FEW_ROWS, false);
-      if (few.at > c.at) c.at = few.at;
-    }
   }
   *nbytes = c.at;
   return ARTLITE_OK;

@@ -5,7 +5,8 @@
 
 namespace artlite {
 
-enum HEpilogue { H_STORE = 0, H_GLU = 1, H_DGLU = 2 };
+// what becomes of the sums: H_STORE y (bf16 or fp32); H_ROWS fp16 rows; H_GLU h of a gated pair; H_DGLU its gradients
+enum HEpilogue { H_STORE = 0, H_ROWS = 1, H_GLU = 2, H_DGLU = 3 };
 
 // out[m][n] = sum over the segments and K of a[m][k] b[n][k]; a, b fp16 rows of lda, ldb values (K a multiple of 64; both
 // multiples of 8). A segment names its operands: planes of split values, or parts of a longer sum.
@@ -22,20 +23,24 @@ struct HGemm {
   const int32_t* row_e;
   const int32_t *e0, *e1;
   int e, e2;
-  // H_STORE: y[m][n] = the sum + bias[n], bf16 or fp32; or (y16) fp16 scaled by 2^-out_e[m] in `planes` planes
+  // H_STORE: y[m][n] = the sum + bias[n], bf16 or fp32
   const float* bias;
   void* y;
   int64_t y_stride;
   int dtype;
-  // H_GLU: h = act(g) u as fp16 planes of rows of h_stride values, times 2^-out_e[m]; columns N .. h_stride zeros
-  // H_DGLU: from dh (fp32, rows of h_stride values): dg and du likewise (2^-out_e[m]), and (h set) h times 2^-h_e[m]
+  // the others: fp16 planes of rows of h_stride values (a multiple of 64), times 2^-out_e[m]; columns N .. h_stride zeros.
+  // H_ROWS: h; H_GLU: h = act(g) u; H_DGLU: from dh (planes as these, worth 2^dh_e[m]) dg and du, and (h set) h times 2^-h_e[m]
   int act;
-  const int32_t *out_e, *h_e;
-  const float* dh;
+  const int32_t *out_e, *h_e, *dh_e;
+  const uint16_t* dh;
   uint16_t *h, *dg, *du;
   int64_t h_stride, h_plane;
   int planes;
+  // scratch for sums in parts: hgemm_parts_bytes of it
+  float* parts;
 };
+// the scratch that a product may take (gated: N columns of each matrix)
+size_t hgemm_parts_bytes(int64_t M, int64_t N, int64_t K, int segs, bool gated);
 int launch_hgemm(const HGemm& g, hipStream_t s);
 
 }  // namespace artlite

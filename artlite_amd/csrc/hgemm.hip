@@ -7,7 +7,7 @@
 // does not wait for it), three steps ahead; operands go from LDS to registers a step ahead of the MFMAs that use them, so one
 // barrier a step is all that a wave waits for. At its barrier a step's successor has landed (every wave has waited for its
 // own loads) and the slot that is filled next has been read (a step before the last).
-// Rows of a slot are 64 bytes, four 16-byte chunks, chunk c of row r at c ^ (r / 4 % 4): the 16 rows that a lane group reads
+// Rows of a slot are 64 bytes, four 16-byte chunks, chunk c of row r at c ^ (r / 2 % 4): the 16 rows that a lane group reads
 // take all banks. Rows past the matrices' ends repeat the last one, their outputs are not stored.
 // The weights' block is the MFMA's first operand, so a lane holds four consecutive columns of one output row.
 // Tiles are dealt so that the workgroups that run on an XCD at a time share rows and columns (its L2 holds them).
@@ -56,39 +56,133 @@ __device__ __forceinline__ void hg_for(F&& f) {
   hg_for_impl(f, std::make_integer_sequence<int, N>{});
 }
 
-constexpr int BK = 32, RING = 4;
+constexpr int BK = 32;
 
 template <int MB>
 struct HT {
   static constexpr int TM = 32 * MB;                 // rows and columns of a tile
   static constexpr int HALF = TM * BK * 2;           // bytes of an operand's step
   static constexpr int SLOT = 2 * HALF;
+  static constexpr int RING = MB == 8 ? 4 : 5;       // (all of LDS, or half: two small tiles a CU)
   static constexpr int LPW = SLOT / 1024 / 4;        // DMAs of a wave a step
   static constexpr int LDS = RING * SLOT;
-  static_assert(LDS <= LDS_BYTES, "LDS");
+  static_assert(LDS <= (MB == 8 ? LDS_BYTES : LDS_BYTES / 2), "LDS");
 };
 
-__device__ __forceinline__ uint16_t f16_bits(float v) { return __builtin_bit_cast(uint16_t, _Float16(v)); }
-
-// four fp16 values times 2^-e at p, and with a second plane what their rounding left
-__device__ __forceinline__ void store16(uint16_t* p, int64_t plane, int planes, const float (&v)[4], int e) {
-  uint16_t a[4], b[4];
+// eight fp16 values times 2^-e at p, and with a second plane what their rounding left
+__device__ __forceinline__ void store16(uint16_t* p, int64_t plane, int planes, const float (&v)[8], int e) {
+  uint16_t a[8], b[8];
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const float x = ldexpf(v[i], -e);
+  for (int i = 0; i < 8; i++) {
+    const float x = __builtin_amdgcn_ldexpf(v[i], -e);
     const _Float16 hi = _Float16(x);
     a[i] = __builtin_bit_cast(uint16_t, hi);
-    b[i] = f16_bits(x - float(hi));
+    b[i] = __builtin_bit_cast(uint16_t, _Float16(x - float(hi)));
   }
-  __builtin_memcpy(__builtin_assume_aligned(p, 8), a, 8);
-  if (planes == 2) __builtin_memcpy(__builtin_assume_aligned(p + plane, 8), b, 8);
+  __builtin_memcpy(__builtin_assume_aligned(p, 16), a, 16);
+  if (planes == 2) __builtin_memcpy(__builtin_assume_aligned(p + plane, 16), b, 16);
 }
 
-template <int MB, int EPI>
-__global__ __launch_bounds__(256, MB == 8 ? 1 : 2) void k_hgemm(const HGemm g, int gm, int gn) {
+// a row's exponents: of its sums, of what is written, of h beside dg and du, of dh
+struct RowExp {
+  int sum, out, h, dh;
+};
+
+// columns n .. n + 8 of row m from their sums v (gated: and the second matrix's u)
+template <int EPI>
+__device__ __forceinline__ void finish(const HGemm& g, int es, const RowExp& r, int64_t m, int64_t n, float (&v)[8],
+                                       float (&u)[8], const float (&bias)[8]) {
+  const int there = int(max(int64_t(0), min(int64_t(8), g.N - n)));  // (columns that there are)
+  if constexpr (EPI == H_STORE) {
+    if (there == 0) return;
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = __builtin_amdgcn_ldexpf(v[k], es + r.sum) + bias[k];
+    const int64_t at = m * g.y_stride + n;
+    if (g.dtype == ARTLITE_X_BF16) {
+      uint16_t* y = static_cast<uint16_t*>(g.y) + at;
+      if (there == 8 && (reinterpret_cast<uintptr_t>(y) & 15) == 0) {
+        u32x4 w;
+#pragma unroll
+        for (int k = 0; k < 4; k++) w[k] = bf16_pair(v[2 * k], v[2 * k + 1]);
+        __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(y));
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          if (k < there) y[k] = uint16_t(f32_to_bf16(v[k]));
+      }
+    } else {
+      float* y = static_cast<float*>(g.y) + at;
+      if (there == 8 && (reinterpret_cast<uintptr_t>(y) & 15) == 0) {
+        __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4*>(y));
+        __builtin_nontemporal_store(f32x4{v[4], v[5], v[6], v[7]}, reinterpret_cast<f32x4*>(y + 4));
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          if (k < there) y[k] = v[k];
+      }
+    }
+  } else {
+    if (n >= g.h_stride) return;
+    const int64_t at = m * g.h_stride + n;
+    if constexpr (EPI == H_ROWS) {
+#pragma unroll
+      for (int k = 0; k < 8; k++) v[k] = k < there ? __builtin_amdgcn_ldexpf(v[k], es + r.sum) : 0.0f;
+      store16(g.h + at, g.h_plane, g.planes, v, r.out);
+    } else if constexpr (EPI == H_GLU) {
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        v[k] = k < there ? gate_act(g.act, __builtin_amdgcn_ldexpf(v[k], es + r.sum)) *
+                               __builtin_amdgcn_ldexpf(u[k], es - g.e + g.e2 + r.sum)
+                         : 0.0f;
+      store16(g.h + at, g.h_plane, g.planes, v, r.out);
+    } else {
+      float d[8], h[8];
+      const f16x8 d0 = *reinterpret_cast<const f16x8*>(g.dh + at);
+#pragma unroll
+      for (int k = 0; k < 8; k++) d[k] = float(d0[k]);
+      if (g.planes == 2) {
+        const f16x8 d1 = *reinterpret_cast<const f16x8*>(g.dh + g.h_plane + at);
+#pragma unroll
+        for (int k = 0; k < 8; k++) d[k] += float(d1[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const bool is = k < there;
+        const float gv = __builtin_amdgcn_ldexpf(v[k], es + r.sum), uv = __builtin_amdgcn_ldexpf(u[k], es - g.e + g.e2 + r.sum),
+                    dh = __builtin_amdgcn_ldexpf(d[k], r.dh);
+        float a, da;
+        gate_act_grad(g.act, gv, a, da);
+        h[k] = is ? a * uv : 0.0f;
+        v[k] = is ? dh * uv * da : 0.0f;
+        u[k] = is ? dh * a : 0.0f;
+      }
+      store16(g.dg + at, g.h_plane, g.planes, v, r.out);
+      store16(g.du + at, g.h_plane, g.planes, u, r.out);
+      if (g.h) store16(g.h + at, g.h_plane, g.planes, h, r.h);
+    }
+  }
+}
+
+template <int EPI>
+constexpr bool gated = EPI == H_GLU || EPI == H_DGLU;
+template <int EPI>
+__device__ __forceinline__ RowExp row_exp(const HGemm& g, int64_t m) {
+  return RowExp{g.row_e ? g.row_e[m] : 0, EPI != H_STORE ? g.out_e[m] : 0, EPI == H_DGLU && g.h ? g.h_e[m] : 0,
+                EPI == H_DGLU ? g.dh_e[m] : 0};
+}
+// a part's sums: rows of pad64(N) floats, of a gated pair both matrices' side by side
+template <int EPI>
+__host__ __device__ __forceinline__ int64_t part_row(const HGemm& g) {
+  return (gated<EPI> ? 2 : 1) * pad64(g.N);
+}
+
+// tiles from column n_off on, gm x gn of them; K in gridDim.y parts (PART: their sums into g.parts, for k_join)
+template <int MB, int EPI, bool PART>
+__global__ __launch_bounds__(256, MB == 8 ? 1 : 2) void k_hgemm(const HGemm g, int64_t n_off, int gm, int gn) {
   using T = HT<MB>;
-  constexpr int TM = T::TM;
-  constexpr int TN = EPI == H_STORE ? TM : TM / 2;  // output columns of a tile
+  constexpr int TM = T::TM, RING = T::RING;
+  constexpr bool GATED = gated<EPI>;
+  constexpr int TN = GATED ? TM / 2 : TM;  // output columns of a tile
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lg = lane >> 4, lr = lane & 15;
   const int wm = wv >> 1, wn = wv & 1;
@@ -104,7 +198,7 @@ __global__ __launch_bounds__(256, MB == 8 ? 1 : 2) void k_hgemm(const HGemm g, i
     mt = __builtin_amdgcn_readfirstlane(band * GR + in % rows);
     nt = __builtin_amdgcn_readfirstlane(in / rows);
   }
-  const int64_t m0 = int64_t(mt) * TM, n0 = int64_t(nt) * TN;
+  const int64_t m0 = int64_t(mt) * TM, n0 = n_off + int64_t(nt) * TN;
   const int mv = int(min(int64_t(TM), g.M - m0)), nv = int(min(int64_t(TN), g.N - n0));  // (rows, columns that there are)
 
   // ---- the issue side: a wave's DMAs of a step take 16 rows each, HPW of A's and HPW of B's (a wave's columns of a gated
@@ -114,174 +208,250 @@ __global__ __launch_bounds__(256, MB == 8 ? 1 : 2) void k_hgemm(const HGemm g, i
   uint32_t offa[HPW], offb[HPW];
 #pragma unroll
   for (int i = 0; i < HPW; i++) {
-    const int r = 16 * (HPW * wv + i) + (lane >> 2), c = (lane & 3) ^ ((r >> 2) & 3);
-    const int rb = EPI == H_STORE ? r : r / (TM / 2) * (TM / 4) + r % (TM / 4);
+    const int r = 16 * (HPW * wv + i) + (lane >> 2), c = (lane & 3) ^ ((r >> 1) & 3);
+    const int rb = GATED ? r / (TM / 2) * (TM / 4) + r % (TM / 4) : r;
     offa[i] = uint32_t(min(r, mv - 1)) * uint32_t(g.lda) * 2 + 16 * c;
     offb[i] = uint32_t(min(rb, nv - 1)) * uint32_t(g.ldb) * 2 + 16 * c;
   }
-  const int steps_seg = int(g.K / BK), steps = steps_seg * g.segs;
-  int iseg = 0, ik = 0, islot = 0;
+  // K in pairs of steps (64 values), a part of them; pair j's first values at (pa, pb): a segment's, then the next one's,
+  // past the last pair its own again (loads into slots that are not read: the counts stay)
+  const int pairs_seg = int(g.K / (2 * BK)), all = pairs_seg * g.segs;
+  const int first = PART ? int(int64_t(all) * blockIdx.y / gridDim.y) : 0;
+  const int pairs = PART ? int(int64_t(all) * (blockIdx.y + 1) / gridDim.y) - first : all;
+  int iseg = PART ? first / pairs_seg : 0, ipair = PART ? first % pairs_seg : 0;
   const uint16_t *pa, *pb;
   auto open_seg = [&]() {
-    pa = g.a[iseg] + m0 * g.lda;
-    pb = (EPI != H_STORE && (wv & 1) ? g.b2[iseg] : g.b[iseg]) + n0 * g.ldb;
+    pa = hg_uniform(g.a[iseg] + m0 * g.lda + ipair * (2 * BK));
+    pb = hg_uniform((GATED && (wv & 1) ? g.b2[iseg] : g.b[iseg]) + n0 * g.ldb + ipair * (2 * BK));
   };
-  open_seg();
-  auto issue = [&]() {
-    const uint32_t d = __builtin_amdgcn_readfirstlane(lds0 + islot * T::SLOT + HPW * wv * 1024);
-    const uint16_t *ua = hg_uniform(pa), *ub = hg_uniform(pb);
-#pragma unroll
-    for (int i = 0; i < HPW; i++) {
-      hg_dma(ua, offa[i], d + 1024 * i);
-      hg_dma(ub, offb[i], d + T::HALF + 1024 * i);
-    }
-    islot = (islot + 1) % RING;
-    // (past the last step its loads are made again, into slots that are not read: the counts stay)
-    if (++ik < steps_seg) {
-      pa += BK, pb += BK;
+  auto next_pair = [&]() {
+    if (++ipair < pairs_seg) {
+      pa += 2 * BK, pb += 2 * BK;
     } else if (iseg + 1 < g.segs) {
-      ik = 0;
-      iseg++;
+      ipair = 0, iseg++;
       open_seg();
     } else {
-      ik = steps_seg - 1;
+      ipair = pairs_seg - 1;
     }
+  };
+  // DMA i of a step at (a, b) into slot
+  auto dma = [&](int i, const uint16_t* a, const uint16_t* b, int slot) __attribute__((always_inline)) {
+    const uint32_t d = __builtin_amdgcn_readfirstlane(lds0 + slot * T::SLOT + (HPW * wv + (i >> 1)) * 1024);
+    if (i & 1)
+      hg_dma(hg_uniform(b), offb[i >> 1], d + T::HALF);
+    else
+      hg_dma(hg_uniform(a), offa[i >> 1], d);
   };
 
   f32x4 acc[MB][MB];
   hg_for<MB>([&](auto i) {
     hg_for<MB>([&](auto j) { acc[i][j] = f32x4{0, 0, 0, 0}; });
   });
-  const uint32_t lo = lr * 64 + ((lg ^ ((lr >> 2) & 3)) << 4);
+  const uint32_t lo = lr * 64 + ((lg ^ ((lr >> 1) & 3)) << 4);
   const uint8_t* const la = lds + wm * (TM / 2) * 64 + lo;
   const uint8_t* const lb = lds + T::HALF + wn * (TM / 2) * 64 + lo;
-  // B's operands of a step, and the next step's as they are read; A's in a window of 4, read two blocks ahead
+  // B's operands of a step, and the next step's as they are read; A's in a window of 4, read two blocks ahead. Each block's
+  // products stay behind its loads and reads (sched_barrier: the scheduler would gather the reads before their uses).
   u32x4 fa[4], fb[2][MB];
-  int rslot = 0;
   auto ld = [](const uint8_t* p) __attribute__((always_inline)) { return *reinterpret_cast<const u32x4*>(p); };
-  auto step = [&](auto set) __attribute__((always_inline)) {
+  // a step of a pair (SET: which of its two) on the slot `slot`, its successor in the next one; loads from (a, b) into the
+  // slot before it
+  int slot = 0;
+  auto step = [&](auto set, const uint16_t* a, const uint16_t* b) __attribute__((always_inline)) {
     constexpr int S = decltype(set)::value;
-    hg_wait<T::LPW>();
+    const int nslot = slot + 1 < RING ? slot + 1 : 0, islot = slot > 0 ? slot - 1 : RING - 1;
+    hg_wait<(RING - 3) * T::LPW>();
     hg_barrier();
-    issue();
-    const int nslot = (rslot + 1) % RING;
-    const uint8_t *a = la + rslot * T::SLOT, *an = la + nslot * T::SLOT, *bn = lb + nslot * T::SLOT;
-    rslot = nslot;
+    const uint8_t *sa = la + slot * T::SLOT, *na = la + nslot * T::SLOT, *nb = lb + nslot * T::SLOT;
     hg_for<MB>([&](auto ic) __attribute__((always_inline)) {
       constexpr int i = decltype(ic)::value;
-      fb[1 - S][i] = ld(bn + 1024 * i);
-      fa[(i + 2) % 4] = i + 2 < MB ? ld(a + 1024 * (i + 2)) : ld(an + 1024 * (i + 2 - MB));
+      fb[1 - S][i] = ld(nb + 1024 * i);
+      fa[(i + 2) % 4] = i + 2 < MB ? ld(sa + 1024 * (i + 2)) : ld(na + 1024 * (i + 2 - MB));
+      dma(i, a, b, islot);
       hg_for<MB>([&](auto j) __attribute__((always_inline)) { acc[i][j] = hg_mfma(fb[S][j], fa[i % 4], acc[i][j]); });
+      __builtin_amdgcn_sched_barrier(0);
     });
+    slot = nslot;
   };
-  issue();
-  issue();
-  issue();
-  hg_wait<2 * T::LPW>();
+  static_assert(T::LPW == MB && (RING == 4 || RING == 5), "a DMA a block; 3 or 4 steps ahead");
+  open_seg();
+  for (int i = 0; i < MB; i++) dma(i, pa, pb, 0);
+  for (int i = 0; i < MB; i++) dma(i, pa + BK, pb + BK, 1);
+  next_pair();
+  for (int i = 0; i < MB; i++) dma(i, pa, pb, 2);
+  if constexpr (RING == 5)
+    for (int i = 0; i < MB; i++) dma(i, pa + BK, pb + BK, 3);
+  hg_wait<(RING - 2) * T::LPW>();
   hg_barrier();
   hg_for<MB>([&](auto j) { fb[0][j] = ld(lb + 1024 * decltype(j)::value); });
   fa[0] = ld(la);
   fa[1] = ld(la + 1024);
-  for (int s = 0; s < steps; s += 2) {  // (K is a multiple of 64: an even number of steps)
-    step(std::integral_constant<int, 0>{});
-    step(std::integral_constant<int, 1>{});
+  // pair p's two steps; loaded meanwhile the steps RING - 1 after them: the second of pair p + 1 and the first of pair p + 2,
+  // or both of pair p + 2
+  for (int p = 0; p < pairs; p++) {
+    const uint16_t *a1 = pa + BK, *b1 = pb + BK;
+    next_pair();
+    step(std::integral_constant<int, 0>{}, RING == 4 ? a1 : pa, RING == 4 ? b1 : pb);
+    step(std::integral_constant<int, 1>{}, RING == 4 ? pa : pa + BK, RING == 4 ? pb : pb + BK);
   }
-  hg_wait<0>();  // (no load may land after the workgroup's LDS is another's)
+  hg_wait<0>();  // (every load of the workgroup has landed: the sums take its LDS)
+  hg_barrier();
 
-  // ---- outputs: block (i, j), lane: row m0 + wm TM / 2 + 16 i + lr, four columns from 16 j + 4 lg of the wave's
-  const int es = g.e + (g.e0 ? *g.e0 : 0) + (g.e1 ? *g.e1 : 0);
-  hg_for<MB>([&](auto ic) {
-    constexpr int i = decltype(ic)::value;
-    const int64_t m = m0 + wm * (TM / 2) + 16 * i + lr;
-    if (m >= g.M) return;
-    const int re = g.row_e ? g.row_e[m] : 0;
-    if constexpr (EPI == H_STORE) {
-      hg_for<MB>([&](auto jc) {
-        constexpr int j = decltype(jc)::value;
-        const int64_t n = n0 + wn * (TM / 2) + 16 * j + 4 * lg;
-        if (n >= g.N) return;
-        float v[4];
+  // (the rows' exponents, so that no load is waited for row by row)
+  RowExp* const rows_e = reinterpret_cast<RowExp*>(lds + T::LDS - TM * sizeof(RowExp));
+  if constexpr (!PART) {
+    for (int r = threadIdx.x; r < TM; r += 256) rows_e[r] = row_exp<EPI>(g, m0 + min(r, mv - 1));
+    __syncthreads();
+  }
+
+  // ---- outputs, 32 of the wave's rows at a time by way of its own part of LDS, from where a lane takes 8 columns of a row
+  constexpr int LROW = 16 * MB + 4;                    // (a row's floats and 4 more: banks)
+  constexpr int COLS = GATED ? 8 * MB : 16 * MB;       // the wave's output columns
+  constexpr int LPR = COLS / 8, RPI = 64 / LPR;        // lanes a row, rows an iteration
+  float* const buf = reinterpret_cast<float*>(lds) + wv * 32 * LROW;
+  static_assert(4 * 32 * LROW * 4 + TM * sizeof(RowExp) <= T::LDS, "LDS");
+  const int es = PART ? 0 : g.e + (g.e0 ? *g.e0 : 0) + (g.e1 ? *g.e1 : 0);
+  const int64_t n = n0 + wn * COLS + 8 * (lane % LPR);
+  const float* const from = buf + (lane / LPR) * LROW + 8 * (lane % LPR);
+  const auto get = [](const float* p, float(&v)[8]) __attribute__((always_inline)) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-          v[k] = ldexpf(acc[i][j][k], es + re) + (g.bias && n + k < g.N ? g.bias[n + k] : 0.0f);
-        const int64_t at = m * g.y_stride + n;
-        if (g.dtype == ARTLITE_X_BF16) {
-          uint16_t* y = static_cast<uint16_t*>(g.y) + at;
-          if (n + 3 < g.N && (reinterpret_cast<uintptr_t>(y) & 7) == 0) {
-            *reinterpret_cast<uint2*>(y) = uint2{f32_to_bf16(v[0]) | f32_to_bf16(v[1]) << 16,
-                                                 f32_to_bf16(v[2]) | f32_to_bf16(v[3]) << 16};
-          } else {
+    for (int k = 0; k < 4; k++) v[k] = a[k], v[4 + k] = b[k];
+  };
+  float bias[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (EPI == H_STORE && !PART && g.bias)
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-              if (n + k < g.N) y[k] = uint16_t(f32_to_bf16(v[k]));
-          }
-        } else {
-          float* y = static_cast<float*>(g.y) + at;
-          if (n + 3 < g.N && (reinterpret_cast<uintptr_t>(y) & 15) == 0) {
-            *reinterpret_cast<float4*>(y) = float4{v[0], v[1], v[2], v[3]};
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-              if (n + k < g.N) y[k] = v[k];
-          }
-        }
+    for (int k = 0; k < 8; k++)
+      if (n + k < g.N) bias[k] = g.bias[n + k];
+  auto put = [&](auto pc) __attribute__((always_inline)) {
+    hg_for<2>([&](auto ic) __attribute__((always_inline)) {
+      hg_for<MB>([&](auto jc) __attribute__((always_inline)) {
+        constexpr int i = decltype(ic)::value, j = decltype(jc)::value;
+        *reinterpret_cast<f32x4*>(buf + (16 * i + lr) * LROW + 16 * j + 4 * lg) = acc[2 * decltype(pc)::value + i][j];
       });
-    } else {
-      const int oe = g.out_e[m], he = EPI == H_DGLU && g.h ? g.h_e[m] : 0;
-      hg_for<MB / 2>([&](auto jc) {
-        constexpr int j = decltype(jc)::value;
-        const int64_t n = n0 + wn * (TM / 4) + 16 * j + 4 * lg;
-        if (n >= g.h_stride) return;
-        const int64_t at = m * g.h_stride + n;
-        float h[4], dg[4], du[4];
-        float4 dh = {0, 0, 0, 0};
-        if constexpr (EPI == H_DGLU) dh = *reinterpret_cast<const float4*>(g.dh + at);
-        const float d[4] = {dh.x, dh.y, dh.z, dh.w};
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const bool there = n + k < g.N;
-          const float gv = ldexpf(acc[i][j][k], g.e + re), uv = ldexpf(acc[i][j + MB / 2][k], g.e2 + re);
-          const float a = gate_act(g.act, gv);
-          h[k] = there ? a * uv : 0.0f;
-          if constexpr (EPI == H_DGLU) {
-            dg[k] = there ? d[k] * uv * gate_act_grad(g.act, gv) : 0.0f;
-            du[k] = there ? d[k] * a : 0.0f;
+    });
+  };
+  // (one copy of the rows' code: instructions that run once come from memory)
+#pragma unroll 1
+  for (int P = 0; P < MB / 2; P++) {
+    if (P == 0)
+      put(std::integral_constant<int, 0>{});
+    else if (P == 1)
+      put(std::integral_constant<int, 1>{});
+    else if (P == 2)
+      put(std::integral_constant<int, (MB > 4 ? 2 : 0)>{});
+    else
+      put(std::integral_constant<int, (MB > 4 ? 3 : 0)>{});
+#pragma unroll 2
+    for (int r = 0; r < 32; r += RPI) {
+      const int row = wm * (TM / 2) + 32 * P + r + lane / LPR;
+      const int64_t m = m0 + row;
+      if (m >= g.M) continue;
+      const float* p = from + r * LROW;
+      float v[8], u[8];
+      get(p, v);
+      if constexpr (GATED) get(p + 8 * MB, u);
+      if constexpr (PART) {
+        const int64_t pr = part_row<EPI>(g);
+        float* o = g.parts + (int64_t(blockIdx.y) * g.M + m) * pr + n;
+        if (n < pad64(g.N)) {
+          *reinterpret_cast<f32x4*>(o) = f32x4{v[0], v[1], v[2], v[3]};
+          *reinterpret_cast<f32x4*>(o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+          if constexpr (GATED) {
+            *reinterpret_cast<f32x4*>(o + pr / 2) = f32x4{u[0], u[1], u[2], u[3]};
+            *reinterpret_cast<f32x4*>(o + pr / 2 + 4) = f32x4{u[4], u[5], u[6], u[7]};
           }
         }
-        if constexpr (EPI == H_GLU) {
-          store16(g.h + at, g.h_plane, g.planes, h, oe);
-        } else {
-          store16(g.dg + at, g.h_plane, g.planes, dg, oe);
-          store16(g.du + at, g.h_plane, g.planes, du, oe);
-          if (g.h) store16(g.h + at, g.h_plane, g.planes, h, he);
-        }
-      });
+      } else {
+        finish<EPI>(g, es, rows_e[row], m, n, v, u, bias);
+      }
     }
-  });
+  }
 }
 
-template <int MB, int EPI>
-int launch_t(const HGemm& g, hipStream_t s) {
+// the parts' sums, in order, and what becomes of them: 8 columns a thread
+template <int EPI>
+__global__ __launch_bounds__(256) void k_join(const HGemm g, int parts) {
+  const int64_t cols = pad64(g.N) / 8, i = int64_t(blockIdx.x) * 256 + threadIdx.x, m = i / cols, n = 8 * (i % cols);
+  if (m >= g.M) return;
+  const int64_t pr = part_row<EPI>(g);
+  const float* p = g.parts + m * pr + n;
+  float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, u[8] = {0, 0, 0, 0, 0, 0, 0, 0}, bias[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int k = 0; k < parts; k++, p += g.M * pr)
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(p + 4 * h);
+#pragma unroll
+      for (int c = 0; c < 4; c++) v[4 * h + c] += a[c];
+      if constexpr (gated<EPI>) {
+        const f32x4 b = *reinterpret_cast<const f32x4*>(p + pr / 2 + 4 * h);
+#pragma unroll
+        for (int c = 0; c < 4; c++) u[4 * h + c] += b[c];
+      }
+    }
+  if (EPI == H_STORE && g.bias)
+    for (int k = 0; k < 8; k++)
+      if (n + k < g.N) bias[k] = g.bias[n + k];
+  finish<EPI>(g, g.e + (g.e0 ? *g.e0 : 0) + (g.e1 ? *g.e1 : 0), row_exp<EPI>(g, m), m, n, v, u, bias);
+}
+
+// How a product is cut: `big` columns in tiles of 256 x 256, the rest in tiles of 128 x 128, K in `parts`.
+struct Cut {
+  int64_t big, small;  // columns of tiles
+  int parts;
+};
+constexpr int CUS = 256;
+Cut cut(int64_t M, int64_t N, int64_t K, int segs, bool gate) {
+  const int64_t cols = gate ? 2 * N : N, gm = (M + 255) / 256, gn = (cols + 255) / 256, sm = (M + 127) / 128;
+  const int64_t tiles = gm * gn, left = tiles % CUS;
+  if (tiles >= CUS) {
+    // a last round of few tiles takes as long as a full one: where half the CUs would idle in it its columns go in small tiles
+    const int64_t keep = tiles / CUS * CUS / gm;
+    if (left && left <= CUS / 2 && keep >= 1) return Cut{keep, (cols - keep * 256 + 127) / 128, 1};
+    return Cut{gn, 0, 1};
+  }
+  const int64_t sn = (cols + 127) / 128, pairs = K / (2 * BK) * segs;
+  int parts = 1;
+  // (two small tiles a CU; a part of at least 4 pairs, 256 values)
+  while (parts < 16 && sm * sn * parts * 2 <= 2 * CUS && pairs / (2 * parts) >= 4) parts *= 2;
+  return Cut{0, sn, parts};
+}
+
+template <int MB, int EPI, bool PART>
+int launch_t(const HGemm& g, int64_t n_off, int64_t gn, int parts, hipStream_t s) {
   using T = HT<MB>;
-  constexpr int TN = EPI == H_STORE ? T::TM : T::TM / 2;
-  static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(k_hgemm<MB, EPI>),
+  static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(k_hgemm<MB, EPI, PART>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS) == hipSuccess;
   if (!ok) return fail(ARTLITE_EHIP, "large tiles: kernel set-up failed");
-  const int64_t gm = (g.M + T::TM - 1) / T::TM, gn = (g.N + TN - 1) / TN;
+  const int64_t gm = (g.M + T::TM - 1) / T::TM;
   if (gm * gn > (int64_t(1) << 30)) return fail(ARTLITE_EINVAL, "large tiles: %lld tiles", (long long)(gm * gn));
-  k_hgemm<MB, EPI><<<unsigned(gm * gn), 256, T::LDS, s>>>(g, int(gm), int(gn));
+  k_hgemm<MB, EPI, PART><<<dim3(unsigned(gm * gn), unsigned(parts)), 256, T::LDS, s>>>(g, n_off, int(gm), int(gn));
   ART_HIP(hipGetLastError());
   return ARTLITE_OK;
 }
 
 template <int EPI>
 int launch_e(const HGemm& g, hipStream_t s) {
-  const int64_t cols = EPI == H_STORE ? g.N : 2 * g.N;
-  const int64_t big = ((g.M + 255) / 256) * ((cols + 255) / 256);
-  return big >= 256 ? launch_t<8, EPI>(g, s) : launch_t<4, EPI>(g, s);
+  const Cut c = cut(g.M, g.N, g.K, g.segs, gated<EPI>);
+  if (c.parts > 1) {
+    if (!g.parts) return fail(ARTLITE_EINVAL, "large tiles: no scratch for parts");
+    ART_TRY((launch_t<4, EPI, true>(g, 0, c.small, c.parts, s)));
+    const int64_t threads = g.M * (pad64(g.N) / 8);
+    k_join<EPI><<<unsigned((threads + 255) / 256), 256, 0, s>>>(g, c.parts);
+    ART_HIP(hipGetLastError());
+    return ARTLITE_OK;
+  }
+  if (c.big) ART_TRY((launch_t<8, EPI, false>(g, 0, c.big, 1, s)));
+  if (c.small) ART_TRY((launch_t<4, EPI, false>(g, c.big * (gated<EPI> ? 128 : 256), c.small, 1, s)));
+  return ARTLITE_OK;
 }
 
 }  // namespace
+
+size_t hgemm_parts_bytes(int64_t M, int64_t N, int64_t K, int segs, bool gate) {
+  const Cut c = cut(M, N, K, segs, gate);
+  return c.parts > 1 ? size_t(c.parts) * M * (gate ? 2 : 1) * pad64(N) * 4 : 0;
+}
 
 int launch_hgemm(const HGemm& g, hipStream_t s) {
   if (g.M <= 0 || g.N <= 0) return ARTLITE_OK;
@@ -289,9 +459,10 @@ int launch_hgemm(const HGemm& g, hipStream_t s) {
       g.lda > (int64_t(1) << 22) || g.ldb > (int64_t(1) << 22) || g.K * g.segs / BK >= (int64_t(1) << 30))
     return fail(ARTLITE_EINVAL, "large tiles: K %lld of rows of %lld and %lld", (long long)g.K, (long long)g.lda,
                 (long long)g.ldb);
-  return g.epilogue == H_STORE ? launch_e<H_STORE>(g, s)
-         : g.epilogue == H_GLU ? launch_e<H_GLU>(g, s)
-                               : launch_e<H_DGLU>(g, s);
+  return g.epilogue == H_STORE  ? launch_e<H_STORE>(g, s)
+         : g.epilogue == H_ROWS ? launch_e<H_ROWS>(g, s)
+         : g.epilogue == H_GLU  ? launch_e<H_GLU>(g, s)
+                                : launch_e<H_DGLU>(g, s);
 }
 
 }  // namespace artlite

@@ -111,20 +111,37 @@ __device__ __forceinline__ void tile_values(uint32_t w, float s, float o, float 
   }
 }
 
-// the gated block's activation and its derivative (artlite_act), fp32
-__device__ __forceinline__ float gate_act(int act, float g) {
-  if (act == ARTLITE_ACT_SILU) return g / (1.0f + expf(-g));
-  const float z = 0.7978845608028654f * (g + 0.044715f * g * g * g);
-  return 0.5f * g * (1.0f + tanhf(z));
+// two fp32 -> two bf16, rounded to nearest even (one instruction)
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
 }
-__device__ __forceinline__ float gate_act_grad(int act, float g) {
-  if (act == ARTLITE_ACT_SILU) {
-    const float s = 1.0f / (1.0f + expf(-g));
-    return s * (1.0f + g * (1.0f - s));
-  }
-  const float z = 0.7978845608028654f * (g + 0.044715f * g * g * g), t = tanhf(z);
-  const float d = 1.0f - t * t;  // (0 where z is large: nothing times a large g stays nothing)
-  return 0.5f * (1.0f + t) + (d > 0.0f ? 0.5f * g * d * 0.7978845608028654f * (1.0f + 3.0f * 0.044715f * g * g) : 0.0f);
+
+// 1 / (1 + e^-v) to about 2 ulp: e^-v as 2^t with t = -v log2 e in two parts (the product's rounding, put back to first order),
+// the hardware's 2^t and reciprocal, the latter with a step of Newton's
+__device__ __forceinline__ float sigmoid(float v) {
+  constexpr float L2E = 1.44269504f, L2E_LO = 1.92596303e-8f;  // (log2 e and what its rounding leaves)
+  const float t = v * -L2E;
+  const float r = __builtin_fmaf(v, -L2E, -t) - v * L2E_LO;
+  const float e = __builtin_amdgcn_exp2f(t) * __builtin_fmaf(r, 0.69314718f, 1.0f);
+  const float d = 1.0f + e;
+  float q = __builtin_amdgcn_rcpf(d);
+  q = __builtin_fmaf(__builtin_fmaf(-d, q, 1.0f), q, q);
+  return t > 126.0f ? 0.0f : v > 100.0f ? 1.0f : q;
+}
+// the gated block's activation a and its derivative da at g (artlite_act); gelu's (1 + tanh z) / 2 is sigmoid(2 z)
+__device__ __forceinline__ float gate_act(int act, float g) {
+  if (act == ARTLITE_ACT_SILU) return g * sigmoid(g);
+  return g * sigmoid(1.5957691216f * __builtin_fmaf(0.044715f * g * g, g, g));
+}
+__device__ __forceinline__ void gate_act_grad(int act, float g, float& a, float& da) {
+  const float c = 0.044715f * g * g;
+  const float s = sigmoid(act == ARTLITE_ACT_SILU ? g : 1.5957691216f * __builtin_fmaf(c, g, g));
+  a = g * s;
+  // (0 where s is 0 or 1: nothing times a large slope stays nothing)
+  const float w = s * (1.0f - s), k = act == ARTLITE_ACT_SILU ? 1.0f : 1.5957691216f * __builtin_fmaf(3.0f, c, 1.0f);
+  da = w > 0.0f ? __builtin_fmaf(a * (1.0f - s), k, s) : s;
 }
 
 // the least e with |v| < 2^e of a finite v (0 and what is no number: a very small one)
@@ -236,6 +253,6 @@ int launch_unpack(const artlite_matrix* m, bool transposed, int e, uint16_t* out
 // the scale that brings a matrix's largest value into [2^14, 2^15)
 inline int wexp16(const artlite_matrix* m) { return m->max_exp - 15; }
 
-inline int64_t pad64(int64_t v) { return (v + 63) / 64 * 64; }
+__host__ __device__ inline int64_t pad64(int64_t v) { return (v + 63) / 64 * 64; }
 
 }  // namespace artlite

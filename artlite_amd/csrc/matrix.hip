@@ -1,8 +1,8 @@
 // Matrices of 4-bit GGUF blocks in the tile layout (matrix.h): upload, the bounds that scale their 16-bit forms, those forms
 // (unpacked into a workspace for the large tiles); workspaces; the C entry points of both and of device arrays.
 //
-// What bounds the kernels here: memory. k_unpack reads 0.56 bytes a value and writes 2: 4096 x 11008 in about 18 us. Uploads
-// happen once a matrix and are not tuned.
+// What bounds the kernels here: memory (k_unpack reads 0.56 bytes a value and writes 2). Uploads happen once a matrix and are
+// not tuned.
 #include "matrix.h"
 
 #include <cmath>
@@ -86,18 +86,34 @@ __global__ __launch_bounds__(128) void k_tile(const uint8_t* __restrict__ raw, i
   }
 }
 
-// a lane's 32 values of half h of a unit: groups 4 h + j, values 8 lg .. + 8 of each
-template <int QT, class F>
-__device__ __forceinline__ void tile_half(const uint8_t* ub, int h, int lane, F&& f) {
+// a lane's 32 values of half H of a unit: f(g, v) with values 8 lg .. + 8 of each of its groups g
+template <int QT, int H, class F>
+__device__ __forceinline__ void tile_half(const uint8_t* ub, int lane, F&& f) {
   TileHdr<QT> hd;
   hd.load(ub + 2048 + hdr_bytes<QT>() * (lane & 15));
-  const uint4 c = *reinterpret_cast<const uint4*>(ub + 1024 * h + 16 * lane);
+  const uint4 c = *reinterpret_cast<const uint4*>(ub + 1024 * H + 16 * lane);
   const uint32_t w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
   for (int j = 0; j < 4; j++) {
     float v[8];
-    tile_values<QT>(w[j], hd.scale(4 * h + j), has_offset<QT> ? hd.offset(4 * h + j) : 0.0f, v);
-    f(j, v);
+    tile_values<QT>(w[j], hd.scale(4 * H + j), has_offset<QT> ? hd.offset(4 * H + j) : 0.0f, v);
+    f(4 * H + j, v);
+  }
+}
+template <int QT, class F>
+__device__ __forceinline__ void tile_unit(const uint8_t* ub, int lane, F&& f) {
+  tile_half<QT, 0>(ub, lane, f);
+  tile_half<QT, 1>(ub, lane, f);
+}
+
+// eight values times 2^-e as fp16, and what that rounding left
+__device__ __forceinline__ void halves(const float (&v)[8], int e, uint16_t (&a)[8], uint16_t (&b)[8]) {
+#pragma unroll
+  for (int p = 0; p < 8; p++) {
+    const float x = __builtin_amdgcn_ldexpf(v[p], -e);
+    const _Float16 hi = _Float16(x);
+    a[p] = __builtin_bit_cast(uint16_t, hi);
+    b[p] = __builtin_bit_cast(uint16_t, _Float16(x - float(hi)));
   }
 }
 
@@ -109,9 +125,9 @@ __global__ __launch_bounds__(256) void k_bounds(const uint8_t* __restrict__ w, i
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const uint8_t* t = w + int64_t(blockIdx.x) * units * unit_bytes<QT>();
   float mx = 0.0f, ss = 0.0f;
-  for (int i = wv; i < 2 * units; i += 4)
-    tile_half<QT>(t + int64_t(i >> 1) * unit_bytes<QT>(), i & 1, lane, [&](int j, const float(&v)[8]) {
-      if (int64_t(i >> 1) * UNIT + 128 * (i & 1) + 32 * j >= K) return;
+  for (int u = wv; u < units; u += 4)
+    tile_unit<QT>(t + int64_t(u) * unit_bytes<QT>(), lane, [&](int g, const float(&v)[8]) {
+      if (int64_t(u) * UNIT + 32 * g >= K) return;
 #pragma unroll
       for (int p = 0; p < 8; p++) {
         mx = fmaxf(mx, fabsf(v[p]));
@@ -130,61 +146,64 @@ __global__ __launch_bounds__(256) void k_bounds(const uint8_t* __restrict__ w, i
   }
 }
 
-// W as fp16 rows of ld values: a wave per half unit of a tile; plane 1 (where there is one) what plane 0's rounding left
-template <int QT>
-__global__ __launch_bounds__(256) void k_unpack(const uint8_t* __restrict__ w, int units, int64_t N, int64_t K, int e,
-                                                uint16_t* __restrict__ out, int64_t ld, int64_t plane, int planes) {
-  const int64_t i = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6), tile = i / (2 * units);
-  const int r = int(i % (2 * units)), lane = threadIdx.x & 63;
+// W as fp16 rows of ld values: a wave per unit of a tile; plane 1 (where there is one) what plane 0's rounding left
+template <int QT, int PLANES>
+__global__ __launch_bounds__(256) void k_unpack(const uint8_t* __restrict__ w, int units, int64_t all, int64_t N, int64_t K,
+                                                int e, uint16_t* __restrict__ out, int64_t ld, int64_t plane) {
+  const int64_t i = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6), tile = i / units;
+  const int u = int(i % units), lane = threadIdx.x & 63;
   const int64_t n = tile * TROWS + (lane & 15);
-  if (n >= N) return;
-  const int64_t k0 = int64_t(r >> 1) * UNIT + 128 * (r & 1) + 8 * (lane >> 4);
+  if (i >= all || n >= N) return;
+  const int64_t k0 = int64_t(u) * UNIT + 8 * (lane >> 4);
   uint16_t* o = out + n * ld + k0;
-  tile_half<QT>(w + (tile * units + (r >> 1)) * unit_bytes<QT>(), r & 1, lane, [&](int j, const float(&v)[8]) {
-    const int64_t k = k0 + 32 * j;
+  tile_unit<QT>(w + i * unit_bytes<QT>(), lane, [&](int g, const float(&v)[8]) {
+    const int64_t k = k0 + 32 * g;
     if (k >= ld) return;
     uint16_t a[8], b[8];
-#pragma unroll
-    for (int p = 0; p < 8; p++) {
-      const float x = k < K ? ldexpf(v[p], -e) : 0.0f;
-      const _Float16 hi = _Float16(x);
-      a[p] = __builtin_bit_cast(uint16_t, hi);
-      b[p] = __builtin_bit_cast(uint16_t, _Float16(x - float(hi)));
-    }
-    __builtin_memcpy(__builtin_assume_aligned(o + 32 * j, 16), a, 16);
-    if (planes == 2) __builtin_memcpy(__builtin_assume_aligned(o + plane + 32 * j, 16), b, 16);
+    halves(v, e, a, b);
+    if (k >= K)
+      for (int p = 0; p < 8; p++) a[p] = b[p] = 0;
+    __builtin_memcpy(__builtin_assume_aligned(o + 32 * g, 16), a, 16);
+    if (PLANES == 2) __builtin_memcpy(__builtin_assume_aligned(o + plane + 32 * g, 16), b, 16);
   });
 }
 
-// W's transpose as fp16 rows of ld values: a workgroup per half unit of 4 tiles (64 rows of W), turned in LDS
-template <int QT>
+// W's transpose as fp16 rows of ld values: a workgroup per unit of 4 tiles (64 rows of W), a half at a time turned in LDS
+template <int QT, int PLANES>
 __global__ __launch_bounds__(256) void k_unpack_t(const uint8_t* __restrict__ w, int units, int64_t tiles, int64_t N,
-                                                  int64_t K, int e, uint16_t* __restrict__ out, int64_t ld, int64_t plane,
-                                                  int planes) {
+                                                  int64_t K, int e, uint16_t* __restrict__ out, int64_t ld, int64_t plane) {
   constexpr int LD = 72;  // (a row's 64 values and 8 more: 16-byte rows, their banks spread)
-  __shared__ __attribute__((aligned(16))) uint16_t t[2][128][LD];
+  __shared__ __attribute__((aligned(16))) uint16_t t[PLANES][UNIT / 2][LD];
   const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, lg = lane >> 4, lr = lane & 15;
-  const int64_t g4 = int64_t(blockIdx.x) / (2 * units), tile = 4 * g4 + wv;
-  const int r = int(int64_t(blockIdx.x) % (2 * units));
-  const int64_t k0 = int64_t(r >> 1) * UNIT + 128 * (r & 1);
+  const int64_t g4 = int64_t(blockIdx.x) / units, tile = 4 * g4 + wv;
+  const int u = int(int64_t(blockIdx.x) % units);
   const bool live = tile < tiles && tile * TROWS + lr < N;
-  const uint8_t* ub = w + ((tile < tiles ? tile : 0) * units + (r >> 1)) * unit_bytes<QT>();
-  tile_half<QT>(ub, r & 1, lane, [&](int j, const float(&v)[8]) {
+  const uint8_t* ub = w + ((tile < tiles ? tile : 0) * units + u) * unit_bytes<QT>();
+  const auto put = [&](int g, const float(&v)[8]) {
+    uint16_t a[8], b[8];
+    halves(v, e, a, b);
 #pragma unroll
     for (int p = 0; p < 8; p++) {
-      const float x = live ? ldexpf(v[p], -e) : 0.0f;
-      const _Float16 hi = _Float16(x);
-      t[0][32 * j + 8 * lg + p][16 * wv + lr] = __builtin_bit_cast(uint16_t, hi);
-      if (planes == 2) t[1][32 * j + 8 * lg + p][16 * wv + lr] = __builtin_bit_cast(uint16_t, _Float16(x - float(hi)));
+      t[0][32 * (g & 3) + 8 * lg + p][16 * wv + lr] = live ? a[p] : 0;
+      if (PLANES == 2) t[PLANES - 1][32 * (g & 3) + 8 * lg + p][16 * wv + lr] = live ? b[p] : 0;
     }
-  });
-  __syncthreads();
-  for (int i = threadIdx.x; i < 128 * 8; i += 256) {
-    const int row = i >> 3, c = i & 7;
-    const int64_t k = k0 + row, n = 64 * g4 + 8 * c;
-    if (k >= K || n >= ld) continue;
-    for (int pl = 0; pl < planes; pl++)
-      *reinterpret_cast<uint4*>(out + pl * plane + k * ld + n) = *reinterpret_cast<const uint4*>(&t[pl][row][8 * c]);
+  };
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    if (h == 0)
+      tile_half<QT, 0>(ub, lane, put);
+    else
+      tile_half<QT, 1>(ub, lane, put);
+    __syncthreads();
+    for (int i = threadIdx.x; i < UNIT / 2 * 8; i += 256) {
+      const int row = i >> 3, c = i & 7;
+      const int64_t k = int64_t(u) * UNIT + 128 * h + row, n = 64 * g4 + 8 * c;
+      if (k >= K || n >= ld) continue;
+#pragma unroll
+      for (int pl = 0; pl < PLANES; pl++)
+        *reinterpret_cast<uint4*>(out + pl * plane + k * ld + n) = *reinterpret_cast<const uint4*>(&t[pl][row][8 * c]);
+    }
+    __syncthreads();
   }
 }
 
@@ -193,13 +212,17 @@ __global__ __launch_bounds__(256) void k_unpack_t(const uint8_t* __restrict__ w,
 int launch_unpack(const artlite_matrix* m, bool transposed, int e, uint16_t* out, int64_t ld, int64_t plane, int planes,
                   hipStream_t s) {
   const uint8_t* w = m->w.as<uint8_t>();
-  const int64_t rows = transposed ? (m->tiles + 3) / 4 : m->tiles;
-  const unsigned grid = unsigned(transposed ? rows * 2 * m->units : (rows * 2 * m->units + 3) / 4);
+  const int64_t all = m->tiles * m->units;
+  const unsigned grid = unsigned(transposed ? (m->tiles + 3) / 4 * m->units : (all + 3) / 4);
 #define ART_U(QT)                                                                                          \
-  if (transposed)                                                                                          \
-    k_unpack_t<QT><<<grid, 256, 0, s>>>(w, m->units, m->tiles, m->N, m->K, e, out, ld, plane, planes);     \
+  if (transposed && planes == 1)                                                                           \
+    k_unpack_t<QT, 1><<<grid, 256, 0, s>>>(w, m->units, m->tiles, m->N, m->K, e, out, ld, plane);          \
+  else if (transposed)                                                                                     \
+    k_unpack_t<QT, 2><<<grid, 256, 0, s>>>(w, m->units, m->tiles, m->N, m->K, e, out, ld, plane);          \
+  else if (planes == 1)                                                                                    \
+    k_unpack<QT, 1><<<grid, 256, 0, s>>>(w, m->units, all, m->N, m->K, e, out, ld, plane);                 \
   else                                                                                                     \
-    k_unpack<QT><<<grid, 256, 0, s>>>(w, m->units, m->N, m->K, e, out, ld, plane, planes);                 \
+    k_unpack<QT, 2><<<grid, 256, 0, s>>>(w, m->units, all, m->N, m->K, e, out, ld, plane);                 \
   break
   ART_TILE_QTYPES(m->t->id, ART_U)
 #undef ART_U

@@ -41,8 +41,9 @@ class DeviceArray:
         self.dtype = np.dtype(dtype)
         _code(self.dtype)
         self.shape = (int(shape[0]), int(shape[1]))
+        self._lib = _hip.lib()  # (close() may run when the module is gone)
         p, dev = ctypes.c_void_p(), ctypes.c_int(0)
-        _hip.check(_hip.lib().artlite_device_alloc(self.nbytes, ctypes.byref(p), ctypes.byref(dev)))
+        _hip.check(self._lib.artlite_device_alloc(self.nbytes, ctypes.byref(p), ctypes.byref(dev)))
         self._p, self.device = p, dev.value
 
     @classmethod
@@ -78,7 +79,7 @@ class DeviceArray:
 
     def close(self) -> None:
         if getattr(self, "_p", None) is not None:
-            _hip.lib().artlite_device_free(self._p)
+            self._lib.artlite_device_free(self._p)
             self._p = None
 
     def __del__(self) -> None:
@@ -90,8 +91,9 @@ class Workspace:
     a stream capture order themselves on it; graphs that run beside each other, or beside calls, take one each."""
 
     def __init__(self, nbytes: int):
+        self._lib = _hip.lib()  # (close() may run when the module is gone)
         h = ctypes.c_void_p()
-        _hip.check(_hip.lib().artlite_workspace_create(nbytes, ctypes.byref(h)))
+        _hip.check(self._lib.artlite_workspace_create(nbytes, ctypes.byref(h)))
         self._h, self.nbytes = h, nbytes
 
     @property
@@ -102,7 +104,7 @@ class Workspace:
 
     def close(self) -> None:
         if getattr(self, "_h", None) is not None:
-            _hip.lib().artlite_workspace_destroy(self._h)
+            self._lib.artlite_workspace_destroy(self._h)
             self._h = None
 
     def __del__(self) -> None:

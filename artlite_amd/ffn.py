@@ -57,7 +57,8 @@ class GatedFFN:
         self._scratch.close()
 
     def workspace_bytes(self, n: int, dtype: str = "bf16", *, backward: bool = False, weights: bool = False) -> int:
-        """What calls of up to n rows need: forward, backward, or backward with the weights' gradients."""
+        """What a call of n rows needs: forward, backward, or backward with the weights' gradients. (Not always less for fewer
+        rows.)"""
         return self._need({"f32": 0, "bf16": 1}[dtype], n, 2 if weights else int(backward))
 
     def _need(self, code: int, n: int, backward: int) -> int:

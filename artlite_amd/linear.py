@@ -18,8 +18,9 @@ class Matrix:
 
     def __init__(self, qtype: str, rows: int, cols: int):
         self.qtype, self.rows, self.cols = qtype, rows, cols
+        self._lib = _hip.lib()  # (close() may run when the module is gone)
         h = ctypes.c_void_p()
-        _hip.check(_hip.lib().artlite_matrix_create(TYPE_ID.get(qtype, -1), rows, cols, ctypes.byref(h)))
+        _hip.check(self._lib.artlite_matrix_create(TYPE_ID.get(qtype, -1), rows, cols, ctypes.byref(h)))
         self._h = h
 
     @property
@@ -38,7 +39,7 @@ class Matrix:
 
     def close(self) -> None:
         if getattr(self, "_h", None) is not None:
-            _hip.lib().artlite_matrix_destroy(self._h)
+            self._lib.artlite_matrix_destroy(self._h)
             self._h = None
 
     def __del__(self) -> None:

@@ -209,7 +209,8 @@ typedef struct artlite_ffn {
   const artlite_matrix *gate, *up, *down;
   int32_t act; /* artlite_act */
 } artlite_ffn;
-/* the most that forward calls of at most n rows (backward = 0), or backward ones (1: dx alone, 2: weights' gradients) need */
+/* The bytes of workspace that a forward call of n rows needs (backward = 0), or a backward one (1: dx alone, 2: weights'
+ * gradients). (Not always less for fewer rows: few rows' sums are taken in parts.) */
 int artlite_ffn_workspace(const artlite_ffn* f, int dtype, int64_t n, int backward, size_t* nbytes);
 int artlite_ffn_forward(const artlite_ffn* f, const void* x, int dtype, int64_t n, int64_t x_stride, void* y,
                         int64_t y_stride, artlite_workspace* work, void* stream);
