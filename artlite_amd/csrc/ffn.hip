@@ -207,9 +207,11 @@ struct LinearPlan {
 };
 LinearPlan linear_plan(Carve& c, const artlite_matrix* w, int dtype, int64_t n, bool direct) {
   LinearPlan p;
-  p.few = n <= FEW_ROWS;
+  p.few = n <= (dtype == ARTLITE_X_BF16 ? FEW_ROWS : FEW_ROWS_F32);
   if (p.few) {
-    if (!direct) p.planes = c.take<uint16_t>(size_t(dtype == ARTLITE_X_BF16 ? 1 : 3) * n * w->K);
+    const int pl = dtype == ARTLITE_X_BF16 ? 1 : 3;
+    if (!direct) p.planes = c.take<uint16_t>(size_t(pl) * n * w->K);
+    p.parts = c.take<float>(few_parts_bytes(w, pl, false, n) / 4);
   } else {
     const int pl = dtype == ARTLITE_X_BF16 ? 1 : 2;
     const int64_t Kp = pad64(w->K);
@@ -260,6 +262,7 @@ int linear(const artlite_matrix* w, const void* x, int dtype, int64_t n, int64_t
     }
     a.M = n;
     a.y = y, a.y_stride = y_stride, a.dtype = dtype;
+    a.parts = p.parts;
     return launch_few(a, s);
   }
   const int pl = dtype == ARTLITE_X_BF16 ? 1 : 2, e = wexp16(w);
@@ -310,11 +313,12 @@ struct FfnPlan {
 };
 FfnPlan ffn_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool direct) {
   FfnPlan p{};
-  p.few = n <= FEW_ROWS;
+  p.few = n <= FEW_ROWS_FFN;
   const bool b = dtype == ARTLITE_X_BF16;
   if (p.few) {
     if (!direct) p.planes = c.take<uint16_t>(size_t(b ? 1 : 3) * n * f.H);
     p.hp = c.take<uint16_t>(size_t(b ? 2 : 3) * n * f.F);
+    p.parts = c.take<float>(std::max(few_parts_bytes(f.gate, b ? 1 : 3, true, n), few_parts_bytes(f.down, b ? 2 : 3, false, n)) / 4);
     return p;
   }
   const size_t pl = b ? 1 : 2;
@@ -347,6 +351,7 @@ int ffn_forward(const Ffn& f, const void* x, int dtype, int64_t n, int64_t x_str
     }
     a.M = n;
     a.h = p.hp, a.h_stride = f.F, a.h_plane = n * f.F, a.h_planes = b ? 2 : 3;
+    a.parts = p.parts;
     ART_TRY(launch_few(a, s));
     FewArgs d{};
     d.w = f.down;
@@ -354,6 +359,7 @@ int ffn_forward(const Ffn& f, const void* x, int dtype, int64_t n, int64_t x_str
     d.x = p.hp, d.x_stride = f.F, d.x_plane = n * f.F;
     d.M = n;
     d.y = y, d.y_stride = y_stride, d.dtype = dtype;
+    d.parts = p.parts;
     return launch_few(d, s);
   }
   const int pl = b ? 1 : 2;

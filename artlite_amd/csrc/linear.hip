@@ -19,6 +19,8 @@
 // and two dependent round trips.
 #include "matrix.h"
 
+#include <utility>
+
 namespace artlite {
 
 namespace {
@@ -71,6 +73,7 @@ constexpr int code_kind() {
 
 struct FewK {
   const uint8_t *w, *up;
+  int64_t tiles;
   int units;
   int64_t N, K, M;
   const uint16_t* x;
@@ -82,6 +85,7 @@ struct FewK {
   uint16_t* h;
   int64_t h_stride, h_plane;
   int h_planes;
+  float* parts;
 };
 
 __device__ __forceinline__ void store_planes(uint16_t* p, int64_t plane, int planes, float v) {
@@ -93,36 +97,66 @@ __device__ __forceinline__ void store_planes(uint16_t* p, int64_t plane, int pla
   }
 }
 
-template <int QT, int P, int NC, bool GLU>
-__global__ __launch_bounds__(P* NC == 1 ? 1024 : 512) void k_few(const FewK a) {
-  constexpr int RB = GLU ? 2 : 1, KIND = code_kind<QT, P>(), UB = unit_bytes<QT>();
+// an output of row m, column n from its sum (gated: and the second matrix's)
+template <bool GLU>
+__device__ __forceinline__ void few_out(const FewK& a, int64_t m, int64_t n, float s, float u) {
+  if constexpr (GLU) {
+    store_planes(a.h + m * a.h_stride + n, a.h_plane, a.h_planes, gate_act(a.act, s) * u);
+  } else {
+    const float v = s + (a.bias ? a.bias[n] : 0.0f);
+    if (a.dtype == ARTLITE_X_BF16)
+      static_cast<uint16_t*>(a.y)[m * a.y_stride + n] = uint16_t(f32_to_bf16(v));
+    else
+      static_cast<float*>(a.y)[m * a.y_stride + n] = v;
+  }
+}
+
+// A launch's shape: tiles of a workgroup (each wave takes its units of all of them, so that an x operand serves them all),
+// most waves (registers: 128 a lane of 16 waves)
+constexpr int few_tiles(int nc, bool glu) { return nc == 2 ? (glu ? 2 : 4) : nc == 4 ? (glu ? 1 : 2) : 1; }
+constexpr int few_most(int planes, int nc, bool glu) { return nc == 1 && planes <= 2 && !glu ? 16 : 8; }
+
+// P planes of x, NC blocks of 16 rows, RI rows of a block a lane: block row 4 g + i is x's row g + 4 i, so that up to 4 rows
+// are in each lane's first sum (RI 1) and up to 8 in its first two, and the others take no scaling. The units in gridDim.z
+// parts (PART: their sums into a.parts, for k_few_join).
+template <int QT, int P, int NC, int RI, bool GLU, bool PART>
+__global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a) {
+  constexpr int TB = few_tiles(NC, GLU), RB = GLU ? 2 * TB : TB, KIND = code_kind<QT, P>(), UB = unit_bytes<QT>();
   constexpr bool CIN = KIND < 0 || has_offset<QT>;  // (sum(x) times a constant is wanted)
   constexpr float CC = KIND < 0 ? (QT == ARTLITE_Q4_0 ? -136.0f : -128.0f) : -1.0f;
   constexpr uint32_t CB = bf16_of(int(CC)) * 0x10001u;
-  constexpr int XG = P * NC <= 2 ? 4 : P * NC <= 4 ? 2 : 1;  // (groups whose x is loaded together: registers)
-  extern __shared__ f32x4 red[];  // [wave][block][lane]
+  // groups whose x is in flight, whether the next unit's codes are (registers)
+  constexpr int XD = P * NC == 1 ? (GLU ? 4 : 8) : P * NC <= 2 ? 4 : 2;
+  constexpr bool AHEAD = NC == 1;
+  extern __shared__ float red[];  // [wave][tile of a matrix][block][row][lane]
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6,
             lg = lane >> 4, lr = lane & 15;
-  const int64_t tile = blockIdx.x, m0 = int64_t(blockIdx.y) * (16 * NC);
-  const int64_t tb = tile * a.units * UB;
-  const uint8_t* wp[2] = {a.w + tb, GLU ? a.up + tb : nullptr};
+  const int64_t t0 = int64_t(blockIdx.x) * TB, m0 = int64_t(blockIdx.y) * (16 * NC);
+  const int first = PART ? int(int64_t(a.units) * blockIdx.z / gridDim.z) : 0;
+  const int end = PART ? int(int64_t(a.units) * (blockIdx.z + 1) / gridDim.z) : a.units;
+  const uint8_t* wp[RB];  // (a tile past the last: the last one's, unused)
+#pragma unroll
+  for (int b = 0; b < RB; b++)
+    wp[b] = (GLU && b >= TB ? a.up : a.w) + min(t0 + b % TB, a.tiles - 1) * a.units * UB;
   const uint16_t* xp[NC];
   bool live[NC];
 #pragma unroll
   for (int c = 0; c < NC; c++) {
-    const int64_t m = m0 + 16 * c + lr;
+    const int64_t m = m0 + 16 * c + (lr >> 2) + 4 * (lr & 3);
     live[c] = m < a.M;
     xp[c] = a.x + (live[c] ? m : 0) * a.x_stride + 8 * lg;
   }
-  f32x4 acc[RB][NC];
+  float acc[RB][NC][RI];
 #pragma unroll
   for (int b = 0; b < RB; b++)
 #pragma unroll
-    for (int c = 0; c < NC; c++) acc[b][c] = f32x4{0, 0, 0, 0};
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+      for (int i = 0; i < RI; i++) acc[b][c][i] = 0.0f;
 
   uint4 code[RB][2];
   TileHdr<QT> hd[RB];
-  auto load = [&](int u) {
+  auto load = [&](int u) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < RB; b++) {
       const uint8_t* p = wp[b] + int64_t(u) * UB;
@@ -131,34 +165,50 @@ __global__ __launch_bounds__(P* NC == 1 ? 1024 : 512) void k_few(const FewK a) {
       hd[b].load(p + 2048 + hdr_bytes<QT>() * lr);
     }
   };
-  if (wv < a.units) load(wv);
-  for (int u = wv; u < a.units; u += W) {
+  // x of a group; past the last group of K the last one's (the scales there are 0). Rows that there are not take row 0, or with
+  // three planes keep what the registers hold: each row of the products is its own. (Loading only the rows there are took 1 row
+  // of 4096 x 4096 from 4.3 to 5.0 us, 16 rows from 6.8 to 10.8; but 5 rows in three planes, 1536 x 2880, from 6.7 to 6.3.)
+  u32x4 x[XD][NC][P];
+#pragma unroll
+  for (int j = 0; j < XD; j++)
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+      for (int p = 0; p < P; p++) x[j][c][p] = u32x4{0, 0, 0, 0};
+  const int klast = int(a.K) - 32;
+  auto load_x = [&](int j, int u, int g) __attribute__((always_inline)) {
+    const int k = min(u * UNIT + 32 * g, klast);
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+      if (P < 3 || NC > 1 || live[c])
+#pragma unroll
+        for (int p = 0; p < P; p++) x[j][c][p] = *reinterpret_cast<const u32x4*>(xp[c] + p * a.x_plane + k);
+  };
+  if (first + wv < end) {
+    if (AHEAD) load(first + wv);
+#pragma unroll
+    for (int g = 0; g < XD; g++) load_x(g, first + wv, g);
+  }
+  for (int u = first + wv; u < end; u += W) {
+    const bool more = u + W < end;
+    const int un = more ? u + W : u;
     uint4 cur[RB][2];
     TileHdr<QT> hc[RB];
+    if (!AHEAD) load(u);
 #pragma unroll
     for (int b = 0; b < RB; b++) {
       cur[b][0] = code[b][0], cur[b][1] = code[b][1];
       hc[b] = hd[b];
     }
-    if (u + W < a.units) load(u + W);
-    const int64_t k0 = int64_t(u) * UNIT;
+    if (AHEAD && more) load(u + W);
+    const auto half = [&](auto hv) __attribute__((always_inline)) {
+      constexpr int H = decltype(hv)::value;
+      float s[RB][4], o[RB][4];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      u32x4 x[XG][NC][P];
+      for (int b = 0; b < RB; b++) hc[b].template fields<H>(s[b], o[b]);
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const int g = 4 * h + j;
-        if (j % XG == 0)
-#pragma unroll
-          for (int i = 0; i < XG; i++)
-#pragma unroll
-            for (int c = 0; c < NC; c++)
-#pragma unroll
-              for (int p = 0; p < P; p++) {
-                const int64_t k = k0 + 32 * (g + i);
-                x[i][c][p] = u32x4{0, 0, 0, 0};
-                if (live[c] && k < a.K) x[i][c][p] = *reinterpret_cast<const u32x4*>(xp[c] + p * a.x_plane + k);
-              }
+        const int g = 4 * H + j;
         const u32x4 cst{CB, CB, CB, CB};
         f32x4 cin[NC];
 #pragma unroll
@@ -166,60 +216,74 @@ __global__ __launch_bounds__(P* NC == 1 ? 1024 : 512) void k_few(const FewK a) {
           cin[c] = f32x4{0, 0, 0, 0};
           if constexpr (CIN)
 #pragma unroll
-            for (int p = P - 1; p >= 0; p--) cin[c] = mfma(x[j % XG][c][p], cst, cin[c]);
+            for (int p = P - 1; p >= 0; p--) cin[c] = mfma(x[g % XD][c][p], cst, cin[c]);
         }
 #pragma unroll
         for (int b = 0; b < RB; b++) {
-          const uint32_t w = j == 0 ? cur[b][h].x : j == 1 ? cur[b][h].y : j == 2 ? cur[b][h].z : cur[b][h].w;
-          const u32x4 q = operand<KIND>(w);
-          const float s = hc[b].scale(g);
-          float o = 0.0f;
-          if constexpr (has_offset<QT>) o = hc[b].offset(g) * (KIND < 0 ? 1.0f / 128.0f : 1.0f);
+          const uint4& cc = cur[b][H];
+          const u32x4 q = operand<KIND>(j == 0 ? cc.x : j == 1 ? cc.y : j == 2 ? cc.z : cc.w);
 #pragma unroll
           for (int c = 0; c < NC; c++) {
             f32x4 d = KIND < 0 ? cin[c] : f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int p = P - 1; p >= 0; p--) d = mfma(x[j % XG][c][p], q, d);
+            for (int p = P - 1; p >= 0; p--) d = mfma(x[g % XD][c][p], q, d);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              acc[b][c][i] = __builtin_fmaf(s, d[i], acc[b][c][i]);
-              if constexpr (has_offset<QT>) acc[b][c][i] = __builtin_fmaf(o, cin[c][i], acc[b][c][i]);
+            for (int i = 0; i < RI; i++) {
+              acc[b][c][i] = __builtin_fmaf(s[b][j], d[i], acc[b][c][i]);
+              if constexpr (has_offset<QT>)
+                acc[b][c][i] = __builtin_fmaf(KIND < 0 ? o[b][j] * (1.0f / 128.0f) : o[b][j], cin[c][i], acc[b][c][i]);
             }
           }
         }
+        // (past the last unit: its own again, unread)
+        load_x(g % XD, g + XD < 8 ? u : un, (g + XD) % 8);
+        if (P * NC > 1) __builtin_amdgcn_sched_barrier(0);  // (the groups' sums in turn: registers)
       }
-    }
+    };
+    half(std::integral_constant<int, 0>{});
+    half(std::integral_constant<int, 1>{});
   }
+  constexpr int ACC = NC * RI;
 #pragma unroll
   for (int b = 0; b < RB; b++)
 #pragma unroll
-    for (int c = 0; c < NC; c++) red[(wv * (RB * NC) + b * NC + c) * WAVE + lane] = acc[b][c];
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+      for (int i = 0; i < RI; i++) red[((wv * RB + b) * ACC + c * RI + i) * WAVE + lane] = acc[b][c][i];
   __syncthreads();
-  // the waves' sums, in wave order; thread t takes block t / 64 (of a gated launch both matrices')
-  for (int c = wv; c < NC; c += W) {
-    f32x4 s[RB];
-#pragma unroll
-    for (int b = 0; b < RB; b++) {
-      s[b] = red[(b * NC + c) * WAVE + lane];
-      for (int w = 1; w < W; w++) s[b] += red[(w * (RB * NC) + b * NC + c) * WAVE + lane];
+  // the waves' sums, in wave order: 64 outputs a wave at a time
+  for (int q = wv; q < TB * ACC; q += W) {
+    const int b = q / ACC, ci = q % ACC;
+    float s = red[(b * ACC + ci) * WAVE + lane], v = GLU ? red[((b + TB) * ACC + ci) * WAVE + lane] : 0.0f;
+    for (int w = 1; w < W; w++) {
+      s += red[((w * RB + b) * ACC + ci) * WAVE + lane];
+      if (GLU) v += red[((w * RB + b + TB) * ACC + ci) * WAVE + lane];
     }
-    const int64_t n = tile * TROWS + lr;
-    if (n >= a.N) continue;
-    const float bias = !GLU && a.bias ? a.bias[n] : 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int64_t m = m0 + 16 * c + 4 * lg + i;
-      if (m >= a.M) continue;
-      const float v = s[0][i] + bias;
-      if constexpr (GLU) {
-        store_planes(a.h + m * a.h_stride + n, a.h_plane, a.h_planes, gate_act(a.act, v) * s[1][i]);
-      } else if (a.dtype == ARTLITE_X_BF16) {
-        static_cast<uint16_t*>(a.y)[m * a.y_stride + n] = uint16_t(f32_to_bf16(v));
-      } else {
-        static_cast<float*>(a.y)[m * a.y_stride + n] = v;
-      }
+    const int64_t n = (t0 + b) * TROWS + lr, m = m0 + 16 * (ci / RI) + lg + 4 * (ci % RI);
+    if (n >= a.N || m >= a.M) continue;
+    if constexpr (PART) {
+      float* o = a.parts + ((blockIdx.z * a.M + m) * (GLU ? 2 : 1)) * a.N + n;
+      o[0] = s;
+      if (GLU) o[a.N] = v;
+    } else {
+      few_out<GLU>(a, m, n, s, v);
     }
   }
+}
+
+// the parts' sums, in order
+template <bool GLU>
+__global__ __launch_bounds__(256) void k_few_join(const FewK a, int parts) {
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x, m = i / a.N, n = i % a.N;
+  if (m >= a.M) return;
+  const int64_t row = (GLU ? 2 : 1) * a.N;
+  const float* p = a.parts + m * row + n;
+  float s = 0.0f, u = 0.0f;
+  for (int k = 0; k < parts; k++, p += a.M * row) {
+    s += p[0];
+    if (GLU) u += p[a.N];
+  }
+  few_out<GLU>(a, m, n, s, u);
 }
 
 __global__ __launch_bounds__(256) void k_planes(const void* __restrict__ x, int bf16, int64_t K, int64_t stride,
@@ -232,41 +296,70 @@ __global__ __launch_bounds__(256) void k_planes(const void* __restrict__ x, int 
   store_planes(out + m * Kp + k, plane, planes, v);
 }
 
-// Waves of a workgroup: 16 to share K where the tiles alone leave the device's waves few (2048 x 2048, one row: the whole
-// matrix in one round of loads), 4 where there are enough of them, never more than units.
-int few_waves(int64_t groups, int units, bool wide) {
-  int w = 4;
-  while (w < (wide ? 16 : 8) && groups * w < 8192) w *= 2;
-  return int(units < w ? units : w);
+// How a product is shared out: the units of K in `parts` workgroups (where the groups of tiles leave half the CUs idle and a
+// part has 4 units at least: 32 rows of 4096 x 4096, 64 groups, 14.9 us in one part, 12.6 in 4, 15.7 in 8; of 128 groups 20.1
+// in one, 16.0 in 2), a part's units among `waves` waves, 16 of them where the workgroups leave the device's waves few, 4 where
+// they are enough, each with the same number of units but for the last.
+struct FewCut {
+  int64_t groups, blocks;
+  int parts, waves;
+};
+FewCut few_cut(int64_t tiles, int units, int64_t M, int planes, bool glu) {
+  const int nc = M <= 16 ? 1 : M <= 32 ? 2 : 4, tb = few_tiles(nc, glu), most = few_most(planes, nc, glu);
+  FewCut c{(tiles + tb - 1) / tb, (M + 16 * nc - 1) / (16 * nc), 1, 4};
+  const int64_t wgs = c.groups * c.blocks;
+  if (nc > 1)
+    while (wgs * c.parts * 2 <= 256 && units / (2 * c.parts) >= 4) c.parts *= 2;
+  const int own = (units + c.parts - 1) / c.parts;
+  while (c.waves < most && wgs * c.parts * c.waves < 8192) c.waves *= 2;
+  const int each = (own + c.waves - 1) / c.waves;
+  c.waves = (own + each - 1) / each;
+  return c;
 }
 
-template <int QT, int P, int NC, bool GLU>
-int launch_few_t(const FewK& k, int64_t tiles, hipStream_t s) {
-  const int64_t mb = (k.M + 16 * NC - 1) / (16 * NC);
-  const int W = few_waves(tiles * mb, k.units, P * NC == 1);
-  const size_t lds = size_t(W) * (GLU ? 2 : 1) * NC * WAVE * 16;
-  k_few<QT, P, NC, GLU><<<dim3(unsigned(tiles), unsigned(mb)), 64 * W, lds, s>>>(k);
+template <int QT, int P, int NC, int RI, bool GLU>
+int launch_few_t(const FewK& k, hipStream_t s) {
+  constexpr int LDS = few_most(P, NC, GLU) * (GLU ? 2 : 1) * few_tiles(NC, GLU) * NC * RI * WAVE * 4;
+  static_assert(LDS <= 64 * 1024, "LDS");
+  const FewCut c = few_cut(k.tiles, k.units, k.M, P, GLU);
+  const size_t lds = size_t(c.waves) * (GLU ? 2 : 1) * few_tiles(NC, GLU) * NC * RI * WAVE * 4;
+  const dim3 grid(unsigned(c.groups), unsigned(c.blocks), unsigned(c.parts));
+  if (NC > 1 && c.parts > 1) {
+    if (!k.parts) return fail(ARTLITE_EINVAL, "dense rows: no scratch for parts");
+    if constexpr (NC > 1) k_few<QT, P, NC, RI, GLU, true><<<grid, 64 * c.waves, lds, s>>>(k);
+    ART_HIP(hipGetLastError());
+    k_few_join<GLU><<<unsigned((k.M * k.N + 255) / 256), 256, 0, s>>>(k, c.parts);
+  } else {
+    k_few<QT, P, NC, RI, GLU, false><<<grid, 64 * c.waves, lds, s>>>(k);
+  }
   ART_HIP(hipGetLastError());
   return ARTLITE_OK;
 }
 
 template <int QT, int P, bool GLU>
-int launch_few_p(const FewK& k, int64_t tiles, hipStream_t s) {
-  if (k.M <= 16) return launch_few_t<QT, P, 1, GLU>(k, tiles, s);
-  if (k.M <= 32) return launch_few_t<QT, P, 2, GLU>(k, tiles, s);
-  return launch_few_t<QT, P, 4, GLU>(k, tiles, s);
+int launch_few_p(const FewK& k, hipStream_t s) {
+  if (k.M <= 4) return launch_few_t<QT, P, 1, 1, GLU>(k, s);
+  if (k.M <= 8) return launch_few_t<QT, P, 1, 2, GLU>(k, s);
+  if (k.M <= 16) return launch_few_t<QT, P, 1, 4, GLU>(k, s);
+  if (k.M <= 32) return launch_few_t<QT, P, 2, 4, GLU>(k, s);
+  return launch_few_t<QT, P, 4, 4, GLU>(k, s);
 }
 
 template <int QT>
 int launch_few_q(const FewArgs& a, const FewK& k, hipStream_t s) {
-  const int64_t t = a.w->tiles;
-  if (a.up) return a.planes == 1 ? launch_few_p<QT, 1, true>(k, t, s) : launch_few_p<QT, 3, true>(k, t, s);
-  return a.planes == 1   ? launch_few_p<QT, 1, false>(k, t, s)
-         : a.planes == 2 ? launch_few_p<QT, 2, false>(k, t, s)
-                         : launch_few_p<QT, 3, false>(k, t, s);
+  if (a.up) return a.planes == 1 ? launch_few_p<QT, 1, true>(k, s) : launch_few_p<QT, 3, true>(k, s);
+  return a.planes == 1   ? launch_few_p<QT, 1, false>(k, s)
+         : a.planes == 2 ? launch_few_p<QT, 2, false>(k, s)
+                         : launch_few_p<QT, 3, false>(k, s);
 }
 
 }  // namespace
+
+size_t few_parts_bytes(const artlite_matrix* w, int planes, bool gated, int64_t M) {
+  if (M <= 16) return 0;
+  const FewCut c = few_cut(w->tiles, w->units, M, planes, gated);
+  return c.parts > 1 ? size_t(c.parts) * M * w->N * (gated ? 2 : 1) * 4 : 0;
+}
 
 int launch_few(const FewArgs& a, hipStream_t s) {
   if (a.M <= 0) return ARTLITE_OK;
@@ -274,12 +367,13 @@ int launch_few(const FewArgs& a, hipStream_t s) {
   FewK k{};
   k.w = a.w->w.as<uint8_t>();
   k.up = a.up ? a.up->w.as<uint8_t>() : nullptr;
-  k.units = a.w->units;
+  k.tiles = a.w->tiles, k.units = a.w->units;
   k.N = a.w->N, k.K = a.w->K, k.M = a.M;
   k.x = a.x, k.x_stride = a.x_stride, k.x_plane = a.x_plane;
   k.bias = a.w->has_bias ? a.w->bias.as<float>() : nullptr;
   k.y = a.y, k.y_stride = a.y_stride, k.dtype = a.dtype, k.act = a.act;
   k.h = a.h, k.h_stride = a.h_stride, k.h_plane = a.h_plane, k.h_planes = a.h_planes;
+  k.parts = a.parts;
 #define ART_F(QT) return launch_few_q<QT>(a, k, s)
   ART_TILE_QTYPES(a.w->t->id, ART_F)
 #undef ART_F

@@ -60,29 +60,31 @@ struct TileHdr {
       }
     }
   }
-  __device__ __forceinline__ float scale(int g) const {
+  // s and o of groups 4 H .. + 4; K-quants' 6-bit fields four at a time, as the bytes of a word
+  template <int H>
+  __device__ __forceinline__ void fields(float (&s)[4], float (&o)[4]) const {
     if constexpr (QT == ARTLITE_Q4_0 || QT == ARTLITE_IQ4_NL) {
-      return h2f((h[g >> 1] >> (16 * (g & 1))) & 0xFFFFu);
+#pragma unroll
+      for (int g = 0; g < 4; g++) s[g] = h2f((h[2 * H + (g >> 1)] >> (16 * (g & 1))) & 0xFFFFu);
     } else if constexpr (QT == ARTLITE_Q4_1) {
-      return h2f(h[g] & 0xFFFFu);
+#pragma unroll
+      for (int g = 0; g < 4; g++) s[g] = h2f(h[4 * H + g] & 0xFFFFu), o[g] = -h2f(h[4 * H + g] >> 16);
     } else if constexpr (QT == ARTLITE_Q4_K) {
-      const int sh = 8 * (g & 3);
-      const uint32_t q = g < 4 ? (h[1] >> sh) & 63 : ((h[3] >> sh) & 15) | (((h[1] >> (sh + 6)) & 3) << 4);
-      return __fmul_rn(h2f(h[0] & 0xFFFFu), float(q));
+      const float d = h2f(h[0] & 0xFFFFu), dm = h2f(h[0] >> 16);
+      const uint32_t sc = H == 0 ? h[1] & 0x3F3F3F3Fu : (h[3] & 0x0F0F0F0Fu) | ((h[1] >> 2) & 0x30303030u);
+      const uint32_t mn = H == 0 ? h[2] & 0x3F3F3F3Fu : ((h[3] >> 4) & 0x0F0F0F0Fu) | ((h[2] >> 2) & 0x30303030u);
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        s[g] = __fmul_rn(d, float((sc >> (8 * g)) & 0xFFu));
+        o[g] = __fmul_rn(dm, float((mn >> (8 * g)) & 0xFFu));
+      }
     } else {
-      const int ls = int((h[1] >> (4 * g)) & 15) | (int((h[0] >> (16 + 2 * g)) & 3) << 4);
-      return __fmul_rn(h2f(h[0] & 0xFFFFu), float(ls - 32));
-    }
-  }
-  __device__ __forceinline__ float offset(int g) const {
-    if constexpr (QT == ARTLITE_Q4_1) {
-      return -h2f(h[g] >> 16);
-    } else if constexpr (QT == ARTLITE_Q4_K) {
-      const int sh = 8 * (g & 3);
-      const uint32_t m = g < 4 ? (h[2] >> sh) & 63 : ((h[3] >> (sh + 4)) & 15) | (((h[2] >> (sh + 6)) & 3) << 4);
-      return __fmul_rn(h2f(h[0] >> 16), float(m));
-    } else {
-      return 0.0f;
+      const float d = h2f(h[0] & 0xFFFFu);
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int k = 4 * H + g;
+        s[g] = __fmul_rn(d, float((int((h[1] >> (4 * k)) & 15) | (int((h[0] >> (16 + 2 * k)) & 3) << 4)) - 32));
+      }
     }
   }
 };
@@ -236,10 +238,14 @@ struct FewArgs {
   uint16_t* h;              // gated: h_planes planes of M rows of h_stride values
   int64_t h_stride, h_plane;
   int h_planes;
+  float* parts;             // scratch for sums in parts: few_parts_bytes of it
 };
 int launch_few(const FewArgs& a, hipStream_t s);
-// rows past which the dense products go by way of 16-bit weights and the large tiles
-constexpr int FEW_ROWS = 64;
+size_t few_parts_bytes(const artlite_matrix* w, int planes, bool gated, int64_t M);
+// Rows past which the dense products go by way of 16-bit weights and the large tiles: one matrix's of bf16 rows (4096 x 4096,
+// 128 rows: 22 us against 43; 256: 41 against 45; 12288 x 2048, 129 rows: 49 against 47), of fp32 rows (65 rows: 61 against
+// 54), the gated block's (2880 x 7680, 65 rows: 113 against 96)
+constexpr int FEW_ROWS = 128, FEW_ROWS_F32 = 64, FEW_ROWS_FFN = 64;
 // x (M rows of K values of dtype, stride apart) as planes of bf16 (1: bf16 as it is; 3: fp32), rows of Kp values (zeros past K)
 int launch_planes(const void* x, int dtype, int64_t M, int64_t K, int64_t stride, uint16_t* out, int64_t Kp, int64_t plane,
                   int planes, hipStream_t s);

@@ -93,10 +93,12 @@ __device__ __forceinline__ void tile_half(const uint8_t* ub, int lane, F&& f) {
   hd.load(ub + 2048 + hdr_bytes<QT>() * (lane & 15));
   const uint4 c = *reinterpret_cast<const uint4*>(ub + 1024 * H + 16 * lane);
   const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  float s[4], o[4] = {0, 0, 0, 0};
+  hd.template fields<H>(s, o);
 #pragma unroll
   for (int j = 0; j < 4; j++) {
     float v[8];
-    tile_values<QT>(w[j], hd.scale(4 * H + j), has_offset<QT> ? hd.offset(4 * H + j) : 0.0f, v);
+    tile_values<QT>(w[j], s[j], o[j], v);
     f(4 * H + j, v);
   }
 }

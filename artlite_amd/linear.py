@@ -107,7 +107,7 @@ class QLinear:
         handle = self._m.handle
         w = work.handle if work is not None else None
         lib = _hip.lib()
-        if work is None and (n > 64 or a.code == 0 or a.at % 16 or (n > 1 and a.row % 8)):
+        if work is None and (n > 16 or a.code == 0 or a.at % 16 or (n > 1 and a.row % 8)):
             z = ctypes.c_size_t(0)
             _hip.check(lib.artlite_linear_workspace(handle, a.code, n, 0, ctypes.byref(z)))
             w = self._scratch.get(z.value).handle if z.value else None

@@ -36,7 +36,7 @@ def linear_streams_and_graphs() -> None:
         assert (y.cpu().double() - want).norm() <= 2.0 ** -7 * want.norm()
 
     streams = [torch.cuda.Stream() for _ in range(3)]
-    xs = [torch.randn(100 + i, K, device="cuda").bfloat16() for i in range(12)]
+    xs = [torch.randn(125 + i, K, device="cuda").bfloat16() for i in range(12)]
     ys = [torch.empty(x.shape[0], N, device="cuda", dtype=torch.bfloat16) for x in xs]
     torch.cuda.synchronize()
     for i, (x, y) in enumerate(zip(xs, ys)):
@@ -45,7 +45,7 @@ def linear_streams_and_graphs() -> None:
     for x, y in zip(xs, ys):
         near(y, x)
     graphs = []
-    for M in (1, 100):
+    for M in (1, 100, 150):
         x = torch.randn(M, K, device="cuda").bfloat16()
         y = torch.empty(M, N, device="cuda", dtype=torch.bfloat16)
         work = Workspace(max(1, lin.workspace_bytes(M, "bf16")))

@@ -1,8 +1,8 @@
-"""``QLinear`` against 64-bit math in every format and on every path: few rows (1 to 64: one, two and four blocks of 16), the
+"""``QLinear`` against 64-bit math in every format and on every path: few rows (bf16 1 to 128, fp32 1 to 64: one, two and four blocks of 16), the
 large tiles past them (both sizes), widths of a single block, of partial units and of partial 64 values, odd numbers of
 outputs, rows at any stride and address; bias, zeros, infinities and NaN.
 
-Tolerances (relative L2). A bf16 output is rounded once: half a step is 2^-8. Up to 64 rows no weight is rounded and sums are
+Tolerances (relative L2). A bf16 output is rounded once: half a step is 2^-8. Of few rows no weight is rounded and sums are
 fp32: 2^-8 + 2^-14. Past that each weight is rounded to fp16 (half a step 2^-11; the errors of a sum's terms are independent,
 so the sum's is 2^-11 of its size): 2^-8 + 2^-10. fp32: a sum of n terms in fp32 is off by about sqrt(n) 2^-24 (n the groups
 of 32 values and their MFMA steps, at most 2 * 90 * 3 here: 1.4e-6), the three bf16 planes by 2^-24, two fp16 planes by 2^-22
@@ -20,7 +20,7 @@ from .dense_helpers import Rows, check, encode, values
 
 pytestmark = pytest.mark.gpu
 
-FEW = 64
+FEW = {"bf16": 128, "f32": 64}
 TOL = {("bf16", True): 2.0 ** -8 + 2.0 ** -14, ("bf16", False): 2.0 ** -8 + 2.0 ** -10, ("f32", True): 4e-6,
        ("f32", False): 4e-6}
 
@@ -48,9 +48,9 @@ def test_rows_and_widths(q: str, dtype: str) -> None:
     for K in widths(q):
         for N in (1, 17, 100):
             lin, w, _ = make(q, N, K, 7 * N + K)
-            for M in (1, 2, 15, 16, 17, 33, 64, 65, 131):
+            for M in (1, 4, 5, 8, 9, 16, 17, 33, 64, 65, 128, 129):
                 x = x_rows(M, K, dtype, M + K)
-                check(lin(x), values(x) @ w.T, TOL[dtype, M <= FEW], np.sqrt(values(x) ** 2 @ (w ** 2).T))
+                check(lin(x), values(x) @ w.T, TOL[dtype, M <= FEW[dtype]], np.sqrt(values(x) ** 2 @ (w ** 2).T))
             lin.close()
 
 
@@ -60,9 +60,9 @@ def test_rows_and_widths(q: str, dtype: str) -> None:
 def test_larger(q: str, N: int, K: int, dtype: str) -> None:
     """Units shared by every number of waves; tiles of the large products in several rows and columns."""
     lin, w, b = make(q, N, K, 5, bias=True)
-    for M in (1, 5, 40, 300):
+    for M in (1, 5, 20, 40, 100, 300):
         x = x_rows(M, K, dtype, M)
-        check(lin(x), values(x) @ w.T + b, TOL[dtype, M <= FEW])
+        check(lin(x), values(x) @ w.T + b, TOL[dtype, M <= FEW[dtype]])
 
 
 def test_large_tiles() -> None:
@@ -79,27 +79,27 @@ def test_strides(at: int, pad: int, out_at: int, out_pad: int, dtype: str) -> No
     """Rows at any address and stride; what lies between and behind the output's rows stays."""
     N, K = 100, 160
     lin, w, _ = make("IQ4_NL", N, K, 2)
-    for M in (1, 3, 16, 70):
+    for M in (1, 3, 16, 70, 150):
         data = x_rows(M, K, dtype, M)
         x = Rows(M, K, dtype, at=at, stride=K + pad, data=data)
         y = Rows(M, N, dtype, at=out_at, stride=N + out_pad)
         assert lin(x, y) is y
-        check(y.numpy(), values(data) @ w.T, TOL[dtype, M <= FEW])
+        check(y.numpy(), values(data) @ w.T, TOL[dtype, M <= FEW[dtype]])
 
 
 def test_one_row_for_all() -> None:
     """A row stride of 0: every output row is the one input row's."""
     lin, w, _ = make("Q4_0", 40, 256, 2)
     data = x_rows(1, 256, "bf16", 1)
-    for M in (3, 80):
+    for M in (3, 80, 150):
         x = Rows(1, 256, "bf16", data=data)
         x.shape, x.row = (M, 256), 0
         y = Rows(M, 40, "bf16")
         lin(x, y)
-        check(y.numpy(), np.repeat(values(data) @ w.T, M, 0), TOL["bf16", M <= FEW])
+        check(y.numpy(), np.repeat(values(data) @ w.T, M, 0), TOL["bf16", M <= FEW["bf16"]])
 
 
-@pytest.mark.parametrize("M", [4, 90])
+@pytest.mark.parametrize("M", [4, 90, 150])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_values_out_of_the_ordinary(dtype: str, M: int) -> None:
     """Rows of zeros, of the type's smallest and largest sizes, with infinities and NaN: each row is its own, the others are
@@ -112,10 +112,10 @@ def test_values_out_of_the_ordinary(dtype: str, M: int) -> None:
     a[2] *= 1e30
     base = encode(a, dtype)
     y0 = lin(base)
-    check(y0[3:], values(base)[3:] @ w.T, TOL[dtype, M <= FEW])
+    check(y0[3:], values(base)[3:] @ w.T, TOL[dtype, M <= FEW[dtype]])
     assert not values(y0)[0].any()
     for r in (1, 2):
-        check(y0[r:r + 1], values(base)[r:r + 1] @ w.T, TOL[dtype, M <= FEW])
+        check(y0[r:r + 1], values(base)[r:r + 1] @ w.T, TOL[dtype, M <= FEW[dtype]])
     a[3, 5] = np.nan
     bad = encode(a, dtype)
     bad[2, 7] = encode(np.array([np.inf]), dtype)[0]
@@ -126,7 +126,7 @@ def test_values_out_of_the_ordinary(dtype: str, M: int) -> None:
 
 def test_zero_blocks_and_large_scales() -> None:
     """A matrix of zeros, and one whose scales are the largest fp16 ones, on both paths."""
-    for M in (3, 70):
+    for M in (3, 70, 150):
         x = x_rows(M, 64, "bf16", M)
         lin = QLinear("Q4_0", 20, 64)
         lin.upload(np.zeros((20, 36), np.uint8))
@@ -136,14 +136,14 @@ def test_zero_blocks_and_large_scales() -> None:
         raw[..., :2] = np.array([65504.0], np.float16).view(np.uint8)
         lin.upload(raw)
         w = dense.gguf_ref.dequantize("Q4_0", raw.reshape(20, 36), 64).astype(np.float64)
-        check(lin(x), values(x) @ w.T, TOL["bf16", M <= FEW])
+        check(lin(x), values(x) @ w.T, TOL["bf16", M <= FEW["bf16"]])
 
 
 def test_no_rows_and_repeats() -> None:
     """0 rows write nothing; the same call twice gives the same bits, on every path."""
     lin, _, _ = make("IQ4_XS", 100, 512, 3)
     assert lin(np.empty((0, 512), np.uint16)).shape == (0, 100)
-    for M in (1, 20, 64, 65, 300):
+    for M in (1, 20, 64, 65, 128, 129, 300):
         for dtype in ("bf16", "f32"):
             x = x_rows(M, 512, dtype, M)
             assert np.array_equal(lin(x), lin(x))
@@ -151,21 +151,21 @@ def test_no_rows_and_repeats() -> None:
 
 def test_refusals() -> None:
     lin, _, _ = make("Q4_0", 64, 64, 3)
-    x, y = DeviceArray((70, 64), np.uint16), DeviceArray((70, 64), np.uint16)
+    x, y = DeviceArray((140, 64), np.uint16), DeviceArray((140, 64), np.uint16)
     with pytest.raises(_hip.Error, match="out overlaps x"):
         lin(x, x)
     with pytest.raises(_hip.Error, match="for 64 rows of 64 values"):
-        lin(x, DeviceArray((70, 64), np.float32))
+        lin(x, DeviceArray((140, 64), np.float32))
     with pytest.raises(_hip.Error, match="for 64 rows of 64 values"):
-        lin(x, DeviceArray((69, 64), np.uint16))
+        lin(x, DeviceArray((139, 64), np.uint16))
     with pytest.raises(_hip.Error, match="is no array"):
         lin(x)
     with pytest.raises(_hip.Error, match="a workspace of 1024 bytes, not"):
         lin(x, y, work=Workspace(1024))
 
     class Host:  # (an address that is the host's)
-        shape, dtype = (70, 64), np.dtype(np.uint16)
-        mem = np.zeros((70, 64), np.uint16)
+        shape, dtype = (140, 64), np.dtype(np.uint16)
+        mem = np.zeros((140, 64), np.uint16)
 
         def stride(self) -> tuple[int, int]:
             return 64, 1
