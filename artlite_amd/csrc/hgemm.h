@@ -35,6 +35,7 @@ struct HGemm {
   const uint16_t* dh;
   uint16_t *h, *dg, *du;
   int64_t h_stride, h_plane;
+  int64_t h_cols;  // (set by the launch: the columns of the planes from the first on)
   int planes;
   // scratch for sums in parts: hgemm_parts_bytes of it
   float* parts;

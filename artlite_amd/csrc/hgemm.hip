@@ -122,7 +122,7 @@ __device__ __forceinline__ void finish(const HGemm& g, int es, const RowExp& r, 
       }
     }
   } else {
-    if (n >= g.h_stride) return;
+    if (n >= g.h_cols) return;
     const int64_t at = m * g.h_stride + n;
     if constexpr (EPI == H_ROWS) {
 #pragma unroll
@@ -176,9 +176,9 @@ __host__ __device__ __forceinline__ int64_t part_row(const HGemm& g) {
   return (gated<EPI> ? 2 : 1) * pad64(g.N);
 }
 
-// tiles from column n_off on, gm x gn of them; K in gridDim.y parts (PART: their sums into g.parts, for k_join)
+// gm x gn tiles from column 0 on; K in gridDim.y parts (PART: their sums into g.parts, for k_join)
 template <int MB, int EPI, bool PART>
-__global__ __launch_bounds__(256, MB == 8 ? 1 : 2) void k_hgemm(const HGemm g, int64_t n_off, int gm, int gn) {
+__global__ __launch_bounds__(256, MB == 8 ? 1 : 2) void k_hgemm(const HGemm g, int gm, int gn) {
   using T = HT<MB>;
   constexpr int TM = T::TM, RING = T::RING;
   constexpr bool GATED = gated<EPI>;
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(256, MB == 8 ? 1 : 2) void k_hgemm(const HGemm g, i
     mt = __builtin_amdgcn_readfirstlane(band * GR + in % rows);
     nt = __builtin_amdgcn_readfirstlane(in / rows);
   }
-  const int64_t m0 = int64_t(mt) * TM, n0 = n_off + int64_t(nt) * TN;
+  const int64_t m0 = int64_t(mt) * TM, n0 = int64_t(nt) * TN;
   const int mv = int(min(int64_t(TM), g.M - m0)), nv = int(min(int64_t(TN), g.N - n0));  // (rows, columns that there are)
 
   // ---- the issue side: a wave's DMAs of a step take 16 rows each, HPW of A's and HPW of B's (a wave's columns of a gated
@@ -395,62 +395,109 @@ __global__ __launch_bounds__(256) void k_join(const HGemm g, int parts) {
   finish<EPI>(g, g.e + (g.e0 ? *g.e0 : 0) + (g.e1 ? *g.e1 : 0), row_exp<EPI>(g, m), m, n, v, u, bias);
 }
 
-// How a product is cut: `big` columns in tiles of 256 x 256, the rest in tiles of 128 x 128, K in `parts`.
+// How a product is cut: `gn` columns of tiles, big (256 x 256) or small (128 x 128), K in `parts`; columns past them are cut
+// anew. The choice goes by what a product takes as measured on the card (us; a step is 32 values of K):
+//   a round of 256 big tiles: 0.76 a step and 18 for its start and its outputs;
+//   a round of 512 small ones, two a CU: 0.53 a step and 10; with one a CU 0.31 a step;
+//   parts: the sums written and read again at 4 TB/s, and 5 for the launch that joins them.
+// (3001 x 4096 of 11008 values, 192 big tiles: 283 us, 366 in small ones; 2048 x 2048 of 16384, 64 big tiles: 4 parts 130 us,
+// 256 small ones in 2 parts 170; 1000 x 6144 of 2048: 96 big 66 us, 384 small 39.)
 struct Cut {
-  int64_t big, small;  // columns of tiles
+  bool big;
+  int64_t gn;
   int parts;
+  double us;
 };
 constexpr int CUS = 256;
-Cut cut(int64_t M, int64_t N, int64_t K, int segs, bool gate) {
-  const int64_t cols = gate ? 2 * N : N, gm = (M + 255) / 256, gn = (cols + 255) / 256, sm = (M + 127) / 128;
-  const int64_t tiles = gm * gn, left = tiles % CUS;
-  if (tiles >= CUS) {
-    // a last round of few tiles takes as long as a full one: where half the CUs would idle in it its columns go in small tiles
-    const int64_t keep = tiles / CUS * CUS / gm;
-    if (left && left <= CUS / 2 && keep >= 1) return Cut{keep, (cols - keep * 256 + 127) / 128, 1};
-    return Cut{gn, 0, 1};
+double round_us(int64_t tiles, bool big, double steps) {
+  if (big) return double((tiles + CUS - 1) / CUS) * (0.76 * steps + 18);
+  const int64_t left = tiles % (2 * CUS);
+  return double(tiles / (2 * CUS)) * (0.53 * steps + 10) + (left ? (left > CUS ? 0.53 : 0.31) * steps + 10 : 0);
+}
+Cut best_cut(int64_t M, int64_t cols, int64_t K, int segs, bool mixed) {
+  const int64_t pairs = K / (2 * BK) * segs;
+  Cut best{false, 0, 0, 1e30};
+  const auto size = [](int64_t v, bool big) { return (v + (big ? 255 : 127)) / (big ? 256 : 128); };
+  for (int big = 0; big < 2; big++)
+    for (int parts = 1; parts <= (big ? 4 : 16); parts *= 2) {
+      if (parts > 1 && pairs / parts < 4) break;
+      const int64_t gn = size(cols, big);
+      double us = round_us(size(M, big) * gn * parts, big, 2.0 * double(pairs) / parts);
+      if (parts > 1) us += 5 + 2.0 * 4 * parts * double(M) * double(cols) / 4e6;
+      if (us < best.us) best = Cut{big != 0, gn, parts, us};
+    }
+  const int64_t gm = size(M, true), tiles = gm * size(cols, true), keep = tiles / CUS * CUS / gm;
+  if (mixed && tiles > CUS && keep >= 1 && keep < size(cols, true)) {  // (whole rounds big, the columns left as is best for them)
+    const double us = round_us(gm * keep, true, 2.0 * double(pairs)) + 2 + best_cut(M, cols - 256 * keep, K, segs, false).us;
+    if (us < best.us) best = Cut{true, keep, 1, us};
   }
-  const int64_t sn = (cols + 127) / 128, pairs = K / (2 * BK) * segs;
-  int parts = 1;
-  // (two small tiles a CU; a part of at least 4 pairs, 256 values)
-  while (parts < 16 && sm * sn * parts * 2 <= 2 * CUS && pairs / (2 * parts) >= 4) parts *= 2;
-  return Cut{0, sn, parts};
+  return best;
 }
 
 template <int MB, int EPI, bool PART>
-int launch_t(const HGemm& g, int64_t n_off, int64_t gn, int parts, hipStream_t s) {
+int launch_t(const HGemm& g, int64_t gn, int parts, hipStream_t s) {
   using T = HT<MB>;
   static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(k_hgemm<MB, EPI, PART>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS) == hipSuccess;
   if (!ok) return fail(ARTLITE_EHIP, "large tiles: kernel set-up failed");
   const int64_t gm = (g.M + T::TM - 1) / T::TM;
   if (gm * gn > (int64_t(1) << 30)) return fail(ARTLITE_EINVAL, "large tiles: %lld tiles", (long long)(gm * gn));
-  k_hgemm<MB, EPI, PART><<<dim3(unsigned(gm * gn), unsigned(parts)), 256, T::LDS, s>>>(g, n_off, int(gm), int(gn));
+  k_hgemm<MB, EPI, PART><<<dim3(unsigned(gm * gn), unsigned(parts)), 256, T::LDS, s>>>(g, int(gm), int(gn));
   ART_HIP(hipGetLastError());
   return ARTLITE_OK;
 }
 
 template <int EPI>
-int launch_e(const HGemm& g, hipStream_t s) {
-  const Cut c = cut(g.M, g.N, g.K, g.segs, gated<EPI>);
+int launch_e(HGemm g, bool mixed, hipStream_t s) {
+  const int64_t cols = gated<EPI> ? 2 * g.N : g.N;
+  const Cut c = best_cut(g.M, cols, g.K, g.segs, mixed);
   if (c.parts > 1) {
     if (!g.parts) return fail(ARTLITE_EINVAL, "large tiles: no scratch for parts");
-    ART_TRY((launch_t<4, EPI, true>(g, 0, c.small, c.parts, s)));
+    if (c.big)
+      ART_TRY((launch_t<8, EPI, true>(g, c.gn, c.parts, s)));
+    else
+      ART_TRY((launch_t<4, EPI, true>(g, c.gn, c.parts, s)));
     const int64_t threads = g.M * (pad64(g.N) / 8);
     k_join<EPI><<<unsigned((threads + 255) / 256), 256, 0, s>>>(g, c.parts);
     ART_HIP(hipGetLastError());
     return ARTLITE_OK;
   }
-  if (c.big) ART_TRY((launch_t<8, EPI, false>(g, 0, c.big, 1, s)));
-  if (c.small) ART_TRY((launch_t<4, EPI, false>(g, c.big * (gated<EPI> ? 128 : 256), c.small, 1, s)));
-  return ARTLITE_OK;
+  if (c.big)
+    ART_TRY((launch_t<8, EPI, false>(g, c.gn, 1, s)));
+  else
+    ART_TRY((launch_t<4, EPI, false>(g, c.gn, 1, s)));
+  const int64_t done = c.gn * (c.big ? 256 : 128);
+  if (done >= cols) return ARTLITE_OK;
+  // the columns left, as a product of their own
+  const int64_t n = gated<EPI> ? done / 2 : done;
+  for (int i = 0; i < g.segs; i++) {
+    g.b[i] += n * g.ldb;
+    if (gated<EPI>) g.b2[i] += n * g.ldb;
+  }
+  g.N -= n;
+  if (EPI == H_STORE) {
+    if (g.bias) g.bias += n;
+    g.y = static_cast<char*>(g.y) + n * (g.dtype == ARTLITE_X_BF16 ? 2 : 4);
+  } else {
+    g.h_cols -= n;
+    for (uint16_t** p : {&g.h, &g.dg, &g.du})
+      if (*p) *p += n;
+    if (g.dh) g.dh += n;
+  }
+  return launch_e<EPI>(g, false, s);
 }
 
 }  // namespace
 
 size_t hgemm_parts_bytes(int64_t M, int64_t N, int64_t K, int segs, bool gate) {
-  const Cut c = cut(M, N, K, segs, gate);
-  return c.parts > 1 ? size_t(c.parts) * M * (gate ? 2 : 1) * pad64(N) * 4 : 0;
+  size_t most = 0;
+  for (int64_t cols = gate ? 2 * N : N, mixed = 1; cols > 0; mixed = 0) {
+    const Cut c = best_cut(M, cols, K, segs, mixed);
+    const int64_t n = gate ? (cols + 1) / 2 : cols;
+    if (c.parts > 1) most = size_t(c.parts) * M * (gate ? 2 : 1) * pad64(n) * 4;
+    cols -= c.gn * (c.big ? 256 : 128);
+  }
+  return most;
 }
 
 int launch_hgemm(const HGemm& g, hipStream_t s) {
@@ -459,10 +506,12 @@ int launch_hgemm(const HGemm& g, hipStream_t s) {
       g.lda > (int64_t(1) << 22) || g.ldb > (int64_t(1) << 22) || g.K * g.segs / BK >= (int64_t(1) << 30))
     return fail(ARTLITE_EINVAL, "large tiles: K %lld of rows of %lld and %lld", (long long)g.K, (long long)g.lda,
                 (long long)g.ldb);
-  return g.epilogue == H_STORE  ? launch_e<H_STORE>(g, s)
-         : g.epilogue == H_ROWS ? launch_e<H_ROWS>(g, s)
-         : g.epilogue == H_GLU  ? launch_e<H_GLU>(g, s)
-                                : launch_e<H_DGLU>(g, s);
+  HGemm h = g;
+  h.h_cols = g.h_stride;
+  return g.epilogue == H_STORE  ? launch_e<H_STORE>(h, true, s)
+         : g.epilogue == H_ROWS ? launch_e<H_ROWS>(h, true, s)
+         : g.epilogue == H_GLU  ? launch_e<H_GLU>(h, true, s)
+                                : launch_e<H_DGLU>(h, true, s);
 }
 
 }  // namespace artlite
