@@ -69,18 +69,29 @@ struct HT {
   static_assert(LDS <= (MB == 8 ? LDS_BYTES : LDS_BYTES / 2), "LDS");
 };
 
-// eight fp16 values times 2^-e at p, and with a second plane what their rounding left
-__device__ __forceinline__ void store16(uint16_t* p, int64_t plane, int planes, const float (&v)[8], int e) {
-  uint16_t a[8], b[8];
+// eight values as fp16 at p, and with a second plane what their rounding left
+template <bool TWO>
+__device__ __forceinline__ void store16(uint16_t* p, int64_t plane, const float (&v)[8]) {
+  f16x8 a, b;
 #pragma unroll
   for (int i = 0; i < 8; i++) {
-    const float x = __builtin_amdgcn_ldexpf(v[i], -e);
-    const _Float16 hi = _Float16(x);
-    a[i] = __builtin_bit_cast(uint16_t, hi);
-    b[i] = __builtin_bit_cast(uint16_t, _Float16(x - float(hi)));
+    a[i] = _Float16(v[i]);
+    if constexpr (TWO) b[i] = _Float16(v[i] - float(a[i]));
   }
-  __builtin_memcpy(__builtin_assume_aligned(p, 16), a, 16);
-  if (planes == 2) __builtin_memcpy(__builtin_assume_aligned(p + plane, 16), b, 16);
+  *reinterpret_cast<f16x8*>(p) = a;
+  if constexpr (TWO) *reinterpret_cast<f16x8*>(p + plane) = b;
+}
+// eight fp16 values, the sum of two planes where there are
+template <bool TWO>
+__device__ __forceinline__ void load16(const uint16_t* p, int64_t plane, float (&v)[8]) {
+  const f16x8 a = *reinterpret_cast<const f16x8*>(p);
+#pragma unroll
+  for (int k = 0; k < 8; k++) v[k] = float(a[k]);
+  if constexpr (TWO) {
+    const f16x8 b = *reinterpret_cast<const f16x8*>(p + plane);
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] += float(b[k]);
+  }
 }
 
 // a row's exponents: of its sums, of what is written, of h beside dg and du, of dh
@@ -88,15 +99,57 @@ struct RowExp {
   int sum, out, h, dh;
 };
 
+// columns n .. n + 8 of row m of the planes from their sums v (gated: and the second matrix's u); the exponents of what is
+// written go into its factors, so that each value takes one scaling
+template <int EPI, bool TWO>
+__device__ __forceinline__ void finish16(const HGemm& g, int es, const RowExp& r, int64_t m, int64_t n, float (&v)[8],
+                                         float (&u)[8]) {
+  const int64_t at = m * g.h_stride + n;
+  const int ev = es + r.sum, eu = es - g.e + g.e2 + r.sum;
+  const int there = int(max(int64_t(0), min(int64_t(8), g.N - n)));  // (columns that there are)
+  float d[8], h[8];
+  if constexpr (EPI == H_DGLU) load16<TWO>(g.dh + at, g.h_plane, d);
+#pragma unroll
+  for (int k = 0; k < 8; k++) {
+    if constexpr (EPI == H_ROWS) {
+      v[k] = __builtin_amdgcn_ldexpf(v[k], ev - r.out);
+    } else if constexpr (EPI == H_GLU) {
+      v[k] = gate_act<TWO>(g.act, __builtin_amdgcn_ldexpf(v[k], ev)) * __builtin_amdgcn_ldexpf(u[k], eu - r.out);
+    } else {
+      const float uv = __builtin_amdgcn_ldexpf(u[k], eu), dh = __builtin_amdgcn_ldexpf(d[k], r.dh - r.out);
+      float a, da;
+      gate_act_grad<TWO>(g.act, __builtin_amdgcn_ldexpf(v[k], ev), a, da);
+      h[k] = a * __builtin_amdgcn_ldexpf(u[k], eu - r.h);
+      v[k] = dh * uv * da;
+      u[k] = dh * a;
+    }
+  }
+  if (there < 8) {
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      if (k >= there) v[k] = u[k] = h[k] = 0.0f;
+  }
+  if constexpr (EPI == H_DGLU) {
+    store16<TWO>(g.dg + at, g.h_plane, v);
+    store16<TWO>(g.du + at, g.h_plane, u);
+    if (g.h) store16<TWO>(g.h + at, g.h_plane, h);
+  } else {
+    store16<TWO>(g.h + at, g.h_plane, v);
+  }
+}
+
 // columns n .. n + 8 of row m from their sums v (gated: and the second matrix's u)
 template <int EPI>
 __device__ __forceinline__ void finish(const HGemm& g, int es, const RowExp& r, int64_t m, int64_t n, float (&v)[8],
                                        float (&u)[8], const float (&bias)[8]) {
-  const int there = int(max(int64_t(0), min(int64_t(8), g.N - n)));  // (columns that there are)
   if constexpr (EPI == H_STORE) {
+    const int there = int(max(int64_t(0), min(int64_t(8), g.N - n)));  // (columns that there are)
     if (there == 0) return;
 #pragma unroll
-    for (int k = 0; k < 8; k++) v[k] = __builtin_amdgcn_ldexpf(v[k], es + r.sum) + bias[k];
+    for (int k = 0; k < 8; k++) v[k] = __builtin_amdgcn_ldexpf(v[k], es + r.sum);
+    if (g.bias)
+#pragma unroll
+      for (int k = 0; k < 8; k++) v[k] += bias[k];
     const int64_t at = m * g.y_stride + n;
     if (g.dtype == ARTLITE_X_BF16) {
       uint16_t* y = static_cast<uint16_t*>(g.y) + at;
@@ -123,43 +176,10 @@ __device__ __forceinline__ void finish(const HGemm& g, int es, const RowExp& r, 
     }
   } else {
     if (n >= g.h_cols) return;
-    const int64_t at = m * g.h_stride + n;
-    if constexpr (EPI == H_ROWS) {
-#pragma unroll
-      for (int k = 0; k < 8; k++) v[k] = k < there ? __builtin_amdgcn_ldexpf(v[k], es + r.sum) : 0.0f;
-      store16(g.h + at, g.h_plane, g.planes, v, r.out);
-    } else if constexpr (EPI == H_GLU) {
-#pragma unroll
-      for (int k = 0; k < 8; k++)
-        v[k] = k < there ? gate_act(g.act, __builtin_amdgcn_ldexpf(v[k], es + r.sum)) *
-                               __builtin_amdgcn_ldexpf(u[k], es - g.e + g.e2 + r.sum)
-                         : 0.0f;
-      store16(g.h + at, g.h_plane, g.planes, v, r.out);
-    } else {
-      float d[8], h[8];
-      const f16x8 d0 = *reinterpret_cast<const f16x8*>(g.dh + at);
-#pragma unroll
-      for (int k = 0; k < 8; k++) d[k] = float(d0[k]);
-      if (g.planes == 2) {
-        const f16x8 d1 = *reinterpret_cast<const f16x8*>(g.dh + g.h_plane + at);
-#pragma unroll
-        for (int k = 0; k < 8; k++) d[k] += float(d1[k]);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const bool is = k < there;
-        const float gv = __builtin_amdgcn_ldexpf(v[k], es + r.sum), uv = __builtin_amdgcn_ldexpf(u[k], es - g.e + g.e2 + r.sum),
-                    dh = __builtin_amdgcn_ldexpf(d[k], r.dh);
-        float a, da;
-        gate_act_grad(g.act, gv, a, da);
-        h[k] = is ? a * uv : 0.0f;
-        v[k] = is ? dh * uv * da : 0.0f;
-        u[k] = is ? dh * a : 0.0f;
-      }
-      store16(g.dg + at, g.h_plane, g.planes, v, r.out);
-      store16(g.du + at, g.h_plane, g.planes, u, r.out);
-      if (g.h) store16(g.h + at, g.h_plane, g.planes, h, r.h);
-    }
+    if (g.planes == 2)
+      finish16<EPI, true>(g, es, r, m, n, v, u);
+    else
+      finish16<EPI, false>(g, es, r, m, n, v, u);
   }
 }
 

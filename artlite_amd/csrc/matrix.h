@@ -120,11 +120,14 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
 }
 
-// 1 / (1 + e^-v) to about 2 ulp: e^-v as 2^t with t = -v log2 e in two parts (the product's rounding, put back to first order),
-// the hardware's 2^t and reciprocal, the latter with a step of Newton's
+// 1 / (1 + e^-v). EXACT: to about 2 ulp, e^-v as 2^t with t = -v log2 e in two parts (the product's rounding, put back to
+// first order), the hardware's 2^t and reciprocal, the latter with a step of Newton's. Else without either correction, for
+// results of 11 bits: off by |v| 2^-24 and 2 ulp (a fourth of the instructions, two of them the quarter-rate ones).
+template <bool EXACT>
 __device__ __forceinline__ float sigmoid(float v) {
   constexpr float L2E = 1.44269504f, L2E_LO = 1.92596303e-8f;  // (log2 e and what its rounding leaves)
   const float t = v * -L2E;
+  if constexpr (!EXACT) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
   const float r = __builtin_fmaf(v, -L2E, -t) - v * L2E_LO;
   const float e = __builtin_amdgcn_exp2f(t) * __builtin_fmaf(r, 0.69314718f, 1.0f);
   const float d = 1.0f + e;
@@ -133,13 +136,15 @@ __device__ __forceinline__ float sigmoid(float v) {
   return t > 126.0f ? 0.0f : v > 100.0f ? 1.0f : q;
 }
 // the gated block's activation a and its derivative da at g (artlite_act); gelu's (1 + tanh z) / 2 is sigmoid(2 z)
+template <bool EXACT = true>
 __device__ __forceinline__ float gate_act(int act, float g) {
-  if (act == ARTLITE_ACT_SILU) return g * sigmoid(g);
-  return g * sigmoid(1.5957691216f * __builtin_fmaf(0.044715f * g * g, g, g));
+  if (act == ARTLITE_ACT_SILU) return g * sigmoid<EXACT>(g);
+  return g * sigmoid<EXACT>(1.5957691216f * __builtin_fmaf(0.044715f * g * g, g, g));
 }
+template <bool EXACT = true>
 __device__ __forceinline__ void gate_act_grad(int act, float g, float& a, float& da) {
   const float c = 0.044715f * g * g;
-  const float s = sigmoid(act == ARTLITE_ACT_SILU ? g : 1.5957691216f * __builtin_fmaf(c, g, g));
+  const float s = sigmoid<EXACT>(act == ARTLITE_ACT_SILU ? g : 1.5957691216f * __builtin_fmaf(c, g, g));
   a = g * s;
   // (0 where s is 0 or 1: nothing times a large slope stays nothing)
   const float w = s * (1.0f - s), k = act == ARTLITE_ACT_SILU ? 1.0f : 1.5957691216f * __builtin_fmaf(3.0f, c, 1.0f);
