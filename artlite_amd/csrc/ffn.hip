@@ -23,31 +23,25 @@ namespace artlite {
 
 namespace {
 
-// x (a row a workgroup) -> fp16 planes of Kp values times 2^-xe, xe and the exponent of its 2-norm
+// A launch of k_rows16: x, or x and dy, and the exponents of their rows (and of h, dh, dg and du, from the rows' 2-norms and
+// the matrices' bounds)
+struct Rows16 {
+  const void* x[2];
+  int64_t stride[2];
+  uint16_t* out[2];
+  int32_t *e[2];            // (their values are times 2^-e)
+  int arrays;
+  int64_t K, Kp, plane;
+  int32_t *he, *dhe, *de;   // (those that are wanted)
+  int lh, ld, lw;           // gate's and up's bounds together; down's; the larger of gate's and up's and 1 for the derivative
+};
+
+// a row a workgroup -> fp16 planes of Kp values
 template <bool BF16>
-__global__ __launch_bounds__(256) void k_rows16(const void* __restrict__ x, int64_t K, int64_t stride, int vec,
-                                                uint16_t* __restrict__ out, int64_t Kp, int64_t plane, int planes,
-                                                int32_t* __restrict__ xe, int32_t* __restrict__ ne) {
+__global__ __launch_bounds__(256) void k_rows16(const Rows16 a) {
   __shared__ float red[4];
   const int64_t m = blockIdx.x;
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  auto load = [&](int64_t k, float(&v)[8]) {
-    if constexpr (BF16) {
-      const uint16_t* p = static_cast<const uint16_t*>(x) + m * stride + k;
-      uint16_t b[8];
-      if (vec)
-        __builtin_memcpy(b, __builtin_assume_aligned(p, 16), 16);
-      else
-        for (int i = 0; i < 8; i++) b[i] = p[i];
-      for (int i = 0; i < 8; i++) v[i] = bf16_to_f32(b[i]);
-    } else {
-      const float* p = static_cast<const float*>(x) + m * stride + k;
-      if (vec)
-        __builtin_memcpy(v, __builtin_assume_aligned(p, 16), 32);
-      else
-        for (int i = 0; i < 8; i++) v[i] = p[i];
-    }
-  };
   auto all = [&](float v, bool add) {
     for (int o = 32; o; o >>= 1) {
       const float u = __shfl_xor(v, o);
@@ -58,48 +52,51 @@ __global__ __launch_bounds__(256) void k_rows16(const void* __restrict__ x, int6
     __syncthreads();
     return add ? red[0] + red[1] + red[2] + red[3] : fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   };
-  float mx = 0.0f;
-  for (int64_t k = threadIdx.x * 8; k < K; k += 2048) {
-    float v[8];
-    load(k, v);
-    for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(v[i]));
-  }
-  mx = all(mx, false);
-  const int e = exp_above(mx);
-  float ss = 0.0f;
-  for (int64_t k = threadIdx.x * 8; k < Kp; k += 2048) {
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (k < K) load(k, v);
-    uint16_t a[8], b[8];
-    for (int i = 0; i < 8; i++) {
-      const float r = __builtin_amdgcn_ldexpf(v[i], -e), s = __builtin_amdgcn_ldexpf(r, 15);
-      ss = __builtin_fmaf(r, r, ss);
-      const _Float16 hi = _Float16(s);
-      a[i] = __builtin_bit_cast(uint16_t, hi);
-      // (an infinite value is its first plane)
-      b[i] = __builtin_bit_cast(uint16_t, _Float16(__builtin_isinf(s) ? 0.0f : s - float(hi)));
+  int norm[2] = {0, 0};
+  for (int i = 0; i < a.arrays; i++) {
+    auto load = [&](int64_t k, float(&v)[8]) {  // (at any address: rows need not be aligned)
+      if constexpr (BF16) {
+        uint16_t b[8];
+        __builtin_memcpy(b, static_cast<const uint16_t*>(a.x[i]) + m * a.stride[i] + k, 16);
+        for (int j = 0; j < 8; j++) v[j] = bf16_to_f32(b[j]);
+      } else {
+        __builtin_memcpy(v, static_cast<const float*>(a.x[i]) + m * a.stride[i] + k, 32);
+      }
+    };
+    float mx = 0.0f;
+    for (int64_t k = threadIdx.x * 8; k < a.K; k += 2048) {
+      float v[8];
+      load(k, v);
+      for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(v[j]));
     }
-    __builtin_memcpy(__builtin_assume_aligned(out + m * Kp + k, 16), a, 16);
-    if (planes == 2) __builtin_memcpy(__builtin_assume_aligned(out + plane + m * Kp + k, 16), b, 16);
-  }
-  ss = all(ss, true);
-  if (threadIdx.x == 0) {
-    xe[m] = e - 15;
+    mx = all(mx, false);
+    const int e = exp_above(mx);
+    float ss = 0.0f;
+    uint16_t* out = a.out[i] + m * a.Kp;
+    for (int64_t k = threadIdx.x * 8; k < a.Kp; k += 2048) {
+      float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (k < a.K) load(k, v);
+      uint16_t hi[8], lo[8];
+      for (int j = 0; j < 8; j++) {
+        const float r = __builtin_amdgcn_ldexpf(v[j], -e), s = __builtin_amdgcn_ldexpf(r, 15);
+        ss = __builtin_fmaf(r, r, ss);
+        const _Float16 h = _Float16(s);
+        hi[j] = __builtin_bit_cast(uint16_t, h);
+        // (an infinite value is its first plane)
+        lo[j] = __builtin_bit_cast(uint16_t, _Float16(__builtin_isinf(s) ? 0.0f : s - float(h)));
+      }
+      __builtin_memcpy(__builtin_assume_aligned(out + k, 16), hi, 16);
+      if (!BF16) __builtin_memcpy(__builtin_assume_aligned(out + a.plane + k, 16), lo, 16);
+    }
     // (|x| < 2^e sqrt(ss); ss is at most K and its fp32 sum off by less than the step to the next exponent)
-    if (ne) ne[m] = e + (exp_above(sqrtf(ss) * 1.01f));
+    ss = all(ss, true);
+    norm[i] = e + exp_above(sqrtf(ss) * 1.01f);
+    if (threadIdx.x == 0) a.e[i][m] = e - 15;
   }
-}
-
-// the rows' scales of h, dh and dg, du, from the exponents of the rows' norms and of the matrices' bounds (lh: gate's and up's
-// together, ld: down's, lw: the larger of gate's and up's and 1 for the derivative)
-__global__ void k_exps(int64_t M, const int32_t* __restrict__ nx, const int32_t* __restrict__ ny, int lh, int ld, int lw,
-                       int32_t* __restrict__ he, int32_t* __restrict__ dhe, int32_t* __restrict__ de) {
-  const int64_t m = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (m >= M) return;
-  he[m] = 2 * nx[m] + lh - 15;
-  if (ny) {
-    dhe[m] = ny[m] + ld - 15;
-    de[m] = ny[m] + ld + nx[m] + lw - 15;
+  if (threadIdx.x == 0) {
+    if (a.he) a.he[m] = 2 * norm[0] + a.lh - 15;
+    if (a.dhe) a.dhe[m] = norm[1] + a.ld - 15;
+    if (a.de) a.de[m] = norm[1] + a.ld + norm[0] + a.lw - 15;
   }
 }
 
@@ -107,39 +104,57 @@ __global__ void k_exps(int64_t M, const int32_t* __restrict__ nx, const int32_t*
 struct MaxE {
   const int32_t* a[4];
 };
-__global__ __launch_bounds__(256) void k_max_e(const MaxE in, int64_t M, int32_t* __restrict__ out) {
-  __shared__ int red[4];
+__global__ __launch_bounds__(1024) void k_max_e(const MaxE in, int64_t M, int32_t* __restrict__ out) {
+  __shared__ int red[16];
   const int32_t* a = in.a[blockIdx.x];
   int v = INT32_MIN;
-  for (int64_t m = threadIdx.x; m < M; m += 256) v = max(v, a[m]);
+  for (int64_t m = threadIdx.x; m < M; m += 1024) v = max(v, a[m]);
   for (int o = 32; o; o >>= 1) v = max(v, __shfl_xor(v, o));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  if (threadIdx.x == 0) out[blockIdx.x] = max(max(red[0], red[1]), max(red[2], red[3]));
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < 16; w++) v = max(v, red[w]);
+    out[blockIdx.x] = v;
+  }
 }
 
-// rows of C fp16 values (ld apart, row t worth 2^e[t]) turned: C rows of Tp values worth 2^*top, zeros past T
-__global__ __launch_bounds__(256) void k_turn(const uint16_t* __restrict__ in, int64_t ld, int64_t T, int64_t C,
-                                              const int32_t* __restrict__ e, const int32_t* __restrict__ top,
-                                              uint16_t* __restrict__ out, int64_t Tp) {
+// Turns of a launch: rows of C fp16 values (ld apart, row t worth 2^e[t]) into C rows of Tp values worth 2^*top, zeros past T
+struct Turn {
+  const uint16_t* in;
+  int64_t ld, C;
+  const int32_t *e, *top;
+  uint16_t* out;
+};
+struct Turns {
+  Turn t[5];
+  int64_t T, Tp;
+  int planes;
+};
+__global__ __launch_bounds__(256) void k_turn(const Turns a) {
   __shared__ __attribute__((aligned(16))) uint16_t t[64][72];
+  const Turn& j = a.t[blockIdx.z / a.planes];
   const int64_t c0 = int64_t(blockIdx.x) * 64, t0 = int64_t(blockIdx.y) * 64;
-  const int E = *top;
+  if (c0 >= j.C) return;
+  const int64_t pl = blockIdx.z % a.planes;
+  const uint16_t* in = j.in + pl * a.T * j.ld;
+  uint16_t* out = j.out + pl * j.C * a.Tp;
+  const int E = *j.top;
   for (int i = threadIdx.x; i < 64 * 8; i += 256) {
     const int r = i >> 3, c = 8 * (i & 7);
     uint16_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (t0 + r < T && c0 + c < ld) {  // (ld is a multiple of 64: the row's padding is read at most)
-      __builtin_memcpy(v, __builtin_assume_aligned(in + (t0 + r) * ld + c0 + c, 16), 16);
-      const int sh = e[t0 + r] - E;
+    if (t0 + r < a.T && c0 + c < j.ld) {  // (ld is a multiple of 64: the row's padding is read at most)
+      __builtin_memcpy(v, __builtin_assume_aligned(in + (t0 + r) * j.ld + c0 + c, 16), 16);
+      const int sh = j.e[t0 + r] - E;
       for (int k = 0; k < 8; k++)
-        v[k] = __builtin_bit_cast(uint16_t, _Float16(__builtin_amdgcn_ldexpf(float(__builtin_bit_cast(_Float16, v[k])), sh)));
+        v[k] = __builtin_bit_cast(uint16_t,
+                                  _Float16(__builtin_amdgcn_ldexpf(float(__builtin_bit_cast(_Float16, v[k])), sh)));
     }
     for (int k = 0; k < 8; k++) t[c + k][r] = v[k];
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 64 * 8; i += 256) {
     const int c = i >> 3, r = 8 * (i & 7);
-    if (c0 + c < C) *reinterpret_cast<uint4*>(out + (c0 + c) * Tp + t0 + r) = *reinterpret_cast<const uint4*>(&t[c][r]);
+    if (c0 + c < j.C) *reinterpret_cast<uint4*>(out + (c0 + c) * a.Tp + t0 + r) = *reinterpret_cast<const uint4*>(&t[c][r]);
   }
 }
 
@@ -147,23 +162,11 @@ __global__ __launch_bounds__(256) void k_zero(uint16_t* p, int64_t n) {
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) p[i] = 0;
 }
 
-int rows16(const void* x, int dtype, int64_t M, int64_t K, int64_t stride, uint16_t* out, int64_t Kp, int planes,
-           int32_t* xe, int32_t* ne, hipStream_t s) {
-  const bool b = dtype == ARTLITE_X_BF16;
-  const int vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (stride * (b ? 2 : 4)) % 16 == 0;
-  if (b)
-    k_rows16<true><<<unsigned(M), 256, 0, s>>>(x, K, stride, vec, out, Kp, M * Kp, planes, xe, ne);
+int rows16(const Rows16& a, int dtype, int64_t M, hipStream_t s) {
+  if (dtype == ARTLITE_X_BF16)
+    k_rows16<true><<<unsigned(M), 256, 0, s>>>(a);
   else
-    k_rows16<false><<<unsigned(M), 256, 0, s>>>(x, K, stride, vec, out, Kp, M * Kp, planes, xe, ne);
-  ART_HIP(hipGetLastError());
-  return ARTLITE_OK;
-}
-
-int turn(const uint16_t* in, int64_t ld, int64_t T, int64_t C, int planes, const int32_t* e, const int32_t* top,
-         uint16_t* out, int64_t Tp, hipStream_t s) {
-  for (int p = 0; p < planes; p++)
-    k_turn<<<dim3(unsigned((C + 63) / 64), unsigned(Tp / 64)), 256, 0, s>>>(in + p * T * ld, ld, T, C, e, top,
-                                                                            out + p * C * Tp, Tp);
+    k_rows16<false><<<unsigned(M), 256, 0, s>>>(a);
   ART_HIP(hipGetLastError());
   return ARTLITE_OK;
 }
@@ -190,11 +193,7 @@ void segments(HGemm& g, std::initializer_list<Pair> pairs, int planes) {
 }
 
 // the most rows of a call of the large tiles (their launches' grids and a workspace's sizes stay in range)
-constexpr int64_t MOST_ROWS = int64_t(1) << 22;
-
-bool aligned_rows(const void* x, int dtype, int64_t n, int64_t stride) {
-  return dtype == ARTLITE_X_BF16 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (n <= 1 || stride % 8 == 0);
-}
+constexpr int64_t MOST_ROWS = int64_t(1) << 21;
 
 // ---- one matrix's product
 
@@ -205,12 +204,12 @@ struct LinearPlan {
   int32_t* xe = nullptr;
   float* parts = nullptr;
 };
-LinearPlan linear_plan(Carve& c, const artlite_matrix* w, int dtype, int64_t n, bool direct) {
+LinearPlan linear_plan(Carve& c, const artlite_matrix* w, int dtype, int64_t n) {
   LinearPlan p;
   p.few = n <= (dtype == ARTLITE_X_BF16 ? FEW_ROWS : FEW_ROWS_F32);
   if (p.few) {
     const int pl = dtype == ARTLITE_X_BF16 ? 1 : 3;
-    if (!direct) p.planes = c.take<uint16_t>(size_t(pl) * n * w->K);
+    if (pl == 3 && n > FEW_X32) p.planes = c.take<uint16_t>(3 * size_t(n) * w->K);
     p.parts = c.take<float>(few_parts_bytes(w, pl, false, n) / 4);
   } else {
     const int pl = dtype == ARTLITE_X_BF16 ? 1 : 2;
@@ -246,20 +245,24 @@ int check_array(const void* p, int64_t n, int64_t cols, int64_t stride, bool wri
   return check_device(p, device, what);
 }
 
+// x as a launch over few rows takes it: bf16 and up to FEW_X32 fp32 rows as they are, more fp32 rows as planes
+int few_x(FewArgs& a, const void* x, int dtype, int64_t n, int64_t K, int64_t stride, uint16_t* planes, hipStream_t s) {
+  a.planes = dtype == ARTLITE_X_BF16 ? 1 : 3;
+  a.x32 = dtype == ARTLITE_X_F32 && !planes;
+  a.x = x, a.x_stride = stride;
+  if (!planes) return ARTLITE_OK;
+  a.x = planes, a.x_stride = K, a.x_plane = n * K;
+  return launch_planes(x, dtype, n, K, stride, planes, K, n * K, 3, s);
+}
+
 int linear(const artlite_matrix* w, const void* x, int dtype, int64_t n, int64_t x_stride, void* y, int64_t y_stride,
            char* base, hipStream_t s) {
   Carve c(base);
-  const bool direct = aligned_rows(x, dtype, n, x_stride);
-  const LinearPlan p = linear_plan(c, w, dtype, n, direct);
+  const LinearPlan p = linear_plan(c, w, dtype, n);
   if (p.few) {
     FewArgs a{};
     a.w = w;
-    a.planes = dtype == ARTLITE_X_BF16 ? 1 : 3;
-    a.x = static_cast<const uint16_t*>(x), a.x_stride = x_stride;
-    if (!direct) {
-      ART_TRY(launch_planes(x, dtype, n, w->K, x_stride, p.planes, w->K, n * w->K, a.planes, s));
-      a.x = p.planes, a.x_stride = w->K, a.x_plane = n * w->K;
-    }
+    ART_TRY(few_x(a, x, dtype, n, w->K, x_stride, p.planes, s));
     a.M = n;
     a.y = y, a.y_stride = y_stride, a.dtype = dtype;
     a.parts = p.parts;
@@ -267,8 +270,11 @@ int linear(const artlite_matrix* w, const void* x, int dtype, int64_t n, int64_t
   }
   const int pl = dtype == ARTLITE_X_BF16 ? 1 : 2, e = wexp16(w);
   const int64_t Kp = pad64(w->K);
-  ART_TRY(rows16(x, dtype, n, w->K, x_stride, p.x16, Kp, pl, p.xe, nullptr, s));
-  ART_TRY(launch_unpack(w, false, e, p.w16, Kp, w->N * Kp, pl, s));
+  Rows16 r{};
+  r.x[0] = x, r.stride[0] = x_stride, r.out[0] = p.x16, r.e[0] = p.xe;
+  r.arrays = 1, r.K = w->K, r.Kp = Kp, r.plane = n * Kp;
+  ART_TRY(rows16(r, dtype, n, s));
+  ART_TRY(launch_unpack(w, nullptr, false, e, 0, p.w16, nullptr, Kp, w->N * Kp, pl, s));
   HGemm g{};
   segments(g, {{p.x16, n * Kp, p.w16, w->N * Kp}}, pl);
   g.lda = g.ldb = g.K = Kp;
@@ -308,15 +314,15 @@ struct FfnPlan {
   bool few;
   uint16_t *planes = nullptr, *hp = nullptr;  // few rows: x as planes (where it is not read as it is), h as planes
   uint16_t *x16, *w16, *u16, *d16, *h16;      // else: x, the unpacked matrices, h
-  int32_t *xe, *nx, *he;
+  int32_t *xe, *he;
   float* parts;
 };
-FfnPlan ffn_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool direct) {
+FfnPlan ffn_plan(Carve& c, const Ffn& f, int dtype, int64_t n) {
   FfnPlan p{};
   p.few = n <= FEW_ROWS_FFN;
   const bool b = dtype == ARTLITE_X_BF16;
   if (p.few) {
-    if (!direct) p.planes = c.take<uint16_t>(size_t(b ? 1 : 3) * n * f.H);
+    if (!b && n > FEW_X32) p.planes = c.take<uint16_t>(3 * size_t(n) * f.H);
     p.hp = c.take<uint16_t>(size_t(b ? 2 : 3) * n * f.F);
     p.parts = c.take<float>(std::max(few_parts_bytes(f.gate, b ? 1 : 3, true, n), few_parts_bytes(f.down, b ? 2 : 3, false, n)) / 4);
     return p;
@@ -328,7 +334,6 @@ FfnPlan ffn_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool direct) {
   p.d16 = c.take<uint16_t>(pl * f.H * f.Fp);
   p.h16 = c.take<uint16_t>(pl * n * f.Fp);
   p.xe = c.take<int32_t>(n);
-  p.nx = c.take<int32_t>(n);
   p.he = c.take<int32_t>(n);
   const int sg = b ? 1 : 3;
   p.parts = c.take<float>(std::max(hgemm_parts_bytes(n, f.F, f.Hp, sg, true), hgemm_parts_bytes(n, f.H, f.Fp, sg, false)) / 4);
@@ -338,17 +343,12 @@ FfnPlan ffn_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool direct) {
 int ffn_forward(const Ffn& f, const void* x, int dtype, int64_t n, int64_t x_stride, void* y, int64_t y_stride, char* base,
                 hipStream_t s) {
   Carve c(base);
-  const bool direct = aligned_rows(x, dtype, n, x_stride), b = dtype == ARTLITE_X_BF16;
-  const FfnPlan p = ffn_plan(c, f, dtype, n, direct);
+  const bool b = dtype == ARTLITE_X_BF16;
+  const FfnPlan p = ffn_plan(c, f, dtype, n);
   if (p.few) {
     FewArgs a{};
     a.w = f.gate, a.up = f.up, a.act = f.act;
-    a.planes = b ? 1 : 3;
-    a.x = static_cast<const uint16_t*>(x), a.x_stride = x_stride;
-    if (!direct) {
-      ART_TRY(launch_planes(x, dtype, n, f.H, x_stride, p.planes, f.H, n * f.H, a.planes, s));
-      a.x = p.planes, a.x_stride = f.H, a.x_plane = n * f.H;
-    }
+    ART_TRY(few_x(a, x, dtype, n, f.H, x_stride, p.planes, s));
     a.M = n;
     a.h = p.hp, a.h_stride = f.F, a.h_plane = n * f.F, a.h_planes = b ? 2 : 3;
     a.parts = p.parts;
@@ -363,12 +363,13 @@ int ffn_forward(const Ffn& f, const void* x, int dtype, int64_t n, int64_t x_str
     return launch_few(d, s);
   }
   const int pl = b ? 1 : 2;
-  ART_TRY(rows16(x, dtype, n, f.H, x_stride, p.x16, f.Hp, pl, p.xe, p.nx, s));
-  k_exps<<<unsigned((n + 255) / 256), 256, 0, s>>>(n, p.nx, nullptr, f.gate->row_exp + f.up->row_exp, 0, 0, p.he, nullptr,
-                                                   nullptr);
-  ART_TRY(launch_unpack(f.gate, false, wexp16(f.gate), p.w16, f.Hp, f.F * f.Hp, pl, s));
-  ART_TRY(launch_unpack(f.up, false, wexp16(f.up), p.u16, f.Hp, f.F * f.Hp, pl, s));
-  ART_TRY(launch_unpack(f.down, false, wexp16(f.down), p.d16, f.Fp, f.H * f.Fp, pl, s));
+  Rows16 r{};
+  r.x[0] = x, r.stride[0] = x_stride, r.out[0] = p.x16, r.e[0] = p.xe;
+  r.arrays = 1, r.K = f.H, r.Kp = f.Hp, r.plane = n * f.Hp;
+  r.he = p.he, r.lh = f.gate->row_exp + f.up->row_exp;
+  ART_TRY(rows16(r, dtype, n, s));
+  ART_TRY(launch_unpack(f.gate, f.up, false, wexp16(f.gate), wexp16(f.up), p.w16, p.u16, f.Hp, f.F * f.Hp, pl, s));
+  ART_TRY(launch_unpack(f.down, nullptr, false, wexp16(f.down), 0, p.d16, nullptr, f.Fp, f.H * f.Fp, pl, s));
   HGemm g{};
   segments(g, {{p.x16, n * f.Hp, p.w16, f.F * f.Hp, p.u16}}, pl);
   g.lda = g.ldb = g.K = f.Hp;
@@ -393,7 +394,7 @@ struct GradPlan {
   uint16_t *x16, *dy16, *a16, *b16, *c16;        // x, dy; gate and up, later their transposes; down's transpose
   uint16_t *h16, *dh16, *dg16, *du16;
   uint16_t *xt, *dyt, *ht, *dgt, *dut;           // (weights' gradients) turned
-  int32_t *xe, *nx, *ye, *ny, *he, *dhe, *de, *top;
+  int32_t *xe, *ye, *he, *dhe, *de, *top;
   float* parts;
 };
 GradPlan grad_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool weights) {
@@ -409,9 +410,7 @@ GradPlan grad_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool weights) {
   p.du16 = c.take<uint16_t>(pl * n * f.Fp);
   p.dh16 = c.take<uint16_t>(pl * n * f.Fp);
   p.xe = c.take<int32_t>(n);
-  p.nx = c.take<int32_t>(n);
   p.ye = c.take<int32_t>(n);
-  p.ny = c.take<int32_t>(n);
   p.he = c.take<int32_t>(n);
   p.dhe = c.take<int32_t>(n);
   p.de = c.take<int32_t>(n);
@@ -440,16 +439,19 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
   Carve c(base);
   const GradPlan p = grad_plan(c, f, dtype, n, weights);
   const int pl = dtype == ARTLITE_X_BF16 ? 1 : 2;
-  ART_TRY(rows16(x, dtype, n, f.H, x_stride, p.x16, f.Hp, pl, p.xe, p.nx, s));
-  ART_TRY(rows16(dy, dtype, n, f.H, dy_stride, p.dy16, f.Hp, pl, p.ye, p.ny, s));
   const int lg = f.gate->row_exp, lu = f.up->row_exp;
-  const int ld = f.down->max_exp + int(std::ceil(0.5 * std::log2(double(f.H))));
-  k_exps<<<unsigned((n + 255) / 256), 256, 0, s>>>(n, p.nx, p.ny, lg + lu, ld, (lg > lu ? lg : lu) + 1, p.he, p.dhe, p.de);
+  Rows16 r{};
+  r.x[0] = x, r.stride[0] = x_stride, r.out[0] = p.x16, r.e[0] = p.xe;
+  r.x[1] = dy, r.stride[1] = dy_stride, r.out[1] = p.dy16, r.e[1] = p.ye;
+  r.arrays = 2, r.K = f.H, r.Kp = f.Hp, r.plane = n * f.Hp;
+  r.he = p.he, r.dhe = p.dhe, r.de = p.de;
+  r.lh = lg + lu, r.lw = (lg > lu ? lg : lu) + 1;
+  r.ld = f.down->max_exp + int(std::ceil(0.5 * std::log2(double(f.H))));
+  ART_TRY(rows16(r, dtype, n, s));
   // (gate and up share a scale: dx sums over both)
   const int e = wexp16(f.gate) > wexp16(f.up) ? wexp16(f.gate) : wexp16(f.up), ed = wexp16(f.down);
-  ART_TRY(launch_unpack(f.gate, false, e, p.a16, f.Hp, f.F * f.Hp, pl, s));
-  ART_TRY(launch_unpack(f.up, false, e, p.b16, f.Hp, f.F * f.Hp, pl, s));
-  ART_TRY(launch_unpack(f.down, true, ed, p.c16, f.Hp, f.F * f.Hp, pl, s));
+  ART_TRY(launch_unpack(f.gate, f.up, false, e, e, p.a16, p.b16, f.Hp, f.F * f.Hp, pl, s));
+  ART_TRY(launch_unpack(f.down, nullptr, true, ed, 0, p.c16, nullptr, f.Hp, f.F * f.Hp, pl, s));
   HGemm d{};
   segments(d, {{p.dy16, n * f.Hp, p.c16, f.F * f.Hp}}, pl);
   d.lda = d.ldb = d.K = f.Hp;
@@ -473,8 +475,7 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
   g.parts = p.parts;
   ART_TRY(launch_hgemm(g, s));
   if (dx) {
-    ART_TRY(launch_unpack(f.gate, true, e, p.a16, f.Fp, f.H * f.Fp, pl, s));
-    ART_TRY(launch_unpack(f.up, true, e, p.b16, f.Fp, f.H * f.Fp, pl, s));
+    ART_TRY(launch_unpack(f.gate, f.up, true, e, e, p.a16, p.b16, f.Fp, f.H * f.Fp, pl, s));
     HGemm x2{};
     segments(x2, {{p.dg16, n * f.Fp, p.a16, f.H * f.Fp}, {p.du16, n * f.Fp, p.b16, f.H * f.Fp}}, pl);
     x2.lda = x2.ldb = x2.K = f.Fp;
@@ -486,14 +487,19 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
   }
   if (!weights) return ARTLITE_OK;
   const int64_t Tp = pad64(n);
-  k_max_e<<<4, 256, 0, s>>>(MaxE{{p.xe, p.ye, p.he, p.de}}, n, p.top);
-  if (dgate || dup) ART_TRY(turn(p.x16, f.Hp, n, f.H, pl, p.xe, p.top, p.xt, Tp, s));
-  if (dgate) ART_TRY(turn(p.dg16, f.Fp, n, f.F, pl, p.de, p.top + 3, p.dgt, Tp, s));
-  if (dup) ART_TRY(turn(p.du16, f.Fp, n, f.F, pl, p.de, p.top + 3, p.dut, Tp, s));
+  k_max_e<<<4, 1024, 0, s>>>(MaxE{{p.xe, p.ye, p.he, p.de}}, n, p.top);
+  Turns t{};
+  t.T = n, t.Tp = Tp, t.planes = pl;
+  int turns = 0;
+  if (dgate || dup) t.t[turns++] = Turn{p.x16, f.Hp, f.H, p.xe, p.top, p.xt};
+  if (dgate) t.t[turns++] = Turn{p.dg16, f.Fp, f.F, p.de, p.top + 3, p.dgt};
+  if (dup) t.t[turns++] = Turn{p.du16, f.Fp, f.F, p.de, p.top + 3, p.dut};
   if (ddown) {
-    ART_TRY(turn(p.dy16, f.Hp, n, f.H, pl, p.ye, p.top + 1, p.dyt, Tp, s));
-    ART_TRY(turn(p.h16, f.Fp, n, f.F, pl, p.he, p.top + 2, p.ht, Tp, s));
+    t.t[turns++] = Turn{p.dy16, f.Hp, f.H, p.ye, p.top + 1, p.dyt};
+    t.t[turns++] = Turn{p.h16, f.Fp, f.F, p.he, p.top + 2, p.ht};
   }
+  k_turn<<<dim3(unsigned((std::max(f.H, f.F) + 63) / 64), unsigned(Tp / 64), unsigned(turns * pl)), 256, 0, s>>>(t);
+  ART_HIP(hipGetLastError());
   const auto grad = [&](const uint16_t* a, int64_t M, const int32_t* ea, const uint16_t* b, int64_t N, const int32_t* eb,
                         void* out) {
     HGemm w{};
@@ -517,12 +523,12 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
 
 using namespace artlite;
 
-extern "C" int artlite_linear_workspace(const artlite_matrix* w, int dtype, int64_t n, int aligned, size_t* nbytes) {
+extern "C" int artlite_linear_workspace(const artlite_matrix* w, int dtype, int64_t n, size_t* nbytes) {
   if (!w || !nbytes) return fail(ARTLITE_EINVAL, "linear: null");
   ART_TRY(check_dtype(dtype, "linear"));
   ART_TRY(check_rows(n, "linear"));
   Carve c(nullptr);
-  if (n) (void)linear_plan(c, w, dtype, n, aligned && dtype == ARTLITE_X_BF16);
+  if (n) (void)linear_plan(c, w, dtype, n);
   *nbytes = c.at;
   return ARTLITE_OK;
 }
@@ -536,7 +542,7 @@ extern "C" int artlite_linear(const artlite_matrix* w, const void* x, int dtype,
   ART_TRY(check_array(x, n, w->K, x_stride, false, dtype, w->device, "linear: x"));
   ART_TRY(check_array(y, n, w->N, y_stride, true, dtype, w->device, "linear: y"));
   Carve c(nullptr);
-  (void)linear_plan(c, w, dtype, n, aligned_rows(x, dtype, n, x_stride));
+  (void)linear_plan(c, w, dtype, n);
   if (c.at && work && work->w.device != w->device)
     return fail(ARTLITE_EINVAL, "linear: a workspace of device %d, not %d", work->w.device, w->device);
   OnDevice on;
@@ -557,7 +563,7 @@ extern "C" int artlite_ffn_workspace(const artlite_ffn* d, int dtype, int64_t n,
   if (n && backward) {
     (void)grad_plan(c, f, dtype, n, backward == 2);
   } else if (n) {
-    (void)ffn_plan(c, f, dtype, n, false);
+    (void)ffn_plan(c, f, dtype, n);
   }
   *nbytes = c.at;
   return ARTLITE_OK;
@@ -574,7 +580,7 @@ extern "C" int artlite_ffn_forward(const artlite_ffn* d, const void* x, int dtyp
   ART_TRY(check_array(x, n, f.H, x_stride, false, dtype, dev, "ffn: x"));
   ART_TRY(check_array(y, n, f.H, y_stride, true, dtype, dev, "ffn: y"));
   Carve c(nullptr);
-  (void)ffn_plan(c, f, dtype, n, aligned_rows(x, dtype, n, x_stride));
+  (void)ffn_plan(c, f, dtype, n);
   if (work && work->w.device != dev) return fail(ARTLITE_EINVAL, "ffn: a workspace of device %d, not %d", work->w.device, dev);
   OnDevice on;
   ART_TRY(on.set(dev));

@@ -97,6 +97,19 @@ __device__ __forceinline__ void store_planes(uint16_t* p, int64_t plane, int pla
   }
 }
 
+// eight fp32 values (a, b) -> their planes: two values' bf16 in a dword each, x = hi + mid + lo to 2^-24
+__device__ __forceinline__ void split3(const u32x4& a, const u32x4& b, u32x4& hi, u32x4& mid, u32x4& lo) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    float u = __uint_as_float(i < 2 ? a[2 * i] : b[2 * i - 4]), v = __uint_as_float(i < 2 ? a[2 * i + 1] : b[2 * i - 3]);
+    hi[i] = bf16_pair(u, v);
+    u -= __uint_as_float(hi[i] << 16), v -= __uint_as_float(hi[i] & 0xFFFF0000u);
+    mid[i] = bf16_pair(u, v);
+    u -= __uint_as_float(mid[i] << 16), v -= __uint_as_float(mid[i] & 0xFFFF0000u);
+    lo[i] = bf16_pair(u, v);
+  }
+}
+
 // an output of row m, column n from its sum (gated: and the second matrix's)
 template <bool GLU>
 __device__ __forceinline__ void few_out(const FewK& a, int64_t m, int64_t n, float s, float u) {
@@ -118,15 +131,15 @@ constexpr int few_most(int planes, int nc, bool glu) { return nc == 1 && planes 
 
 // P planes of x, NC blocks of 16 rows, RI rows of a block a lane: block row 4 g + i is x's row g + 4 i, so that up to 4 rows
 // are in each lane's first sum (RI 1) and up to 8 in its first two, and the others take no scaling. The units in gridDim.z
-// parts (PART: their sums into a.parts, for k_few_join).
-template <int QT, int P, int NC, int RI, bool GLU, bool PART>
+// parts (PART: their sums into a.parts, for k_few_join). X32: x is fp32, split into its planes as it is used.
+template <int QT, int P, int NC, int RI, bool GLU, bool PART, bool X32>
 __global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a) {
   constexpr int TB = few_tiles(NC, GLU), RB = GLU ? 2 * TB : TB, KIND = code_kind<QT, P>(), UB = unit_bytes<QT>();
   constexpr bool CIN = KIND < 0 || has_offset<QT>;  // (sum(x) times a constant is wanted)
   constexpr float CC = KIND < 0 ? (QT == ARTLITE_Q4_0 ? -136.0f : -128.0f) : -1.0f;
   constexpr uint32_t CB = bf16_of(int(CC)) * 0x10001u;
   // groups whose x is in flight, whether the next unit's codes are (registers)
-  constexpr int XD = P * NC == 1 ? (GLU ? 4 : 8) : P * NC <= 2 ? 4 : 2;
+  constexpr int XD = X32 ? 2 : P * NC == 1 ? (GLU ? 4 : 8) : P * NC <= 2 ? 4 : 2;
   constexpr bool AHEAD = NC == 1;
   extern __shared__ float red[];  // [wave][tile of a matrix][block][row][lane]
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6,
@@ -144,7 +157,7 @@ __global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a)
   for (int c = 0; c < NC; c++) {
     const int64_t m = m0 + 16 * c + (lr >> 2) + 4 * (lr & 3);
     live[c] = m < a.M;
-    xp[c] = a.x + (live[c] ? m : 0) * a.x_stride + 8 * lg;
+    xp[c] = a.x + ((live[c] ? m : 0) * a.x_stride + 8 * lg) * (X32 ? 2 : 1);
   }
   float acc[RB][NC][RI];
 #pragma unroll
@@ -168,21 +181,23 @@ __global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a)
   // x of a group; past the last group of K the last one's (the scales there are 0). Rows that there are not take row 0, or with
   // three planes keep what the registers hold: each row of the products is its own. (Loading only the rows there are took 1 row
   // of 4096 x 4096 from 4.3 to 5.0 us, 16 rows from 6.8 to 10.8; but 5 rows in three planes, 1536 x 2880, from 6.7 to 6.3.)
-  u32x4 x[XD][NC][P];
+  constexpr int XP = X32 ? 2 : P;  // (a group's loads: its planes, or 8 fp32 values in two)
+  u32x4 x[XD][NC][XP];
 #pragma unroll
   for (int j = 0; j < XD; j++)
 #pragma unroll
     for (int c = 0; c < NC; c++)
 #pragma unroll
-      for (int p = 0; p < P; p++) x[j][c][p] = u32x4{0, 0, 0, 0};
+      for (int p = 0; p < XP; p++) x[j][c][p] = u32x4{0, 0, 0, 0};
   const int klast = int(a.K) - 32;
   auto load_x = [&](int j, int u, int g) __attribute__((always_inline)) {
     const int k = min(u * UNIT + 32 * g, klast);
 #pragma unroll
     for (int c = 0; c < NC; c++)
-      if (P < 3 || NC > 1 || live[c])
+      if (!X32 || live[c])
 #pragma unroll
-        for (int p = 0; p < P; p++) x[j][c][p] = *reinterpret_cast<const u32x4*>(xp[c] + p * a.x_plane + k);
+        for (int p = 0; p < XP; p++)  // (at any address: rows need not be aligned)
+          __builtin_memcpy(&x[j][c][p], X32 ? xp[c] + 2 * k + 8 * p : xp[c] + p * a.x_plane + k, 16);
   };
   if (first + wv < end) {
     if (AHEAD) load(first + wv);
@@ -210,13 +225,21 @@ __global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a)
       for (int j = 0; j < 4; j++) {
         const int g = 4 * H + j;
         const u32x4 cst{CB, CB, CB, CB};
+        u32x4 xo[NC][P];
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+          if constexpr (X32)
+            split3(x[g % XD][c][0], x[g % XD][c][XP - 1], xo[c][0], xo[c][P > 1 ? 1 : 0], xo[c][P - 1]);
+          else
+#pragma unroll
+            for (int p = 0; p < P; p++) xo[c][p] = x[g % XD][c][p];
         f32x4 cin[NC];
 #pragma unroll
         for (int c = 0; c < NC; c++) {
           cin[c] = f32x4{0, 0, 0, 0};
           if constexpr (CIN)
 #pragma unroll
-            for (int p = P - 1; p >= 0; p--) cin[c] = mfma(x[g % XD][c][p], cst, cin[c]);
+            for (int p = P - 1; p >= 0; p--) cin[c] = mfma(xo[c][p], cst, cin[c]);
         }
 #pragma unroll
         for (int b = 0; b < RB; b++) {
@@ -226,7 +249,7 @@ __global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a)
           for (int c = 0; c < NC; c++) {
             f32x4 d = KIND < 0 ? cin[c] : f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int p = P - 1; p >= 0; p--) d = mfma(x[g % XD][c][p], q, d);
+            for (int p = P - 1; p >= 0; p--) d = mfma(xo[c][p], q, d);
 #pragma unroll
             for (int i = 0; i < RI; i++) {
               acc[b][c][i] = __builtin_fmaf(s[b][j], d[i], acc[b][c][i]);
@@ -317,7 +340,7 @@ FewCut few_cut(int64_t tiles, int units, int64_t M, int planes, bool glu) {
   return c;
 }
 
-template <int QT, int P, int NC, int RI, bool GLU>
+template <int QT, int P, int NC, int RI, bool GLU, bool X32>
 int launch_few_t(const FewK& k, hipStream_t s) {
   constexpr int LDS = few_most(P, NC, GLU) * (GLU ? 2 : 1) * few_tiles(NC, GLU) * NC * RI * WAVE * 4;
   static_assert(LDS <= 64 * 1024, "LDS");
@@ -326,27 +349,28 @@ int launch_few_t(const FewK& k, hipStream_t s) {
   const dim3 grid(unsigned(c.groups), unsigned(c.blocks), unsigned(c.parts));
   if (NC > 1 && c.parts > 1) {
     if (!k.parts) return fail(ARTLITE_EINVAL, "dense rows: no scratch for parts");
-    if constexpr (NC > 1) k_few<QT, P, NC, RI, GLU, true><<<grid, 64 * c.waves, lds, s>>>(k);
+    if constexpr (NC > 1) k_few<QT, P, NC, RI, GLU, true, X32><<<grid, 64 * c.waves, lds, s>>>(k);
     ART_HIP(hipGetLastError());
     k_few_join<GLU><<<unsigned((k.M * k.N + 255) / 256), 256, 0, s>>>(k, c.parts);
   } else {
-    k_few<QT, P, NC, RI, GLU, false><<<grid, 64 * c.waves, lds, s>>>(k);
+    k_few<QT, P, NC, RI, GLU, false, X32><<<grid, 64 * c.waves, lds, s>>>(k);
   }
   ART_HIP(hipGetLastError());
   return ARTLITE_OK;
 }
 
-template <int QT, int P, bool GLU>
+template <int QT, int P, bool GLU, bool X32 = false>
 int launch_few_p(const FewK& k, hipStream_t s) {
-  if (k.M <= 4) return launch_few_t<QT, P, 1, 1, GLU>(k, s);
-  if (k.M <= 8) return launch_few_t<QT, P, 1, 2, GLU>(k, s);
-  if (k.M <= 16) return launch_few_t<QT, P, 1, 4, GLU>(k, s);
-  if (k.M <= 32) return launch_few_t<QT, P, 2, 4, GLU>(k, s);
-  return launch_few_t<QT, P, 4, 4, GLU>(k, s);
+  if (k.M <= 4) return launch_few_t<QT, P, 1, 1, GLU, X32>(k, s);
+  if (k.M <= 8) return launch_few_t<QT, P, 1, 2, GLU, X32>(k, s);
+  if (k.M <= 16 || X32) return launch_few_t<QT, P, 1, 4, GLU, X32>(k, s);
+  if (k.M <= 32) return launch_few_t<QT, P, 2, 4, GLU, false>(k, s);
+  return launch_few_t<QT, P, 4, 4, GLU, false>(k, s);
 }
 
 template <int QT>
 int launch_few_q(const FewArgs& a, const FewK& k, hipStream_t s) {
+  if (a.x32) return a.up ? launch_few_p<QT, 3, true, true>(k, s) : launch_few_p<QT, 3, false, true>(k, s);
   if (a.up) return a.planes == 1 ? launch_few_p<QT, 1, true>(k, s) : launch_few_p<QT, 3, true>(k, s);
   return a.planes == 1   ? launch_few_p<QT, 1, false>(k, s)
          : a.planes == 2 ? launch_few_p<QT, 2, false>(k, s)
@@ -363,13 +387,14 @@ size_t few_parts_bytes(const artlite_matrix* w, int planes, bool gated, int64_t 
 
 int launch_few(const FewArgs& a, hipStream_t s) {
   if (a.M <= 0) return ARTLITE_OK;
+  if (a.x32 && a.M > FEW_X32) return fail(ARTLITE_EINVAL, "dense rows: %lld fp32 rows", (long long)a.M);
   if (a.M > int64_t(65535) * 16) return fail(ARTLITE_EINVAL, "dense rows: %lld rows", (long long)a.M);
   FewK k{};
   k.w = a.w->w.as<uint8_t>();
   k.up = a.up ? a.up->w.as<uint8_t>() : nullptr;
   k.tiles = a.w->tiles, k.units = a.w->units;
   k.N = a.w->N, k.K = a.w->K, k.M = a.M;
-  k.x = a.x, k.x_stride = a.x_stride, k.x_plane = a.x_plane;
+  k.x = static_cast<const uint16_t*>(a.x), k.x_stride = a.x_stride, k.x_plane = a.x_plane;
   k.bias = a.w->has_bias ? a.w->bias.as<float>() : nullptr;
   k.y = a.y, k.y_stride = a.y_stride, k.dtype = a.dtype, k.act = a.act;
   k.h = a.h, k.h_stride = a.h_stride, k.h_plane = a.h_plane, k.h_planes = a.h_planes;

@@ -228,14 +228,15 @@ namespace artlite {
 
 // ---- the dense products over few rows (linear.hip)
 
-// One launch: out[m][n] = sum_k x[m][k] W[n][k] (+ bias[n]) for M rows of A given as P planes of bf16 (x = the sum of its
-// planes), or with `up` set the gated products act(x W^T) (x U^T), written as planes of bf16 for the launch after.
+// One launch: out[m][n] = sum_k x[m][k] W[n][k] (+ bias[n]) for M rows of x given as planes of bf16 (x = the sum of its
+// planes) or, up to FEW_X32 of them, as fp32, or with `up` set the gated products act(x W^T) (x U^T), written as planes of bf16 for the launch after.
 struct FewArgs {
   const artlite_matrix *w, *up;
   int act;                  // (gated) artlite_act
-  const uint16_t* x;        // plane p of row m at x + p x_plane + m x_stride, 16-byte aligned rows
+  const void* x;            // plane p of row m at x + p x_plane + m x_stride (bf16), at any address
   int64_t x_stride, x_plane;
   int planes;               // 1, 2 or 3
+  bool x32;                 // x is fp32 (3 planes as it is used)
   int64_t M;
   void* y;                  // plain: bf16 or fp32 rows, y_stride values apart
   int64_t y_stride;
@@ -245,6 +246,7 @@ struct FewArgs {
   int h_planes;
   float* parts;             // scratch for sums in parts: few_parts_bytes of it
 };
+constexpr int FEW_X32 = 16;
 int launch_few(const FewArgs& a, hipStream_t s);
 size_t few_parts_bytes(const artlite_matrix* w, int planes, bool gated, int64_t M);
 // Rows past which the dense products go by way of 16-bit weights and the large tiles: one matrix's of bf16 rows (4096 x 4096,
@@ -259,8 +261,9 @@ int launch_planes(const void* x, int dtype, int64_t M, int64_t K, int64_t stride
 
 // W (or its transpose) as fp16 rows of ld values, times 2^-e (e: `wexp16`): plane 0, with planes 2 also what its rounding
 // left (at out + plane). Values past the matrix's columns (transposed: rows) up to ld are zeros.
-int launch_unpack(const artlite_matrix* m, bool transposed, int e, uint16_t* out, int64_t ld, int64_t plane, int planes,
-                  hipStream_t s);
+// m2: with a second matrix of the same shape and format, into out2.
+int launch_unpack(const artlite_matrix* m, const artlite_matrix* m2, bool transposed, int e, int e2, uint16_t* out,
+                  uint16_t* out2, int64_t ld, int64_t plane, int planes, hipStream_t s);
 // the scale that brings a matrix's largest value into [2^14, 2^15)
 inline int wexp16(const artlite_matrix* m) { return m->max_exp - 15; }
 

@@ -148,10 +148,20 @@ __global__ __launch_bounds__(256) void k_bounds(const uint8_t* __restrict__ w, i
   }
 }
 
+// one or two matrices of a launch: their blocks, where their values go, times 2^-e
+struct Unpack {
+  const uint8_t* w[2];
+  uint16_t* out[2];
+  int e[2];
+};
+
 // W as fp16 rows of ld values: a wave per unit of a tile; plane 1 (where there is one) what plane 0's rounding left
 template <int QT, int PLANES>
-__global__ __launch_bounds__(256) void k_unpack(const uint8_t* __restrict__ w, int units, int64_t all, int64_t N, int64_t K,
-                                                int e, uint16_t* __restrict__ out, int64_t ld, int64_t plane) {
+__global__ __launch_bounds__(256) void k_unpack(const Unpack two, int units, int64_t all, int64_t N, int64_t K, int64_t ld,
+                                                int64_t plane) {
+  const uint8_t* w = two.w[blockIdx.y];
+  uint16_t* out = two.out[blockIdx.y];
+  const int e = two.e[blockIdx.y];
   const int64_t i = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6), tile = i / units;
   const int u = int(i % units), lane = threadIdx.x & 63;
   const int64_t n = tile * TROWS + (lane & 15);
@@ -172,8 +182,11 @@ __global__ __launch_bounds__(256) void k_unpack(const uint8_t* __restrict__ w, i
 
 // W's transpose as fp16 rows of ld values: a workgroup per unit of 4 tiles (64 rows of W), a half at a time turned in LDS
 template <int QT, int PLANES>
-__global__ __launch_bounds__(256) void k_unpack_t(const uint8_t* __restrict__ w, int units, int64_t tiles, int64_t N,
-                                                  int64_t K, int e, uint16_t* __restrict__ out, int64_t ld, int64_t plane) {
+__global__ __launch_bounds__(256) void k_unpack_t(const Unpack two, int units, int64_t tiles, int64_t N, int64_t K,
+                                                  int64_t ld, int64_t plane) {
+  const uint8_t* w = two.w[blockIdx.y];
+  uint16_t* out = two.out[blockIdx.y];
+  const int e = two.e[blockIdx.y];
   constexpr int LD = 72;  // (a row's 64 values and 8 more: 16-byte rows, their banks spread)
   __shared__ __attribute__((aligned(16))) uint16_t t[PLANES][UNIT / 2][LD];
   const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63, lg = lane >> 4, lr = lane & 15;
@@ -211,20 +224,20 @@ __global__ __launch_bounds__(256) void k_unpack_t(const uint8_t* __restrict__ w,
 
 }  // namespace
 
-int launch_unpack(const artlite_matrix* m, bool transposed, int e, uint16_t* out, int64_t ld, int64_t plane, int planes,
-                  hipStream_t s) {
-  const uint8_t* w = m->w.as<uint8_t>();
+int launch_unpack(const artlite_matrix* m, const artlite_matrix* m2, bool transposed, int e, int e2, uint16_t* out,
+                  uint16_t* out2, int64_t ld, int64_t plane, int planes, hipStream_t s) {
+  const Unpack w{{m->w.as<uint8_t>(), m2 ? m2->w.as<uint8_t>() : nullptr}, {out, out2}, {e, e2}};
   const int64_t all = m->tiles * m->units;
-  const unsigned grid = unsigned(transposed ? (m->tiles + 3) / 4 * m->units : (all + 3) / 4);
+  const dim3 grid(unsigned(transposed ? (m->tiles + 3) / 4 * m->units : (all + 3) / 4), m2 ? 2 : 1);
 #define ART_U(QT)                                                                                          \
   if (transposed && planes == 1)                                                                           \
-    k_unpack_t<QT, 1><<<grid, 256, 0, s>>>(w, m->units, m->tiles, m->N, m->K, e, out, ld, plane);          \
+    k_unpack_t<QT, 1><<<grid, 256, 0, s>>>(w, m->units, m->tiles, m->N, m->K, ld, plane);          \
   else if (transposed)                                                                                     \
-    k_unpack_t<QT, 2><<<grid, 256, 0, s>>>(w, m->units, m->tiles, m->N, m->K, e, out, ld, plane);          \
+    k_unpack_t<QT, 2><<<grid, 256, 0, s>>>(w, m->units, m->tiles, m->N, m->K, ld, plane);          \
   else if (planes == 1)                                                                                    \
-    k_unpack<QT, 1><<<grid, 256, 0, s>>>(w, m->units, all, m->N, m->K, e, out, ld, plane);                 \
+    k_unpack<QT, 1><<<grid, 256, 0, s>>>(w, m->units, all, m->N, m->K, ld, plane);                 \
   else                                                                                                     \
-    k_unpack<QT, 2><<<grid, 256, 0, s>>>(w, m->units, all, m->N, m->K, e, out, ld, plane);                 \
+    k_unpack<QT, 2><<<grid, 256, 0, s>>>(w, m->units, all, m->N, m->K, ld, plane);                 \
   break
   ART_TILE_QTYPES(m->t->id, ART_U)
 #undef ART_U

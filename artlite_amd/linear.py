@@ -80,11 +80,13 @@ class QLinear:
         self._m.close()
         self._scratch.close()
 
-    def workspace_bytes(self, n: int, dtype: str = "bf16", aligned: bool = True) -> int:
-        """What a call of n rows needs (``aligned``: bf16 rows that start on 16 bytes)."""
+    def workspace_bytes(self, n: int, dtype: str = "bf16") -> int:
+        """What a call of n rows needs (0 for up to 16)."""
+        return self._need({"f32": 0, "bf16": 1}[dtype], n)
+
+    def _need(self, code: int, n: int) -> int:
         z = ctypes.c_size_t(0)
-        _hip.check(_hip.lib().artlite_linear_workspace(self._m.handle, {"f32": 0, "bf16": 1}[dtype], n, int(aligned),
-                                                       ctypes.byref(z)))
+        _hip.check(_hip.lib().artlite_linear_workspace(self._m.handle, code, n, ctypes.byref(z)))
         return z.value
 
     def __call__(self, x: object, out: object = None, *, stream: int = 0, work: Workspace | None = None) -> object:
@@ -106,10 +108,8 @@ class QLinear:
             raise _hip.Error("linear: out overlaps x")
         handle = self._m.handle
         w = work.handle if work is not None else None
-        lib = _hip.lib()
-        if work is None and (n > 16 or a.code == 0 or a.at % 16 or (n > 1 and a.row % 8)):
-            z = ctypes.c_size_t(0)
-            _hip.check(lib.artlite_linear_workspace(handle, a.code, n, 0, ctypes.byref(z)))
-            w = self._scratch.get(z.value).handle if z.value else None
-        _hip.check(lib.artlite_linear(handle, a.at, a.code, n, a.row, y.at, y.row, w, stream))
+        if work is None and n > 16:
+            need = self._need(a.code, n)
+            w = self._scratch.get(need).handle if need else None
+        _hip.check(_hip.lib().artlite_linear(handle, a.at, a.code, n, a.row, y.at, y.row, w, stream))
         return out

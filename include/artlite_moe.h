@@ -191,10 +191,11 @@ int artlite_workspace_create(size_t nbytes, artlite_workspace** out);
 int artlite_workspace_destroy(artlite_workspace* work); /* its calls have come to their end */
 
 /* y (n x rows) = x (n x cols) W^T (+ bias). x's products with the blocks' values are summed in fp32 and rounded once to y's
- * type (up to 64 rows without rounding a weight; past that weights are fp16 of 11 bits for bf16 x, of 22 for fp32 x).
- * artlite_linear_workspace: the bytes of workspace that such a call of n rows needs (aligned: x's rows start on 16 bytes and
- * cols are a multiple of 32 anyhow; 0: they may not); work may be null where that is 0. */
-int artlite_linear_workspace(const artlite_matrix* w, int dtype, int64_t n, int aligned, size_t* nbytes);
+ * type (up to 128 bf16 rows, or 64 fp32 ones, without rounding a weight; past that weights are fp16 of 11 bits for bf16 x, of
+ * 22 for fp32 x).
+ * artlite_linear_workspace: the bytes of workspace that a call of n rows needs (0 for up to 16 rows); work may be null where
+ * that is 0. */
+int artlite_linear_workspace(const artlite_matrix* w, int dtype, int64_t n, size_t* nbytes);
 int artlite_linear(const artlite_matrix* w, const void* x, int dtype, int64_t n, int64_t x_stride, void* y,
                    int64_t y_stride, artlite_workspace* work, void* stream);
 
