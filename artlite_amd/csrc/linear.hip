@@ -129,6 +129,21 @@ __device__ __forceinline__ void few_out(const FewK& a, int64_t m, int64_t n, flo
 constexpr int few_tiles(int nc, bool glu) { return nc == 2 ? (glu ? 2 : 4) : nc == 4 ? (glu ? 1 : 2) : 1; }
 constexpr int few_most(int planes, int nc, bool glu) { return nc == 1 && planes <= 2 && !glu ? 16 : 8; }
 
+// whether x goes by way of LDS: past 4 rows (1 row's operand loads take few cache accesses; 5 rows of 4096 x 4096 5.7 us as
+// operands, 5.0 through LDS), of fp32 past 8 (5 rows of 1536 x 2880 8.4 us as operands, 9.1 through LDS)
+constexpr bool few_stage(int ri, bool x32) { return ri > (x32 ? 2 : 1); }
+
+// x's slot of a wave: NC blocks of 16 rows, CG groups of them (8 KiB or so: registers hold the next chunk), by planes
+template <int P, int NC, bool X32>
+struct FewStage {
+  static constexpr int PL = X32 ? 1 : P, SIZE = X32 ? 128 : 64;  // (planes; bytes of a row's group in one)
+  static constexpr int CG = NC * PL * SIZE <= 64 ? 8 : NC * PL * SIZE <= 128 ? 4 : NC * PL * SIZE <= 384 ? 2 : 1;
+  static constexpr int PIECES = CG * SIZE / 16;                  // (of a row in a plane)
+  static constexpr int PLANE = NC * 16 * CG * SIZE, BYTES = PL * PLANE, LOADS = BYTES / 1024;
+  static_assert(PIECES % 4 == 0 && 64 % PIECES == 0, "pieces");
+  __device__ static int turn(int r) { return PIECES >= 8 ? r & 7 : (r >> 1) & 3; }
+};
+
 // P planes of x, NC blocks of 16 rows, RI rows of a block a lane: block row 4 g + i is x's row g + 4 i, so that up to 4 rows
 // are in each lane's first sum (RI 1) and up to 8 in its first two, and the others take no scaling. The units in gridDim.z
 // parts (PART: their sums into a.parts, for k_few_join). X32: x is fp32, split into its planes as it is used.
@@ -139,9 +154,11 @@ __global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a)
   constexpr float CC = KIND < 0 ? (QT == ARTLITE_Q4_0 ? -136.0f : -128.0f) : -1.0f;
   constexpr uint32_t CB = bf16_of(int(CC)) * 0x10001u;
   // groups whose x is in flight, whether the next unit's codes are (registers)
-  constexpr int XD = X32 ? 2 : P * NC == 1 ? (GLU ? 4 : 8) : P * NC <= 2 ? 4 : 2;
+  constexpr int XD = X32 ? 2 : P > 1 || GLU ? 4 : 8;
   constexpr bool AHEAD = NC == 1;
-  extern __shared__ float red[];  // [wave][tile of a matrix][block][row][lane]
+  using S = FewStage<P, NC, X32>;
+  constexpr bool STAGE = few_stage(RI, X32);
+  extern __shared__ __attribute__((aligned(16))) float red[];  // x's slots; then [wave][tile of a matrix][block][row][lane]
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6,
             lg = lane >> 4, lr = lane & 15;
   const int64_t t0 = int64_t(blockIdx.x) * TB, m0 = int64_t(blockIdx.y) * (16 * NC);
@@ -151,14 +168,12 @@ __global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a)
 #pragma unroll
   for (int b = 0; b < RB; b++)
     wp[b] = (GLU && b >= TB ? a.up : a.w) + min(t0 + b % TB, a.tiles - 1) * a.units * UB;
-  const uint16_t* xp[NC];
-  bool live[NC];
-#pragma unroll
-  for (int c = 0; c < NC; c++) {
-    const int64_t m = m0 + 16 * c + (lr >> 2) + 4 * (lr & 3);
-    live[c] = m < a.M;
-    xp[c] = a.x + ((live[c] ? m : 0) * a.x_stride + 8 * lg) * (X32 ? 2 : 1);
-  }
+  // rows that there are not take row 0: each row of the products is its own
+  constexpr int XE = X32 ? 4 : 2, PL = X32 ? 1 : P;  // (bytes of a value of x; its planes in memory)
+  const auto xrow = [&](int r) __attribute__((always_inline)) {  // (row r of the NC blocks)
+    const int64_t m = m0 + 16 * (r >> 4) + ((r & 15) >> 2) + 4 * (r & 3);
+    return reinterpret_cast<const uint8_t*>(a.x) + (m < a.M ? m : 0) * a.x_stride * XE;
+  };
   float acc[RB][NC][RI];
 #pragma unroll
   for (int b = 0; b < RB; b++)
@@ -178,35 +193,50 @@ __global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a)
       hd[b].load(p + 2048 + hdr_bytes<QT>() * lr);
     }
   };
-  // x of a group; past the last group of K the last one's (the scales there are 0). Rows that there are not take row 0, or with
-  // three planes keep what the registers hold: each row of the products is its own. (Loading only the rows there are took 1 row
-  // of 4096 x 4096 from 4.3 to 5.0 us, 16 rows from 6.8 to 10.8; but 5 rows in three planes, 1536 x 2880, from 6.7 to 6.3.)
+  // Up to 4 rows: x of a group as its operand, loaded so. Past the last group of K the last one's (the scales there are 0).
   constexpr int XP = X32 ? 2 : P;  // (a group's loads: its planes, or 8 fp32 values in two)
-  u32x4 x[XD][NC][XP];
-#pragma unroll
-  for (int j = 0; j < XD; j++)
-#pragma unroll
-    for (int c = 0; c < NC; c++)
-#pragma unroll
-      for (int p = 0; p < XP; p++) x[j][c][p] = u32x4{0, 0, 0, 0};
+  u32x4 x[STAGE ? 1 : XD][XP];
+  const uint8_t* const xd = xrow(lr) + 8 * XE * lg;
   const int klast = int(a.K) - 32;
   auto load_x = [&](int j, int u, int g) __attribute__((always_inline)) {
-    const int k = min(u * UNIT + 32 * g, klast);
+    const int64_t k = min(u * UNIT + 32 * g, klast);
 #pragma unroll
-    for (int c = 0; c < NC; c++)
-      if (!X32 || live[c])
+    for (int p = 0; p < XP; p++)  // (at any address: rows need not be aligned)
+      __builtin_memcpy(&x[j][p], xd + (X32 ? 4 * k + 16 * p : 2 * (p * a.x_plane + k)), 16);
+  };
+  // More rows: x a chunk of CG groups at a time by way of the wave's own slot in LDS, in lines' order (an operand's own order
+  // has 16 rows in a quarter of a wave: 64 cache accesses a load against 16, which bound 77 rows of 4096 x 4096 at 13 of 21
+  // us), the next chunk's loads in flight while one is used. 16-byte pieces swizzled by row.
+  uint8_t* const slot = reinterpret_cast<uint8_t*>(red) + wv * S::BYTES;
+  u32x4 st[STAGE ? S::LOADS : 1];
+  const uint8_t* sp[STAGE ? S::LOADS : 1];
+  uint32_t sk = 0, sl[STAGE ? S::LOADS : 1];
+  if constexpr (STAGE) {
 #pragma unroll
-        for (int p = 0; p < XP; p++)  // (at any address: rows need not be aligned)
-          __builtin_memcpy(&x[j][c][p], X32 ? xp[c] + 2 * k + 8 * p : xp[c] + p * a.x_plane + k, 16);
+    for (int i = 0; i < S::LOADS; i++) {
+      const int q = (i % (S::LOADS / PL)) * 64 + lane, r = q / S::PIECES, c = q % S::PIECES;
+      sp[i] = xrow(r) + 2 * int64_t(X32 ? 0 : i / (S::LOADS / PL)) * a.x_plane;
+      sl[i] = (i / (S::LOADS / PL)) * S::PLANE + r * (16 * S::PIECES) + ((c ^ S::turn(r)) << 4);
+      sk = 16 * c;  // (the same of every load: 64 is a multiple of PIECES)
+    }
+  }
+  auto load_chunk = [&](int u, int g) __attribute__((always_inline)) {
+    const int64_t at = min(int64_t(u * UNIT + 32 * g) * XE + sk, a.K * XE - 16);
+#pragma unroll
+    for (int i = 0; i < S::LOADS; i++) __builtin_memcpy(&st[i], sp[i] + at, 16);
   };
   if (first + wv < end) {
     if (AHEAD) load(first + wv);
+    if constexpr (STAGE) {
+      load_chunk(first + wv, 0);
+    } else {
 #pragma unroll
-    for (int g = 0; g < XD; g++) load_x(g, first + wv, g);
+      for (int g = 0; g < XD; g++) load_x(g, first + wv, g);
+    }
   }
   for (int u = first + wv; u < end; u += W) {
     const bool more = u + W < end;
-    const int un = more ? u + W : u;
+    const int un = more ? u + W : u;  // (past the last unit x's loads are its own again, unread)
     uint4 cur[RB][2];
     TileHdr<QT> hc[RB];
     if (!AHEAD) load(u);
@@ -226,13 +256,31 @@ __global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a)
         const int g = 4 * H + j;
         const u32x4 cst{CB, CB, CB, CB};
         u32x4 xo[NC][P];
+        if constexpr (STAGE) {
+          if (g % S::CG == 0) {  // (the chunk's loads to the slot; the next chunk's go out)
 #pragma unroll
-        for (int c = 0; c < NC; c++)
-          if constexpr (X32)
-            split3(x[g % XD][c][0], x[g % XD][c][XP - 1], xo[c][0], xo[c][P > 1 ? 1 : 0], xo[c][P - 1]);
-          else
+            for (int i = 0; i < S::LOADS; i++) *reinterpret_cast<u32x4*>(slot + sl[i]) = st[i];
+            load_chunk(g + S::CG < 8 ? u : un, (g + S::CG) % 8);
+          }
 #pragma unroll
-            for (int p = 0; p < P; p++) xo[c][p] = x[g % XD][c][p];
+          for (int c = 0; c < NC; c++) {
+            const uint8_t* r = slot + (16 * c + lr) * (16 * S::PIECES);
+            const int piece = (g % S::CG) * (X32 ? 8 : 4);
+            if constexpr (X32)
+              split3(*reinterpret_cast<const u32x4*>(r + (((piece + 2 * lg) ^ S::turn(lr)) << 4)),
+                     *reinterpret_cast<const u32x4*>(r + (((piece + 2 * lg + 1) ^ S::turn(lr)) << 4)), xo[c][0],
+                     xo[c][P > 1 ? 1 : 0], xo[c][P - 1]);
+            else
+#pragma unroll
+              for (int p = 0; p < P; p++)
+                xo[c][p] = *reinterpret_cast<const u32x4*>(r + p * S::PLANE + (((piece + lg) ^ S::turn(lr)) << 4));
+          }
+        } else if constexpr (X32) {
+          split3(x[g % XD][0], x[g % XD][XP - 1], xo[0][0], xo[0][P > 1 ? 1 : 0], xo[0][P - 1]);
+        } else {
+#pragma unroll
+          for (int p = 0; p < P; p++) xo[0][p] = x[g % XD][p];
+        }
         f32x4 cin[NC];
 #pragma unroll
         for (int c = 0; c < NC; c++) {
@@ -258,8 +306,7 @@ __global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a)
             }
           }
         }
-        // (past the last unit: its own again, unread)
-        load_x(g % XD, g + XD < 8 ? u : un, (g + XD) % 8);
+        if constexpr (!STAGE) load_x(g % XD, g + XD < 8 ? u : un, (g + XD) % 8);
         if (P * NC > 1) __builtin_amdgcn_sched_barrier(0);  // (the groups' sums in turn: registers)
       }
     };
@@ -267,6 +314,7 @@ __global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a)
     half(std::integral_constant<int, 1>{});
   }
   constexpr int ACC = NC * RI;
+  if constexpr (STAGE) __syncthreads();  // (the slots' place)
 #pragma unroll
   for (int b = 0; b < RB; b++)
 #pragma unroll
@@ -320,9 +368,10 @@ __global__ __launch_bounds__(256) void k_planes(const void* __restrict__ x, int 
 }
 
 // How a product is shared out: the units of K in `parts` workgroups (where the groups of tiles leave half the CUs idle and a
-// part has 4 units at least: 32 rows of 4096 x 4096, 64 groups, 14.9 us in one part, 12.6 in 4, 15.7 in 8; of 128 groups 20.1
-// in one, 16.0 in 2), a part's units among `waves` waves, 16 of them where the workgroups leave the device's waves few, 4 where
-// they are enough, each with the same number of units but for the last.
+// part has 4 units at least: 32 rows of 4096 x 4096, 64 groups, 13.8 us in one part, 12.8 in 4; 64 rows, 128 groups, 14.6 in
+// one, 13.3 in 2; 77 rows, 256 groups, 14.8 in one, 21.2 in 2), a part's units among `waves` waves, up to 16 of them where the workgroups leave the device's waves few (16 rows
+// of 4096 x 4096 in 16: 5.5 us, in 8 6.2; of 8192 x 4096 10.4 and 9.4), 4 where they are enough, each with the same number of
+// units but for the last.
 struct FewCut {
   int64_t groups, blocks;
   int parts, waves;
@@ -334,7 +383,7 @@ FewCut few_cut(int64_t tiles, int units, int64_t M, int planes, bool glu) {
   if (nc > 1)
     while (wgs * c.parts * 2 <= 256 && units / (2 * c.parts) >= 4) c.parts *= 2;
   const int own = (units + c.parts - 1) / c.parts;
-  while (c.waves < most && wgs * c.parts * c.waves < 8192) c.waves *= 2;
+  while (c.waves < most && wgs * c.parts * c.waves < (nc > 1 ? 2048 : 4096)) c.waves *= 2;
   const int each = (own + c.waves - 1) / c.waves;
   c.waves = (own + each - 1) / each;
   return c;
@@ -342,11 +391,16 @@ FewCut few_cut(int64_t tiles, int units, int64_t M, int planes, bool glu) {
 
 template <int QT, int P, int NC, int RI, bool GLU, bool X32>
 int launch_few_t(const FewK& k, hipStream_t s) {
-  constexpr int LDS = few_most(P, NC, GLU) * (GLU ? 2 : 1) * few_tiles(NC, GLU) * NC * RI * WAVE * 4;
-  static_assert(LDS <= 64 * 1024, "LDS");
+  constexpr int RED = (GLU ? 2 : 1) * few_tiles(NC, GLU) * NC * RI * WAVE * 4, SLOT = few_stage(RI, X32) ? FewStage<P, NC, X32>::BYTES : 0;
+  constexpr int WAVE_LDS = RED > SLOT ? RED : SLOT, LDS = few_most(P, NC, GLU) * WAVE_LDS;
+  static_assert(LDS <= LDS_BYTES, "LDS");
   const FewCut c = few_cut(k.tiles, k.units, k.M, P, GLU);
-  const size_t lds = size_t(c.waves) * (GLU ? 2 : 1) * few_tiles(NC, GLU) * NC * RI * WAVE * 4;
+  const size_t lds = size_t(c.waves) * WAVE_LDS;
   const dim3 grid(unsigned(c.groups), unsigned(c.blocks), unsigned(c.parts));
+  const auto set = [](const void* f) { return hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) == hipSuccess; };
+  static const bool ok = set(reinterpret_cast<const void*>(k_few<QT, P, NC, RI, GLU, false, X32>)) &&
+                         (NC == 1 || set(reinterpret_cast<const void*>(k_few<QT, P, NC, RI, GLU, NC != 1, X32>)));
+  if (!ok) return fail(ARTLITE_EHIP, "dense rows: kernel set-up failed");
   if (NC > 1 && c.parts > 1) {
     if (!k.parts) return fail(ARTLITE_EINVAL, "dense rows: no scratch for parts");
     if constexpr (NC > 1) k_few<QT, P, NC, RI, GLU, true, X32><<<grid, 64 * c.waves, lds, s>>>(k);

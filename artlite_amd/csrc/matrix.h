@@ -249,10 +249,11 @@ struct FewArgs {
 constexpr int FEW_X32 = 16;
 int launch_few(const FewArgs& a, hipStream_t s);
 size_t few_parts_bytes(const artlite_matrix* w, int planes, bool gated, int64_t M);
-// Rows past which the dense products go by way of 16-bit weights and the large tiles: one matrix's of bf16 rows (4096 x 4096,
-// 128 rows: 22 us against 43; 256: 41 against 45; 12288 x 2048, 129 rows: 49 against 47), of fp32 rows (65 rows: 61 against
-// 54), the gated block's (2880 x 7680, 65 rows: 113 against 96)
-constexpr int FEW_ROWS = 128, FEW_ROWS_F32 = 64, FEW_ROWS_FFN = 64;
+// Rows past which the dense products go by way of 16-bit weights and the large tiles. One matrix's of bf16 rows: 4096 x 4096
+// Q4_K, 256 rows, 27 us against 40, 384 rows 40 against 45; 12288 x 2048 IQ4_XS, 256 rows, 37 against 46, 384 rows 54 against
+// 58, 512 rows 73 against 60. Of fp32 rows: 4096 x 4096, 128 rows, 45 against 55, 192 rows 68 against 62. The gated block's:
+// 2048 x 8192, 128 rows, 61 against 78, 192 rows 82 against 78.
+constexpr int FEW_ROWS = 256, FEW_ROWS_F32 = 128, FEW_ROWS_FFN = 128;
 // x (M rows of K values of dtype, stride apart) as planes of bf16 (1: bf16 as it is; 3: fp32), rows of Kp values (zeros past K)
 int launch_planes(const void* x, int dtype, int64_t M, int64_t K, int64_t stride, uint16_t* out, int64_t Kp, int64_t plane,
                   int planes, hipStream_t s);

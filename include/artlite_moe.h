@@ -191,7 +191,7 @@ int artlite_workspace_create(size_t nbytes, artlite_workspace** out);
 int artlite_workspace_destroy(artlite_workspace* work); /* its calls have come to their end */
 
 /* y (n x rows) = x (n x cols) W^T (+ bias). x's products with the blocks' values are summed in fp32 and rounded once to y's
- * type (up to 128 bf16 rows, or 64 fp32 ones, without rounding a weight; past that weights are fp16 of 11 bits for bf16 x, of
+ * type (up to 256 bf16 rows, or 128 fp32 ones, without rounding a weight; past that weights are fp16 of 11 bits for bf16 x, of
  * 22 for fp32 x).
  * artlite_linear_workspace: the bytes of workspace that a call of n rows needs (0 for up to 16 rows); work may be null where
  * that is 0. */

@@ -36,7 +36,7 @@ def linear_streams_and_graphs() -> None:
         assert (y.cpu().double() - want).norm() <= 2.0 ** -7 * want.norm()
 
     streams = [torch.cuda.Stream() for _ in range(3)]
-    xs = [torch.randn(125 + i, K, device="cuda").bfloat16() for i in range(12)]
+    xs = [torch.randn(253 + i, K, device="cuda").bfloat16() for i in range(12)]
     ys = [torch.empty(x.shape[0], N, device="cuda", dtype=torch.bfloat16) for x in xs]
     torch.cuda.synchronize()
     for i, (x, y) in enumerate(zip(xs, ys)):
@@ -45,7 +45,7 @@ def linear_streams_and_graphs() -> None:
     for x, y in zip(xs, ys):
         near(y, x)
     graphs = []
-    for M in (1, 100, 150):
+    for M in (1, 100, 300):
         x = torch.randn(M, K, device="cuda").bfloat16()
         y = torch.empty(M, N, device="cuda", dtype=torch.bfloat16)
         work = Workspace(max(1, lin.workspace_bytes(M, "bf16")))
@@ -86,7 +86,7 @@ def ffn_streams_and_graphs() -> None:
         return torch.randn(n, H, device="cuda").bfloat16()
 
     streams = [torch.cuda.Stream() for _ in range(3)]
-    xs = [rand(n) for n in (5, 100, 64, 70, 1, 33)]
+    xs = [rand(n) for n in (5, 150, 64, 129, 1, 33)]
     ys = [torch.empty_like(x) for x in xs]
     torch.cuda.synchronize()
     for i, (x, y) in enumerate(zip(xs, ys)):
@@ -95,7 +95,7 @@ def ffn_streams_and_graphs() -> None:
     for x, y in zip(xs, ys):
         near(y, dense.ffn("silu", host(x), *w), TOL)
     graphs = []
-    for n in (4, 90):
+    for n in (4, 150):
         x, dy = rand(n), rand(n)
         out = {"y": torch.empty_like(x), "dx": torch.empty_like(x),
                "dgate": torch.empty(F, H, device="cuda", dtype=torch.bfloat16)}

@@ -1,4 +1,4 @@
-"""``QLinear`` against 64-bit math in every format and on every path: few rows (bf16 1 to 128, fp32 1 to 64: one, two and four blocks of 16), the
+"""``QLinear`` against 64-bit math in every format and on every path: few rows (bf16 1 to 256, fp32 1 to 128: one, two and four blocks of 16), the
 large tiles past them (both sizes), widths of a single block, of partial units and of partial 64 values, odd numbers of
 outputs, rows at any stride and address; bias, zeros, infinities and NaN.
 
@@ -20,7 +20,7 @@ from .dense_helpers import Rows, check, encode, values
 
 pytestmark = pytest.mark.gpu
 
-FEW = {"bf16": 128, "f32": 64}
+FEW = {"bf16": 256, "f32": 128}
 TOL = {("bf16", True): 2.0 ** -8 + 2.0 ** -14, ("bf16", False): 2.0 ** -8 + 2.0 ** -10, ("f32", True): 4e-6,
        ("f32", False): 4e-6}
 
@@ -48,7 +48,7 @@ def test_rows_and_widths(q: str, dtype: str) -> None:
     for K in widths(q):
         for N in (1, 17, 100):
             lin, w, _ = make(q, N, K, 7 * N + K)
-            for M in (1, 4, 5, 8, 9, 16, 17, 33, 64, 65, 128, 129):
+            for M in (1, 4, 5, 8, 9, 16, 17, 33, 65, 128, 129, 256, 257):
                 x = x_rows(M, K, dtype, M + K)
                 check(lin(x), values(x) @ w.T, TOL[dtype, M <= FEW[dtype]], np.sqrt(values(x) ** 2 @ (w ** 2).T))
             lin.close()
@@ -79,7 +79,7 @@ def test_strides(at: int, pad: int, out_at: int, out_pad: int, dtype: str) -> No
     """Rows at any address and stride; what lies between and behind the output's rows stays."""
     N, K = 100, 160
     lin, w, _ = make("IQ4_NL", N, K, 2)
-    for M in (1, 3, 16, 70, 150):
+    for M in (1, 3, 16, 70, 300):
         data = x_rows(M, K, dtype, M)
         x = Rows(M, K, dtype, at=at, stride=K + pad, data=data)
         y = Rows(M, N, dtype, at=out_at, stride=N + out_pad)
@@ -91,7 +91,7 @@ def test_one_row_for_all() -> None:
     """A row stride of 0: every output row is the one input row's."""
     lin, w, _ = make("Q4_0", 40, 256, 2)
     data = x_rows(1, 256, "bf16", 1)
-    for M in (3, 80, 150):
+    for M in (3, 80, 300):
         x = Rows(1, 256, "bf16", data=data)
         x.shape, x.row = (M, 256), 0
         y = Rows(M, 40, "bf16")
@@ -99,7 +99,7 @@ def test_one_row_for_all() -> None:
         check(y.numpy(), np.repeat(values(data) @ w.T, M, 0), TOL["bf16", M <= FEW["bf16"]])
 
 
-@pytest.mark.parametrize("M", [4, 90, 150])
+@pytest.mark.parametrize("M", [4, 90, 300])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_values_out_of_the_ordinary(dtype: str, M: int) -> None:
     """Rows of zeros, of the type's smallest and largest sizes, with infinities and NaN: each row is its own, the others are
@@ -126,7 +126,7 @@ def test_values_out_of_the_ordinary(dtype: str, M: int) -> None:
 
 def test_zero_blocks_and_large_scales() -> None:
     """A matrix of zeros, and one whose scales are the largest fp16 ones, on both paths."""
-    for M in (3, 70, 150):
+    for M in (3, 70, 300):
         x = x_rows(M, 64, "bf16", M)
         lin = QLinear("Q4_0", 20, 64)
         lin.upload(np.zeros((20, 36), np.uint8))
@@ -143,7 +143,7 @@ def test_no_rows_and_repeats() -> None:
     """0 rows write nothing; the same call twice gives the same bits, on every path."""
     lin, _, _ = make("IQ4_XS", 100, 512, 3)
     assert lin(np.empty((0, 512), np.uint16)).shape == (0, 100)
-    for M in (1, 20, 64, 65, 128, 129, 300):
+    for M in (1, 20, 65, 128, 129, 300):
         for dtype in ("bf16", "f32"):
             x = x_rows(M, 512, dtype, M)
             assert np.array_equal(lin(x), lin(x))
@@ -151,21 +151,21 @@ def test_no_rows_and_repeats() -> None:
 
 def test_refusals() -> None:
     lin, _, _ = make("Q4_0", 64, 64, 3)
-    x, y = DeviceArray((140, 64), np.uint16), DeviceArray((140, 64), np.uint16)
+    x, y = DeviceArray((280, 64), np.uint16), DeviceArray((280, 64), np.uint16)
     with pytest.raises(_hip.Error, match="out overlaps x"):
         lin(x, x)
     with pytest.raises(_hip.Error, match="for 64 rows of 64 values"):
-        lin(x, DeviceArray((140, 64), np.float32))
+        lin(x, DeviceArray((280, 64), np.float32))
     with pytest.raises(_hip.Error, match="for 64 rows of 64 values"):
-        lin(x, DeviceArray((139, 64), np.uint16))
+        lin(x, DeviceArray((279, 64), np.uint16))
     with pytest.raises(_hip.Error, match="is no array"):
         lin(x)
     with pytest.raises(_hip.Error, match="a workspace of 1024 bytes, not"):
         lin(x, y, work=Workspace(1024))
 
     class Host:  # (an address that is the host's)
-        shape, dtype = (140, 64), np.dtype(np.uint16)
-        mem = np.zeros((140, 64), np.uint16)
+        shape, dtype = (280, 64), np.dtype(np.uint16)
+        mem = np.zeros((280, 64), np.uint16)
 
         def stride(self) -> tuple[int, int]:
             return 64, 1
