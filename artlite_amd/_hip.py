@@ -79,16 +79,18 @@ SIGNATURES = {
     "artlite_matrix_destroy": (_I, [_P]),
     "artlite_matrix_upload": (_I, [_P, _P, _Z]),
     "artlite_matrix_upload_bias": (_I, [_P, _P, _Z]),
-    "artlite_workspace_create": (_I, [_Z, ctypes.POINTER(_P)]),
+    "artlite_matrix_device": (_I, [_P, ctypes.POINTER(_I)]),
+    "artlite_workspace_create": (_I, [_I, _Z, _I, ctypes.POINTER(_P)]),
     "artlite_workspace_destroy": (_I, [_P]),
+    "artlite_stream_capturing": (_I, [_P, ctypes.POINTER(_I)]),
     "artlite_linear_workspace": (_I, [_P, _I, _I64, ctypes.POINTER(_Z)]),
     "artlite_linear": (_I, [_P, _P, _I, _I64, _I64, _P, _I64, _P, _P]),
     "artlite_ffn_workspace": (_I, [ctypes.POINTER(Ffn), _I, _I64, _I, ctypes.POINTER(_Z)]),
     "artlite_ffn_forward": (_I, [ctypes.POINTER(Ffn), _P, _I, _I64, _I64, _P, _I64, _P, _P]),
     "artlite_ffn_backward": (_I, [ctypes.POINTER(Ffn), _P, _I64, _P, _I64, _I, _I64, _P, _I64, _P, _P, _P, _P, _P]),
-    "artlite_device_alloc": (_I, [_Z, ctypes.POINTER(_P), ctypes.POINTER(_I)]),
+    "artlite_device_alloc": (_I, [ctypes.POINTER(_I), _Z, ctypes.POINTER(_P)]),
     "artlite_device_free": (_I, [_P]),
-    "artlite_device_copy": (_I, [_P, _P, _Z, _I]),
+    "artlite_device_copy": (_I, [_I, _P, _P, _Z, _I]),
 }
 
 _lib: ctypes.CDLL | None = None

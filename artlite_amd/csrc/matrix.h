@@ -169,7 +169,7 @@ struct Work {
   std::mutex mu;
   hipEvent_t done = nullptr;
   hipStream_t last = nullptr;
-  bool used = false;
+  bool used = false, eager = false;
 };
 // Around the launches of a call that uses a workspace: `begin` locks it, checks its size and orders the call behind the last
 // one; the destructor notes where the call ends. (Inside a stream capture nothing is ordered: a graph's replays and other

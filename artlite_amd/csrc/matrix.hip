@@ -275,7 +275,8 @@ int WorkScope::begin(Work* work, size_t need, hipStream_t stream, const char* wh
   s = stream;
   hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
   ART_HIP(hipStreamIsCapturing(stream, &st));
-  if (st != hipStreamCaptureStatusNone) return ARTLITE_OK;
+  if (st != hipStreamCaptureStatusNone)
+    return w->eager ? fail(ARTLITE_EINVAL, "%s: a captured call takes a workspace of its own", what) : ARTLITE_OK;
   if (w->used && w->last != stream) ART_HIP(hipStreamWaitEvent(stream, w->done, 0));
   note = true;
   return ARTLITE_OK;
@@ -391,15 +392,24 @@ extern "C" int artlite_matrix_upload_bias(artlite_matrix* m, const float* data, 
   return ARTLITE_OK;
 }
 
-extern "C" int artlite_workspace_create(size_t nbytes, artlite_workspace** out) {
+extern "C" int artlite_matrix_device(const artlite_matrix* m, int* device) {
+  if (!m || !device) return fail(ARTLITE_EINVAL, "matrix: null");
+  *device = m->device;
+  return ARTLITE_OK;
+}
+
+extern "C" int artlite_workspace_create(int device, size_t nbytes, int eager_only, artlite_workspace** out) {
   if (!out) return fail(ARTLITE_EINVAL, "workspace: null");
   *out = nullptr;
   HostCtx* c;
   ART_TRY(host_ctx(&c, false));
+  OnDevice on;
+  ART_TRY(on.set(device < 0 ? c->device : device));
   artlite_workspace* w = new (std::nothrow) artlite_workspace;
   if (!w) return fail(ARTLITE_ENOMEM, "workspace: no memory");
-  w->w.device = c->device;
+  w->w.device = device < 0 ? c->device : device;
   w->w.n = nbytes;
+  w->w.eager = eager_only != 0;
   hipError_t e = hipMalloc(reinterpret_cast<void**>(&w->w.p), nbytes ? nbytes : 256);
   if (e == hipSuccess) e = hipEventCreateWithFlags(&w->w.done, hipEventDisableTiming);
   if (e != hipSuccess) {
@@ -409,6 +419,14 @@ extern "C" int artlite_workspace_create(size_t nbytes, artlite_workspace** out) 
     return fail(ARTLITE_ENOMEM, "workspace of %zu bytes: %s", nbytes, hipGetErrorString(e));
   }
   *out = w;
+  return ARTLITE_OK;
+}
+
+extern "C" int artlite_stream_capturing(void* stream, int* out) {
+  if (!out) return fail(ARTLITE_EINVAL, "stream: null");
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  ART_HIP(hipStreamIsCapturing(static_cast<hipStream_t>(stream), &st));
+  *out = st != hipStreamCaptureStatusNone;
   return ARTLITE_OK;
 }
 
@@ -422,16 +440,18 @@ extern "C" int artlite_workspace_destroy(artlite_workspace* w) {
   return rc;
 }
 
-extern "C" int artlite_device_alloc(size_t nbytes, void** out, int* device) {
+extern "C" int artlite_device_alloc(int* device, size_t nbytes, void** out) {
   if (!out || !device) return fail(ARTLITE_EINVAL, "device memory: null");
   *out = nullptr;
   HostCtx* c;
   ART_TRY(host_ctx(&c, false));
+  OnDevice on;
+  if (*device < 0) *device = c->device;
+  ART_TRY(on.set(*device));
   if (hipMalloc(out, nbytes ? nbytes : 1) != hipSuccess) {
     (void)hipGetLastError();
     return fail(ARTLITE_ENOMEM, "device memory: %zu bytes", nbytes);
   }
-  *device = c->device;
   return ARTLITE_OK;
 }
 
@@ -440,9 +460,11 @@ extern "C" int artlite_device_free(void* p) {
   return ARTLITE_OK;
 }
 
-extern "C" int artlite_device_copy(void* dst, const void* src, size_t nbytes, int to_host) {
+extern "C" int artlite_device_copy(int device, void* dst, const void* src, size_t nbytes, int to_host) {
   if (!nbytes) return ARTLITE_OK;
   if (!dst || !src) return fail(ARTLITE_EINVAL, "device copy: null");
+  OnDevice on;
+  ART_TRY(on.set(device));
   // (behind everything queued on the device, whichever streams it is on)
   ART_HIP(hipDeviceSynchronize());
   ART_HIP(hipMemcpy(dst, src, nbytes, to_host ? hipMemcpyDeviceToHost : hipMemcpyHostToDevice));

@@ -34,22 +34,23 @@ def _code(dtype: object) -> int:
 
 
 class DeviceArray:
-    """(rows, values) in GPU memory, on the device that is current when it is made. dtype: ``float32``, or ``uint16`` for
-    bf16 bits."""
+    """(rows, values) in GPU memory, on a device (-1: the current one). dtype: ``float32``, or ``uint16`` for bf16 bits."""
 
-    def __init__(self, shape: tuple[int, int], dtype: object = np.float32):
+    def __init__(self, shape: tuple[int, int], dtype: object = np.float32, device: int = -1):
         self.dtype = np.dtype(dtype)
         _code(self.dtype)
         self.shape = (int(shape[0]), int(shape[1]))
         self._lib = _hip.lib()  # (close() may run when the module is gone)
-        p, dev = ctypes.c_void_p(), ctypes.c_int(0)
-        _hip.check(self._lib.artlite_device_alloc(self.nbytes, ctypes.byref(p), ctypes.byref(dev)))
+        p, dev = ctypes.c_void_p(), ctypes.c_int(device)
+        _hip.check(self._lib.artlite_device_alloc(ctypes.byref(dev), self.nbytes, ctypes.byref(p)))
         self._p, self.device = p, dev.value
 
     @classmethod
-    def of(cls, a: np.ndarray) -> "DeviceArray":
+    def of(cls, a: np.ndarray, device: int = -1) -> "DeviceArray":
         """A host array's copy."""
-        d = cls(a.shape, a.dtype)
+        if a.ndim != 2:
+            raise _hip.Error(f"DeviceArray: {a.shape}, not (rows, values)")
+        d = cls(a.shape, a.dtype, device)
         d.copy_from(a)
         return d
 
@@ -69,12 +70,12 @@ class DeviceArray:
         a = np.ascontiguousarray(a)
         if a.shape != self.shape or a.dtype != self.dtype:
             raise _hip.Error(f"DeviceArray: {a.dtype} {a.shape} into {self.dtype} {self.shape}")
-        _hip.check(_hip.lib().artlite_device_copy(self.data_ptr(), a.ctypes.data, a.nbytes, 0))
+        _hip.check(_hip.lib().artlite_device_copy(self.device, self.data_ptr(), a.ctypes.data, a.nbytes, 0))
 
     def numpy(self) -> np.ndarray:
         """A host copy, behind everything queued on the device."""
         a = np.empty(self.shape, self.dtype)
-        _hip.check(_hip.lib().artlite_device_copy(a.ctypes.data, self.data_ptr(), a.nbytes, 1))
+        _hip.check(_hip.lib().artlite_device_copy(self.device, a.ctypes.data, self.data_ptr(), a.nbytes, 1))
         return a
 
     def close(self) -> None:
@@ -87,13 +88,14 @@ class DeviceArray:
 
 
 class Workspace:
-    """Scratch memory of the operators' calls, of a fixed size, on the device that is current when it is made. Calls outside
-    a stream capture order themselves on it; graphs that run beside each other, or beside calls, take one each."""
+    """Scratch memory of the operators' calls, of a fixed size, on a device (-1: the current one). Calls outside a stream
+    capture order themselves on it; graphs that run beside each other, or beside calls, take one each. eager_only: calls
+    under capture are refused."""
 
-    def __init__(self, nbytes: int):
+    def __init__(self, nbytes: int, device: int = -1, *, eager_only: bool = False):
         self._lib = _hip.lib()  # (close() may run when the module is gone)
         h = ctypes.c_void_p()
-        _hip.check(self._lib.artlite_workspace_create(nbytes, ctypes.byref(h)))
+        _hip.check(self._lib.artlite_workspace_create(device, nbytes, int(eager_only), ctypes.byref(h)))
         self._h, self.nbytes = h, nbytes
 
     @property
@@ -111,24 +113,23 @@ class Workspace:
         self.close()
 
 
-class Scratch:
-    """An operator's own workspace, grown as its calls need more. A workspace that it outgrows is kept: a graph captured on
-    it may be replayed yet (each is at least twice the one before, so that all take at most twice the last)."""
+_shared: dict[int, list[Workspace]] = {}
+_shared_lock = threading.Lock()
 
-    def __init__(self) -> None:
-        self._all: list[Workspace] = []
-        self._lock = threading.Lock()
 
-    def get(self, nbytes: int) -> Workspace:
-        with self._lock:
-            if not self._all or self._all[-1].nbytes < nbytes:
-                self._all.append(Workspace(max(nbytes, 2 * self._all[-1].nbytes if self._all else 0)))
-            return self._all[-1]
-
-    def close(self) -> None:
-        for w in self._all:
-            w.close()
-        self._all = []
+def shared_workspace(device: int, nbytes: int, stream: object) -> Workspace:
+    """The workspace of a device's calls that are given none, grown as they need more (not while ``stream`` is captured: such
+    a call is refused). One that is outgrown stays until the process ends (a thread may be about to use it); each is at least
+    twice the one before."""
+    with _shared_lock:
+        all_ = _shared.setdefault(device, [])
+        if not all_ or all_[-1].nbytes < nbytes:
+            capturing = ctypes.c_int(0)
+            _hip.check(_hip.lib().artlite_stream_capturing(stream, ctypes.byref(capturing)))
+            if capturing.value:
+                raise _hip.Error("a captured call takes a workspace of its own")
+            all_.append(Workspace(max(nbytes, 2 * all_[-1].nbytes if all_ else 0), device, eager_only=True))
+        return all_[-1]
 
 
 class View:
@@ -148,11 +149,13 @@ class View:
             if len(shape) != 2:
                 raise _hip.Error(f"{what}: {tuple(shape)}, not (rows, values)")
             size = 4 if self.code == F32 else 2
-            strides = [s // size for s in d["strides"]] if d.get("strides") else (shape[1], 1)
+            strides = [s / size for s in d["strides"]] if d.get("strides") else (shape[1], 1)
         else:
             raise _hip.Error(f"{what}: {type(a).__name__} is no array of device memory")
         self.rows, self.cols = shape
-        self.row = strides[0]
+        self.row = int(strides[0])
+        if self.row != strides[0]:
+            raise _hip.Error(f"{what}: rows {strides[0]} values apart")
         if strides[1] != 1 and self.cols > 1:
             raise _hip.Error(f"{what}: a row's values are {strides[1]} apart")
 

@@ -7,7 +7,7 @@ import ctypes
 import numpy as np
 
 from . import _hip
-from .device import DeviceArray, Scratch, View, Workspace, overlap
+from .device import DeviceArray, View, Workspace, overlap, shared_workspace
 from .gguf_model import GGUFFile
 from .linear import FORMATS, Matrix
 
@@ -25,7 +25,6 @@ class GatedFFN:
         self._m = {"ffn_gate": Matrix(gate_type, ffn, hidden), "ffn_up": Matrix(gate_type, ffn, hidden),
                    "ffn_down": Matrix(down_type, hidden, ffn)}
         self._d = _hip.Ffn(*(m.handle.value for m in self._m.values()), ACTS[act])
-        self._scratch = Scratch()
 
     @classmethod
     def from_gguf(cls, gguf: GGUFFile, block: int, *, act: str = "silu") -> "GatedFFN":
@@ -54,7 +53,6 @@ class GatedFFN:
     def close(self) -> None:
         for m in self._m.values():
             m.close()
-        self._scratch.close()
 
     def workspace_bytes(self, n: int, dtype: str = "bf16", *, backward: bool = False, weights: bool = False) -> int:
         """What a call of n rows needs: forward, backward, or backward with the weights' gradients. (Not always less for fewer
@@ -71,10 +69,12 @@ class GatedFFN:
             m.handle  # (raises when closed)
         return self._d
 
-    def _work(self, work: Workspace | None, code: int, n: int, backward: int) -> object:
+    def _work(self, work: Workspace | None, code: int, n: int, backward: int, stream: object) -> object:
         if work is not None:
             return work.handle
-        return self._scratch.get(self._need(code, n, backward)).handle if n else None
+        if not n:
+            return None
+        return shared_workspace(self._m["ffn_gate"].device, self._need(code, n, backward), stream).handle
 
     def _views(self, what: str, shapes: dict[str, tuple[object, int, int]]) -> dict[str, View]:
         """The views of the arrays (array, rows, cols) that are given: all of one dtype, none of the written ones (all but
@@ -94,21 +94,21 @@ class GatedFFN:
 
     def __call__(self, x: object, out: object = None, *, stream: int = 0, work: Workspace | None = None) -> object:
         """x (n, hidden) -> out (n, hidden). Device arrays (``device``): enqueued on ``stream`` (a hipStream_t's address; 0:
-        the null stream), ``out`` given by the caller, ``work`` its workspace (none: the object's own). A numpy x (fp32, or
+        the null stream), ``out`` given by the caller, ``work`` its workspace (none: one that the device's calls
+        share, which a captured call may not use). A numpy x (fp32, or
         uint16 bf16 bits): the result as a numpy array."""
         if isinstance(x, np.ndarray):
             if out is not None:
                 raise _hip.Error("ffn: out goes with device arrays")
-            y = DeviceArray(x.shape, x.dtype)
-            self(DeviceArray.of(x), y, stream=stream, work=work)
-            return y.numpy()
+            d = DeviceArray.of(x, self._m["ffn_gate"].device)
+            return self(d, DeviceArray(d.shape, x.dtype, d.device), stream=stream, work=work).numpy()
         n = x.shape[0]
         v = self._views("ffn", {"x": (x, n, self.hidden), "out": (out, n, self.hidden)})
         if "out" not in v:
             raise _hip.Error("ffn: device arrays need out")
         a, y = v["x"], v["out"]
         _hip.check(_hip.lib().artlite_ffn_forward(ctypes.byref(self._open()), a.at, a.code, n, a.row, y.at, y.row,
-                                                  self._work(work, a.code, n, 0), stream))
+                                                  self._work(work, a.code, n, 0, stream), stream))
         return out
 
     def backward(self, x: object, dy: object, *, dx: object = None, dgate: object = None, dup: object = None,
@@ -120,8 +120,9 @@ class GatedFFN:
         outs = {"dx": (dx, n, H), "dgate": (dgate, F, H), "dup": (dup, F, H), "ddown": (ddown, H, F)}
         if isinstance(x, np.ndarray):
             host = {k: a for k, (a, _, _) in outs.items() if a is not None}
-            dev = {k: DeviceArray(a.shape, a.dtype) for k, a in host.items()}
-            self.backward(DeviceArray.of(x), DeviceArray.of(dy), **dev, stream=stream, work=work)
+            on = self._m["ffn_gate"].device
+            dev = {k: DeviceArray(a.shape, a.dtype, on) for k, a in host.items()}
+            self.backward(DeviceArray.of(x, on), DeviceArray.of(dy, on), **dev, stream=stream, work=work)
             for k, a in host.items():
                 a[...] = dev[k].numpy()
             return
@@ -136,4 +137,4 @@ class GatedFFN:
         at = [v[k].at if k in v else None for k in ("dgate", "dup", "ddown")]
         _hip.check(_hip.lib().artlite_ffn_backward(
             ctypes.byref(self._open()), a.at, a.row, d.at, d.row, a.code, n, o.at if o else None, o.row if o else 0, *at,
-            self._work(work, a.code, n, 2 if weights else 1), stream))
+            self._work(work, a.code, n, 2 if weights else 1, stream), stream))

@@ -7,7 +7,7 @@ import ctypes
 import numpy as np
 
 from . import _hip
-from .device import DeviceArray, Scratch, View, Workspace, overlap
+from .device import DeviceArray, View, Workspace, overlap, shared_workspace
 from .gguf_model import TYPE_ID, GGUFFile
 
 FORMATS = ("Q4_0", "Q4_1", "Q4_K", "IQ4_NL", "IQ4_XS")
@@ -22,6 +22,9 @@ class Matrix:
         h = ctypes.c_void_p()
         _hip.check(self._lib.artlite_matrix_create(TYPE_ID.get(qtype, -1), rows, cols, ctypes.byref(h)))
         self._h = h
+        d = ctypes.c_int(0)
+        _hip.check(self._lib.artlite_matrix_device(h, ctypes.byref(d)))
+        self.device = d.value
 
     @property
     def handle(self) -> ctypes.c_void_p:
@@ -53,7 +56,6 @@ class QLinear:
     def __init__(self, qtype: str, rows: int, cols: int):
         self.rows, self.cols = rows, cols
         self._m = Matrix(qtype, rows, cols)
-        self._scratch = Scratch()
 
     @classmethod
     def from_gguf(cls, gguf: GGUFFile, name: str, bias: str = "") -> "QLinear":
@@ -78,7 +80,6 @@ class QLinear:
 
     def close(self) -> None:
         self._m.close()
-        self._scratch.close()
 
     def workspace_bytes(self, n: int, dtype: str = "bf16") -> int:
         """What a call of n rows needs (0 for up to 16)."""
@@ -91,14 +92,14 @@ class QLinear:
 
     def __call__(self, x: object, out: object = None, *, stream: int = 0, work: Workspace | None = None) -> object:
         """x (n, cols) -> out (n, rows). Device arrays (``device``): enqueued on ``stream`` (a hipStream_t's address; 0: the
-        null stream), ``out`` given by the caller, ``work`` its workspace (none: the object's own). A numpy x (fp32, or
-        uint16 bf16 bits): the result as a numpy array."""
+        null stream), ``out`` given by the caller, ``work`` its workspace (none: one that the device's
+        calls share, which a captured call may not use; up to 16 rows need none). A numpy x (fp32, or uint16 bf16 bits): the
+        result as a numpy array."""
         if isinstance(x, np.ndarray):
             if out is not None:
                 raise _hip.Error("linear: out goes with device arrays")
-            y = DeviceArray((x.shape[0], self.rows), x.dtype)
-            self(DeviceArray.of(x), y, stream=stream, work=work)
-            return y.numpy()
+            d = DeviceArray.of(x, self._m.device)
+            return self(d, DeviceArray((d.shape[0], self.rows), x.dtype, d.device), stream=stream, work=work).numpy()
         a, y = View(x, "linear: x"), View(out, "linear: out")
         n = a.rows
         if a.cols != self.cols or y.rows != n or y.cols != self.rows or y.code != a.code:
@@ -110,6 +111,6 @@ class QLinear:
         w = work.handle if work is not None else None
         if work is None and n > 16:
             need = self._need(a.code, n)
-            w = self._scratch.get(need).handle if need else None
+            w = shared_workspace(self._m.device, need, stream).handle if need else None
         _hip.check(_hip.lib().artlite_linear(handle, a.at, a.code, n, a.row, y.at, y.row, w, stream))
         return out

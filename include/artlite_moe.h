@@ -185,9 +185,14 @@ int artlite_matrix_upload(artlite_matrix* m, const void* data, size_t nbytes);
 /* n = rows fp32 values added to every output row of artlite_linear; n = 0: none. */
 int artlite_matrix_upload_bias(artlite_matrix* m, const float* data, size_t n);
 
-/* Scratch memory of calls, of a fixed size. */
+int artlite_matrix_device(const artlite_matrix* m, int* device);
+
+/* Scratch memory of calls, of a fixed size, on a device (-1: the current one). eager_only: a call under stream capture that
+ * would use it is refused (for one that many callers share). A stream's calls have come to their end before it is destroyed.
+ * artlite_stream_capturing: whether a stream is being captured (memory is then not to be allocated). */
 typedef struct artlite_workspace artlite_workspace;
-int artlite_workspace_create(size_t nbytes, artlite_workspace** out);
+int artlite_workspace_create(int device, size_t nbytes, int eager_only, artlite_workspace** out);
+int artlite_stream_capturing(void* stream, int* out);
 int artlite_workspace_destroy(artlite_workspace* work); /* its calls have come to their end */
 
 /* y (n x rows) = x (n x cols) W^T (+ bias). x's products with the blocks' values are summed in fp32 and rounded once to y's
@@ -219,11 +224,11 @@ int artlite_ffn_backward(const artlite_ffn* f, const void* x, int64_t x_stride, 
                          int dtype, int64_t n, void* dx, int64_t dx_stride, void* dgate, void* dup, void* ddown,
                          artlite_workspace* work, void* stream);
 
-/* Device memory for callers that have no allocator of their own: allocated on the current device (*device), and copied to
- * (to_host 0) or from the host behind everything queued on the current device. */
-int artlite_device_alloc(size_t nbytes, void** out, int* device);
+/* Device memory for callers that have no allocator of their own: allocated on *device (-1: the current one, which it becomes),
+ * and copied to (to_host 0) or from the host behind everything queued on the device. */
+int artlite_device_alloc(int* device, size_t nbytes, void** out);
 int artlite_device_free(void* p);
-int artlite_device_copy(void* dst, const void* src, size_t nbytes, int to_host);
+int artlite_device_copy(int device, void* dst, const void* src, size_t nbytes, int to_host);
 
 #ifdef __cplusplus
 }

@@ -11,12 +11,23 @@ import torch
 
 sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 
+from artlite_amd import _hip  # noqa: E402
 from artlite_amd.device import Workspace  # noqa: E402
 from artlite_amd.ffn import GatedFFN  # noqa: E402
 from artlite_amd.linear import QLinear  # noqa: E402
 from oracle import dense  # noqa: E402
 
 TOL = 2.0 ** -8 + 8 * 2.0 ** -11
+
+
+def refused(call: object) -> None:
+    """A captured call on the workspace that a device's calls share (there already, or to be grown)."""
+    try:
+        call()
+    except _hip.Error as e:
+        assert "a captured call takes a workspace of its own" in str(e), e
+    else:
+        raise AssertionError("captured")
 
 
 def linear_streams_and_graphs() -> None:
@@ -45,6 +56,7 @@ def linear_streams_and_graphs() -> None:
     for x, y in zip(xs, ys):
         near(y, x)
     graphs = []
+    wide, out = (torch.empty(50000, c, device="cuda", dtype=torch.bfloat16) for c in (K, N))
     for M in (1, 100, 300):
         x = torch.randn(M, K, device="cuda").bfloat16()
         y = torch.empty(M, N, device="cuda", dtype=torch.bfloat16)
@@ -52,7 +64,11 @@ def linear_streams_and_graphs() -> None:
         torch.cuda.synchronize()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
-            lin(x, y, stream=torch.cuda.current_stream().cuda_stream, work=work)
+            s = torch.cuda.current_stream().cuda_stream
+            if lin.workspace_bytes(M, "bf16"):  # (nothing has been queued or allocated: the capture goes on)
+                refused(lambda: lin(x, y, stream=s))
+                refused(lambda: lin(wide, out, stream=s))
+            lin(x, y, stream=s, work=work)
         graphs.append((g, x, y, work))
     for _ in range(3):
         for g, x, y, _ in graphs:

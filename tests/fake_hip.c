@@ -28,6 +28,19 @@ static int map(void** p, size_t n) {
 
 int hipGetDeviceCount(int* n) { return *n = 1, OK; }
 int hipGetDevice(int* d) { return *d = 0, OK; }
+int hipSetDevice(int d) { return d ? INVALID : OK; }
+int hipDeviceSynchronize(void) {
+  for (int i = 0; i < 64; i++) pending_of[i] = 0;
+  return fake_pending = 0, OK;
+}
+int fake_host_pointers, fake_capturing; /* switches: pointers are the host's; streams are being captured */
+int hipPointerGetAttributes(int* a, const void* p) {  /* (the type and the device, the first two fields) */
+  return (void)p, a[0] = fake_host_pointers ? 1 : 2, a[1] = 0, OK;
+}
+int hipStreamIsCapturing(stream_t s, int* st) { return (void)s, *st = fake_capturing, OK; }
+int hipEventCreateWithFlags(void** e, unsigned flags) { return (void)flags, *e = NULL, OK; }
+int fake_waits; /* streams made to wait for an event */
+int hipStreamWaitEvent(stream_t s, void* e, unsigned flags) { return (void)s, (void)e, (void)flags, fake_waits++, OK; }
 int hipDeviceGetAttribute(int* v, int attr, int dev) { return (void)attr, (void)dev, *v = 256, OK; }
 int hipFuncSetAttribute(const void* f, int attr, int v) { return (void)f, (void)attr, (void)v, OK; }
 int hipOccupancyMaxActiveBlocksPerMultiprocessor(int* n, const void* f, int threads, size_t lds) {
