@@ -206,10 +206,12 @@ struct LinearPlan {
 };
 LinearPlan linear_plan(Carve& c, const artlite_matrix* w, int dtype, int64_t n) {
   LinearPlan p;
-  p.few = n <= (dtype == ARTLITE_X_BF16 ? FEW_ROWS : FEW_ROWS_F32);
+  const int few_pl = dtype == ARTLITE_X_BF16 ? 1 : 3;
+  const bool apart = few_apart(w, few_pl, false, n);
+  p.few = apart || n <= (dtype == ARTLITE_X_BF16 ? FEW_ROWS : FEW_ROWS_F32);
   if (p.few) {
-    const int pl = dtype == ARTLITE_X_BF16 ? 1 : 3;
-    if (pl == 3 && n > FEW_X32) p.planes = c.take<uint16_t>(3 * size_t(n) * w->K);
+    const int pl = few_pl;
+    if (pl == 3 && !apart) p.planes = c.take<uint16_t>(3 * size_t(n) * w->K);
     p.parts = c.take<float>(few_parts_bytes(w, pl, false, n) / 4);
   } else {
     const int pl = dtype == ARTLITE_X_BF16 ? 1 : 2;
@@ -245,7 +247,7 @@ int check_array(const void* p, int64_t n, int64_t cols, int64_t stride, bool wri
   return check_device(p, device, what);
 }
 
-// x as a launch over few rows takes it: bf16 and up to FEW_X32 fp32 rows as they are, more fp32 rows as planes
+// x as a launch over few rows takes it: bf16 as it is, fp32 too where the blocks of rows are apart, else as planes
 int few_x(FewArgs& a, const void* x, int dtype, int64_t n, int64_t K, int64_t stride, uint16_t* planes, hipStream_t s) {
   a.planes = dtype == ARTLITE_X_BF16 ? 1 : 3;
   a.x32 = dtype == ARTLITE_X_F32 && !planes;
@@ -319,10 +321,10 @@ struct FfnPlan {
 };
 FfnPlan ffn_plan(Carve& c, const Ffn& f, int dtype, int64_t n) {
   FfnPlan p{};
-  p.few = n <= FEW_ROWS_FFN;
-  const bool b = dtype == ARTLITE_X_BF16;
+  const bool b = dtype == ARTLITE_X_BF16, apart = few_apart(f.gate, b ? 1 : 3, true, n);
+  p.few = n <= FEW_ROWS_FFN || (apart && few_apart(f.down, b ? 2 : 3, false, n));
   if (p.few) {
-    if (!b && n > FEW_X32) p.planes = c.take<uint16_t>(3 * size_t(n) * f.H);
+    if (!b && !apart) p.planes = c.take<uint16_t>(3 * size_t(n) * f.H);
     p.hp = c.take<uint16_t>(size_t(b ? 2 : 3) * n * f.F);
     p.parts = c.take<float>(std::max(few_parts_bytes(f.gate, b ? 1 : 3, true, n), few_parts_bytes(f.down, b ? 2 : 3, false, n)) / 4);
     return p;

@@ -457,9 +457,9 @@ Cut best_cut(int64_t M, int64_t cols, int64_t K, int segs, bool mixed) {
 template <int MB, int EPI, bool PART>
 int launch_t(const HGemm& g, int64_t gn, int parts, hipStream_t s) {
   using T = HT<MB>;
-  static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(k_hgemm<MB, EPI, PART>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS) == hipSuccess;
-  if (!ok) return fail(ARTLITE_EHIP, "large tiles: kernel set-up failed");
+  static DeviceOnce set;
+  if (!set.lds(reinterpret_cast<const void*>(k_hgemm<MB, EPI, PART>), T::LDS))
+    return fail(ARTLITE_EHIP, "large tiles: kernel set-up failed");
   const int64_t gm = (g.M + T::TM - 1) / T::TM;
   if (gm * gn > (int64_t(1) << 30)) return fail(ARTLITE_EINVAL, "large tiles: %lld tiles", (long long)(gm * gn));
   k_hgemm<MB, EPI, PART><<<dim3(unsigned(gm * gn), unsigned(parts)), 256, T::LDS, s>>>(g, int(gm), int(gn));

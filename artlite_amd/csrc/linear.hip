@@ -51,12 +51,16 @@ __device__ __forceinline__ void lut_bytes(uint32_t c, uint32_t& lo, uint32_t& hi
   hi = (__builtin_amdgcn_perm(T.hi[3], T.hi[2], s) & m) | (__builtin_amdgcn_perm(T.hi[1], T.hi[0], s) & ~m);
 }
 
+// the constants of a code dword's operand in registers: an and-or takes them so, literals make it two instructions
+struct Nibbles {
+  uint32_t mask = 0x000F000Fu, top = 0x43004300u;
+  __device__ __forceinline__ Nibbles() { asm("" : "+s"(mask), "+v"(top)); }
+};
 // the operand of a code dword: 128 + c, or by table the codes' own values
 template <int KIND>
-__device__ __forceinline__ u32x4 operand(uint32_t w) {
+__device__ __forceinline__ u32x4 operand(uint32_t w, const Nibbles& n) {
   if constexpr (KIND < 0) {
-    return u32x4{(w & 0x000F000Fu) | 0x43004300u, ((w >> 4) & 0x000F000Fu) | 0x43004300u,
-                 ((w >> 8) & 0x000F000Fu) | 0x43004300u, ((w >> 12) & 0x000F000Fu) | 0x43004300u};
+    return u32x4{(w & n.mask) | n.top, ((w >> 4) & n.mask) | n.top, ((w >> 8) & n.mask) | n.top, ((w >> 12) & n.mask) | n.top};
   } else {
     uint32_t l0, h0, l1, h1;  // (nibbles 0, 2, 4, 6 and 1, 3, 5, 7)
     lut_bytes<KIND>(w & 0x0F0F0F0Fu, l0, h0);
@@ -110,17 +114,19 @@ __device__ __forceinline__ void split3(const u32x4& a, const u32x4& b, u32x4& hi
   }
 }
 
+__device__ __forceinline__ void store_row(const FewK& a, int64_t m, int64_t n, float v) {
+  if (a.dtype == ARTLITE_X_BF16)
+    static_cast<uint16_t*>(a.y)[m * a.y_stride + n] = uint16_t(f32_to_bf16(v));
+  else
+    static_cast<float*>(a.y)[m * a.y_stride + n] = v;
+}
 // an output of row m, column n from its sum (gated: and the second matrix's)
 template <bool GLU>
 __device__ __forceinline__ void few_out(const FewK& a, int64_t m, int64_t n, float s, float u) {
   if constexpr (GLU) {
     store_planes(a.h + m * a.h_stride + n, a.h_plane, a.h_planes, gate_act(a.act, s) * u);
   } else {
-    const float v = s + (a.bias ? a.bias[n] : 0.0f);
-    if (a.dtype == ARTLITE_X_BF16)
-      static_cast<uint16_t*>(a.y)[m * a.y_stride + n] = uint16_t(f32_to_bf16(v));
-    else
-      static_cast<float*>(a.y)[m * a.y_stride + n] = v;
+    store_row(a, m, n, s + (a.bias ? a.bias[n] : 0.0f));
   }
 }
 
@@ -153,6 +159,8 @@ __global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a)
   constexpr bool CIN = KIND < 0 || has_offset<QT>;  // (sum(x) times a constant is wanted)
   constexpr float CC = KIND < 0 ? (QT == ARTLITE_Q4_0 ? -136.0f : -128.0f) : -1.0f;
   constexpr uint32_t CB = bf16_of(int(CC)) * 0x10001u;
+  constexpr float OM = KIND < 0 ? 1.0f / 128.0f : 1.0f;
+  const Nibbles nib;
   // groups whose x is in flight, whether the next unit's codes are (registers)
   constexpr int XD = X32 ? 2 : P > 1 || GLU ? 4 : 8;
   constexpr bool AHEAD = NC == 1;
@@ -250,7 +258,7 @@ __global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a)
       constexpr int H = decltype(hv)::value;
       float s[RB][4], o[RB][4];
 #pragma unroll
-      for (int b = 0; b < RB; b++) hc[b].template fields<H>(s[b], o[b]);
+      for (int b = 0; b < RB; b++) hc[b].template fields<H>(s[b], o[b], OM);
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         const int g = 4 * H + j;
@@ -292,7 +300,7 @@ __global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a)
 #pragma unroll
         for (int b = 0; b < RB; b++) {
           const uint4& cc = cur[b][H];
-          const u32x4 q = operand<KIND>(j == 0 ? cc.x : j == 1 ? cc.y : j == 2 ? cc.z : cc.w);
+          const u32x4 q = operand<KIND>(j == 0 ? cc.x : j == 1 ? cc.y : j == 2 ? cc.z : cc.w, nib);
 #pragma unroll
           for (int c = 0; c < NC; c++) {
             f32x4 d = KIND < 0 ? cin[c] : f32x4{0, 0, 0, 0};
@@ -302,7 +310,7 @@ __global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a)
             for (int i = 0; i < RI; i++) {
               acc[b][c][i] = __builtin_fmaf(s[b][j], d[i], acc[b][c][i]);
               if constexpr (has_offset<QT>)
-                acc[b][c][i] = __builtin_fmaf(KIND < 0 ? o[b][j] * (1.0f / 128.0f) : o[b][j], cin[c][i], acc[b][c][i]);
+                acc[b][c][i] = __builtin_fmaf(o[b][j], cin[c][i], acc[b][c][i]);
             }
           }
         }
@@ -367,23 +375,191 @@ __global__ __launch_bounds__(256) void k_planes(const void* __restrict__ x, int 
   store_planes(out + m * Kp + k, plane, planes, v);
 }
 
+// Tall matrices, up to 16 rows of x: a workgroup a CU; the tiles shared out among workgroups, a workgroup's units, tile after
+// tile, evenly among its waves, so that a wave reads one run of memory from beginning to end with the next units in flight and
+// leaves a sum only at a tile's end. x (as its planes) and the workgroup's biases are in LDS. A tile that several waves share:
+// the one that begins it adds the others' shares, in order. What bounds it: the weights' bytes, and nearly as much the
+// instructions (about 120 a unit and wave for one bf16 row).
+constexpr int TALL_WAVES = 16, TALL_WGS = 256;
+// From 1024 tiles of together 32768 units on (Q4_K, one row: 131072 x 2048 32 us against k_few's 39, 32768 x 4096 18.6
+// against 21.9, 16384 x 12288 25 against 33; 16384 x 4096 13.2 against 10.4, 65536 x 1024 11.5 against 9.9). 16 rows of 131072
+// x 2048: 41 us against 57; 3 rows of fp32: 59 against 89.
+constexpr int64_t TALL_TILES = 1024, TALL_UNITS = 32768;
+
+template <int QT, int P, int RI, bool X32>
+__global__ __launch_bounds__(TALL_WAVES * 64) void k_tall(const FewK a) {
+  constexpr int KIND = code_kind<QT, P>(), UB = unit_bytes<QT>(), D = 3;  // (units in flight)
+  constexpr bool CIN = KIND < 0 || has_offset<QT>;
+  constexpr float CC = KIND < 0 ? (QT == ARTLITE_Q4_0 ? -136.0f : -128.0f) : -1.0f;
+  constexpr uint32_t CB = bf16_of(int(CC)) * 0x10001u;
+  constexpr float OM = KIND < 0 ? 1.0f / 128.0f : 1.0f;
+  const Nibbles nib;
+  extern __shared__ __attribute__((aligned(16))) float red[];  // [wave][RI][lane]; x: [plane][row][units 256 + 8]; biases
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lg = lane >> 4, lr = lane & 15;
+  uint8_t* const xs = reinterpret_cast<uint8_t*>(red) + TALL_WAVES * RI * WAVE * 4;
+  const int K = int(a.K), pitch = 2 * a.units * UNIT + 16, rows = int(a.M), plane = rows * pitch;
+  float* const bias = reinterpret_cast<float*>(xs + P * plane);
+  const int64_t t0 = a.tiles * blockIdx.x / gridDim.x, t1 = a.tiles * (blockIdx.x + 1) / gridDim.x;
+  const int64_t all = (t1 - t0) * a.units;
+  if (all == 0) return;
+  const int64_t first = all * wv / TALL_WAVES, end = all * (wv + 1) / TALL_WAVES;
+  const uint8_t* const last = a.w + (t1 * a.units - 1) * UB;
+
+  u32x4 code[D][2];
+  TileHdr<QT> hd[D];
+  const uint8_t* next = a.w + (t0 * a.units + first) * UB;
+  auto load = [&](auto sv) __attribute__((always_inline)) {
+    constexpr int S = decltype(sv)::value;
+    const uint8_t* p = next < last ? next : last;  // (past the run: unread)
+#pragma unroll
+    for (int h = 0; h < 2; h++) code[S][h] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 1024 * h + 16 * lane));
+    hd[S].load(p + 2048 + hdr_bytes<QT>() * lr);
+    next += UB;
+  };
+  load(std::integral_constant<int, 0>{});
+  load(std::integral_constant<int, 1>{});
+  load(std::integral_constant<int, 2>{});
+  for (int m = 0; m < rows; m++)
+    for (int k = 8 * threadIdx.x; k < a.units * UNIT; k += 8 * TALL_WAVES * 64) {
+      u32x4 v[P];
+#pragma unroll
+      for (int i = 0; i < P; i++) v[i] = u32x4{0, 0, 0, 0};
+      if (k < K) {
+        const uint8_t* p = reinterpret_cast<const uint8_t*>(a.x) + (m * a.x_stride + k) * (X32 ? 4 : 2);
+        if constexpr (X32) {
+          u32x4 u[2];
+          __builtin_memcpy(u, p, 32);
+          split3(u[0], u[1], v[0], v[P > 1 ? 1 : 0], v[P - 1]);
+        } else {
+          __builtin_memcpy(v, p, 16);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < P; i++) *reinterpret_cast<u32x4*>(xs + i * plane + m * pitch + 2 * k) = v[i];
+    }
+  for (int64_t n = t0 * TROWS + threadIdx.x; n < t1 * TROWS; n += TALL_WAVES * 64)
+    bias[n - t0 * TROWS] = a.bias && n < a.N ? a.bias[n] : 0.0f;
+  __syncthreads();
+
+  const int xr = (lr >> 2) + 4 * (lr & 3);
+  const uint8_t* const x0 = xs + (xr < rows ? xr : 0) * pitch + 16 * lg;
+  float acc[RI];
+#pragma unroll
+  for (int i = 0; i < RI; i++) acc[i] = 0.0f;
+  int t = int(first / a.units), u = int(first - int64_t(t) * a.units);  // (the workgroup's tile)
+  bool begun = u == 0;                                                // (the wave has the tile's first unit)
+  const auto put = [&]() __attribute__((always_inline)) {
+    const int64_t n = (t0 + t) * TROWS + lr;
+    const float b = bias[t * TROWS + lr];
+#pragma unroll
+    for (int i = 0; i < RI; i++)
+      if (n < a.N && lg + 4 * i < rows) store_row(a, lg + 4 * i, n, acc[i] + b);
+  };
+  const auto leave = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < RI; i++) red[(wv * RI + i) * WAVE + lane] = acc[i];
+  };
+  const auto step = [&](auto sv) __attribute__((always_inline)) {
+    constexpr int S = decltype(sv)::value;
+    const uint8_t* const xu = x0 + 2 * UNIT * u;
+    const auto half = [&](auto hv) __attribute__((always_inline)) {
+      constexpr int H = decltype(hv)::value;
+      float s[4], o[4];
+      hd[S].template fields<H>(s, o, OM);
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const u32x4 cst{CB, CB, CB, CB};
+        u32x4 xo[P];
+#pragma unroll
+        for (int p = 0; p < P; p++) xo[p] = *reinterpret_cast<const u32x4*>(xu + p * plane + 64 * (4 * H + j));
+        f32x4 cin{0, 0, 0, 0};
+        if constexpr (CIN)
+#pragma unroll
+          for (int p = P - 1; p >= 0; p--) cin = mfma(xo[p], cst, cin);
+        const u32x4 q = operand<KIND>(code[S][H][j], nib);
+        f32x4 d = KIND < 0 ? cin : f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int p = P - 1; p >= 0; p--) d = mfma(xo[p], q, d);
+#pragma unroll
+        for (int i = 0; i < RI; i++) {
+          acc[i] = __builtin_fmaf(s[j], d[i], acc[i]);
+          if constexpr (has_offset<QT>) acc[i] = __builtin_fmaf(o[j], cin[i], acc[i]);
+        }
+      }
+    };
+    half(std::integral_constant<int, 0>{});
+    half(std::integral_constant<int, 1>{});
+    load(sv);
+    if (++u == a.units) {
+      if (begun)
+        put();
+      else
+        leave();
+#pragma unroll
+      for (int i = 0; i < RI; i++) acc[i] = 0.0f;
+      u = 0, t++, begun = true;
+    }
+  };
+  int64_t n = end - first;
+  for (; n >= D; n -= D) {
+    step(std::integral_constant<int, 0>{});
+    step(std::integral_constant<int, 1>{});
+    step(std::integral_constant<int, 2>{});
+  }
+  if (n > 0) step(std::integral_constant<int, 0>{});
+  if (n > 1) step(std::integral_constant<int, 1>{});
+  if (!begun) leave();  // (a share with neither of the tile's ends, or none)
+  __syncthreads();
+  if (begun && u) {
+    const int64_t until = int64_t(t + 1) * a.units;
+    for (int w = wv + 1; w < TALL_WAVES && all * w / TALL_WAVES < until; w++)
+#pragma unroll
+      for (int i = 0; i < RI; i++) acc[i] += red[(w * RI + i) * WAVE + lane];
+    put();
+  }
+}
+
+size_t tall_lds(const FewK& k, int planes, int ri) {
+  return size_t(TALL_WAVES) * ri * WAVE * 4 + size_t(planes) * size_t(k.M) * (size_t(k.units) * UNIT * 2 + 16) +
+         size_t((k.tiles + TALL_WGS - 1) / TALL_WGS) * TROWS * 4;
+}
+template <int QT, int P, int RI, bool X32>
+int launch_tall_t(const FewK& k, hipStream_t s) {
+  static DeviceOnce set;
+  if (!set.lds(reinterpret_cast<const void*>(k_tall<QT, P, RI, X32>), LDS_BYTES)) return fail(ARTLITE_EHIP, "dense rows: kernel set-up failed");
+  k_tall<QT, P, RI, X32><<<TALL_WGS, TALL_WAVES * 64, tall_lds(k, P, RI), s>>>(k);
+  ART_HIP(hipGetLastError());
+  return ARTLITE_OK;
+}
+
 // How a product is shared out: the units of K in `parts` workgroups (where the groups of tiles leave half the CUs idle and a
 // part has 4 units at least: 32 rows of 4096 x 4096, 64 groups, 13.8 us in one part, 12.8 in 4; 64 rows, 128 groups, 14.6 in
-// one, 13.3 in 2; 77 rows, 256 groups, 14.8 in one, 21.2 in 2), a part's units among `waves` waves, up to 16 of them where the workgroups leave the device's waves few (16 rows
-// of 4096 x 4096 in 16: 5.5 us, in 8 6.2; of 8192 x 4096 10.4 and 9.4), 4 where they are enough, each with the same number of
-// units but for the last.
+// one, 13.3 in 2; 77 rows, 256 groups, 14.8 in one, 21.2 in 2), a part's units among `waves` waves: up to 16 of them where the
+// workgroups leave the device's waves few (16 rows of 4096 x 4096, 256 workgroups, in 16: 5.5 us, in 8 6.2; of 4608 x 8192,
+// 288 workgroups, which are no longer all there at once, 14.5 and 12.5), 4 where they are enough, each with the same number
+// of units but for the last.
 struct FewCut {
   int64_t groups, blocks;
   int parts, waves;
 };
+// Blocks of 16 rows a workgroup's pass takes. More than one shares the weights' expansion and x's loads among tiles, but leaves
+// few workgroups, which then take parts and a launch more (about 4 us): one where the products are few. 16384 unit products of
+// one plane (4096 x 4096 Q4_K: 24 rows 12.1 us in passes of 32, 8.0 in blocks apart; 64 rows 13.1 and 12.3; 96 rows 15 and 17;
+// 2048 x 2048, 64 rows, 10.7 and 5.2), half as many of more (2048 x 8192, two planes: 24 rows 14.3 and 14.3, 48 rows 16.5 and
+// 22; 4096 x 4096, three: 24 rows 17.1 and 13.3, 48 rows 19.4 and 19.1).
+constexpr int64_t FEW_APART = 16384;
+int few_nc(int64_t tiles, int units, int64_t M, int planes, bool glu) {
+  if (M <= 16 || tiles * units * (glu ? 2 : 1) * ((M + 15) / 16) <= FEW_APART / (planes > 1 ? 2 : 1)) return 1;
+  return M <= 32 ? 2 : 4;
+}
 FewCut few_cut(int64_t tiles, int units, int64_t M, int planes, bool glu) {
-  const int nc = M <= 16 ? 1 : M <= 32 ? 2 : 4, tb = few_tiles(nc, glu), most = few_most(planes, nc, glu);
+  const int nc = few_nc(tiles, units, M, planes, glu), tb = few_tiles(nc, glu), most = few_most(planes, nc, glu);
   FewCut c{(tiles + tb - 1) / tb, (M + 16 * nc - 1) / (16 * nc), 1, 4};
   const int64_t wgs = c.groups * c.blocks;
   if (nc > 1)
     while (wgs * c.parts * 2 <= 256 && units / (2 * c.parts) >= 4) c.parts *= 2;
   const int own = (units + c.parts - 1) / c.parts;
-  while (c.waves < most && wgs * c.parts * c.waves < (nc > 1 ? 2048 : 4096)) c.waves *= 2;
+  while (c.waves < (wgs > 256 ? 8 : most) && wgs * c.parts * c.waves < (nc > 1 ? 2048 : 4096)) c.waves *= 2;
   const int each = (own + c.waves - 1) / c.waves;
   c.waves = (own + each - 1) / each;
   return c;
@@ -397,10 +573,10 @@ int launch_few_t(const FewK& k, hipStream_t s) {
   const FewCut c = few_cut(k.tiles, k.units, k.M, P, GLU);
   const size_t lds = size_t(c.waves) * WAVE_LDS;
   const dim3 grid(unsigned(c.groups), unsigned(c.blocks), unsigned(c.parts));
-  const auto set = [](const void* f) { return hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) == hipSuccess; };
-  static const bool ok = set(reinterpret_cast<const void*>(k_few<QT, P, NC, RI, GLU, false, X32>)) &&
-                         (NC == 1 || set(reinterpret_cast<const void*>(k_few<QT, P, NC, RI, GLU, NC != 1, X32>)));
-  if (!ok) return fail(ARTLITE_EHIP, "dense rows: kernel set-up failed");
+  static DeviceOnce set, set_part;
+  if (!set.lds(reinterpret_cast<const void*>(k_few<QT, P, NC, RI, GLU, false, X32>), LDS) ||
+      (NC > 1 && !set_part.lds(reinterpret_cast<const void*>(k_few<QT, P, NC, RI, GLU, NC != 1, X32>), LDS)))
+    return fail(ARTLITE_EHIP, "dense rows: kernel set-up failed");
   if (NC > 1 && c.parts > 1) {
     if (!k.parts) return fail(ARTLITE_EINVAL, "dense rows: no scratch for parts");
     if constexpr (NC > 1) k_few<QT, P, NC, RI, GLU, true, X32><<<grid, 64 * c.waves, lds, s>>>(k);
@@ -415,9 +591,14 @@ int launch_few_t(const FewK& k, hipStream_t s) {
 
 template <int QT, int P, bool GLU, bool X32 = false>
 int launch_few_p(const FewK& k, hipStream_t s) {
+  if constexpr (!GLU && (P == 1 || X32))
+    if (k.M <= 16 && k.tiles >= TALL_TILES && k.tiles * k.units >= TALL_UNITS && tall_lds(k, P, 4) <= size_t(LDS_BYTES))
+      return k.M <= 4   ? launch_tall_t<QT, P, 1, X32>(k, s)
+             : k.M <= 8 ? launch_tall_t<QT, P, 2, X32>(k, s)
+                        : launch_tall_t<QT, P, 4, X32>(k, s);
   if (k.M <= 4) return launch_few_t<QT, P, 1, 1, GLU, X32>(k, s);
   if (k.M <= 8) return launch_few_t<QT, P, 1, 2, GLU, X32>(k, s);
-  if (k.M <= 16 || X32) return launch_few_t<QT, P, 1, 4, GLU, X32>(k, s);
+  if (X32 || few_nc(k.tiles, k.units, k.M, P, GLU) == 1) return launch_few_t<QT, P, 1, 4, GLU, X32>(k, s);
   if (k.M <= 32) return launch_few_t<QT, P, 2, 4, GLU, false>(k, s);
   return launch_few_t<QT, P, 4, 4, GLU, false>(k, s);
 }
@@ -433,15 +614,19 @@ int launch_few_q(const FewArgs& a, const FewK& k, hipStream_t s) {
 
 }  // namespace
 
+bool few_apart(const artlite_matrix* w, int planes, bool gated, int64_t M) {
+  return few_nc(w->tiles, w->units, M, planes, gated) == 1;
+}
+
 size_t few_parts_bytes(const artlite_matrix* w, int planes, bool gated, int64_t M) {
-  if (M <= 16) return 0;
+  if (few_apart(w, planes, gated, M)) return 0;
   const FewCut c = few_cut(w->tiles, w->units, M, planes, gated);
   return c.parts > 1 ? size_t(c.parts) * M * w->N * (gated ? 2 : 1) * 4 : 0;
 }
 
 int launch_few(const FewArgs& a, hipStream_t s) {
   if (a.M <= 0) return ARTLITE_OK;
-  if (a.x32 && a.M > FEW_X32) return fail(ARTLITE_EINVAL, "dense rows: %lld fp32 rows", (long long)a.M);
+  if (a.x32 && !few_apart(a.w, 3, a.up != nullptr, a.M)) return fail(ARTLITE_EINVAL, "dense rows: %lld fp32 rows", (long long)a.M);
   if (a.M > int64_t(65535) * 16) return fail(ARTLITE_EINVAL, "dense rows: %lld rows", (long long)a.M);
   FewK k{};
   k.w = a.w->w.as<uint8_t>();

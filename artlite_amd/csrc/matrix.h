@@ -2,6 +2,7 @@
 // it, workspaces, the checks of device arguments, the launches of the dense products.
 #pragma once
 
+#include <atomic>
 #include <mutex>
 
 #include "codes.h"
@@ -60,19 +61,20 @@ struct TileHdr {
       }
     }
   }
-  // s and o of groups 4 H .. + 4; K-quants' 6-bit fields four at a time, as the bytes of a word
+  // s and o (times om, a power of two) of groups 4 H .. + 4; K-quants' 6-bit fields four at a time, as the bytes of a word
   template <int H>
-  __device__ __forceinline__ void fields(float (&s)[4], float (&o)[4]) const {
+  __device__ __forceinline__ void fields(float (&s)[4], float (&o)[4], float om = 1.0f) const {
     if constexpr (QT == ARTLITE_Q4_0 || QT == ARTLITE_IQ4_NL) {
 #pragma unroll
       for (int g = 0; g < 4; g++) s[g] = h2f((h[2 * H + (g >> 1)] >> (16 * (g & 1))) & 0xFFFFu);
     } else if constexpr (QT == ARTLITE_Q4_1) {
 #pragma unroll
-      for (int g = 0; g < 4; g++) s[g] = h2f(h[4 * H + g] & 0xFFFFu), o[g] = -h2f(h[4 * H + g] >> 16);
+      for (int g = 0; g < 4; g++) s[g] = h2f(h[4 * H + g] & 0xFFFFu), o[g] = -om * h2f(h[4 * H + g] >> 16);
     } else if constexpr (QT == ARTLITE_Q4_K) {
-      const float d = h2f(h[0] & 0xFFFFu), dm = h2f(h[0] >> 16);
-      const uint32_t sc = H == 0 ? h[1] & 0x3F3F3F3Fu : (h[3] & 0x0F0F0F0Fu) | ((h[1] >> 2) & 0x30303030u);
-      const uint32_t mn = H == 0 ? h[2] & 0x3F3F3F3Fu : ((h[3] >> 4) & 0x0F0F0F0Fu) | ((h[2] >> 2) & 0x30303030u);
+      const float d = h2f(h[0] & 0xFFFFu), dm = om * h2f(h[0] >> 16);
+      uint32_t sc = H == 0 ? h[1] & 0x3F3F3F3Fu : (h[3] & 0x0F0F0F0Fu) | ((h[1] >> 2) & 0x30303030u);
+      uint32_t mn = H == 0 ? h[2] & 0x3F3F3F3Fu : ((h[3] >> 4) & 0x0F0F0F0Fu) | ((h[2] >> 2) & 0x30303030u);
+      asm("" : "+v"(sc), "+v"(mn));  // (else a field is taken out of its word by an instruction of its own)
 #pragma unroll
       for (int g = 0; g < 4; g++) {
         s[g] = __fmul_rn(d, float((sc >> (8 * g)) & 0xFFu));
@@ -202,6 +204,19 @@ struct OnDevice {
     if (was >= 0) (void)hipSetDevice(was);
   }
 };
+// a kernel's dynamic LDS beyond the default, set once on each device (current when it is launched)
+struct DeviceOnce {
+  std::atomic<uint64_t> done{0};
+  bool lds(const void* kernel, size_t bytes) {
+    int d = 0;
+    if (hipGetDevice(&d) != hipSuccess) return false;
+    const uint64_t bit = uint64_t(1) << (d & 63);
+    if (done.load(std::memory_order_acquire) & bit) return true;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)) != hipSuccess) return false;
+    done.fetch_or(bit, std::memory_order_release);
+    return true;
+  }
+};
 // p: device memory of `device`
 int check_device(const void* p, int device, const char* what);
 
@@ -229,7 +244,7 @@ namespace artlite {
 // ---- the dense products over few rows (linear.hip)
 
 // One launch: out[m][n] = sum_k x[m][k] W[n][k] (+ bias[n]) for M rows of x given as planes of bf16 (x = the sum of its
-// planes) or, up to FEW_X32 of them, as fp32, or with `up` set the gated products act(x W^T) (x U^T), written as planes of bf16 for the launch after.
+// planes) or, where few_apart, as fp32, or with `up` set the gated products act(x W^T) (x U^T), written as planes of bf16 for the launch after.
 struct FewArgs {
   const artlite_matrix *w, *up;
   int act;                  // (gated) artlite_act
@@ -246,13 +261,15 @@ struct FewArgs {
   int h_planes;
   float* parts;             // scratch for sums in parts: few_parts_bytes of it
 };
-constexpr int FEW_X32 = 16;
 int launch_few(const FewArgs& a, hipStream_t s);
+// Whether a workgroup takes 16 rows of x of one tile, and blocks of 16 rows are workgroups of their own: up to 16 rows, and
+// where the product is small (below).
+bool few_apart(const artlite_matrix* w, int planes, bool gated, int64_t M);
 size_t few_parts_bytes(const artlite_matrix* w, int planes, bool gated, int64_t M);
 // Rows past which the dense products go by way of 16-bit weights and the large tiles. One matrix's of bf16 rows: 4096 x 4096
 // Q4_K, 256 rows, 27 us against 40, 384 rows 40 against 45; 12288 x 2048 IQ4_XS, 256 rows, 37 against 46, 384 rows 54 against
 // 58, 512 rows 73 against 60. Of fp32 rows: 4096 x 4096, 128 rows, 45 against 55, 192 rows 68 against 62. The gated block's:
-// 2048 x 8192, 128 rows, 61 against 78, 192 rows 82 against 78.
+// 2048 x 8192, 128 rows, 61 against 78, 192 rows 82 against 78. And any number of rows that are few_apart.
 constexpr int FEW_ROWS = 256, FEW_ROWS_F32 = 128, FEW_ROWS_FFN = 128;
 // x (M rows of K values of dtype, stride apart) as planes of bf16 (1: bf16 as it is; 3: fp32), rows of Kp values (zeros past K)
 int launch_planes(const void* x, int dtype, int64_t M, int64_t K, int64_t stride, uint16_t* out, int64_t Kp, int64_t plane,

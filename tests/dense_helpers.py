@@ -8,6 +8,18 @@ from oracle.tensors import bf16_bits, from_bf16_bits
 DTYPE = {"bf16": np.uint16, "f32": np.float32}
 
 
+def small(rows: int, cols: int, M: int, planes: int, gated: bool = False) -> bool:
+    """Whether a product's blocks of 16 rows are workgroups of their own (and stay with the few rows' path)."""
+    units = -(-rows // 16) * -(-cols // 256) * (2 if gated else 1)
+    return M <= 16 or units * -(-M // 16) <= 16384 // (2 if planes > 1 else 1)
+
+
+def past_small(rows: int, cols: int, planes: int, gated: bool = False) -> int:
+    """The first number of rows that is not."""
+    units = -(-rows // 16) * -(-cols // 256) * (2 if gated else 1)
+    return 16 * max(1, 16384 // (2 if planes > 1 else 1) // units) + 1
+
+
 def values(a: np.ndarray) -> np.ndarray:
     """A host array's values in 64 bits."""
     return (from_bf16_bits(a) if a.dtype == np.uint16 else a).astype(np.float64)

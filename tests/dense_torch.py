@@ -33,7 +33,7 @@ def refused(call: object) -> None:
 def linear_streams_and_graphs() -> None:
     """Torch tensors: calls that alternate between streams on one object's workspace; captured calls replayed with other
     inputs, beside eager ones on workspaces of their own."""
-    N, K = 200, 512
+    N, K = 2000, 512
     lin = QLinear("Q4_1", N, K)
     raw, w = dense.matrix("Q4_1", N, K, 8)
     lin.upload(raw)
@@ -47,7 +47,7 @@ def linear_streams_and_graphs() -> None:
         assert (y.cpu().double() - want).norm() <= 2.0 ** -7 * want.norm()
 
     streams = [torch.cuda.Stream() for _ in range(3)]
-    xs = [torch.randn(253 + i, K, device="cuda").bfloat16() for i in range(12)]
+    xs = [torch.randn(1034 + i, K, device="cuda").bfloat16() for i in range(12)]
     ys = [torch.empty(x.shape[0], N, device="cuda", dtype=torch.bfloat16) for x in xs]
     torch.cuda.synchronize()
     for i, (x, y) in enumerate(zip(xs, ys)):
@@ -57,7 +57,7 @@ def linear_streams_and_graphs() -> None:
         near(y, x)
     graphs = []
     wide, out = (torch.empty(50000, c, device="cuda", dtype=torch.bfloat16) for c in (K, N))
-    for M in (1, 100, 300):
+    for M in (1, 100, 1100):
         x = torch.randn(M, K, device="cuda").bfloat16()
         y = torch.empty(M, N, device="cuda", dtype=torch.bfloat16)
         work = Workspace(max(1, lin.workspace_bytes(M, "bf16")))
@@ -102,7 +102,7 @@ def ffn_streams_and_graphs() -> None:
         return torch.randn(n, H, device="cuda").bfloat16()
 
     streams = [torch.cuda.Stream() for _ in range(3)]
-    xs = [rand(n) for n in (5, 150, 64, 129, 1, 33)]
+    xs = [rand(n) for n in (5, 4200, 64, 129, 1, 33)]
     ys = [torch.empty_like(x) for x in xs]
     torch.cuda.synchronize()
     for i, (x, y) in enumerate(zip(xs, ys)):
@@ -111,7 +111,7 @@ def ffn_streams_and_graphs() -> None:
     for x, y in zip(xs, ys):
         near(y, dense.ffn("silu", host(x), *w), TOL)
     graphs = []
-    for n in (4, 150):
+    for n in (4, 150, 4200):
         x, dy = rand(n), rand(n)
         out = {"y": torch.empty_like(x), "dx": torch.empty_like(x),
                "dgate": torch.empty(F, H, device="cuda", dtype=torch.bfloat16)}

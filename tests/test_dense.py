@@ -109,9 +109,9 @@ def test_device_arguments_refused(tmp_path: Path) -> None:
     run_fake(tmp_path, PRELUDE + """
 import ctypes
 lib = _hip.lib()
-l, f = linear(64, 64), block(64, 96)
-x, y = arr(400, 64), arr(400, 64)
-def call(x=x.data_ptr(), n=4, xs=64, y=y.data_ptr(), ys=64, dtype=1, work=None):
+l, f = linear(4096, 1024), block(1024, 96)
+x, y = arr(400, 1024), arr(400, 4096)
+def call(x=x.data_ptr(), n=4, xs=1024, y=y.data_ptr(), ys=4096, dtype=1, work=None):
     _hip.check(lib.artlite_linear(l._m.handle, x, dtype, n, xs, y, ys, work, None))
 before = hip.launches
 call()
@@ -119,8 +119,8 @@ assert hip.launches == before + 1
 call(n=0, x=None, y=None)
 assert hip.launches == before + 1
 refused("x: null", lambda: call(x=None))
-refused("y: rows of 64 values 63 apart", lambda: call(ys=63))
-refused("x: rows of 64 values -1 apart", lambda: call(xs=-1))
+refused("y: rows of 4096 values 63 apart", lambda: call(ys=63))
+refused("x: rows of 1024 values -1 apart", lambda: call(xs=-1))
 refused("not aligned to its values", lambda: call(x=x.data_ptr() + 1))
 refused("not aligned to its values", lambda: call(dtype=0, x=x.data_ptr() + 2))
 refused("dtype 7", lambda: call(dtype=7))
@@ -133,10 +133,11 @@ refused("x: not device memory", call)
 hip.host_pointers = 0
 assert hip.launches == before + 1
 call(n=300, work=enough.handle)
-def back(dx=y, dy=x, **w): f.backward(x, dy, dx=dx, **w)
-refused("dx overlaps dy", lambda: back(dy=y))
+z = arr(400, 1024)
+def back(dx=z, dy=x, **w): f.backward(x, dy, dx=dx, **w)
+refused("dx overlaps dy", lambda: back(dy=z))
 refused("no dy", lambda: back(dy=None))
-refused("ddown is (96, 64)", lambda: back(ddown=arr(96, 64)))
+refused("ddown is (96, 1024)", lambda: back(ddown=arr(96, 1024)))
 """.replace("hip.fake_host = 0\n", ""))
 
 
@@ -144,7 +145,7 @@ def test_workspaces(tmp_path: Path) -> None:
     """Calls that are given no workspace share one a device; it grows, refuses captures and is free again after a call that
     failed; calls on another stream than the last one's wait for it."""
     run_fake(tmp_path, PRELUDE + """
-l, f = linear(64, 64), block(64, 96)
+l, f = linear(4096, 1024), block(1024, 96)
 mallocs = lambda: hip.mallocs
 def run(n, stream=0, **k): l(X[:n], Y[:n], stream=stream, **k)
 class Rows:
@@ -154,11 +155,12 @@ class Rows:
 class Whole:
     def __init__(self, n, c): self.a = arr(n, c)
     def __getitem__(self, s): return Rows(self.a, s.stop)
-X, Y = Whole(5000, 64), Whole(5000, 64)
+X, Y = Whole(5000, 1024), Whole(5000, 4096)
 assert l.workspace_bytes(16) == 0 == l.workspace_bytes(16, "f32") and l.workspace_bytes(300) > 0
 run(300)
+Z = Whole(200, 1024)
 at = hip.mallocs
-run(300); f(X[:200], Y[:200]); run(290)
+run(300); f(X[:200], Z[:200]); run(290)
 assert hip.mallocs <= at + 1
 big = hip.mallocs
 run(5000); run(5000); run(300)
@@ -168,7 +170,7 @@ run(300); run(300)
 assert hip.waits == waits
 run(300, stream=5); run(300, stream=5); run(300)
 assert hip.waits == waits + 2
-big_rows = arr(50000, 64), arr(50000, 64)
+big_rows = arr(50000, 1024), arr(50000, 4096)
 hip.capturing = 1
 refused("a captured call takes a workspace of its own", lambda: run(300))
 at = hip.mallocs

@@ -1,5 +1,5 @@
-"""``QLinear`` against 64-bit math in every format and on every path: few rows (bf16 1 to 256, fp32 1 to 128: one, two and four blocks of 16), the
-large tiles past them (both sizes), widths of a single block, of partial units and of partial 64 values, odd numbers of
+"""``QLinear`` against 64-bit math in every format and on every path: few rows (bf16 1 to 256, fp32 1 to 128, more of
+a small matrix: one, two and four blocks of 16), tall matrices, the large tiles past them (both sizes), widths of a single block, of partial units and of partial 64 values, odd numbers of
 outputs, rows at any stride and address; bias, zeros, infinities and NaN.
 
 Tolerances (relative L2). A bf16 output is rounded once: half a step is 2^-8. Of few rows no weight is rounded and sums are
@@ -16,13 +16,17 @@ from artlite_amd.device import DeviceArray, Workspace
 from artlite_amd.linear import QLinear
 from oracle import dense
 
-from .dense_helpers import Rows, check, encode, values
+from .dense_helpers import Rows, check, encode, past_small, small, values
 
 pytestmark = pytest.mark.gpu
 
 FEW = {"bf16": 256, "f32": 128}
 TOL = {("bf16", True): 2.0 ** -8 + 2.0 ** -14, ("bf16", False): 2.0 ** -8 + 2.0 ** -10, ("f32", True): 4e-6,
        ("f32", False): 4e-6}
+
+
+def few(N: int, K: int, M: int, dtype: str) -> bool:
+    return M <= FEW[dtype] or small(N, K, M, 1 if dtype == "bf16" else 3)
 
 
 def widths(q: str) -> list[int]:
@@ -48,9 +52,10 @@ def test_rows_and_widths(q: str, dtype: str) -> None:
     for K in widths(q):
         for N in (1, 17, 100):
             lin, w, _ = make(q, N, K, 7 * N + K)
-            for M in (1, 4, 5, 8, 9, 16, 17, 33, 65, 128, 129, 256, 257):
+            past = [max(FEW[dtype] + 1, past_small(N, K, 1 if dtype == "bf16" else 3))] if N == 100 else []
+            for M in (1, 4, 5, 8, 9, 16, 17, 33, 65, 128, 129, 256, 257, *past):
                 x = x_rows(M, K, dtype, M + K)
-                check(lin(x), values(x) @ w.T, TOL[dtype, M <= FEW[dtype]], np.sqrt(values(x) ** 2 @ (w ** 2).T))
+                check(lin(x), values(x) @ w.T, TOL[dtype, few(N, K, M, dtype)], np.sqrt(values(x) ** 2 @ (w ** 2).T))
             lin.close()
 
 
@@ -60,9 +65,9 @@ def test_rows_and_widths(q: str, dtype: str) -> None:
 def test_larger(q: str, N: int, K: int, dtype: str) -> None:
     """Units shared by every number of waves; tiles of the large products in several rows and columns."""
     lin, w, b = make(q, N, K, 5, bias=True)
-    for M in (1, 5, 20, 40, 100, 300):
+    for M in (1, 5, 20, 40, 100, 300, 1400):
         x = x_rows(M, K, dtype, M)
-        check(lin(x), values(x) @ w.T + b, TOL[dtype, M <= FEW[dtype]])
+        check(lin(x), values(x) @ w.T + b, TOL[dtype, few(N, K, M, dtype)])
 
 
 def test_large_tiles() -> None:
@@ -73,38 +78,60 @@ def test_large_tiles() -> None:
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize(("q", "N", "K"), [("Q4_0", 131077, 1024), ("Q4_K", 33001, 4096), ("Q4_1", 131072, 992),
+                                           ("IQ4_NL", 40003, 3616), ("IQ4_XS", 16387, 8192)])
+def test_tall(q: str, N: int, K: int, dtype: str) -> None:
+    """Matrices of so many rows that a wave reads several tiles or parts of them (the rows those of 1009, a prime, over and
+    over: each of a tile's places has each of them); a bias; x and the output with rows apart; the same bits again."""
+    raw, w = dense.matrix(q, 1009, K, 3)
+    raw = np.tile(raw.reshape(1009, -1), (-(-N // 1009), 1))[:N]
+    b = np.random.default_rng(1).standard_normal(N).astype(np.float32)
+    lin = QLinear(q, N, K)
+    for bias in (None, b):
+        lin.upload(raw, bias=bias)
+        for M in (1, 4, 5, 11, 16):
+            data = x_rows(M, K, dtype, M)
+            x, y = Rows(M, K, dtype, at=3, stride=K + 5, data=data), Rows(M, N, dtype, at=1, stride=N + 3)
+            lin(x, y)
+            got = y.numpy()
+            check(got, np.tile(values(data) @ w.T, (1, -(-N // 1009)))[:, :N] + (0 if bias is None else b), TOL[dtype, True])
+            lin(x, y)
+            assert np.array_equal(got, y.numpy())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize(("at", "pad", "out_at", "out_pad"), [(0, 0, 0, 0), (8, 8, 1, 3), (1, 0, 0, 4), (3, 5, 2, 2),
                                                               (8, 4, 4, 0), (0, 1, 0, 1)])
 def test_strides(at: int, pad: int, out_at: int, out_pad: int, dtype: str) -> None:
     """Rows at any address and stride; what lies between and behind the output's rows stays."""
     N, K = 100, 160
     lin, w, _ = make("IQ4_NL", N, K, 2)
-    for M in (1, 3, 16, 70, 300):
+    for M in (1, 3, 16, 70, 300, 37500):
         data = x_rows(M, K, dtype, M)
         x = Rows(M, K, dtype, at=at, stride=K + pad, data=data)
         y = Rows(M, N, dtype, at=out_at, stride=N + out_pad)
         assert lin(x, y) is y
-        check(y.numpy(), values(data) @ w.T, TOL[dtype, M <= FEW[dtype]])
+        check(y.numpy(), values(data) @ w.T, TOL[dtype, few(N, K, M, dtype)])
 
 
 def test_one_row_for_all() -> None:
     """A row stride of 0: every output row is the one input row's."""
     lin, w, _ = make("Q4_0", 40, 256, 2)
     data = x_rows(1, 256, "bf16", 1)
-    for M in (3, 80, 300):
+    for M in (3, 80, 87400):
         x = Rows(1, 256, "bf16", data=data)
         x.shape, x.row = (M, 256), 0
         y = Rows(M, 40, "bf16")
         lin(x, y)
-        check(y.numpy(), np.repeat(values(data) @ w.T, M, 0), TOL["bf16", M <= FEW["bf16"]])
+        check(y.numpy(), np.repeat(values(data) @ w.T, M, 0), TOL["bf16", few(40, 256, M, "bf16")])
 
 
-@pytest.mark.parametrize("M", [4, 90, 300])
+@pytest.mark.parametrize("M", [4, 90, 1300])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_values_out_of_the_ordinary(dtype: str, M: int) -> None:
     """Rows of zeros, of the type's smallest and largest sizes, with infinities and NaN: each row is its own, the others are
     unmoved."""
-    N, K = 48, 512
+    N, K = 1600, 512
     lin, w, _ = make("Q4_K", N, K, 4)
     a = np.random.default_rng(1).standard_normal((M, K))
     a[0] = 0.0
@@ -112,10 +139,10 @@ def test_values_out_of_the_ordinary(dtype: str, M: int) -> None:
     a[2] *= 1e30
     base = encode(a, dtype)
     y0 = lin(base)
-    check(y0[3:], values(base)[3:] @ w.T, TOL[dtype, M <= FEW[dtype]])
+    check(y0[3:], values(base)[3:] @ w.T, TOL[dtype, few(N, K, M, dtype)])
     assert not values(y0)[0].any()
     for r in (1, 2):
-        check(y0[r:r + 1], values(base)[r:r + 1] @ w.T, TOL[dtype, M <= FEW[dtype]])
+        check(y0[r:r + 1], values(base)[r:r + 1] @ w.T, TOL[dtype, few(N, K, M, dtype)])
     a[3, 5] = np.nan
     bad = encode(a, dtype)
     bad[2, 7] = encode(np.array([np.inf]), dtype)[0]
@@ -126,7 +153,7 @@ def test_values_out_of_the_ordinary(dtype: str, M: int) -> None:
 
 def test_zero_blocks_and_large_scales() -> None:
     """A matrix of zeros, and one whose scales are the largest fp16 ones, on both paths."""
-    for M in (3, 70, 300):
+    for M in (3, 70, 131100):
         x = x_rows(M, 64, "bf16", M)
         lin = QLinear("Q4_0", 20, 64)
         lin.upload(np.zeros((20, 36), np.uint8))
@@ -136,14 +163,14 @@ def test_zero_blocks_and_large_scales() -> None:
         raw[..., :2] = np.array([65504.0], np.float16).view(np.uint8)
         lin.upload(raw)
         w = dense.gguf_ref.dequantize("Q4_0", raw.reshape(20, 36), 64).astype(np.float64)
-        check(lin(x), values(x) @ w.T, TOL["bf16", M <= FEW["bf16"]])
+        check(lin(x), values(x) @ w.T, TOL["bf16", few(20, 64, M, "bf16")])
 
 
 def test_no_rows_and_repeats() -> None:
     """0 rows write nothing; the same call twice gives the same bits, on every path."""
     lin, _, _ = make("IQ4_XS", 100, 512, 3)
     assert lin(np.empty((0, 512), np.uint16)).shape == (0, 100)
-    for M in (1, 20, 65, 128, 129, 300):
+    for M in (1, 20, 65, 128, 129, 300, 18800):
         for dtype in ("bf16", "f32"):
             x = x_rows(M, 512, dtype, M)
             assert np.array_equal(lin(x), lin(x))
@@ -161,7 +188,8 @@ def test_refusals() -> None:
     with pytest.raises(_hip.Error, match="is no array"):
         lin(x)
     with pytest.raises(_hip.Error, match="a workspace of 1024 bytes, not"):
-        lin(x, y, work=Workspace(1024))
+        make("Q4_0", 4096, 1024, 3)[0](DeviceArray((300, 1024), np.uint16), DeviceArray((300, 4096), np.uint16),
+                                       work=Workspace(1024))
 
     class Host:  # (an address that is the host's)
         shape, dtype = (280, 64), np.dtype(np.uint16)
