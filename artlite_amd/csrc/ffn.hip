@@ -392,7 +392,14 @@ int ffn_forward(const Ffn& f, const void* x, int dtype, int64_t n, int64_t x_str
   return launch_hgemm(d, s);
 }
 
+// Rows up to which the gradients' products run from the blocks (GRADROWS)
+#ifndef FGR
+#define FGR 128
+#endif
+constexpr int FEW_ROWS_GRAD = FGR;
 struct GradPlan {
+  bool few;
+  uint16_t* planes = nullptr;                    // few rows: x as planes, where it is not read as it is
   uint16_t *x16, *dy16, *a16, *b16, *c16;        // x, dy; gate and up, later their transposes; down's transpose
   uint16_t *h16, *dh16, *dg16, *du16;
   uint16_t *xt, *dyt, *ht, *dgt, *dut;           // (weights' gradients) turned
@@ -403,11 +410,16 @@ GradPlan grad_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool weights) {
   GradPlan p{};
   const size_t pl = dtype == ARTLITE_X_BF16 ? 1 : 2;
   const size_t w = pl * size_t(f.F * f.Hp > f.H * f.Fp ? f.F * f.Hp : f.H * f.Fp);
+  p.few = n <= FEW_ROWS_GRAD;
   p.x16 = c.take<uint16_t>(pl * n * f.Hp);
   p.dy16 = c.take<uint16_t>(pl * n * f.Hp);
-  p.a16 = c.take<uint16_t>(w);
-  p.b16 = c.take<uint16_t>(w);
-  p.c16 = c.take<uint16_t>(pl * f.F * f.Hp);
+  if (!p.few) {
+    p.a16 = c.take<uint16_t>(w);
+    p.b16 = c.take<uint16_t>(w);
+    p.c16 = c.take<uint16_t>(pl * f.F * f.Hp);
+  } else if (pl == 2 && !few_apart(f.gate, 3, true, n)) {
+    p.planes = c.take<uint16_t>(3 * size_t(n) * f.H);
+  }
   p.dg16 = c.take<uint16_t>(pl * n * f.Fp);
   p.du16 = c.take<uint16_t>(pl * n * f.Fp);
   p.dh16 = c.take<uint16_t>(pl * n * f.Fp);
@@ -427,7 +439,12 @@ GradPlan grad_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool weights) {
     p.top = c.take<int32_t>(4);
   }
   const int sg = pl == 2 ? 3 : 1;
-  size_t parts = std::max({hgemm_parts_bytes(n, f.F, f.Hp, sg, false), hgemm_parts_bytes(n, f.F, f.Hp, sg, true),
+  size_t parts = 0;
+  if (p.few)
+    parts = std::max({few_t_bytes(f.down, 1, int(pl), n), few_t_bytes(f.gate, 2, int(pl), n),
+                      size_t(few_raw_parts(f.gate, pl == 2 ? 3 : 1, n)) * n * 2 * f.Fp * 4});
+  else
+    parts = std::max({hgemm_parts_bytes(n, f.F, f.Hp, sg, false), hgemm_parts_bytes(n, f.F, f.Hp, sg, true),
                            hgemm_parts_bytes(n, f.H, f.Fp, 2 * sg, false)});
   if (weights)
     parts = std::max({parts, hgemm_parts_bytes(f.F, f.H, pad64(n), sg, false), hgemm_parts_bytes(f.H, f.F, pad64(n), sg, false)});
@@ -452,19 +469,26 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
   ART_TRY(rows16(r, dtype, n, s));
   // (gate and up share a scale: dx sums over both)
   const int e = wexp16(f.gate) > wexp16(f.up) ? wexp16(f.gate) : wexp16(f.up), ed = wexp16(f.down);
-  ART_TRY(launch_unpack(f.gate, f.up, false, e, e, p.a16, p.b16, f.Hp, f.F * f.Hp, pl, s));
-  ART_TRY(launch_unpack(f.down, nullptr, true, ed, 0, p.c16, nullptr, f.Hp, f.F * f.Hp, pl, s));
+  if (!p.few) {
+    ART_TRY(launch_unpack(f.gate, f.up, false, e, e, p.a16, p.b16, f.Hp, f.F * f.Hp, pl, s));
+    ART_TRY(launch_unpack(f.down, nullptr, true, ed, 0, p.c16, nullptr, f.Hp, f.F * f.Hp, pl, s));
+  }
   HGemm d{};
-  segments(d, {{p.dy16, n * f.Hp, p.c16, f.F * f.Hp}}, pl);
+  if (!p.few) segments(d, {{p.dy16, n * f.Hp, p.c16, f.F * f.Hp}}, pl);
   d.lda = d.ldb = d.K = f.Hp;
   d.M = n, d.N = f.F;
   d.epilogue = H_ROWS;
   d.row_e = p.ye, d.e = ed;
   d.out_e = p.dhe, d.h = p.dh16, d.h_stride = f.Fp, d.h_plane = n * f.Fp, d.planes = pl;
   d.parts = p.parts;
-  ART_TRY(launch_hgemm(d, s));
+  if (p.few) {
+    ART_TRY(launch_few_t(FewTArgs{{f.down}, {p.dy16}, 1, f.Hp, n * f.Hp, pl, ed, n, p.parts}, s));
+    ART_TRY(launch_join(d, few_t_parts(f.down, 1, pl, n), s));
+  } else {
+    ART_TRY(launch_hgemm(d, s));
+  }
   HGemm g{};
-  segments(g, {{p.x16, n * f.Hp, p.a16, f.F * f.Hp, p.b16}}, pl);
+  if (!p.few) segments(g, {{p.x16, n * f.Hp, p.a16, f.F * f.Hp, p.b16}}, pl);
   g.lda = g.ldb = g.K = f.Hp;
   g.M = n, g.N = f.F;
   g.epilogue = H_DGLU;
@@ -475,17 +499,34 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
   g.dg = p.dg16, g.du = p.du16, g.h = p.h16;
   g.h_stride = f.Fp, g.h_plane = n * f.Fp, g.planes = pl;
   g.parts = p.parts;
-  ART_TRY(launch_hgemm(g, s));
+  if (p.few) {
+    FewArgs a{};
+    a.w = f.gate, a.up = f.up;
+    ART_TRY(few_x(a, x, dtype, n, f.H, x_stride, p.planes, s));
+    a.M = n;
+    a.parts = p.parts;
+    a.raw = few_raw_parts(f.gate, a.planes, n);
+    ART_TRY(launch_few(a, s));
+    g.row_e = nullptr, g.e = g.e2 = 0;  // (sums of the values themselves)
+    ART_TRY(launch_join(g, a.raw, s));
+  } else {
+    ART_TRY(launch_hgemm(g, s));
+  }
   if (dx) {
-    ART_TRY(launch_unpack(f.gate, f.up, true, e, e, p.a16, p.b16, f.Fp, f.H * f.Fp, pl, s));
+    if (!p.few) ART_TRY(launch_unpack(f.gate, f.up, true, e, e, p.a16, p.b16, f.Fp, f.H * f.Fp, pl, s));
     HGemm x2{};
-    segments(x2, {{p.dg16, n * f.Fp, p.a16, f.H * f.Fp}, {p.du16, n * f.Fp, p.b16, f.H * f.Fp}}, pl);
+    if (!p.few) segments(x2, {{p.dg16, n * f.Fp, p.a16, f.H * f.Fp}, {p.du16, n * f.Fp, p.b16, f.H * f.Fp}}, pl);
     x2.lda = x2.ldb = x2.K = f.Fp;
     x2.M = n, x2.N = f.H;
     x2.row_e = p.de, x2.e = e;
     x2.y = dx, x2.y_stride = dx_stride, x2.dtype = dtype;
     x2.parts = p.parts;
-    ART_TRY(launch_hgemm(x2, s));
+    if (p.few) {
+      ART_TRY(launch_few_t(FewTArgs{{f.gate, f.up}, {p.dg16, p.du16}, 2, f.Fp, n * f.Fp, pl, e, n, p.parts}, s));
+      ART_TRY(launch_join(x2, few_t_parts(f.gate, 2, pl, n), s));
+    } else {
+      ART_TRY(launch_hgemm(x2, s));
+    }
   }
   if (!weights) return ARTLITE_OK;
   const int64_t Tp = pad64(n);

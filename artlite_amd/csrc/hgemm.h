@@ -43,5 +43,7 @@ struct HGemm {
 // the scratch that a product may take (gated: N columns of each matrix)
 size_t hgemm_parts_bytes(int64_t M, int64_t N, int64_t K, int segs, bool gated);
 int launch_hgemm(const HGemm& g, hipStream_t s);
+// what becomes of sums that are there already, in parts of M rows of pad64(N) values (gated: both matrices' side by side)
+int launch_join(const HGemm& g, int parts, hipStream_t s);
 
 }  // namespace artlite

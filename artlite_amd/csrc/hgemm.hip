@@ -397,6 +397,7 @@ __global__ __launch_bounds__(256) void k_join(const HGemm g, int parts) {
   const int64_t pr = part_row<EPI>(g);
   const float* p = g.parts + m * pr + n;
   float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, u[8] = {0, 0, 0, 0, 0, 0, 0, 0}, bias[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 8
   for (int k = 0; k < parts; k++, p += g.M * pr)
 #pragma unroll
     for (int h = 0; h < 2; h++) {
@@ -468,6 +469,14 @@ int launch_t(const HGemm& g, int64_t gn, int parts, hipStream_t s) {
 }
 
 template <int EPI>
+int join(const HGemm& g, int parts, hipStream_t s) {
+  const int64_t threads = g.M * (pad64(g.N) / 8);
+  k_join<EPI><<<unsigned((threads + 255) / 256), 256, 0, s>>>(g, parts);
+  ART_HIP(hipGetLastError());
+  return ARTLITE_OK;
+}
+
+template <int EPI>
 int launch_e(HGemm g, bool mixed, hipStream_t s) {
   const int64_t cols = gated<EPI> ? 2 * g.N : g.N;
   const Cut c = best_cut(g.M, cols, g.K, g.segs, mixed);
@@ -477,10 +486,7 @@ int launch_e(HGemm g, bool mixed, hipStream_t s) {
       ART_TRY((launch_t<8, EPI, true>(g, c.gn, c.parts, s)));
     else
       ART_TRY((launch_t<4, EPI, true>(g, c.gn, c.parts, s)));
-    const int64_t threads = g.M * (pad64(g.N) / 8);
-    k_join<EPI><<<unsigned((threads + 255) / 256), 256, 0, s>>>(g, c.parts);
-    ART_HIP(hipGetLastError());
-    return ARTLITE_OK;
+    return join<EPI>(g, c.parts, s);
   }
   if (c.big)
     ART_TRY((launch_t<8, EPI, false>(g, c.gn, 1, s)));
@@ -532,6 +538,16 @@ int launch_hgemm(const HGemm& g, hipStream_t s) {
          : g.epilogue == H_ROWS ? launch_e<H_ROWS>(h, true, s)
          : g.epilogue == H_GLU  ? launch_e<H_GLU>(h, true, s)
                                 : launch_e<H_DGLU>(h, true, s);
+}
+
+int launch_join(const HGemm& g, int parts, hipStream_t s) {
+  if (g.M <= 0 || g.N <= 0) return ARTLITE_OK;
+  HGemm h = g;
+  h.h_cols = g.h_stride;
+  return g.epilogue == H_STORE  ? join<H_STORE>(h, parts, s)
+         : g.epilogue == H_ROWS ? join<H_ROWS>(h, parts, s)
+         : g.epilogue == H_GLU  ? join<H_GLU>(h, parts, s)
+                                : join<H_DGLU>(h, parts, s);
 }
 
 }  // namespace artlite

@@ -19,6 +19,7 @@
 // and two dependent round trips.
 #include "matrix.h"
 
+#include <algorithm>
 #include <utility>
 
 namespace artlite {
@@ -90,6 +91,7 @@ struct FewK {
   int64_t h_stride, h_plane;
   int h_planes;
   float* parts;
+  int64_t part_row, part_up;  // (values of a row of the parts; where the second matrix's begin)
 };
 
 __device__ __forceinline__ void store_planes(uint16_t* p, int64_t plane, int planes, float v) {
@@ -341,9 +343,9 @@ __global__ __launch_bounds__(few_most(P, NC, GLU) * 64) void k_few(const FewK a)
     const int64_t n = (t0 + b) * TROWS + lr, m = m0 + 16 * (ci / RI) + lg + 4 * (ci % RI);
     if (n >= a.N || m >= a.M) continue;
     if constexpr (PART) {
-      float* o = a.parts + ((blockIdx.z * a.M + m) * (GLU ? 2 : 1)) * a.N + n;
+      float* o = a.parts + (blockIdx.z * a.M + m) * a.part_row + n;
       o[0] = s;
-      if (GLU) o[a.N] = v;
+      if (GLU) o[a.part_up] = v;
     } else {
       few_out<GLU>(a, m, n, s, v);
     }
@@ -355,12 +357,11 @@ template <bool GLU>
 __global__ __launch_bounds__(256) void k_few_join(const FewK a, int parts) {
   const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x, m = i / a.N, n = i % a.N;
   if (m >= a.M) return;
-  const int64_t row = (GLU ? 2 : 1) * a.N;
-  const float* p = a.parts + m * row + n;
+  const float* p = a.parts + m * a.part_row + n;
   float s = 0.0f, u = 0.0f;
-  for (int k = 0; k < parts; k++, p += a.M * row) {
+  for (int k = 0; k < parts; k++, p += a.M * a.part_row) {
     s += p[0];
-    if (GLU) u += p[a.N];
+    if (GLU) u += p[a.part_up];
   }
   few_out<GLU>(a, m, n, s, u);
 }
@@ -566,21 +567,24 @@ FewCut few_cut(int64_t tiles, int units, int64_t M, int planes, bool glu) {
 }
 
 template <int QT, int P, int NC, int RI, bool GLU, bool X32>
-int launch_few_t(const FewK& k, hipStream_t s) {
+int launch_few_nc(const FewK& k, int raw, hipStream_t s) {
   constexpr int RED = (GLU ? 2 : 1) * few_tiles(NC, GLU) * NC * RI * WAVE * 4, SLOT = few_stage(RI, X32) ? FewStage<P, NC, X32>::BYTES : 0;
   constexpr int WAVE_LDS = RED > SLOT ? RED : SLOT, LDS = few_most(P, NC, GLU) * WAVE_LDS;
   static_assert(LDS <= LDS_BYTES, "LDS");
   const FewCut c = few_cut(k.tiles, k.units, k.M, P, GLU);
   const size_t lds = size_t(c.waves) * WAVE_LDS;
   const dim3 grid(unsigned(c.groups), unsigned(c.blocks), unsigned(c.parts));
+  constexpr bool PARTS = NC > 1 || GLU;
   static DeviceOnce set, set_part;
   if (!set.lds(reinterpret_cast<const void*>(k_few<QT, P, NC, RI, GLU, false, X32>), LDS) ||
-      (NC > 1 && !set_part.lds(reinterpret_cast<const void*>(k_few<QT, P, NC, RI, GLU, NC != 1, X32>), LDS)))
+      (PARTS && !set_part.lds(reinterpret_cast<const void*>(k_few<QT, P, NC, RI, GLU, PARTS, X32>), LDS)))
     return fail(ARTLITE_EHIP, "dense rows: kernel set-up failed");
-  if (NC > 1 && c.parts > 1) {
+  if (raw && (!PARTS || raw != c.parts)) return fail(ARTLITE_EINVAL, "dense rows: %d parts", raw);
+  if (PARTS && (raw || c.parts > 1)) {
     if (!k.parts) return fail(ARTLITE_EINVAL, "dense rows: no scratch for parts");
-    if constexpr (NC > 1) k_few<QT, P, NC, RI, GLU, true, X32><<<grid, 64 * c.waves, lds, s>>>(k);
+    if constexpr (PARTS) k_few<QT, P, NC, RI, GLU, true, X32><<<grid, 64 * c.waves, lds, s>>>(k);
     ART_HIP(hipGetLastError());
+    if (raw) return ARTLITE_OK;
     k_few_join<GLU><<<unsigned((k.M * k.N + 255) / 256), 256, 0, s>>>(k, c.parts);
   } else {
     k_few<QT, P, NC, RI, GLU, false, X32><<<grid, 64 * c.waves, lds, s>>>(k);
@@ -590,26 +594,227 @@ int launch_few_t(const FewK& k, hipStream_t s) {
 }
 
 template <int QT, int P, bool GLU, bool X32 = false>
-int launch_few_p(const FewK& k, hipStream_t s) {
+int launch_few_p(const FewK& k, int raw, hipStream_t s) {
   if constexpr (!GLU && (P == 1 || X32))
     if (k.M <= 16 && k.tiles >= TALL_TILES && k.tiles * k.units >= TALL_UNITS && tall_lds(k, P, 4) <= size_t(LDS_BYTES))
       return k.M <= 4   ? launch_tall_t<QT, P, 1, X32>(k, s)
              : k.M <= 8 ? launch_tall_t<QT, P, 2, X32>(k, s)
                         : launch_tall_t<QT, P, 4, X32>(k, s);
-  if (k.M <= 4) return launch_few_t<QT, P, 1, 1, GLU, X32>(k, s);
-  if (k.M <= 8) return launch_few_t<QT, P, 1, 2, GLU, X32>(k, s);
-  if (X32 || few_nc(k.tiles, k.units, k.M, P, GLU) == 1) return launch_few_t<QT, P, 1, 4, GLU, X32>(k, s);
-  if (k.M <= 32) return launch_few_t<QT, P, 2, 4, GLU, false>(k, s);
-  return launch_few_t<QT, P, 4, 4, GLU, false>(k, s);
+  if (k.M <= 4) return launch_few_nc<QT, P, 1, 1, GLU, X32>(k, raw, s);
+  if (k.M <= 8) return launch_few_nc<QT, P, 1, 2, GLU, X32>(k, raw, s);
+  if (X32 || few_nc(k.tiles, k.units, k.M, P, GLU) == 1) return launch_few_nc<QT, P, 1, 4, GLU, X32>(k, raw, s);
+  if (k.M <= 32) return launch_few_nc<QT, P, 2, 4, GLU, false>(k, raw, s);
+  return launch_few_nc<QT, P, 4, 4, GLU, false>(k, raw, s);
 }
 
 template <int QT>
 int launch_few_q(const FewArgs& a, const FewK& k, hipStream_t s) {
-  if (a.x32) return a.up ? launch_few_p<QT, 3, true, true>(k, s) : launch_few_p<QT, 3, false, true>(k, s);
-  if (a.up) return a.planes == 1 ? launch_few_p<QT, 1, true>(k, s) : launch_few_p<QT, 3, true>(k, s);
-  return a.planes == 1   ? launch_few_p<QT, 1, false>(k, s)
-         : a.planes == 2 ? launch_few_p<QT, 2, false>(k, s)
-                         : launch_few_p<QT, 3, false>(k, s);
+  if (a.x32) return a.up ? launch_few_p<QT, 3, true, true>(k, a.raw, s) : launch_few_p<QT, 3, false, true>(k, 0, s);
+  if (a.up) return a.planes == 1 ? launch_few_p<QT, 1, true>(k, a.raw, s) : launch_few_p<QT, 3, true>(k, a.raw, s);
+  return a.planes == 1   ? launch_few_p<QT, 1, false>(k, 0, s)
+         : a.planes == 2 ? launch_few_p<QT, 2, false>(k, 0, s)
+                         : launch_few_p<QT, 3, false>(k, 0, s);
+}
+
+// ---- the transposed product: out[m][k] = sum_n x[m][n] W[n][k], for few rows
+//
+// Mathematics. W's values as fp16 times 2^-e, rounded once (fp32 calls: two planes), as the large tiles have them; x fp16 rows
+// scaled by rows. The MFMA sums over what lies in a lane's registers, and there a tile has 8 values of one row n, so the codes
+// are turned first, by the MFMA itself: codes (bf16, exact) times a matrix of ones and zeros that picks 16 of the group's 32
+// columns give c[n][k] in fp32 with 4 rows n in a lane, whose scales and offsets make them values, which are rounded and are
+// then an operand of 32 rows (4 and 4 of two tiles) as they are. No weight goes through memory or LDS.
+//
+// Shape. A workgroup takes a unit (256 columns; past 32 rows of x half of one) and a part of the tiles, its waves pairs of
+// tiles in turn; their sums meet in LDS, the parts' in k_join. The scales go to lanes by way of the wave's slot in LDS. What
+// bounds it: about 4 instructions a weight and lane, and the launch.
+struct FewTK {
+  const uint8_t* w[2];
+  const uint16_t* x[2];
+  int pairs;
+  int64_t tiles;
+  int units;
+  int64_t M, ld, x_plane;
+  int e;
+  float* parts;
+  int64_t part_row;
+};
+constexpr int FEW_T_WAVES = 8;
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// PL planes of x and W, NC blocks of 16 rows of x, HU halves of a unit
+template <int QT, int PL, int NC, int HU>
+__global__ __launch_bounds__(FEW_T_WAVES * 64) void k_few_t(const FewTK a) {
+  constexpr int KIND = iq4<QT> ? 0 : -1, UB = unit_bytes<QT>(), G = 4 * HU, CB = 2 * G;
+  constexpr float CC = KIND < 0 ? (QT == ARTLITE_Q4_0 ? -136.0f : -128.0f) : 0.0f;
+  constexpr int RED = 4 * NC * 4 * WAVE;  // (a wave's sums of four blocks of 16 columns)
+  extern __shared__ __attribute__((aligned(16))) float red[];  // [wave][RED]; in the loop the scales: [tile][2][group][row]
+  const Nibbles nib;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lg = lane >> 4, lr = lane & 15;
+  const int u = HU == 2 ? blockIdx.x : blockIdx.x >> 1, h0 = HU == 2 ? 0 : blockIdx.x & 1;
+  const int64_t m0 = int64_t(blockIdx.y) * (16 * NC);
+  const int each = int(a.tiles / 2), all = each * a.pairs;  // (pairs of tiles)
+  const int first = int(int64_t(all) * blockIdx.z / gridDim.z), end = int(int64_t(all) * (blockIdx.z + 1) / gridDim.z);
+  float* const slot = red + wv * RED;
+  static_assert(RED >= 2 * 2 * G * TROWS, "the scales' slot");
+
+  // ones that pick column 16 i + lr of a group's 32
+  u32x4 pick[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+#pragma unroll
+    for (int d = 0; d < 4; d++)
+      pick[i][d] = lg == 2 * i + (lr >> 3) && d == ((lr & 7) >> 1) ? (lr & 1 ? 0x3F800000u : 0x3F80u) : 0u;
+  int64_t xp[NC];
+#pragma unroll
+  for (int c = 0; c < NC; c++) {  // (rows that there are not take the block's first)
+    const int64_t m = m0 + 16 * c + (lr >> 2) + 4 * (lr & 3);
+    xp[c] = (m < a.M ? m : m0) * a.ld + 4 * lg;
+  }
+  f32x4 acc[CB][NC];
+#pragma unroll
+  for (int b = 0; b < CB; b++)
+#pragma unroll
+    for (int c = 0; c < NC; c++) acc[b][c] = f32x4{0, 0, 0, 0};
+
+  uint4 code[2][HU];
+  TileHdr<QT> hd;
+  uint2 x[NC][PL][2];
+  // (lane group lg has the header of tile lg % 2)
+  const auto load = [&](int p) __attribute__((always_inline)) {
+    const int sg = p >= each ? 1 : 0, t = 2 * (p - sg * each);
+    const uint8_t* w = (sg ? a.w[1] : a.w[0]) + (int64_t(t) * a.units + u) * UB;
+    const uint8_t* const wt[2] = {w, w + int64_t(a.units) * UB};
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+      for (int h = 0; h < HU; h++) code[b][h] = *reinterpret_cast<const uint4*>(wt[b] + 1024 * (h0 + h) + 16 * lane);
+    hd.load((lg & 1 ? wt[1] : wt[0]) + 2048 + hdr_bytes<QT>() * lr);
+    const uint16_t* xs = (sg ? a.x[1] : a.x[0]) + 16 * t;
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+      for (int q = 0; q < PL; q++)
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+          x[c][q][b] = *reinterpret_cast<const uint2*>(xs + xp[c] + q * a.x_plane + 16 * b);
+  };
+  if (first + wv < end) load(first + wv);
+  for (int p = first + wv; p < end; p += FEW_T_WAVES) {
+    uint4 cur[2][HU];
+    f16x8 xo[NC][PL];
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+      for (int h = 0; h < HU; h++) cur[b][h] = code[b][h];
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+      for (int q = 0; q < PL; q++)
+        xo[c][q] = __builtin_bit_cast(f16x8, u32x4{x[c][q][0].x, x[c][q][0].y, x[c][q][1].x, x[c][q][1].y});
+    {
+      // the scales of half h of the tile's row lr: of a unit, lane groups 0, 1 have the first half's, 2, 3 the second's
+      float s[4], o[4] = {0, 0, 0, 0}, s1[4], o1[4] = {0, 0, 0, 0};
+      hd.template fields<0>(s, o);
+      hd.template fields<1>(s1, o1);
+      const bool second = HU == 2 ? lg >= 2 : h0 == 1;
+      float* const at = slot + ((lg & 1) * 2 * G + (HU == 2 && second ? 4 : 0)) * TROWS + lr;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        at[j * TROWS] = __builtin_amdgcn_ldexpf(second ? s1[j] : s[j], -a.e);
+        if constexpr (has_offset<QT>) at[(G + j) * TROWS] = __builtin_amdgcn_ldexpf(second ? o1[j] : o[j], -a.e);
+      }
+    }
+    load(p + FEW_T_WAVES < end ? p + FEW_T_WAVES : p);
+    __builtin_amdgcn_wave_barrier();  // (the wave's own slot: its writes come before its reads)
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      u32x4 q[2];
+      f32x4 s[2], o[2];
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+        const uint4& cc = cur[b][g / 4];
+        q[b] = operand<KIND>(g % 4 == 0 ? cc.x : g % 4 == 1 ? cc.y : g % 4 == 2 ? cc.z : cc.w, nib);
+        s[b] = *reinterpret_cast<const f32x4*>(slot + (b * 2 * G + g) * TROWS + 4 * lg);
+        if constexpr (has_offset<QT>) o[b] = *reinterpret_cast<const f32x4*>(slot + ((b * 2 + 1) * G + g) * TROWS + 4 * lg);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        f16x8 hi, lo;
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+          const f32x4 c = mfma(q[b], pick[i], f32x4{CC, CC, CC, CC});
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const float v = has_offset<QT> ? __fsub_rn(__fmul_rn(s[b][r], c[r]), o[b][r]) : s[b][r] * c[r];
+            hi[4 * b + r] = _Float16(v);
+            if constexpr (PL == 2) lo[4 * b + r] = _Float16(v - float(hi[4 * b + r]));
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+          f32x4& d = acc[2 * g + i][c];
+          if constexpr (PL == 2) {
+            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(xo[c][PL - 1], hi, d, 0, 0, 0);
+            d = __builtin_amdgcn_mfma_f32_16x16x32_f16(xo[c][0], lo, d, 0, 0, 0);
+          }
+          d = __builtin_amdgcn_mfma_f32_16x16x32_f16(xo[c][0], hi, d, 0, 0, 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);  // (the groups in turn: registers)
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+  // the waves' sums, in wave order, four blocks of 16 columns at a time: block row 4 g + i is x's row g + 4 i
+#pragma unroll
+  for (int f = 0; f < CB; f += 4) {
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < 4; b++)
+#pragma unroll
+      for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (m0 + 16 * c + 4 * i < a.M) slot[((b * NC + c) * 4 + i) * WAVE + lane] = acc[f + b][c][i];
+    __syncthreads();
+    for (int j = wv; j < 16 * NC; j += FEW_T_WAVES) {
+      const int64_t m = m0 + 16 * (j / 4 % NC) + 4 * (j % 4) + lg, k = u * UNIT + h0 * (UNIT / 2) + 16 * (f + j / (4 * NC)) + lr;
+      if (m >= a.M || k >= a.part_row) continue;
+      float s = 0.0f;
+      for (int w = 0; w < FEW_T_WAVES; w++) s += red[w * RED + j * WAVE + lane];
+      a.parts[(blockIdx.z * a.M + m) * a.part_row + k] = s;
+    }
+  }
+}
+
+struct FewTCut {
+  int nc, cols, parts;
+};
+// blocks of 16 rows and halves of a unit by what registers hold; one workgroup a CU, each wave a pair of tiles at least
+constexpr int few_t_halves(int nc, int planes) { return nc * planes <= 2 ? 2 : 1; }
+FewTCut few_t_cut(int64_t tiles, int units, int pairs, int planes, int64_t M) {
+  FewTCut c{M <= 16 ? 1 : M <= 32 || planes == 2 ? 2 : 4, units, 1};
+  c.cols = units * (3 - few_t_halves(c.nc, planes));
+  const int64_t wgs = c.cols * ((M + 16 * c.nc - 1) / (16 * c.nc)), all = tiles / 2 * pairs;
+  c.parts = int(std::max<int64_t>(1, std::min<int64_t>(256 / wgs, (all + FEW_T_WAVES - 1) / FEW_T_WAVES)));
+  return c;
+}
+template <int QT, int PL, int NC, int HU>
+int launch_few_t_nc(const FewTK& k, const FewTCut& c, hipStream_t s) {
+  constexpr int LDS = FEW_T_WAVES * 4 * NC * 4 * WAVE * 4;
+  static DeviceOnce set;
+  if (!set.lds(reinterpret_cast<const void*>(k_few_t<QT, PL, NC, HU>), LDS)) return fail(ARTLITE_EHIP, "dense rows: kernel set-up failed");
+  k_few_t<QT, PL, NC, HU><<<dim3(unsigned(c.cols), unsigned((k.M + 16 * NC - 1) / (16 * NC)), unsigned(c.parts)),
+                            FEW_T_WAVES * 64, LDS, s>>>(k);
+  ART_HIP(hipGetLastError());
+  return ARTLITE_OK;
+}
+template <int QT, int PL>
+int launch_few_t_p(const FewTK& k, hipStream_t s) {
+  const FewTCut c = few_t_cut(k.tiles, k.units, k.pairs, PL, k.M);
+  if (c.nc == 1) return launch_few_t_nc<QT, PL, 1, few_t_halves(1, PL)>(k, c, s);
+  if (PL == 2 || c.nc == 2) return launch_few_t_nc<QT, PL, 2, few_t_halves(2, PL)>(k, c, s);
+  return launch_few_t_nc<QT, PL, PL == 1 ? 4 : 2, 1>(k, c, s);
 }
 
 }  // namespace
@@ -622,6 +827,10 @@ size_t few_parts_bytes(const artlite_matrix* w, int planes, bool gated, int64_t 
   if (few_apart(w, planes, gated, M)) return 0;
   const FewCut c = few_cut(w->tiles, w->units, M, planes, gated);
   return c.parts > 1 ? size_t(c.parts) * M * w->N * (gated ? 2 : 1) * 4 : 0;
+}
+
+int few_raw_parts(const artlite_matrix* w, int planes, int64_t M) {
+  return few_cut(w->tiles, w->units, M, planes, true).parts;
 }
 
 int launch_few(const FewArgs& a, hipStream_t s) {
@@ -638,9 +847,33 @@ int launch_few(const FewArgs& a, hipStream_t s) {
   k.y = a.y, k.y_stride = a.y_stride, k.dtype = a.dtype, k.act = a.act;
   k.h = a.h, k.h_stride = a.h_stride, k.h_plane = a.h_plane, k.h_planes = a.h_planes;
   k.parts = a.parts;
+  k.part_up = a.raw ? pad64(k.N) : k.N, k.part_row = (a.up ? 2 : 1) * k.part_up;
 #define ART_F(QT) return launch_few_q<QT>(a, k, s)
   ART_TILE_QTYPES(a.w->t->id, ART_F)
 #undef ART_F
+}
+
+int few_t_parts(const artlite_matrix* w, int pairs, int planes, int64_t M) {
+  return few_t_cut(w->tiles, w->units, pairs, planes, M).parts;
+}
+size_t few_t_bytes(const artlite_matrix* w, int pairs, int planes, int64_t M) {
+  return size_t(few_t_parts(w, pairs, planes, M)) * M * pad64(w->K) * 4;
+}
+
+int launch_few_t(const FewTArgs& a, hipStream_t s) {
+  if (a.M <= 0) return ARTLITE_OK;
+  const artlite_matrix *w = a.w[0], *v = a.pairs == 2 ? a.w[1] : w;
+  if (a.pairs < 1 || a.pairs > 2 || v->N != w->N || v->K != w->K || v->t != w->t || w->N % 32 || a.ld % 64 || a.ld < w->N ||
+      a.planes < 1 || a.planes > 2 || !a.parts || a.M > int64_t(65535) * 16)
+    return fail(ARTLITE_EINVAL, "dense rows, transposed: %lld rows of %lld", (long long)a.M, (long long)a.ld);
+  FewTK k{};
+  for (int i = 0; i < a.pairs; i++) k.w[i] = a.w[i]->w.as<uint8_t>(), k.x[i] = a.x[i];
+  k.pairs = a.pairs, k.tiles = w->tiles, k.units = w->units, k.M = a.M;
+  k.ld = a.ld, k.x_plane = a.x_plane, k.e = a.e;
+  k.parts = a.parts, k.part_row = pad64(w->K);
+#define ART_T(QT) return a.planes == 1 ? launch_few_t_p<QT, 1>(k, s) : launch_few_t_p<QT, 2>(k, s)
+  ART_TILE_QTYPES(w->t->id, ART_T)
+#undef ART_T
 }
 
 int launch_planes(const void* x, int dtype, int64_t M, int64_t K, int64_t stride, uint16_t* out, int64_t Kp, int64_t plane,

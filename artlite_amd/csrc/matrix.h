@@ -260,12 +260,33 @@ struct FewArgs {
   int64_t h_stride, h_plane;
   int h_planes;
   float* parts;             // scratch for sums in parts: few_parts_bytes of it
+  // (gated) the two products' sums as they are: `raw` parts of them in parts (few_raw_parts), rows of 2 pad64(N) values, the
+  // second matrix's behind the first's
+  int raw;
 };
 int launch_few(const FewArgs& a, hipStream_t s);
 // Whether a workgroup takes 16 rows of x of one tile, and blocks of 16 rows are workgroups of their own: up to 16 rows, and
 // where the product is small (below).
 bool few_apart(const artlite_matrix* w, int planes, bool gated, int64_t M);
+int few_raw_parts(const artlite_matrix* w, int planes, int64_t M);
 size_t few_parts_bytes(const artlite_matrix* w, int planes, bool gated, int64_t M);
+
+// The transposed product, for few rows: sum over one or two (W, x) of x W -> parts of M rows of pad64(K) fp32 sums each (of
+// the values times 2^-e as they are rounded to fp16: few_t_parts of them, few_t_bytes). x: `planes` (1 or 2) planes of fp16
+// rows, ld a multiple of 64 and at least the matrix's rows, zeros behind them. The matrices are alike, with a
+// multiple of 32 rows.
+struct FewTArgs {
+  const artlite_matrix* w[2];
+  const uint16_t* x[2];
+  int pairs;                // 1 or 2
+  int64_t ld, x_plane;
+  int planes, e;
+  int64_t M;
+  float* parts;
+};
+int few_t_parts(const artlite_matrix* w, int pairs, int planes, int64_t M);
+size_t few_t_bytes(const artlite_matrix* w, int pairs, int planes, int64_t M);
+int launch_few_t(const FewTArgs& a, hipStream_t s);
 // Rows past which the dense products go by way of 16-bit weights and the large tiles. One matrix's of bf16 rows: 4096 x 4096
 // Q4_K, 256 rows, 27 us against 40, 384 rows 40 against 45; 12288 x 2048 IQ4_XS, 256 rows, 37 against 46, 384 rows 54 against
 // 58, 512 rows 73 against 60. Of fp32 rows: 4096 x 4096, 128 rows, 45 against 55, 192 rows 68 against 62. The gated block's:

@@ -70,7 +70,7 @@ def test_forward(H: int, F: int, q: str, down: str, act: str, dtype: str) -> Non
 def test_backward(H: int, F: int, q: str, down: str, act: str, dtype: str) -> None:
     """Every gradient, of rows of very different sizes with rows of zeros among them."""
     f, w = make(H, F, q, down, act)
-    for n in (1, 2, 31, 64, 65, 200):
+    for n in (1, 2, 5, 16, 17, 31, 33, 64, 65, 128, 129, 200):
         x = rows(n, H, dtype, n, 3.0)
         size = 10.0 ** np.random.default_rng(n).uniform(-6, 1, (n, 1))
         size[2::5] = 0.0
