@@ -290,8 +290,9 @@ int launch_few_t(const FewTArgs& a, hipStream_t s);
 // Rows past which the dense products go by way of 16-bit weights and the large tiles. One matrix's of bf16 rows: 4096 x 4096
 // Q4_K, 256 rows, 27 us against 40, 384 rows 40 against 45; 12288 x 2048 IQ4_XS, 256 rows, 37 against 46, 384 rows 54 against
 // 58, 512 rows 73 against 60. Of fp32 rows: 4096 x 4096, 128 rows, 45 against 55, 192 rows 68 against 62. The gated block's:
-// 2048 x 8192, 128 rows, 61 against 78, 192 rows 82 against 78. And any number of rows that are few_apart.
-constexpr int FEW_ROWS = 256, FEW_ROWS_F32 = 128, FEW_ROWS_FFN = 128;
+// 2048 x 8192 Q4_K, 144 rows, 72 against 77, 192 rows 76 against 75, 256 rows 95 against 76; fp32 143, 150 and 217 against 153,
+// 149 and 155; 4096 x 11008 Q4_0, 192 rows, 182 against 220. And any number of rows that are few_apart.
+constexpr int FEW_ROWS = 256, FEW_ROWS_F32 = 128, FEW_ROWS_FFN = 192;
 // x (M rows of K values of dtype, stride apart) as planes of bf16 (1: bf16 as it is; 3: fp32), rows of Kp values (zeros past K)
 int launch_planes(const void* x, int dtype, int64_t M, int64_t K, int64_t stride, uint16_t* out, int64_t Kp, int64_t plane,
                   int planes, hipStream_t s);

@@ -111,7 +111,7 @@ def ffn_streams_and_graphs() -> None:
     for x, y in zip(xs, ys):
         near(y, dense.ffn("silu", host(x), *w), TOL)
     graphs = []
-    for n in (4, 150, 4200):
+    for n in (4, 150, 220, 4200):
         x, dy = rand(n), rand(n)
         out = {"y": torch.empty_like(x), "dx": torch.empty_like(x),
                "dgate": torch.empty(F, H, device="cuda", dtype=torch.bfloat16)}

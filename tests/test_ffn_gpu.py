@@ -58,7 +58,7 @@ def grads(f: GatedFFN, x: np.ndarray, dy: np.ndarray, names: tuple[str, ...] = G
 def test_forward(H: int, F: int, q: str, down: str, act: str, dtype: str) -> None:
     f, w = make(H, F, q, down, act)
     past = min(past_small(F, H, 1 if dtype == "bf16" else 3, True), past_small(H, F, 2))
-    for n in (1, 3, 6, 16, 17, 40, 65, 128, 129, 200, past):
+    for n in (1, 3, 6, 16, 17, 40, 65, 128, 129, 192, 193, 240, past):
         x = rows(n, H, dtype, n, 3.0)
         check(f(x), dense.ffn(act, values(x), *w), FORWARD[dtype])
     assert f(np.empty((0, H), DTYPE[dtype])).shape == (0, H)
@@ -70,7 +70,7 @@ def test_forward(H: int, F: int, q: str, down: str, act: str, dtype: str) -> Non
 def test_backward(H: int, F: int, q: str, down: str, act: str, dtype: str) -> None:
     """Every gradient, of rows of very different sizes with rows of zeros among them."""
     f, w = make(H, F, q, down, act)
-    for n in (1, 2, 5, 16, 17, 31, 33, 64, 65, 128, 129, 200):
+    for n in (1, 2, 5, 16, 17, 31, 33, 64, 65, 128, 129, 192, 193, 240):
         x = rows(n, H, dtype, n, 3.0)
         size = 10.0 ** np.random.default_rng(n).uniform(-6, 1, (n, 1))
         size[2::5] = 0.0
@@ -131,7 +131,7 @@ def test_strides(dtype: str) -> None:
     """Rows at any address and stride; what surrounds the outputs stays; a broadcast dy."""
     H, F = 96, 160
     f, w = make(H, F, "IQ4_NL", "Q4_0")
-    for n in (1, 5, 80, 150, 13200):
+    for n in (1, 5, 80, 200, 13200):
         for at, pad, oat, opad in ((0, 0, 0, 0), (1, 3, 2, 5), (8, 8, 1, 0)):
             xd, dyd = rows(n, H, dtype, 1), rows(n, H, dtype, 2)
             x, dy = (Rows(n, H, dtype, at=at, stride=H + pad, data=d) for d in (xd, dyd))
@@ -154,7 +154,7 @@ def test_strides(dtype: str) -> None:
 def test_rows_are_their_own() -> None:
     """A row of infinities or NaN leaves the others' outputs and gradients as they are."""
     f, _ = make(96, 160, "Q4_0", "Q4_1")
-    for n in (9, 80, 150, 13200):
+    for n in (9, 80, 200, 13200):
         x, dy = rows(n, 96, "bf16", 1), rows(n, 96, "bf16", 2)
         y, dx = f(x), grads(f, x, dy, ("dx",))["dx"]
         bad = x.copy()
