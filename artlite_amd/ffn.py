@@ -48,6 +48,8 @@ class GatedFFN:
 
     def upload(self, name: str, raw: np.ndarray) -> None:
         """A matrix's rows as the file holds them."""
+        if name not in self._m:
+            raise _hip.Error(f"ffn: {name!r}, not one of {', '.join(self._m)}")
         self._m[name].upload(raw)
 
     def close(self) -> None:

@@ -171,11 +171,12 @@ int artlite_hbm_copy(size_t nbytes, int iters, double* ms_per_copy);
  *
  * x, y and the gradients below are DEVICE memory of that device (anything else is refused), bf16 or fp32 (artlite_dtype; y
  * and gradients in x's type), rows of consecutive values `stride` values apart: x's at least 0 (0: one row for all), those
- * of what is written at least the row's values. Calls are enqueued on `stream` (a hipStream_t; null: the null stream) and
+ * of what is written at least the row's values; what is written overlaps nothing else of the call's. Calls are enqueued on `stream` (a hipStream_t; null: the null stream) and
  * return at once; 0 rows write nothing. They may be captured into a graph: its replays use the workspace that was given, and
  * whatever else uses that workspace has to be ordered with them by the caller's streams (a workspace for each graph that
  * runs beside others). Outside captures, calls on one workspace order themselves, whichever streams and threads they come
- * from. */
+ * from. Values of x beyond 2^100 in size may overflow the sums of few rows (the result is then infinite or no number); a
+ * value that is infinite or no number reaches its own row alone. The same call gives the same bits. */
 typedef struct artlite_matrix artlite_matrix;
 int artlite_matrix_supported(int qtype);
 int artlite_matrix_create(int qtype, int64_t rows, int64_t cols, artlite_matrix** out);
@@ -196,8 +197,8 @@ int artlite_stream_capturing(void* stream, int* out);
 int artlite_workspace_destroy(artlite_workspace* work); /* its calls have come to their end */
 
 /* y (n x rows) = x (n x cols) W^T (+ bias). x's products with the blocks' values are summed in fp32 and rounded once to y's
- * type (up to 256 bf16 rows, or 128 fp32 ones, without rounding a weight; past that weights are fp16 of 11 bits for bf16 x, of
- * 22 for fp32 x).
+ * type (up to 256 bf16 rows or 128 fp32 ones, more of a small matrix, without rounding a weight; past that weights are fp16 of
+ * 11 bits for bf16 x, of 22 for fp32 x).
  * artlite_linear_workspace: the bytes of workspace that a call of n rows needs (0 for up to 16 rows); work may be null where
  * that is 0. */
 int artlite_linear_workspace(const artlite_matrix* w, int dtype, int64_t n, size_t* nbytes);

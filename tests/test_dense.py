@@ -84,6 +84,7 @@ refused("100 bytes, not 2304", lambda: l.upload(np.zeros(100, np.uint8)))
 refused("63 values for 64 rows", lambda: l.upload(np.zeros(2304, np.uint8), bias=np.zeros(63, np.float32)))
 refused("activation 'relu'", lambda: GatedFFN(hidden=64, ffn=64, gate_type="Q4_0", down_type="Q4_0", act="relu"))
 lib, f = _hip.lib(), block(64, 96)
+refused("'ffn_norm', not one of ffn_gate, ffn_up, ffn_down", lambda: f.upload("ffn_norm", np.zeros(4, np.uint8)))
 import ctypes
 def matrix(N, K, q="Q4_0", bias=False): return linear(N, K, q, bias)._m
 g, u, d = matrix(96, 64), matrix(96, 64), matrix(64, 96)
