@@ -1,8 +1,9 @@
 // The dense operators' calls: one matrix's product and the gated feed-forward block, forward and backward, on device memory
 // (the C entry points artlite_linear*, artlite_ffn*), and the passes over activations that the large tiles need.
 //
-// Up to FEW_ROWS rows go through k_few (linear.hip), straight from the blocks. More rows go through the large tiles
-// (hgemm.hip), over fp16 operands made for the call in its workspace:
+// Up to FEW_ROWS rows go through k_few (linear.hip; backward also k_few_t), straight from the blocks. More rows go through the
+// large tiles (hgemm.hip), over fp16 operands made for the call in its workspace, or, one matrix's of some hundreds of bf16
+// rows, through tiles that make W's from the blocks (k_qgemm):
 //   x, dy: each row times the power of two that brings its largest value into [2^14, 2^15): bf16 values convert exactly
 //     (those above 2^-29 of their row's largest; smaller ones keep 2^-39 of it), fp32 ones as two planes (hi + lo, 2^-22);
 //   weights: each value times the matrix's power of two, rounded once to fp16 (2^-11; fp32 calls: two planes, 2^-22), an
@@ -198,7 +199,7 @@ constexpr int64_t MOST_ROWS = int64_t(1) << 21;
 // ---- one matrix's product
 
 struct LinearPlan {
-  bool few;
+  bool few, direct = false;
   uint16_t* planes = nullptr;                 // few rows: x as planes, where it is not read as it is
   uint16_t *x16 = nullptr, *w16 = nullptr;    // else
   int32_t* xe = nullptr;
@@ -217,6 +218,12 @@ LinearPlan linear_plan(Carve& c, const artlite_matrix* w, int dtype, int64_t n) 
     const int pl = dtype == ARTLITE_X_BF16 ? 1 : 2;
     const int64_t Kp = pad64(w->K);
     p.x16 = c.take<uint16_t>(size_t(pl) * n * Kp);
+    p.direct = pl == 1 && qgemm_fits(n, w);
+    if (p.direct) {
+      p.xe = c.take<int32_t>(n);
+      p.parts = c.take<float>(qgemm_parts_bytes(n, w) / 4);
+      return p;
+    }
     p.w16 = c.take<uint16_t>(size_t(pl) * w->N * Kp);
     p.xe = c.take<int32_t>(n);
     p.parts = c.take<float>(hgemm_parts_bytes(n, w->N, Kp, pl == 2 ? 3 : 1, false) / 4);
@@ -270,22 +277,26 @@ int linear(const artlite_matrix* w, const void* x, int dtype, int64_t n, int64_t
     a.parts = p.parts;
     return launch_few(a, s);
   }
-  const int pl = dtype == ARTLITE_X_BF16 ? 1 : 2, e = wexp16(w);
+  const int pl = dtype == ARTLITE_X_BF16 ? 1 : 2, e = p.direct ? qexp16(w) : wexp16(w);
   const int64_t Kp = pad64(w->K);
   Rows16 r{};
   r.x[0] = x, r.stride[0] = x_stride, r.out[0] = p.x16, r.e[0] = p.xe;
   r.arrays = 1, r.K = w->K, r.Kp = Kp, r.plane = n * Kp;
   ART_TRY(rows16(r, dtype, n, s));
-  ART_TRY(launch_unpack(w, nullptr, false, e, 0, p.w16, nullptr, Kp, w->N * Kp, pl, s));
   HGemm g{};
-  segments(g, {{p.x16, n * Kp, p.w16, w->N * Kp}}, pl);
+  if (p.direct) {
+    g.a[0] = p.x16, g.segs = 1;
+  } else {
+    ART_TRY(launch_unpack(w, nullptr, false, e, 0, p.w16, nullptr, Kp, w->N * Kp, pl, s));
+    segments(g, {{p.x16, n * Kp, p.w16, w->N * Kp}}, pl);
+  }
   g.lda = g.ldb = g.K = Kp;
   g.M = n, g.N = w->N;
   g.row_e = p.xe, g.e = e;
   g.bias = w->has_bias ? w->bias.as<float>() : nullptr;
   g.y = y, g.y_stride = y_stride, g.dtype = dtype;
   g.parts = p.parts;
-  return launch_hgemm(g, s);
+  return p.direct ? launch_qgemm(g, w, s) : launch_hgemm(g, s);
 }
 
 // ---- the gated block
@@ -313,7 +324,7 @@ int check_ffn(const artlite_ffn* f, Ffn& o, const char* what) {
 }
 
 struct FfnPlan {
-  bool few;
+  bool few, direct;  // (direct: down from its blocks, k_qgemm)
   uint16_t *planes = nullptr, *hp = nullptr;  // few rows: x as planes (where it is not read as it is), h as planes
   uint16_t *x16, *w16, *u16, *d16, *h16;      // else: x, the unpacked matrices, h
   int32_t *xe, *he;
@@ -333,12 +344,14 @@ FfnPlan ffn_plan(Carve& c, const Ffn& f, int dtype, int64_t n) {
   p.x16 = c.take<uint16_t>(pl * n * f.Hp);
   p.w16 = c.take<uint16_t>(pl * f.F * f.Hp);
   p.u16 = c.take<uint16_t>(pl * f.F * f.Hp);
-  p.d16 = c.take<uint16_t>(pl * f.H * f.Fp);
+  p.direct = b && qgemm_fits(n, f.down);
+  if (!p.direct) p.d16 = c.take<uint16_t>(pl * f.H * f.Fp);
   p.h16 = c.take<uint16_t>(pl * n * f.Fp);
   p.xe = c.take<int32_t>(n);
   p.he = c.take<int32_t>(n);
   const int sg = b ? 1 : 3;
-  p.parts = c.take<float>(std::max(hgemm_parts_bytes(n, f.F, f.Hp, sg, true), hgemm_parts_bytes(n, f.H, f.Fp, sg, false)) / 4);
+  p.parts = c.take<float>(std::max(hgemm_parts_bytes(n, f.F, f.Hp, sg, true), p.direct ? qgemm_parts_bytes(n, f.down)
+                                                                                      : hgemm_parts_bytes(n, f.H, f.Fp, sg, false)) / 4);
   return p;
 }
 
@@ -371,7 +384,7 @@ int ffn_forward(const Ffn& f, const void* x, int dtype, int64_t n, int64_t x_str
   r.he = p.he, r.lh = f.gate->row_exp + f.up->row_exp;
   ART_TRY(rows16(r, dtype, n, s));
   ART_TRY(launch_unpack(f.gate, f.up, false, wexp16(f.gate), wexp16(f.up), p.w16, p.u16, f.Hp, f.F * f.Hp, pl, s));
-  ART_TRY(launch_unpack(f.down, nullptr, false, wexp16(f.down), 0, p.d16, nullptr, f.Fp, f.H * f.Fp, pl, s));
+  if (!p.direct) ART_TRY(launch_unpack(f.down, nullptr, false, wexp16(f.down), 0, p.d16, nullptr, f.Fp, f.H * f.Fp, pl, s));
   HGemm g{};
   segments(g, {{p.x16, n * f.Hp, p.w16, f.F * f.Hp, p.u16}}, pl);
   g.lda = g.ldb = g.K = f.Hp;
@@ -383,13 +396,16 @@ int ffn_forward(const Ffn& f, const void* x, int dtype, int64_t n, int64_t x_str
   g.parts = p.parts;
   ART_TRY(launch_hgemm(g, s));
   HGemm d{};
-  segments(d, {{p.h16, n * f.Fp, p.d16, f.H * f.Fp}}, pl);
+  if (p.direct)
+    d.a[0] = p.h16, d.segs = 1;
+  else
+    segments(d, {{p.h16, n * f.Fp, p.d16, f.H * f.Fp}}, pl);
   d.lda = d.ldb = d.K = f.Fp;
   d.M = n, d.N = f.H;
-  d.row_e = p.he, d.e = wexp16(f.down);
+  d.row_e = p.he, d.e = p.direct ? qexp16(f.down) : wexp16(f.down);
   d.y = y, d.y_stride = y_stride, d.dtype = dtype;
   d.parts = p.parts;
-  return launch_hgemm(d, s);
+  return p.direct ? launch_qgemm(d, f.down, s) : launch_hgemm(d, s);
 }
 
 // Rows up to which the gradients' products run from the blocks (dx alone, 2048 x 8192 Q4_K: 192 rows 122 us against 121 by

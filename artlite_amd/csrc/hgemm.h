@@ -3,6 +3,8 @@
 
 #include "common.h"
 
+struct artlite_matrix;
+
 namespace artlite {
 
 // what becomes of the sums: H_STORE y (bf16 or fp32); H_ROWS fp16 rows; H_GLU h of a gated pair; H_DGLU its gradients
@@ -43,6 +45,10 @@ struct HGemm {
 // the scratch that a product may take (gated: N columns of each matrix)
 size_t hgemm_parts_bytes(int64_t M, int64_t N, int64_t K, int segs, bool gated);
 int launch_hgemm(const HGemm& g, hipStream_t s);
+// y = x W^T (H_STORE) with W in its blocks, values times 2^-g.e: a as one segment, no b
+bool qgemm_fits(int64_t M, const artlite_matrix* w);
+size_t qgemm_parts_bytes(int64_t M, const artlite_matrix* w);
+int launch_qgemm(const HGemm& g, const artlite_matrix* w, hipStream_t s);
 // what becomes of sums that are there already, in parts of M rows of pad64(N) values (gated: both matrices' side by side)
 int launch_join(const HGemm& g, int parts, hipStream_t s);
 

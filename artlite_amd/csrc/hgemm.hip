@@ -196,6 +196,17 @@ __host__ __device__ __forceinline__ int64_t part_row(const HGemm& g) {
   return (gated<EPI> ? 2 : 1) * pad64(g.N);
 }
 
+// the tile of a workgroup: those of an XCD (every eighth) take a run of tiles, in columns of 4 tile rows
+__device__ __forceinline__ void deal_tile(int gm, int gn, int& mt, int& nt) {
+  const int total = gm * gn, per = total / 8, rest = total % 8;
+  const int x = int(blockIdx.x) & 7, i = int(blockIdx.x) >> 3;
+  const int t = x * per + (x < rest ? x : rest) + i;
+  constexpr int GR = 4;
+  const int band = t / (GR * gn), in = t % (GR * gn), rows = min(GR, gm - band * GR);
+  mt = __builtin_amdgcn_readfirstlane(band * GR + in % rows);
+  nt = __builtin_amdgcn_readfirstlane(in / rows);
+}
+
 // gm x gn tiles from column 0 on; K in gridDim.y parts (PART: their sums into g.parts, for k_join)
 template <int MB, int EPI, bool PART>
 __global__ __launch_bounds__(256, MB == 8 ? 1 : 2) void k_hgemm(const HGemm g, int gm, int gn) {
@@ -207,17 +218,8 @@ __global__ __launch_bounds__(256, MB == 8 ? 1 : 2) void k_hgemm(const HGemm g, i
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lg = lane >> 4, lr = lane & 15;
   const int wm = wv >> 1, wn = wv & 1;
 
-  // ---- the tile: the workgroups of an XCD (every eighth) take a run of tiles, in columns of 4 tile rows
   int mt, nt;
-  {
-    const int total = gm * gn, per = total / 8, rest = total % 8;
-    const int x = int(blockIdx.x) & 7, i = int(blockIdx.x) >> 3;
-    const int t = x * per + (x < rest ? x : rest) + i;
-    constexpr int GR = 4;
-    const int band = t / (GR * gn), in = t % (GR * gn), rows = min(GR, gm - band * GR);
-    mt = __builtin_amdgcn_readfirstlane(band * GR + in % rows);
-    nt = __builtin_amdgcn_readfirstlane(in / rows);
-  }
+  deal_tile(gm, gn, mt, nt);
   const int64_t m0 = int64_t(mt) * TM, n0 = int64_t(nt) * TN;
   const int mv = int(min(int64_t(TM), g.M - m0)), nv = int(min(int64_t(TN), g.N - n0));  // (rows, columns that there are)
 
@@ -513,6 +515,264 @@ int launch_e(HGemm g, bool mixed, hipStream_t s) {
   return launch_e<EPI>(g, false, s);
 }
 
+
+// ---- the same product with W in its blocks, for hundreds of rows: y = x W^T, x as fp16 rows, W's values made of the codes in
+// registers, as the MFMA's operands
+//
+// A workgroup of 4 waves takes 128 rows of x and 256 of W, a wave 64 of W's and all of x's. x goes through an LDS ring as above;
+// a wave's codes (and headers) go through its own part of LDS by the same DMAs, whose counts then stay one queue, and are
+// values when they are operands: code to fp16 (exact), times its group's scale less its offset in fp16 (both rounded to fp16
+// from fp32 products: a value is off by 2^-11 of its product and of its offset, at most 8 times its group's largest value where
+// `direct` says so, 3 times it where the codes span their range; the large tiles' are by 2^-11 of themselves). That saves the unpacked
+// matrix's way through memory and most of an operand's traffic from L2, which bounds the small tiles; one wave a SIMD does
+// the values' instructions (15 to 28 for 8 of them) between the MFMAs of the step before. A step (32 values of K) takes 0.55 us
+// with one workgroup a CU and 0.95 with two, which is neither the ring's depth (8 slots: the same), the barriers (every second
+// step: the same) nor the operands' latency (read 5 blocks ahead: the same): 1.1 to 1.3 PFLOP/s where the large tiles have 1.4.
+// 1000 rows of 4096 x 4096 Q4_K: 46 us and 7 to join 2 parts; of 6144 x 2048 IQ4_NL 44.
+constexpr int Q_TM = 128, Q_TN = 256, Q_RING = 4, Q_SLOT = Q_TM * BK * 2;
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+// the fp16 values of a code dword, with its scale and offset (twice in a word each)
+template <int QT>
+__device__ __forceinline__ u32x4 q_values(uint32_t w, uint32_t s, uint32_t o, uint32_t mask, uint32_t top) {
+  const f16x2 sc = __builtin_bit_cast(f16x2, s);
+  u32x4 r;
+  if constexpr (iq4<QT>) {
+    r = lut_operand<3>(w);
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, uint32_t(r[i])) * sc);
+  } else {
+    constexpr _Float16 Z = QT == ARTLITE_Q4_0 ? _Float16(-1032.0f) : _Float16(-1024.0f);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const f16x2 c = __builtin_bit_cast(f16x2, ((w >> (4 * i)) & mask) | top) + f16x2{Z, Z};  // (1024 + c)
+      f16x2 v;
+      if constexpr (has_offset<QT>)
+        v = __builtin_elementwise_fma(c, sc, __builtin_bit_cast(f16x2, o));
+      else
+        v = c * sc;
+      r[i] = __builtin_bit_cast(uint32_t, v);
+    }
+  }
+  return r;
+}
+
+template <int QT, bool PART>
+__global__ __launch_bounds__(256, 1) void k_qgemm(const HGemm g, const uint8_t* __restrict__ w, int64_t tiles, int units, int e,
+                                                  int gm, int gn) {
+  constexpr int UB = unit_bytes<QT>(), HB = hdr_bytes<QT>(), HD = HB == 32 ? 2 : 1;  // (header DMAs a unit)
+  constexpr int CODES = Q_RING * Q_SLOT, HDRS = CODES + 4 * 8192, LDS = HDRS + 4 * 2048;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lg = lane >> 4, lr = lane & 15;
+  int mt, nt;
+  deal_tile(gm, gn, mt, nt);
+  const int64_t m0 = int64_t(mt) * Q_TM, n0 = int64_t(nt) * Q_TN;
+  const int mv = int(min(int64_t(Q_TM), g.M - m0));
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(hg_lds_addr(lds));
+  uint32_t mask = 0x000F000Fu, top = 0x64006400u;
+  asm("" : "+s"(mask), "+v"(top));
+
+  uint32_t offa[2];
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int r = 16 * (2 * wv + i) + (lane >> 2), c = (lane & 3) ^ ((r >> 1) & 3);
+    offa[i] = uint32_t(min(r, mv - 1)) * uint32_t(g.lda) * 2 + 16 * c;
+  }
+  // (tiles past the last: the last again, their columns are not stored)
+  const int64_t tw = n0 / TROWS + 4 * wv, t0 = min(tw, tiles - 1);
+  uint32_t tile_at[4], offh[HD];
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+    tile_at[j] = __builtin_amdgcn_readfirstlane(uint32_t(min(tw + j, tiles - 1) - t0) * uint32_t(units) * UB);
+  {
+    constexpr int LT = TROWS * HB / 16;  // lanes of a tile's headers
+#pragma unroll
+    for (int d = 0; d < HD; d++) {
+      const int j = LT >= 64 ? 0 : (lane / LT + d * (64 / LT)) & 3;
+      offh[d] = uint32_t(min(tw + j, tiles - 1) - t0) * uint32_t(units) * UB + 16 * (lane % LT);
+    }
+  }
+  const uint8_t* const wbase = w + t0 * units * UB;
+  const int steps_all = int(g.K / BK);
+  const int u0 = PART ? int(int64_t(units) * blockIdx.y / gridDim.y) : 0;
+  const int u1 = PART ? int(int64_t(units) * (blockIdx.y + 1) / gridDim.y) : units;
+  const int steps = min(8 * u1, steps_all);  // (of K)
+  const uint16_t* const abase = g.a[0] + m0 * g.lda;
+  auto dma_a = [&](int i, int t) __attribute__((always_inline)) {
+    const uint32_t d = __builtin_amdgcn_readfirstlane(lds0 + (t & (Q_RING - 1)) * Q_SLOT + (2 * wv + i) * 1024);
+    hg_dma(hg_uniform(abase + int64_t(min(t, steps - 1)) * BK), offa[i], d);
+  };
+  auto dma_code = [&](int j, int h, int u) __attribute__((always_inline)) {
+    const uint32_t d = __builtin_amdgcn_readfirstlane(lds0 + CODES + wv * 8192 + (h * 4 + j) * 1024);
+    const uint8_t* p = wbase + int64_t(min(u, u1 - 1)) * UB + tile_at[j] + 1024 * h;
+    hg_dma(hg_uniform(reinterpret_cast<const uint16_t*>(p)), 16 * lane, d);
+  };
+  auto dma_hdr = [&](int d, int u) __attribute__((always_inline)) {
+    const uint8_t* p = wbase + int64_t(min(u, u1 - 1)) * UB + 2048;
+    hg_dma(hg_uniform(reinterpret_cast<const uint16_t*>(p)), offh[d],
+           __builtin_amdgcn_readfirstlane(lds0 + HDRS + wv * 2048 + d * 1024));
+  };
+
+  f32x4 acc[8][4];
+  hg_for<8>([&](auto i) {
+    hg_for<4>([&](auto j) { acc[i][j] = f32x4{0, 0, 0, 0}; });
+  });
+  const uint32_t lo = lr * 64 + ((lg ^ ((lr >> 1) & 3)) << 4);
+  auto ld = [](const uint8_t* p) __attribute__((always_inline)) { return *reinterpret_cast<const u32x4*>(p); };
+  u32x4 fa[4], fb[2][4], code[4], code2[4];
+  uint32_t sc[4][4], of[4][4], sc2[4][4], of2[4][4];
+  TileHdr<QT> hd[4];
+  const uint8_t* const mycodes = lds + CODES + wv * 8192 + 16 * lane;
+  const uint8_t* const myhdrs = lds + HDRS + wv * 2048 + HB * lr;
+  auto read_hdrs = [&]() __attribute__((always_inline)) {
+    hg_for<4>([&](auto j) { hd[j].load(myhdrs + decltype(j)::value * TROWS * HB); });
+  };
+  auto read_codes = [&](int h) __attribute__((always_inline)) {
+    hg_for<4>([&](auto j) { code2[j] = ld(mycodes + (4 * h + decltype(j)::value) * 1024); });
+  };
+  // a tile's scales of half H
+  auto scales = [&](auto jc, auto hc) __attribute__((always_inline)) {
+    constexpr int j = decltype(jc)::value, H = decltype(hc)::value;
+    float s[4], o[4] = {0, 0, 0, 0};
+    hd[j].template fields<H>(s, o);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const _Float16 a = _Float16(__builtin_amdgcn_ldexpf(s[k], -e)), b = _Float16(-__builtin_amdgcn_ldexpf(o[k], -e));
+      sc2[j][k] = __builtin_bit_cast(uint32_t, f16x2{a, a});
+      if constexpr (has_offset<QT>) of2[j][k] = __builtin_bit_cast(uint32_t, f16x2{b, b});
+    }
+  };
+  auto next_half = [&]() __attribute__((always_inline)) {
+    hg_for<4>([&](auto jc) __attribute__((always_inline)) {
+      constexpr int j = decltype(jc)::value;
+      code[j] = code2[j];
+      hg_for<4>([&](auto k) { sc[j][k] = sc2[j][k], of[j][k] = has_offset<QT> ? of2[j][k] : 0; });
+    });
+  };
+  // operand j of the group gi of the half at hand
+  auto values = [&](auto jc, auto gc) __attribute__((always_inline)) {
+    constexpr int j = decltype(jc)::value, gi = decltype(gc)::value;
+    return q_values<QT>(code[j][gi], sc[j][gi], of[j][gi], mask, top);
+  };
+
+  const int s0 = 8 * u0;
+  for (int d = 0; d < HD; d++) dma_hdr(d, u0);
+  for (int j = 0; j < 4; j++) dma_code(j, 0, u0);
+  for (int t = 0; t < 2; t++)
+    for (int i = 0; i < 2; i++) dma_a(i, s0 + t);
+  for (int j = 0; j < 4; j++) dma_code(j, 1, u0);
+  for (int i = 0; i < 2; i++) dma_a(i, s0 + 2);
+  hg_wait<6>();
+  hg_barrier();
+  read_hdrs();
+  read_codes(0);
+  hg_for<4>([&](auto j) { scales(j, std::integral_constant<int, 0>{}); });
+  next_half();
+  hg_for<4>([&](auto j) { fb[0][j] = values(j, std::integral_constant<int, 0>{}); });
+  fa[0] = ld(lds + lo);
+  fa[1] = ld(lds + lo + 1024);
+
+  // Step t = 8 u + J on ring slot t % 4: its operands of W are there; the next step's are made meanwhile. Loads issued in it:
+  // a tile's codes of the same half of unit u + 1, at J = 0 its headers, x of step t + 3. At its barrier all that was issued
+  // up to step t - 2 has landed: x of step t + 1, the other half's codes (read into registers at J = 2 and 6, a step before
+  // their first use), the next unit's headers.
+  auto step = [&](auto jc, int u) __attribute__((always_inline)) {
+    constexpr int J = decltype(jc)::value, S = J & 1;
+    const int t = 8 * u + J;
+    hg_wait<(J == 1 ? 3 + HD : 3)>();
+    hg_barrier();
+    const uint8_t *sa = lds + (t & 3) * Q_SLOT + lo, *na = lds + ((t + 1) & 3) * Q_SLOT + lo;
+    if constexpr (J == 6) read_hdrs();
+    if constexpr (J == 2) read_codes(1);
+    if constexpr (J == 6) read_codes(0);
+    hg_for<8>([&](auto ic) __attribute__((always_inline)) {
+      constexpr int i = decltype(ic)::value;
+      fa[(i + 2) % 4] = i + 2 < 8 ? ld(sa + 1024 * (i + 2)) : ld(na + 1024 * (i + 2 - 8));
+      if constexpr (i == 0) dma_code(J & 3, J >> 2, u + 1);
+      if constexpr (i == 1 && J == 0)
+        for (int d = 0; d < HD; d++) dma_hdr(d, u + 1);
+      if constexpr (i == 2 || i == 3) dma_a(i - 2, t + 3);
+      if constexpr (i % 2 == 1 && J % 4 == 2) scales(std::integral_constant<int, i / 2>{}, std::integral_constant<int, J == 2>{});
+      if constexpr (i == 0 && J % 4 == 3) next_half();
+      if constexpr (i % 2 == 0) fb[1 - S][i / 2] = values(std::integral_constant<int, i / 2>{}, std::integral_constant<int, (J + 1) % 4>{});
+      hg_for<4>([&](auto j) __attribute__((always_inline)) { acc[i][j] = hg_mfma(fb[S][j], fa[i % 4], acc[i][j]); });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  for (int u = u0; u < u1; u++)
+    hg_for<4>([&](auto pc) __attribute__((always_inline)) {
+      constexpr int P = decltype(pc)::value;
+      if (P == 0 || 8 * u + 2 * P < steps) {  // (K is a multiple of 64)
+        step(std::integral_constant<int, 2 * P>{}, u);
+        step(std::integral_constant<int, 2 * P + 1>{}, u);
+      }
+    });
+  hg_wait<0>();
+  hg_barrier();
+
+  // ---- outputs, as above
+  RowExp* const rows_e = reinterpret_cast<RowExp*>(lds + LDS - Q_TM * sizeof(RowExp));
+  if constexpr (!PART) {
+    for (int r = threadIdx.x; r < Q_TM; r += 256) rows_e[r] = row_exp<H_STORE>(g, m0 + min(r, mv - 1));
+    __syncthreads();
+  }
+  constexpr int LROW = 64 + 4;
+  float* const buf = reinterpret_cast<float*>(lds) + wv * 32 * LROW;
+  static_assert(4 * 32 * LROW * 4 + Q_TM * sizeof(RowExp) <= LDS, "LDS");
+  const int64_t n = n0 + 64 * wv + 8 * (lane & 7);
+  const float* const from = buf + (lane >> 3) * LROW + 8 * (lane & 7);
+  float bias[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (!PART && g.bias)
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      if (n + k < g.N) bias[k] = g.bias[n + k];
+  hg_for<4>([&](auto pc) __attribute__((always_inline)) {
+    constexpr int P = decltype(pc)::value;
+    hg_for<2>([&](auto i) __attribute__((always_inline)) {
+      hg_for<4>([&](auto j) __attribute__((always_inline)) {
+        *reinterpret_cast<f32x4*>(buf + (16 * i + lr) * LROW + 16 * j + 4 * lg) = acc[2 * P + decltype(i)::value][j];
+      });
+    });
+#pragma unroll 1
+    for (int r = 0; r < 32; r += 8) {
+      const int row = 32 * P + r + (lane >> 3);
+      const int64_t m = m0 + row;
+      if (m >= g.M) continue;
+      const f32x4 a = *reinterpret_cast<const f32x4*>(from + r * LROW), b = *reinterpret_cast<const f32x4*>(from + r * LROW + 4);
+      if constexpr (PART) {
+        const int64_t pr = part_row<H_STORE>(g);
+        float* o = g.parts + (int64_t(blockIdx.y) * g.M + m) * pr + n;
+        if (n < pr) {
+          *reinterpret_cast<f32x4*>(o) = a;
+          *reinterpret_cast<f32x4*>(o + 4) = b;
+        }
+      } else {
+        float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}, none[8];
+        finish<H_STORE>(g, g.e, rows_e[row], m, n, v, none, bias);
+      }
+    }
+  });
+}
+
+template <int QT>
+int launch_q(const HGemm& g, const artlite_matrix* w, int parts, hipStream_t s) {
+  constexpr int LDS = Q_RING * Q_SLOT + 4 * 8192 + 4 * 2048;
+  const int64_t gm = (g.M + Q_TM - 1) / Q_TM, gn = (g.N + Q_TN - 1) / Q_TN;
+  static DeviceOnce set, set_part;
+  if (!set.lds(reinterpret_cast<const void*>(k_qgemm<QT, false>), LDS) ||
+      !set_part.lds(reinterpret_cast<const void*>(k_qgemm<QT, true>), LDS))
+    return fail(ARTLITE_EHIP, "dense tiles: kernel set-up failed");
+  const dim3 grid(unsigned(gm * gn), unsigned(parts));
+  if (parts == 1) {
+    k_qgemm<QT, false><<<grid, 256, LDS, s>>>(g, w->w.as<uint8_t>(), w->tiles, w->units, g.e, int(gm), int(gn));
+    ART_HIP(hipGetLastError());
+    return ARTLITE_OK;
+  }
+  k_qgemm<QT, true><<<grid, 256, LDS, s>>>(g, w->w.as<uint8_t>(), w->tiles, w->units, g.e, int(gm), int(gn));
+  ART_HIP(hipGetLastError());
+  return join<H_STORE>(g, parts, s);
+}
+
 }  // namespace
 
 size_t hgemm_parts_bytes(int64_t M, int64_t N, int64_t K, int segs, bool gate) {
@@ -548,6 +808,37 @@ int launch_join(const HGemm& g, int parts, hipStream_t s) {
          : g.epilogue == H_ROWS ? join<H_ROWS>(h, parts, s)
          : g.epilogue == H_GLU  ? join<H_GLU>(h, parts, s)
                                 : join<H_DGLU>(h, parts, s);
+}
+
+// Where it is the faster way (against unpacking W and the tiles above): for what is one workgroup a CU at most (4096 x 4096 Q4_K,
+// 257 rows 36 us against 42, 2048 rows, 256 workgroups, 80 against 95, 3000 rows, 384, 125 against 115; 4096 x 12288 Q4_0, 512
+// rows 75 against 105, 2048 rows 198 against 225; 12288 x 4096 IQ4_XS, 512 rows 88 against 101, 700 rows, 288, 137 against
+// 118), and where the unpacking is most of the work (32768 x 2048 Q4_K, 512 rows, 512 workgroups, 77 against 98).
+bool qgemm_fits(int64_t M, const artlite_matrix* w) {
+  return w->direct && int64_t(4) * w->units * w->ub < (int64_t(1) << 32) &&
+         (M <= 512 || (M + Q_TM - 1) / Q_TM * ((w->N + Q_TN - 1) / Q_TN) <= CUS);
+}
+// the parts of K: as long as they fill CUs and a part has two units
+int qgemm_parts(int64_t M, const artlite_matrix* w) {
+  const int64_t wgs = (M + Q_TM - 1) / Q_TM * ((w->N + Q_TN - 1) / Q_TN);
+  int parts = 1;
+  while (wgs * parts * 2 <= CUS && w->units / (2 * parts) >= 2) parts *= 2;
+  return parts;
+}
+size_t qgemm_parts_bytes(int64_t M, const artlite_matrix* w) {
+  const int parts = qgemm_parts(M, w);
+  return parts > 1 ? size_t(parts) * M * pad64(w->N) * 4 : 0;
+}
+
+int launch_qgemm(const HGemm& g, const artlite_matrix* w, hipStream_t s) {
+  if (g.M <= 0) return ARTLITE_OK;
+  const int parts = qgemm_parts(g.M, w);
+  if (g.K != pad64(w->K) || g.lda < g.K || g.lda % 8 || g.lda > (int64_t(1) << 22) || g.N != w->N || g.segs != 1 ||
+      !qgemm_fits(g.M, w) || (parts > 1 && !g.parts))
+    return fail(ARTLITE_EINVAL, "dense tiles: K %lld of rows of %lld", (long long)g.K, (long long)g.lda);
+#define ART_Q(QT) return launch_q<QT>(g, w, parts, s)
+  ART_TILE_QTYPES(w->t->id, ART_Q)
+#undef ART_Q
 }
 
 }  // namespace artlite

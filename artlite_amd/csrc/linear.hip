@@ -26,32 +26,6 @@ namespace artlite {
 
 namespace {
 
-constexpr uint32_t bf16_of(int v) { return __builtin_bit_cast(uint32_t, float(v)) >> 16; }
-
-// 16 values as byte tables of their bf16 halves
-struct Lut16 {
-  uint32_t lo[4], hi[4];
-};
-constexpr Lut16 make_lut(int kind) {  // 0: IQ4's values, 1: c - 8, 2: c
-  constexpr int V[16] = {-127, -104, -83, -65, -49, -35, -22, -10, 1, 13, 25, 38, 53, 69, 89, 113};
-  Lut16 t{};
-  for (int i = 0; i < 16; i++) {
-    const uint32_t b = bf16_of(kind == 0 ? V[i] : kind == 1 ? i - 8 : i);
-    t.lo[i / 4] |= (b & 0xFF) << (8 * (i % 4));
-    t.hi[i / 4] |= (b >> 8) << (8 * (i % 4));
-  }
-  return t;
-}
-template <int KIND>
-__device__ __forceinline__ void lut_bytes(uint32_t c, uint32_t& lo, uint32_t& hi) {
-  constexpr Lut16 T = make_lut(KIND);
-  const uint32_t s = c & 0x07070707u;
-  // bytes of ones where the code's bit 3 is set (selectors 8 .. 11: the sign of bytes 1, 3 of the second and first source)
-  const uint32_t m = __builtin_amdgcn_perm(c << 4, c << 12, 0x0B090A08u);
-  lo = (__builtin_amdgcn_perm(T.lo[3], T.lo[2], s) & m) | (__builtin_amdgcn_perm(T.lo[1], T.lo[0], s) & ~m);
-  hi = (__builtin_amdgcn_perm(T.hi[3], T.hi[2], s) & m) | (__builtin_amdgcn_perm(T.hi[1], T.hi[0], s) & ~m);
-}
-
 // the constants of a code dword's operand in registers: an and-or takes them so, literals make it two instructions
 struct Nibbles {
   uint32_t mask = 0x000F000Fu, top = 0x43004300u;
@@ -63,11 +37,7 @@ __device__ __forceinline__ u32x4 operand(uint32_t w, const Nibbles& n) {
   if constexpr (KIND < 0) {
     return u32x4{(w & n.mask) | n.top, ((w >> 4) & n.mask) | n.top, ((w >> 8) & n.mask) | n.top, ((w >> 12) & n.mask) | n.top};
   } else {
-    uint32_t l0, h0, l1, h1;  // (nibbles 0, 2, 4, 6 and 1, 3, 5, 7)
-    lut_bytes<KIND>(w & 0x0F0F0F0Fu, l0, h0);
-    lut_bytes<KIND>((w >> 4) & 0x0F0F0F0Fu, l1, h1);
-    return u32x4{__builtin_amdgcn_perm(h0, l0, 0x06020400u), __builtin_amdgcn_perm(h1, l1, 0x06020400u),
-                 __builtin_amdgcn_perm(h0, l0, 0x07030501u), __builtin_amdgcn_perm(h1, l1, 0x07030501u)};
+    return lut_operand<KIND>(w);
   }
 }
 

@@ -15,7 +15,7 @@
 //     (dword >> 4 p) & 0x000F000F are the codes of values 2 p and 2 p + 1: one 16-bit operand dword of the MFMA;
 //   header: Q4_0, IQ4_NL: the 8 groups' fp16 scales; Q4_1: their (scale, min) pairs; Q4_K: the block's 16 bytes before its
 //     codes (d, dmin, the 6-bit scales and mins); IQ4_XS: its 8 (d and the 6-bit scales).
-// The bytes are the file's (but for the padding), in the order in which a wave reads them: 1 KiB of codes a load, contiguous.
+// The bytes are the file's (but for the padding and the scales of Q4_0's blocks of zeros), in the order in which a wave reads them: 1 KiB of codes a load, contiguous.
 namespace artlite {
 
 constexpr int UNIT = 256;   // values of a unit
@@ -95,6 +95,43 @@ template <int QT>
 constexpr bool has_offset = QT == ARTLITE_Q4_1 || QT == ARTLITE_Q4_K;
 template <int QT>
 constexpr bool iq4 = QT == ARTLITE_IQ4_NL || QT == ARTLITE_IQ4_XS;
+
+constexpr uint32_t bf16_of(int v) { return __builtin_bit_cast(uint32_t, float(v)) >> 16; }
+constexpr uint32_t f16_of(int v) { return __builtin_bit_cast(uint16_t, _Float16(v)); }
+
+// 16 values as byte tables of their 16-bit forms' halves
+struct Lut16 {
+  uint32_t lo[4], hi[4];
+};
+constexpr Lut16 make_lut(int kind) {  // 0: IQ4's values, 1: c - 8, 2: c (bf16), 3: IQ4's values in fp16
+  constexpr int V[16] = {-127, -104, -83, -65, -49, -35, -22, -10, 1, 13, 25, 38, 53, 69, 89, 113};
+  Lut16 t{};
+  for (int i = 0; i < 16; i++) {
+    const uint32_t b = kind == 3 ? f16_of(V[i]) : bf16_of(kind == 0 ? V[i] : kind == 1 ? i - 8 : i);
+    t.lo[i / 4] |= (b & 0xFF) << (8 * (i % 4));
+    t.hi[i / 4] |= (b >> 8) << (8 * (i % 4));
+  }
+  return t;
+}
+template <int KIND>
+__device__ __forceinline__ void lut_bytes(uint32_t c, uint32_t& lo, uint32_t& hi) {
+  constexpr Lut16 T = make_lut(KIND);
+  const uint32_t s = c & 0x07070707u;
+  // bytes of ones where the code's bit 3 is set (selectors 8 .. 11: the sign of bytes 1, 3 of the second and first source)
+  const uint32_t m = __builtin_amdgcn_perm(c << 4, c << 12, 0x0B090A08u);
+  lo = (__builtin_amdgcn_perm(T.lo[3], T.lo[2], s) & m) | (__builtin_amdgcn_perm(T.lo[1], T.lo[0], s) & ~m);
+  hi = (__builtin_amdgcn_perm(T.hi[3], T.hi[2], s) & m) | (__builtin_amdgcn_perm(T.hi[1], T.hi[0], s) & ~m);
+}
+
+// a code dword's 8 values by table, as MFMA operand dwords
+template <int KIND>
+__device__ __forceinline__ u32x4 lut_operand(uint32_t w) {
+  uint32_t l0, h0, l1, h1;  // (nibbles 0, 2, 4, 6 and 1, 3, 5, 7)
+  lut_bytes<KIND>(w & 0x0F0F0F0Fu, l0, h0);
+  lut_bytes<KIND>((w >> 4) & 0x0F0F0F0Fu, l1, h1);
+  return u32x4{__builtin_amdgcn_perm(h0, l0, 0x06020400u), __builtin_amdgcn_perm(h1, l1, 0x06020400u),
+               __builtin_amdgcn_perm(h0, l0, 0x07030501u), __builtin_amdgcn_perm(h1, l1, 0x07030501u)};
+}
 
 // the 8 values of a code dword as fp32, in order (dequantized as the file's: rows of artlite_dequant_rows)
 template <int QT>
@@ -234,6 +271,7 @@ struct artlite_matrix {
   int units = 0;
   int ub = 0;              // bytes a unit of a tile
   bool have = false, has_bias = false;
+  bool direct = false;     // no group's scale and offset are many times its values (k_qgemm, hgemm.hip)
   artlite::DevBuf w, bias;
   int max_exp = 0;         // every |value| < 2^max_exp
   int row_exp = 0;         // every row's 2-norm < 2^row_exp
@@ -304,8 +342,13 @@ int launch_planes(const void* x, int dtype, int64_t M, int64_t K, int64_t stride
 // m2: with a second matrix of the same shape and format, into out2.
 int launch_unpack(const artlite_matrix* m, const artlite_matrix* m2, bool transposed, int e, int e2, uint16_t* out,
                   uint16_t* out2, int64_t ld, int64_t plane, int planes, hipStream_t s);
+// the scale of a `direct` matrix's values where their scales and offsets are fp16 too (offsets up to 8 times the values)
+inline int qexp16(const artlite_matrix* m);
 // the scale that brings a matrix's largest value into [2^14, 2^15)
 inline int wexp16(const artlite_matrix* m) { return m->max_exp - 15; }
+inline int qexp16(const artlite_matrix* m) {
+  return wexp16(m) + (m->t->id == ARTLITE_Q4_1 || m->t->id == ARTLITE_Q4_K ? 3 : 0);
+}
 
 __host__ __device__ inline int64_t pad64(int64_t v) { return (v + 63) / 64 * 64; }
 

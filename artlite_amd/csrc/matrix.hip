@@ -81,6 +81,12 @@ __global__ __launch_bounds__(128) void k_tile(const uint8_t* __restrict__ raw, i
         if (k < K) {
           const uint8_t* b = rr + k / 32 * BYTES + 2 * (w % F);
           x = uint16_t(b[0] | b[1] << 8);
+          if constexpr (QT == ARTLITE_Q4_0) {
+            // (a block of zeros keeps no scale, which the sums' roundings would carry; one that is no number stays)
+            bool zeros = (x & 0x7C00) != 0x7C00;
+            for (int j = 0; j < 16; j++) zeros &= b[2 + j] == 0x88;
+            if (zeros) x = 0;
+          }
         }
       }
     }
@@ -88,7 +94,7 @@ __global__ __launch_bounds__(128) void k_tile(const uint8_t* __restrict__ raw, i
   }
 }
 
-// a lane's 32 values of half H of a unit: f(g, v) with values 8 lg .. + 8 of each of its groups g
+// a lane's 32 values of half H of a unit: f(g, v) with values 8 lg .. + 8 of each of its groups g, or f(g, v, scale, offset)
 template <int QT, int H, class F>
 __device__ __forceinline__ void tile_half(const uint8_t* ub, int lane, F&& f) {
   TileHdr<QT> hd;
@@ -101,7 +107,10 @@ __device__ __forceinline__ void tile_half(const uint8_t* ub, int lane, F&& f) {
   for (int j = 0; j < 4; j++) {
     float v[8];
     tile_values<QT>(w[j], s[j], o[j], v);
-    f(4 * H + j, v);
+    if constexpr (std::is_invocable_v<F, int, const float(&)[8]>)
+      f(4 * H + j, v);
+    else
+      f(4 * H + j, v, s[j], o[j]);
   }
 }
 template <int QT, class F>
@@ -121,7 +130,8 @@ __device__ __forceinline__ void halves(const float (&v)[8], int e, uint16_t (&a)
   }
 }
 
-// out[0] = max |value|, out[1] = the largest 2-norm of a row, as bits (finite values; atomic maxima of floats that are not
+// out[0] = max |value|, out[1] = the largest 2-norm of a row (out[2]: whether a group's scale and offset are many times its
+// values, which are then a small difference of theirs), as bits (finite values; atomic maxima of floats that are not
 // negative): a workgroup of 4 waves per tile
 template <int QT>
 __global__ __launch_bounds__(256) void k_bounds(const uint8_t* __restrict__ w, int units, int64_t K, uint32_t* out) {
@@ -129,15 +139,26 @@ __global__ __launch_bounds__(256) void k_bounds(const uint8_t* __restrict__ w, i
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const uint8_t* t = w + int64_t(blockIdx.x) * units * unit_bytes<QT>();
   float mx = 0.0f, ss = 0.0f;
+  bool far = false;
   for (int u = wv; u < units; u += 4)
-    tile_unit<QT>(t + int64_t(u) * unit_bytes<QT>(), lane, [&](int g, const float(&v)[8]) {
-      if (int64_t(u) * UNIT + 32 * g >= K) return;
+    tile_unit<QT>(
+        t + int64_t(u) * unit_bytes<QT>(), lane,
+        [&](int g, const float(&v)[8], float s, float o) {
+          if (int64_t(u) * UNIT + 32 * g >= K) return;
+          float gx = 0.0f;
 #pragma unroll
-      for (int p = 0; p < 8; p++) {
-        mx = fmaxf(mx, fabsf(v[p]));
-        ss = __builtin_fmaf(v[p], v[p], ss);
-      }
-    });
+          for (int p = 0; p < 8; p++) {
+            gx = fmaxf(gx, fabsf(v[p]));
+            ss = __builtin_fmaf(v[p], v[p], ss);
+          }
+          mx = fmaxf(mx, gx);
+          if constexpr (has_offset<QT>) {
+            gx = fmaxf(gx, __shfl_xor(gx, 16));  // (the row's other lanes)
+            gx = fmaxf(gx, __shfl_xor(gx, 32));
+            far |= !(15.0f * fabsf(s) + fabsf(o) <= 8.0f * gx);
+          }
+        });
+  if (has_offset<QT> && far) atomicMax(out + 2, 1u);
   for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
   ss += __shfl_xor(ss, 16);
   ss += __shfl_xor(ss, 32);
@@ -321,9 +342,9 @@ int matrix_upload(artlite_matrix* m, const void* data) {
   ART_TRY(raw.reserve(nb));
   ART_TRY(c->flag.reserve(256));
   ART_TRY(m->w.reserve(size_t(m->tiles) * m->units * m->ub + WEIGHT_TAIL));
-  uint32_t b[2] = {0, 0};
+  uint32_t b[3] = {0, 0, 0};
   ART_HIP(hipMemcpyAsync(raw.p, data, nb, hipMemcpyHostToDevice, c->stream));
-  ART_HIP(hipMemcpyAsync(c->flag.p, b, 8, hipMemcpyHostToDevice, c->stream));
+  ART_HIP(hipMemcpyAsync(c->flag.p, b, 12, hipMemcpyHostToDevice, c->stream));
   const unsigned grid = unsigned(m->tiles * m->units);
 #define ART_T(QT)                                                                                                   \
   k_tile<QT, QT == ARTLITE_Q4_K || QT == ARTLITE_IQ4_XS ? 256 : 32,                                                 \
@@ -334,13 +355,14 @@ int matrix_upload(artlite_matrix* m, const void* data) {
   ART_TILE_QTYPES(m->t->id, ART_T)
 #undef ART_T
   ART_HIP(hipGetLastError());
-  ART_HIP(hipMemcpyAsync(b, c->flag.p, 8, hipMemcpyDeviceToHost, c->stream));
+  ART_HIP(hipMemcpyAsync(b, c->flag.p, 12, hipMemcpyDeviceToHost, c->stream));
   ART_HIP(hipStreamSynchronize(c->stream));
   float f[2];
   std::memcpy(f, b, 8);
   // (a matrix of zeros, or with scales that are no numbers: any bound will do)
   m->max_exp = f[0] > 0.0f ? exp_above(f[0]) : 0;
   m->row_exp = f[1] > 0.0f ? exp_above(f[1]) : 0;
+  m->direct = b[2] == 0;
   m->have = true;
   return ARTLITE_OK;
 }

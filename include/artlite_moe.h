@@ -175,8 +175,9 @@ int artlite_hbm_copy(size_t nbytes, int iters, double* ms_per_copy);
  * return at once; 0 rows write nothing. They may be captured into a graph: its replays use the workspace that was given, and
  * whatever else uses that workspace has to be ordered with them by the caller's streams (a workspace for each graph that
  * runs beside others). Outside captures, calls on one workspace order themselves, whichever streams and threads they come
- * from. Values of x beyond 2^100 in size may overflow the sums of few rows (the result is then infinite or no number); a
- * value that is infinite or no number reaches its own row alone. The same call gives the same bits. */
+ * from. The same call gives the same bits. A value of x that is infinite or no number reaches its own row alone; values beyond
+ * 2^100 in size may overflow the sums of few rows. Those are of codes, a group's times its scale: exact to about 2^-15 of the
+ * group's scale and offset, also where its values themselves come out far smaller than both. */
 typedef struct artlite_matrix artlite_matrix;
 int artlite_matrix_supported(int qtype);
 int artlite_matrix_create(int qtype, int64_t rows, int64_t cols, artlite_matrix** out);

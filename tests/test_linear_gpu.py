@@ -4,7 +4,9 @@ outputs, rows at any stride and address; bias, zeros, infinities and NaN.
 
 Tolerances (relative L2). A bf16 output is rounded once: half a step is 2^-8. Of few rows no weight is rounded and sums are
 fp32: 2^-8 + 2^-14. Past that each weight is rounded to fp16 (half a step 2^-11; the errors of a sum's terms are independent,
-so the sum's is 2^-11 of its size): 2^-8 + 2^-10. fp32: a sum of n terms in fp32 is off by about sqrt(n) 2^-24 (n the groups
+so the sum's is 2^-11 of its size), or its scale's product, its offset and itself are (uniform codes 0 .. 15 with an offset of
+7.5: 8.8, 7.5 and 4.6 times the scale in the mean square, each off by 2^-11 / sqrt(3) of itself: together 2.7 2^-11 / sqrt(3) =
+1.6 2^-11 of the values): 2^-8 + 2^-10. fp32: a sum of n terms in fp32 is off by about sqrt(n) 2^-24 (n the groups
 of 32 values and their MFMA steps, at most 2 * 90 * 3 here: 1.4e-6), the three bf16 planes by 2^-24, two fp16 planes by 2^-22
 a factor: 4e-6."""
 
@@ -61,7 +63,7 @@ def test_rows_and_widths(q: str, dtype: str) -> None:
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize(("q", "N", "K"), [("Q4_0", 1531, 2880), ("Q4_K", 512, 2048), ("Q4_1", 272, 4128),
-                                           ("IQ4_NL", 4100, 576), ("IQ4_XS", 96, 8192)])
+                                           ("IQ4_NL", 4100, 576), ("IQ4_XS", 96, 8192), ("Q4_1", 2080, 3104)])
 def test_larger(q: str, N: int, K: int, dtype: str) -> None:
     """Units shared by every number of waves; tiles of the large products in several rows and columns."""
     lin, w, b = make(q, N, K, 5, bias=True)
@@ -164,6 +166,28 @@ def test_zero_blocks_and_large_scales() -> None:
         lin.upload(raw)
         w = dense.gguf_ref.dequantize("Q4_0", raw.reshape(20, 36), 64).astype(np.float64)
         check(lin(x), values(x) @ w.T, TOL["bf16", few(20, 64, M, "bf16")])
+
+
+@pytest.mark.parametrize("q", ["Q4_0", "Q4_1", "IQ4_NL"])
+def test_scales_beyond_their_values(q: str) -> None:
+    """Groups whose values are zeros, or small differences, of large scales and offsets."""
+    N, K, per = 1600, 512, {"Q4_0": 18, "Q4_1": 20, "IQ4_NL": 18}[q]
+    raw, _ = dense.matrix(q, N, K, 3)
+    raw = raw.reshape(N, K // 32, per).copy()
+    big = np.array([100.0], np.float16).view(np.uint8)
+    for r, at in ((5, 3), (800, 0), (1599, 15)):
+        if q == "Q4_0":  # (c - 8 = 0)
+            raw[r, at, :2], raw[r, at, 2:] = np.array([65504.0], np.float16).view(np.uint8), 0x88
+        elif q == "Q4_1":  # (15 d + m = 0, and 1 for one value)
+            raw[r, at, :2], raw[r, at, 2:4], raw[r, at, 4:] = big, np.array([-1500.0], np.float16).view(np.uint8), 0xFF
+        else:
+            raw[r, at, :2] = big
+    lin = QLinear(q, N, K)
+    lin.upload(raw.reshape(N, -1))
+    w = dense.gguf_ref.dequantize(q, raw.reshape(N, -1), K).astype(np.float64)
+    for M in (3, 90, 1300):
+        x = x_rows(M, K, "bf16", M)
+        check(lin(x), values(x) @ w.T, TOL["bf16", few(N, K, M, "bf16")], np.sqrt(values(x) ** 2 @ (w ** 2).T))
 
 
 def test_no_rows_and_repeats() -> None:
