@@ -205,7 +205,7 @@ struct LinearPlan {
   int32_t* xe = nullptr;
   float* parts = nullptr;
 };
-LinearPlan linear_plan(Carve& c, const artlite_matrix* w, int dtype, int64_t n) {
+LinearPlan linear_layout(Carve& c, const artlite_matrix* w, int dtype, int64_t n, bool direct) {
   LinearPlan p;
   const int few_pl = dtype == ARTLITE_X_BF16 ? 1 : 3;
   const bool apart = few_apart(w, few_pl, false, n);
@@ -218,7 +218,7 @@ LinearPlan linear_plan(Carve& c, const artlite_matrix* w, int dtype, int64_t n) 
     const int pl = dtype == ARTLITE_X_BF16 ? 1 : 2;
     const int64_t Kp = pad64(w->K);
     p.x16 = c.take<uint16_t>(size_t(pl) * n * Kp);
-    p.direct = pl == 1 && qgemm_fits(n, w);
+    p.direct = direct && pl == 1 && qgemm_fits(n, w);
     if (p.direct) {
       p.xe = c.take<int32_t>(n);
       p.parts = c.take<float>(qgemm_parts_bytes(n, w) / 4);
@@ -228,6 +228,15 @@ LinearPlan linear_plan(Carve& c, const artlite_matrix* w, int dtype, int64_t n) 
     p.xe = c.take<int32_t>(n);
     p.parts = c.take<float>(hgemm_parts_bytes(n, w->N, Kp, pl == 2 ? 3 : 1, false) / 4);
   }
+  return p;
+}
+
+// (the same bytes whatever the matrix holds: a workspace outlives its values)
+LinearPlan linear_plan(Carve& c, const artlite_matrix* w, int dtype, int64_t n) {
+  Carve other(nullptr);
+  (void)linear_layout(other, w, dtype, n, !w->direct);
+  const LinearPlan p = linear_layout(c, w, dtype, n, w->direct);
+  c.at = std::max(c.at, other.at);
   return p;
 }
 
@@ -330,7 +339,7 @@ struct FfnPlan {
   int32_t *xe, *he;
   float* parts;
 };
-FfnPlan ffn_plan(Carve& c, const Ffn& f, int dtype, int64_t n) {
+FfnPlan ffn_layout(Carve& c, const Ffn& f, int dtype, int64_t n, bool direct) {
   FfnPlan p{};
   const bool b = dtype == ARTLITE_X_BF16, apart = few_apart(f.gate, b ? 1 : 3, true, n);
   p.few = n <= FEW_ROWS_FFN || (apart && few_apart(f.down, b ? 2 : 3, false, n));
@@ -344,7 +353,7 @@ FfnPlan ffn_plan(Carve& c, const Ffn& f, int dtype, int64_t n) {
   p.x16 = c.take<uint16_t>(pl * n * f.Hp);
   p.w16 = c.take<uint16_t>(pl * f.F * f.Hp);
   p.u16 = c.take<uint16_t>(pl * f.F * f.Hp);
-  p.direct = b && qgemm_fits(n, f.down);
+  p.direct = direct && b && qgemm_fits(n, f.down);
   if (!p.direct) p.d16 = c.take<uint16_t>(pl * f.H * f.Fp);
   p.h16 = c.take<uint16_t>(pl * n * f.Fp);
   p.xe = c.take<int32_t>(n);
@@ -352,6 +361,14 @@ FfnPlan ffn_plan(Carve& c, const Ffn& f, int dtype, int64_t n) {
   const int sg = b ? 1 : 3;
   p.parts = c.take<float>(std::max(hgemm_parts_bytes(n, f.F, f.Hp, sg, true), p.direct ? qgemm_parts_bytes(n, f.down)
                                                                                       : hgemm_parts_bytes(n, f.H, f.Fp, sg, false)) / 4);
+  return p;
+}
+
+FfnPlan ffn_plan(Carve& c, const Ffn& f, int dtype, int64_t n) {
+  Carve other(nullptr);
+  (void)ffn_layout(other, f, dtype, n, !f.down->direct);
+  const FfnPlan p = ffn_layout(c, f, dtype, n, f.down->direct);
+  c.at = std::max(c.at, other.at);
   return p;
 }
 

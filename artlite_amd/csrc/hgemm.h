@@ -46,7 +46,7 @@ struct HGemm {
 size_t hgemm_parts_bytes(int64_t M, int64_t N, int64_t K, int segs, bool gated);
 int launch_hgemm(const HGemm& g, hipStream_t s);
 // y = x W^T (H_STORE) with W in its blocks, values times 2^-g.e: a as one segment, no b
-bool qgemm_fits(int64_t M, const artlite_matrix* w);
+bool qgemm_fits(int64_t M, const artlite_matrix* w);  // (by its shape; w has to be `direct` besides)
 size_t qgemm_parts_bytes(int64_t M, const artlite_matrix* w);
 int launch_qgemm(const HGemm& g, const artlite_matrix* w, hipStream_t s);
 // what becomes of sums that are there already, in parts of M rows of pad64(N) values (gated: both matrices' side by side)

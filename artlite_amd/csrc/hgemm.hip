@@ -815,7 +815,7 @@ int launch_join(const HGemm& g, int parts, hipStream_t s) {
 // rows 75 against 105, 2048 rows 198 against 225; 12288 x 4096 IQ4_XS, 512 rows 88 against 101, 700 rows, 288, 137 against
 // 118), and where the unpacking is most of the work (32768 x 2048 Q4_K, 512 rows, 512 workgroups, 77 against 98).
 bool qgemm_fits(int64_t M, const artlite_matrix* w) {
-  return w->direct && int64_t(4) * w->units * w->ub < (int64_t(1) << 32) &&
+  return int64_t(4) * w->units * w->ub < (int64_t(1) << 32) &&
          (M <= 512 || (M + Q_TM - 1) / Q_TM * ((w->N + Q_TN - 1) / Q_TN) <= CUS);
 }
 // the parts of K: as long as they fill CUs and a part has two units
@@ -834,7 +834,7 @@ int launch_qgemm(const HGemm& g, const artlite_matrix* w, hipStream_t s) {
   if (g.M <= 0) return ARTLITE_OK;
   const int parts = qgemm_parts(g.M, w);
   if (g.K != pad64(w->K) || g.lda < g.K || g.lda % 8 || g.lda > (int64_t(1) << 22) || g.N != w->N || g.segs != 1 ||
-      !qgemm_fits(g.M, w) || (parts > 1 && !g.parts))
+      !w->direct || !qgemm_fits(g.M, w) || (parts > 1 && !g.parts))
     return fail(ARTLITE_EINVAL, "dense tiles: K %lld of rows of %lld", (long long)g.K, (long long)g.lda);
 #define ART_Q(QT) return launch_q<QT>(g, w, parts, s)
   ART_TILE_QTYPES(w->t->id, ART_Q)

@@ -182,7 +182,8 @@ typedef struct artlite_matrix artlite_matrix;
 int artlite_matrix_supported(int qtype);
 int artlite_matrix_create(int qtype, int64_t rows, int64_t cols, artlite_matrix** out);
 int artlite_matrix_destroy(artlite_matrix* m); /* its calls have come to their end */
-/* The rows' raw blocks (host, exactly their size); replaces earlier ones. */
+/* The rows' raw blocks (host, exactly their size); replaces earlier ones once the device is idle. A graph that captured calls on
+ * the matrix is captured again after that. */
 int artlite_matrix_upload(artlite_matrix* m, const void* data, size_t nbytes);
 /* n = rows fp32 values added to every output row of artlite_linear; n = 0: none. */
 int artlite_matrix_upload_bias(artlite_matrix* m, const float* data, size_t n);

@@ -187,6 +187,13 @@ for i in range(3):
     hip.fail_launch = -1
     run(300)
 own.close()
+# what a call needs does not depend on what a matrix holds
+for q in ("Q4_0", "Q4_1"):
+    w = QLinear(q, 256, 32768)
+    need = [w.workspace_bytes(n) for n in (300, 512, 2000)]
+    for fill in (0, 0x3c, 0x7c):
+        w.upload(np.full(256 * 1024 * BLOCK[q][1], fill, np.uint8))
+        assert need == [w.workspace_bytes(n) for n in (300, 512, 2000)]
 refused("closed", lambda: run(300, work=own))
 """)
 
