@@ -320,7 +320,8 @@ int check_ffn(const artlite_ffn* f, Ffn& o, const char* what) {
   for (const artlite_matrix* m : {f->gate, f->up, f->down}) {
     ART_TRY(check_matrix(m, what));
     if (m->has_bias) return fail(ARTLITE_EINVAL, "%s: a matrix with a bias", what);
-    if (m->device != f->gate->device) return fail(ARTLITE_EINVAL, "%s: matrices of devices %d and %d", what, m->device, f->gate->device);
+    if (m->device != f->gate->device)
+      return fail(ARTLITE_EINVAL, "%s: matrices of devices %d and %d", what, m->device, f->gate->device);
   }
   if (f->act != ARTLITE_ACT_SILU && f->act != ARTLITE_ACT_GELU_TANH)
     return fail(ARTLITE_EINVAL, "%s: activation %d", what, f->act);
@@ -346,7 +347,8 @@ FfnPlan ffn_layout(Carve& c, const Ffn& f, int dtype, int64_t n, bool direct) {
   if (p.few) {
     if (!b && !apart) p.planes = c.take<uint16_t>(3 * size_t(n) * f.H);
     p.hp = c.take<uint16_t>(size_t(b ? 2 : 3) * n * f.F);
-    p.parts = c.take<float>(std::max(few_parts_bytes(f.gate, b ? 1 : 3, true, n), few_parts_bytes(f.down, b ? 2 : 3, false, n)) / 4);
+    p.parts = c.take<float>(
+        std::max(few_parts_bytes(f.gate, b ? 1 : 3, true, n), few_parts_bytes(f.down, b ? 2 : 3, false, n)) / 4);
     return p;
   }
   const size_t pl = b ? 1 : 2;
@@ -359,8 +361,8 @@ FfnPlan ffn_layout(Carve& c, const Ffn& f, int dtype, int64_t n, bool direct) {
   p.xe = c.take<int32_t>(n);
   p.he = c.take<int32_t>(n);
   const int sg = b ? 1 : 3;
-  p.parts = c.take<float>(std::max(hgemm_parts_bytes(n, f.F, f.Hp, sg, true), p.direct ? qgemm_parts_bytes(n, f.down)
-                                                                                      : hgemm_parts_bytes(n, f.H, f.Fp, sg, false)) / 4);
+  const size_t down = p.direct ? qgemm_parts_bytes(n, f.down) : hgemm_parts_bytes(n, f.H, f.Fp, sg, false);
+  p.parts = c.take<float>(std::max(hgemm_parts_bytes(n, f.F, f.Hp, sg, true), down) / 4);
   return p;
 }
 

@@ -519,16 +519,16 @@ int launch_e(HGemm g, bool mixed, hipStream_t s) {
 // ---- the same product with W in its blocks, for hundreds of rows: y = x W^T, x as fp16 rows, W's values made of the codes in
 // registers, as the MFMA's operands
 //
-// A workgroup of 4 waves takes 128 rows of x and 256 of W, a wave 64 of W's and all of x's. x goes through an LDS ring as above;
-// a wave's codes (and headers) go through its own part of LDS by the same DMAs, whose counts then stay one queue, and are
-// values when they are operands: code to fp16 (exact), times its group's scale less its offset in fp16 (both rounded to fp16
-// from fp32 products: a value is off by 2^-11 of its product and of its offset, at most 8 times its group's largest value where
-// `direct` says so, 3 times it where the codes span their range; the large tiles' are by 2^-11 of themselves). That saves the unpacked
-// matrix's way through memory and most of an operand's traffic from L2, which bounds the small tiles; one wave a SIMD does
-// the values' instructions (15 to 28 for 8 of them) between the MFMAs of the step before. A step (32 values of K) takes 0.55 us
-// with one workgroup a CU and 0.95 with two, which is neither the ring's depth (8 slots: the same), the barriers (every second
-// step: the same) nor the operands' latency (read 5 blocks ahead: the same): 1.1 to 1.3 PFLOP/s where the large tiles have 1.4.
-// 1000 rows of 4096 x 4096 Q4_K: 46 us and 7 to join 2 parts; of 6144 x 2048 IQ4_NL 44.
+// A workgroup of 4 waves takes 128 rows of x and 256 of W, a wave 64 of W's and all of x's. x goes through an LDS ring as
+// above; a wave's codes (and headers) go through its own part of LDS by the same DMAs, whose counts then stay one queue, and
+// are values when they are operands: code to fp16 (exact), times its group's scale less its offset in fp16 (both rounded to
+// fp16 from fp32 products: a value is off by 2^-11 of its product and of its offset, at most 8 times its group's largest value
+// where `direct` says so, 3 times it where the codes span their range; the large tiles' are by 2^-11 of themselves). That
+// saves the unpacked matrix's way through memory and most of an operand's traffic from L2, which bounds the small tiles; one
+// wave a SIMD does the values' instructions (15 to 28 for 8 of them) between the MFMAs of the step before. A step (32 values
+// of K) takes 0.55 us with one workgroup a CU and 0.95 with two, which is neither the ring's depth (8 slots: the same), the
+// barriers (every second step: the same) nor the operands' latency (read 5 blocks ahead: the same): 1.1 to 1.3 PFLOP/s where
+// the large tiles have 1.4. 1000 rows of 4096 x 4096 Q4_K: 46 us and 7 to join 2 parts; of 6144 x 2048 IQ4_NL 44.
 constexpr int Q_TM = 128, Q_TN = 256, Q_RING = 4, Q_SLOT = Q_TM * BK * 2;
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -694,7 +694,8 @@ __global__ __launch_bounds__(256, 1) void k_qgemm(const HGemm g, const uint8_t* 
       if constexpr (i == 2 || i == 3) dma_a(i - 2, t + 3);
       if constexpr (i % 2 == 1 && J % 4 == 2) scales(std::integral_constant<int, i / 2>{}, std::integral_constant<int, J == 2>{});
       if constexpr (i == 0 && J % 4 == 3) next_half();
-      if constexpr (i % 2 == 0) fb[1 - S][i / 2] = values(std::integral_constant<int, i / 2>{}, std::integral_constant<int, (J + 1) % 4>{});
+      if constexpr (i % 2 == 0)
+        fb[1 - S][i / 2] = values(std::integral_constant<int, i / 2>{}, std::integral_constant<int, (J + 1) % 4>{});
       hg_for<4>([&](auto j) __attribute__((always_inline)) { acc[i][j] = hg_mfma(fb[S][j], fa[i % 4], acc[i][j]); });
       __builtin_amdgcn_sched_barrier(0);
     });

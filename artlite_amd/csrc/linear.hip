@@ -497,7 +497,8 @@ size_t tall_lds(const FewK& k, int planes, int ri) {
 template <int QT, int P, int RI, bool X32>
 int launch_tall_t(const FewK& k, hipStream_t s) {
   static DeviceOnce set;
-  if (!set.lds(reinterpret_cast<const void*>(k_tall<QT, P, RI, X32>), LDS_BYTES)) return fail(ARTLITE_EHIP, "dense rows: kernel set-up failed");
+  if (!set.lds(reinterpret_cast<const void*>(k_tall<QT, P, RI, X32>), LDS_BYTES))
+    return fail(ARTLITE_EHIP, "dense rows: kernel set-up failed");
   k_tall<QT, P, RI, X32><<<TALL_WGS, TALL_WAVES * 64, tall_lds(k, P, RI), s>>>(k);
   ART_HIP(hipGetLastError());
   return ARTLITE_OK;
@@ -538,7 +539,8 @@ FewCut few_cut(int64_t tiles, int units, int64_t M, int planes, bool glu) {
 
 template <int QT, int P, int NC, int RI, bool GLU, bool X32>
 int launch_few_nc(const FewK& k, int raw, hipStream_t s) {
-  constexpr int RED = (GLU ? 2 : 1) * few_tiles(NC, GLU) * NC * RI * WAVE * 4, SLOT = few_stage(RI, X32) ? FewStage<P, NC, X32>::BYTES : 0;
+  constexpr int RED = (GLU ? 2 : 1) * few_tiles(NC, GLU) * NC * RI * WAVE * 4;
+  constexpr int SLOT = few_stage(RI, X32) ? FewStage<P, NC, X32>::BYTES : 0;
   constexpr int WAVE_LDS = RED > SLOT ? RED : SLOT, LDS = few_most(P, NC, GLU) * WAVE_LDS;
   static_assert(LDS <= LDS_BYTES, "LDS");
   const FewCut c = few_cut(k.tiles, k.units, k.M, P, GLU);
@@ -773,7 +775,8 @@ template <int QT, int PL, int NC, int HU>
 int launch_few_t_nc(const FewTK& k, const FewTCut& c, hipStream_t s) {
   constexpr int LDS = FEW_T_WAVES * 4 * NC * 4 * WAVE * 4;
   static DeviceOnce set;
-  if (!set.lds(reinterpret_cast<const void*>(k_few_t<QT, PL, NC, HU>), LDS)) return fail(ARTLITE_EHIP, "dense rows: kernel set-up failed");
+  if (!set.lds(reinterpret_cast<const void*>(k_few_t<QT, PL, NC, HU>), LDS))
+    return fail(ARTLITE_EHIP, "dense rows: kernel set-up failed");
   k_few_t<QT, PL, NC, HU><<<dim3(unsigned(c.cols), unsigned((k.M + 16 * NC - 1) / (16 * NC)), unsigned(c.parts)),
                             FEW_T_WAVES * 64, LDS, s>>>(k);
   ART_HIP(hipGetLastError());
@@ -805,7 +808,8 @@ int few_raw_parts(const artlite_matrix* w, int planes, int64_t M) {
 
 int launch_few(const FewArgs& a, hipStream_t s) {
   if (a.M <= 0) return ARTLITE_OK;
-  if (a.x32 && !few_apart(a.w, 3, a.up != nullptr, a.M)) return fail(ARTLITE_EINVAL, "dense rows: %lld fp32 rows", (long long)a.M);
+  if (a.x32 && !few_apart(a.w, 3, a.up != nullptr, a.M))
+    return fail(ARTLITE_EINVAL, "dense rows: %lld fp32 rows", (long long)a.M);
   if (a.M > int64_t(65535) * 16) return fail(ARTLITE_EINVAL, "dense rows: %lld rows", (long long)a.M);
   FewK k{};
   k.w = a.w->w.as<uint8_t>();

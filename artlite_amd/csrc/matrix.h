@@ -15,7 +15,8 @@
 //     (dword >> 4 p) & 0x000F000F are the codes of values 2 p and 2 p + 1: one 16-bit operand dword of the MFMA;
 //   header: Q4_0, IQ4_NL: the 8 groups' fp16 scales; Q4_1: their (scale, min) pairs; Q4_K: the block's 16 bytes before its
 //     codes (d, dmin, the 6-bit scales and mins); IQ4_XS: its 8 (d and the 6-bit scales).
-// The bytes are the file's (but for the padding and the scales of Q4_0's blocks of zeros), in the order in which a wave reads them: 1 KiB of codes a load, contiguous.
+// The bytes are the file's (but for the padding and the scales of Q4_0's blocks of zeros), in the order in which a wave reads
+// them: 1 KiB of codes a load, contiguous.
 namespace artlite {
 
 constexpr int UNIT = 256;   // values of a unit
@@ -282,7 +283,8 @@ namespace artlite {
 // ---- the dense products over few rows (linear.hip)
 
 // One launch: out[m][n] = sum_k x[m][k] W[n][k] (+ bias[n]) for M rows of x given as planes of bf16 (x = the sum of its
-// planes) or, where few_apart, as fp32, or with `up` set the gated products act(x W^T) (x U^T), written as planes of bf16 for the launch after.
+// planes) or, where few_apart, as fp32, or with `up` set the gated products act(x W^T) (x U^T), written as planes of bf16 for
+// the launch after.
 struct FewArgs {
   const artlite_matrix *w, *up;
   int act;                  // (gated) artlite_act

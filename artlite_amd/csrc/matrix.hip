@@ -179,8 +179,8 @@ struct Unpack {
 };
 
 // W as fp16 rows of ld values: a wave per unit of a tile, a half at a time turned in its own part of LDS so that a store takes
-// 256 bytes of each of 4 rows (as it is held, 64 bytes of 16 rows: 60 us where this takes 38); plane 1 (where there is one) what plane 0's
-// rounding left. Bound by its writes: 38 us are 2 x 4096 x 11008 Q4_K, 5.9 TB/s.
+// 256 bytes of each of 4 rows (as it is held, 64 bytes of 16 rows: 60 us where this takes 38); plane 1 (where there is one)
+// what plane 0's rounding left. Bound by its writes: 38 us are 2 x 4096 x 11008 Q4_K, 5.9 TB/s.
 template <int QT, int PLANES>
 __global__ __launch_bounds__(256) void k_unpack(const Unpack two, int units, uint32_t all, int64_t N, int64_t K, int64_t ld,
                                                 int64_t plane) {

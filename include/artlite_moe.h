@@ -169,15 +169,16 @@ int artlite_hbm_copy(size_t nbytes, int iters, double* ms_per_copy);
  * kernels; Q4_0, Q4_1, Q4_K, IQ4_NL or IQ4_XS; cols a multiple of the format's block, at most 2^20; at most 2^24 rows.
  * Created on the calling thread's current device, which its calls then use whichever device is current.
  *
- * x, y and the gradients below are DEVICE memory of that device (anything else is refused), bf16 or fp32 (artlite_dtype; y
- * and gradients in x's type), rows of consecutive values `stride` values apart: x's at least 0 (0: one row for all), those
- * of what is written at least the row's values; what is written overlaps nothing else of the call's. Calls are enqueued on `stream` (a hipStream_t; null: the null stream) and
- * return at once; 0 rows write nothing. They may be captured into a graph: its replays use the workspace that was given, and
- * whatever else uses that workspace has to be ordered with them by the caller's streams (a workspace for each graph that
- * runs beside others). Outside captures, calls on one workspace order themselves, whichever streams and threads they come
- * from. The same call gives the same bits. A value of x that is infinite or no number reaches its own row alone; values beyond
- * 2^100 in size may overflow the sums of few rows. Those are of codes, a group's times its scale: exact to about 2^-15 of the
- * group's scale and offset, also where its values themselves come out far smaller than both. */
+ * x, y and the gradients below are DEVICE memory of that device (anything else is refused), bf16 or fp32 (artlite_dtype;
+ * y and gradients in x's type), rows of consecutive values `stride` values apart: x's at least 0 (0: one row for all),
+ * those of what is written at least the row's values; what is written overlaps nothing else of the call's. Calls are
+ * enqueued on `stream` (a hipStream_t; null: the null stream) and return at once; 0 rows write nothing. They may be
+ * captured into a graph: its replays use the workspace that was given, and whatever else uses that workspace has to be
+ * ordered with them by the caller's streams (a workspace for each graph that runs beside others). Outside captures, calls
+ * on one workspace order themselves, whichever streams and threads they come from. The same call gives the same bits. A
+ * value of x that is infinite or no number reaches its own row alone; values beyond 2^100 in size may overflow the sums of
+ * few rows. Those are of codes, a group's times its scale: exact to about 2^-15 of the group's scale and offset, also where
+ * its values themselves come out far smaller than both. */
 typedef struct artlite_matrix artlite_matrix;
 int artlite_matrix_supported(int qtype);
 int artlite_matrix_create(int qtype, int64_t rows, int64_t cols, artlite_matrix** out);

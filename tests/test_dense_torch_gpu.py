@@ -1,5 +1,6 @@
 """The dense operators on torch tensors, in a process that imports torch first."""
 
+import importlib.util
 import subprocess
 import sys
 from pathlib import Path
@@ -10,7 +11,8 @@ pytestmark = pytest.mark.gpu
 
 
 def test_torch_tensors_streams_and_graphs() -> None:
-    pytest.importorskip("torch")
+    if importlib.util.find_spec("torch") is None:  # (not imported here: it brings a HIP runtime of its own)
+        pytest.skip("no torch")
     r = subprocess.run([sys.executable, "-u", str(Path(__file__).with_name("dense_torch.py"))], capture_output=True, text=True,
                        timeout=110)
     assert r.returncode == 0 and r.stdout.count("passed") == 2, r.stdout + r.stderr

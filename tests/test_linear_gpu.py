@@ -1,6 +1,7 @@
-"""``QLinear`` against 64-bit math in every format and on every path: few rows (bf16 1 to 256, fp32 1 to 128, more of
-a small matrix: one, two and four blocks of 16), tall matrices, the large tiles past them (both sizes), widths of a single block, of partial units and of partial 64 values, odd numbers of
-outputs, rows at any stride and address; bias, zeros, infinities and NaN.
+"""``QLinear`` against 64-bit math in every format and on every path: few rows (bf16 1 to 256, fp32 1 to 128, more of a
+small matrix: one, two and four blocks of 16), tall matrices, the large tiles past them (both sizes), widths of a single
+block, of partial units and of partial 64 values, odd numbers of outputs, rows at any stride and address; bias, zeros,
+infinities and NaN.
 
 Tolerances (relative L2). A bf16 output is rounded once: half a step is 2^-8. Of few rows no weight is rounded and sums are
 fp32: 2^-8 + 2^-14. Past that each weight is rounded to fp16 (half a step 2^-11; the errors of a sum's terms are independent,
