@@ -431,6 +431,10 @@ int ffn_forward(const Ffn& f, const void* x, int dtype, int64_t n, int64_t x_str
 // the large tiles, 256 rows 141 against 126, fp32 260 against 262 and 327 against 281; 4096 x 11008 Q4_0: 192 rows 276 against
 // 363, 256 rows 297 against 372; one row 52 against 103 and 65 against 241)
 constexpr int FEW_ROWS_GRAD = 192;
+// Rows (a multiple of 64) up to which the weights' gradients are one launch of small tiles: what they write bounds them, and a
+// launch's start (all gradients of 1024 x 2816 IQ4_NL, 45 rows of fp32: 85 us in three launches, SHORT_US in one; 4096 x 11008
+// Q4_0, 1 row 187 and 161, fp32 332 and 251, 256 rows 1136 and 1065; 2048 x 8192 Q4_K, 256 rows of bf16, 187 and 189)
+constexpr int64_t SHORT_SUMS = 256;
 struct GradPlan {
   bool few;
   uint16_t* planes = nullptr;                    // few rows: x as planes, where it is not read as it is
@@ -577,20 +581,24 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
   }
   k_turn<<<dim3(unsigned((std::max(f.H, f.F) + 63) / 64), unsigned(Tp / 64), unsigned(turns * pl)), 256, 0, s>>>(t);
   ART_HIP(hipGetLastError());
+  HGemm w[3] = {};
+  int count = 0;
   const auto grad = [&](const uint16_t* a, int64_t M, const int32_t* ea, const uint16_t* b, int64_t N, const int32_t* eb,
                         void* out) {
-    HGemm w{};
-    segments(w, {{a, M * Tp, b, N * Tp}}, pl);
-    w.lda = w.ldb = w.K = Tp;
-    w.M = M, w.N = N;
-    w.e0 = ea, w.e1 = eb;
-    w.y = out, w.y_stride = N, w.dtype = dtype;
-    w.parts = p.parts;
-    return launch_hgemm(w, s);
+    if (!out) return;
+    HGemm& g = w[count++];
+    segments(g, {{a, M * Tp, b, N * Tp}}, pl);
+    g.lda = g.ldb = g.K = Tp;
+    g.M = M, g.N = N;
+    g.e0 = ea, g.e1 = eb;
+    g.y = out, g.y_stride = N, g.dtype = dtype;
+    g.parts = p.parts;
   };
-  if (dgate) ART_TRY(grad(p.dgt, f.F, p.top + 3, p.xt, f.H, p.top, dgate));
-  if (dup) ART_TRY(grad(p.dut, f.F, p.top + 3, p.xt, f.H, p.top, dup));
-  if (ddown) ART_TRY(grad(p.dyt, f.H, p.top + 1, p.ht, f.F, p.top + 2, ddown));
+  grad(p.dgt, f.F, p.top + 3, p.xt, f.H, p.top, dgate);
+  grad(p.dut, f.F, p.top + 3, p.xt, f.H, p.top, dup);
+  grad(p.dyt, f.H, p.top + 1, p.ht, f.F, p.top + 2, ddown);
+  if (Tp <= SHORT_SUMS) return launch_hgemms(w, count, s);
+  for (int i = 0; i < count; i++) ART_TRY(launch_hgemm(w[i], s));
   return ARTLITE_OK;
 }
 

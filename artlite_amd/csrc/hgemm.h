@@ -45,6 +45,8 @@ struct HGemm {
 // the scratch that a product may take (gated: N columns of each matrix)
 size_t hgemm_parts_bytes(int64_t M, int64_t N, int64_t K, int segs, bool gated);
 int launch_hgemm(const HGemm& g, hipStream_t s);
+// up to three H_STORE products of as many 128 x 128 tiles each, in one launch without parts: short sums of many outputs
+int launch_hgemms(const HGemm* g, int count, hipStream_t s);
 // y = x W^T (H_STORE) with W in its blocks, values times 2^-g.e: a as one segment, no b
 bool qgemm_fits(int64_t M, const artlite_matrix* w);  // (by its shape; w has to be `direct` besides)
 size_t qgemm_parts_bytes(int64_t M, const artlite_matrix* w);

@@ -209,7 +209,7 @@ __device__ __forceinline__ void deal_tile(int gm, int gn, int& mt, int& nt) {
 
 // gm x gn tiles from column 0 on; K in gridDim.y parts (PART: their sums into g.parts, for k_join)
 template <int MB, int EPI, bool PART>
-__global__ __launch_bounds__(256, MB == 8 ? 1 : 2) void k_hgemm(const HGemm g, int gm, int gn) {
+__device__ __forceinline__ void hgemm_tile(const HGemm& g, int gm, int gn) {
   using T = HT<MB>;
   constexpr int TM = T::TM, RING = T::RING;
   constexpr bool GATED = gated<EPI>;
@@ -389,6 +389,20 @@ __global__ __launch_bounds__(256, MB == 8 ? 1 : 2) void k_hgemm(const HGemm g, i
       }
     }
   }
+}
+
+template <int MB, int EPI, bool PART>
+__global__ __launch_bounds__(256, MB == 8 ? 1 : 2) void k_hgemm(const HGemm g, int gm, int gn) {
+  hgemm_tile<MB, EPI, PART>(g, gm, gn);
+}
+// up to three products of as many small tiles each
+struct HGemms {
+  HGemm g[3];
+  int gm[3], gn[3];
+};
+__global__ __launch_bounds__(256, 2) void k_hgemms(const HGemms all) {
+  const int i = blockIdx.z;
+  hgemm_tile<4, H_STORE, false>(all.g[i], all.gm[i], all.gn[i]);
 }
 
 // the parts' sums, in order, and what becomes of them: 8 columns a thread
@@ -787,18 +801,45 @@ size_t hgemm_parts_bytes(int64_t M, int64_t N, int64_t K, int segs, bool gate) {
   return most;
 }
 
-int launch_hgemm(const HGemm& g, hipStream_t s) {
-  if (g.M <= 0 || g.N <= 0) return ARTLITE_OK;
+namespace {
+int check_hgemm(const HGemm& g) {
   if (g.segs < 1 || g.segs > H_SEGS || g.K < 64 || g.K % 64 || g.lda < g.K || g.ldb < g.K || g.lda % 8 || g.ldb % 8 ||
       g.lda > (int64_t(1) << 22) || g.ldb > (int64_t(1) << 22) || g.K * g.segs / BK >= (int64_t(1) << 30))
     return fail(ARTLITE_EINVAL, "large tiles: K %lld of rows of %lld and %lld", (long long)g.K, (long long)g.lda,
                 (long long)g.ldb);
+  return ARTLITE_OK;
+}
+}  // namespace
+
+int launch_hgemm(const HGemm& g, hipStream_t s) {
+  if (g.M <= 0 || g.N <= 0) return ARTLITE_OK;
+  ART_TRY(check_hgemm(g));
   HGemm h = g;
   h.h_cols = g.h_stride;
   return g.epilogue == H_STORE  ? launch_e<H_STORE>(h, true, s)
          : g.epilogue == H_ROWS ? launch_e<H_ROWS>(h, true, s)
          : g.epilogue == H_GLU  ? launch_e<H_GLU>(h, true, s)
                                 : launch_e<H_DGLU>(h, true, s);
+}
+
+int launch_hgemms(const HGemm* g, int count, hipStream_t s) {
+  using T = HT<4>;
+  HGemms all{};
+  int64_t tiles = 0;
+  if (count > 3) return fail(ARTLITE_EINVAL, "large tiles: %d products", count);
+  for (int i = 0; i < count; i++) {
+    ART_TRY(check_hgemm(g[i]));
+    const int64_t gm = (g[i].M + T::TM - 1) / T::TM, gn = (g[i].N + T::TM - 1) / T::TM;
+    if (g[i].epilogue != H_STORE || gm < 1 || gn < 1 || gm * gn > (int64_t(1) << 30) || (i && gm * gn != tiles))
+      return fail(ARTLITE_EINVAL, "large tiles: products that are not alike");
+    all.g[i] = g[i], all.gm[i] = int(gm), all.gn[i] = int(gn);
+    tiles = gm * gn;
+  }
+  static DeviceOnce set;
+  if (!set.lds(reinterpret_cast<const void*>(k_hgemms), T::LDS)) return fail(ARTLITE_EHIP, "large tiles: kernel set-up failed");
+  if (count) k_hgemms<<<dim3(unsigned(tiles), 1, unsigned(count)), 256, T::LDS, s>>>(all);
+  ART_HIP(hipGetLastError());
+  return ARTLITE_OK;
 }
 
 int launch_join(const HGemm& g, int parts, hipStream_t s) {
