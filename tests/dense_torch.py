@@ -4,6 +4,7 @@ library loads (both then share torch's HIP runtime). Run by test_dense_torch_gpu
 TOL: a bf16 output's half step (2^-8) and the inner roundings' eighths of it (at most 8)."""
 
 import sys
+import threading
 from pathlib import Path
 
 import numpy as np
@@ -139,7 +140,92 @@ def ffn_streams_and_graphs() -> None:
                 near(t, want[k], TOL)
 
 
+def far_rows() -> None:
+    """Rows whose offsets pass 32 bits, in values and in bytes."""
+    N, K = 1600, 512
+    lin = QLinear("Q4_K", N, K)
+    raw, w = dense.matrix("Q4_K", N, K, 8)
+    lin.upload(raw)
+    w = torch.from_numpy(w)
+    f, fw = GatedFFN(hidden=256, ffn=512, gate_type="Q4_0", down_type="IQ4_NL"), []
+    for i, (name, q, r, c) in enumerate((("gate", "Q4_0", 512, 256), ("up", "Q4_0", 512, 256), ("down", "IQ4_NL", 256, 512))):
+        raw, v = dense.matrix(q, r, c, i)
+        f.upload("ffn_" + name, raw)
+        fw.append(v)
+
+    def rows(n: int, cols: int, stride: int) -> object:
+        return torch.empty((n - 1) * stride + cols, device="cuda", dtype=torch.bfloat16).as_strided((n, cols), (stride, 1))
+
+    def near(y: object, want: np.ndarray) -> None:
+        assert np.linalg.norm(y.double().cpu().numpy() - want) <= TOL * np.linalg.norm(want)
+
+    for M, stride in ((3, 2_200_000_001), (90, 50_000_001), (1300, 3_400_003)):
+        x, y = rows(M, K, stride), rows(M, N, stride)
+        x.copy_(torch.randn(M, K, device="cuda"))
+        torch.cuda.synchronize()
+        lin(x, y)
+        near(y, (x.cpu().double() @ w.T).numpy())
+        del x, y
+        x, dy, y, dx = (rows(M, 256, stride) for _ in range(4))
+        for t in (x, dy):
+            t.copy_(torch.randn(M, 256, device="cuda"))
+        torch.cuda.synchronize()
+        f(x, y)
+        f.backward(x, dy, dx=dx)
+        xs, dys = (t.double().cpu().numpy() for t in (x, dy))
+        near(y, dense.ffn("silu", xs, *fw))
+        near(dx, dense.ffn_grad("silu", xs, dys, *fw)["dx"])
+        del x, dy, y, dx
+        torch.cuda.empty_cache()
+
+
+def threads_and_shared_workspaces() -> None:
+    """Threads on streams of their own, over one object and the workspace that they share; graphs that share a workspace,
+    replayed in turn on one stream."""
+    N, K, M = 2000, 512, 1100
+    lin = QLinear("Q4_1", N, K)
+    raw, w = dense.matrix("Q4_1", N, K, 8)
+    lin.upload(raw)
+    w = torch.from_numpy(w).cuda()
+    xs = [torch.randn(M + i, K, device="cuda").bfloat16() for i in range(4)]
+    ys = [torch.empty(M + i, N, device="cuda", dtype=torch.bfloat16) for i in range(4)]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+
+    def near(y: object, x: object) -> None:
+        want = x.double() @ w.T
+        assert (y.double() - want).norm() <= TOL * want.norm()
+
+    def run(i: int) -> None:
+        for _ in range(40):
+            lin(xs[i], ys[i], stream=streams[i].cuda_stream)
+
+    all_ = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in all_:
+        t.start()
+    for t in all_:
+        t.join()
+    torch.cuda.synchronize()
+    for x, y in zip(xs, ys):
+        near(y, x)
+    work = Workspace(max(lin.workspace_bytes(x.shape[0]) for x in xs))
+    graphs = []
+    for x, y in zip(xs, ys):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            lin(x, y, stream=torch.cuda.current_stream().cuda_stream, work=work)
+        graphs.append(g)
+    for _ in range(3):
+        for x, y, g in zip(xs, ys, graphs):
+            x.copy_(torch.randn_like(x))
+            y.zero_()
+            g.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(xs, ys):
+            near(y, x)
+
+
 if __name__ == "__main__":
-    for case in (linear_streams_and_graphs, ffn_streams_and_graphs):
+    for case in (linear_streams_and_graphs, ffn_streams_and_graphs, far_rows, threads_and_shared_workspaces):
         case()
         print(case.__name__, "passed", flush=True)

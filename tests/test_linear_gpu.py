@@ -129,6 +129,23 @@ def test_one_row_for_all() -> None:
         check(y.numpy(), np.repeat(values(data) @ w.T, M, 0), TOL["bf16", few(40, 256, M, "bf16")])
 
 
+def test_widest() -> None:
+    """The most values a row may have, on every path (many rows: one for all of them)."""
+    N, K = 20, 1 << 20
+    lin, w, _ = make("Q4_0", N, K, 6)
+    data = x_rows(1, K, "bf16", 1)
+    want = values(data) @ w.T
+    terms = np.sqrt(values(data) ** 2 @ (w ** 2).T)
+    for M in (1, 7, 40, 100, 256, 257, 600):
+        x = Rows(1, K, "bf16", data=data)
+        x.shape, x.row = (M, K), 0
+        y = Rows(M, N, "bf16")
+        lin(x, y)
+        check(y.numpy(), np.repeat(want, M, 0), TOL["bf16", few(N, K, M, "bf16")], np.repeat(terms, M, 0))
+    with pytest.raises(_hip.Error, match="rows of 1048608 values"):
+        QLinear("Q4_0", N, K + 32)
+
+
 @pytest.mark.parametrize("M", [4, 90, 1300])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_values_out_of_the_ordinary(dtype: str, M: int) -> None:
