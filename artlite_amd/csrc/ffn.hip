@@ -218,10 +218,10 @@ LinearPlan linear_layout(Carve& c, const artlite_matrix* w, int dtype, int64_t n
     const int pl = dtype == ARTLITE_X_BF16 ? 1 : 2;
     const int64_t Kp = pad64(w->K);
     p.x16 = c.take<uint16_t>(size_t(pl) * n * Kp);
-    p.direct = direct && pl == 1 && qgemm_fits(n, w);
+    p.direct = direct && pl == 1 && qgemm_fits(n, w, false);
     if (p.direct) {
       p.xe = c.take<int32_t>(n);
-      p.parts = c.take<float>(qgemm_parts_bytes(n, w) / 4);
+      p.parts = c.take<float>(qgemm_parts_bytes(n, w, false) / 4);
       return p;
     }
     p.w16 = c.take<uint16_t>(size_t(pl) * w->N * Kp);
@@ -305,7 +305,7 @@ int linear(const artlite_matrix* w, const void* x, int dtype, int64_t n, int64_t
   g.bias = w->has_bias ? w->bias.as<float>() : nullptr;
   g.y = y, g.y_stride = y_stride, g.dtype = dtype;
   g.parts = p.parts;
-  return p.direct ? launch_qgemm(g, w, s) : launch_hgemm(g, s);
+  return p.direct ? launch_qgemm(g, w, nullptr, s) : launch_hgemm(g, s);
 }
 
 // ---- the gated block
@@ -334,13 +334,13 @@ int check_ffn(const artlite_ffn* f, Ffn& o, const char* what) {
 }
 
 struct FfnPlan {
-  bool few, direct;  // (direct: down from its blocks, k_qgemm)
+  bool few, direct, gated;  // (direct: down from its blocks, gated: gate and up from theirs, k_qgemm)
   uint16_t *planes = nullptr, *hp = nullptr;  // few rows: x as planes (where it is not read as it is), h as planes
   uint16_t *x16, *w16, *u16, *d16, *h16;      // else: x, the unpacked matrices, h
   int32_t *xe, *he;
   float* parts;
 };
-FfnPlan ffn_layout(Carve& c, const Ffn& f, int dtype, int64_t n, bool direct) {
+FfnPlan ffn_layout(Carve& c, const Ffn& f, int dtype, int64_t n, bool direct, bool gated) {
   FfnPlan p{};
   const bool b = dtype == ARTLITE_X_BF16, apart = few_apart(f.gate, b ? 1 : 3, true, n);
   p.few = n <= FEW_ROWS_FFN || (apart && few_apart(f.down, b ? 2 : 3, false, n));
@@ -353,24 +353,32 @@ FfnPlan ffn_layout(Carve& c, const Ffn& f, int dtype, int64_t n, bool direct) {
   }
   const size_t pl = b ? 1 : 2;
   p.x16 = c.take<uint16_t>(pl * n * f.Hp);
-  p.w16 = c.take<uint16_t>(pl * f.F * f.Hp);
-  p.u16 = c.take<uint16_t>(pl * f.F * f.Hp);
-  p.direct = direct && b && qgemm_fits(n, f.down);
+  p.gated = gated && b && qgemm_fits(n, f.gate, true);
+  if (!p.gated) {
+    p.w16 = c.take<uint16_t>(pl * f.F * f.Hp);
+    p.u16 = c.take<uint16_t>(pl * f.F * f.Hp);
+  }
+  p.direct = direct && b && qgemm_fits(n, f.down, false);
   if (!p.direct) p.d16 = c.take<uint16_t>(pl * f.H * f.Fp);
   p.h16 = c.take<uint16_t>(pl * n * f.Fp);
   p.xe = c.take<int32_t>(n);
   p.he = c.take<int32_t>(n);
   const int sg = b ? 1 : 3;
-  const size_t down = p.direct ? qgemm_parts_bytes(n, f.down) : hgemm_parts_bytes(n, f.H, f.Fp, sg, false);
-  p.parts = c.take<float>(std::max(hgemm_parts_bytes(n, f.F, f.Hp, sg, true), down) / 4);
+  const size_t gate = p.gated ? qgemm_parts_bytes(n, f.gate, true) : hgemm_parts_bytes(n, f.F, f.Hp, sg, true);
+  const size_t down = p.direct ? qgemm_parts_bytes(n, f.down, false) : hgemm_parts_bytes(n, f.H, f.Fp, sg, false);
+  p.parts = c.take<float>(std::max(gate, down) / 4);
   return p;
 }
 
 FfnPlan ffn_plan(Carve& c, const Ffn& f, int dtype, int64_t n) {
-  Carve other(nullptr);
-  (void)ffn_layout(other, f, dtype, n, !f.down->direct);
-  const FfnPlan p = ffn_layout(c, f, dtype, n, f.down->direct);
-  c.at = std::max(c.at, other.at);
+  size_t most = 0;
+  for (int i = 0; i < 4; i++) {
+    Carve any(nullptr);
+    (void)ffn_layout(any, f, dtype, n, i & 1, i & 2);
+    most = std::max(most, any.at);
+  }
+  const FfnPlan p = ffn_layout(c, f, dtype, n, f.down->direct, f.gate->direct && f.up->direct);
+  c.at = most;
   return p;
 }
 
@@ -402,18 +410,22 @@ int ffn_forward(const Ffn& f, const void* x, int dtype, int64_t n, int64_t x_str
   r.arrays = 1, r.K = f.H, r.Kp = f.Hp, r.plane = n * f.Hp;
   r.he = p.he, r.lh = f.gate->row_exp + f.up->row_exp;
   ART_TRY(rows16(r, dtype, n, s));
-  ART_TRY(launch_unpack(f.gate, f.up, false, wexp16(f.gate), wexp16(f.up), p.w16, p.u16, f.Hp, f.F * f.Hp, pl, s));
+  const int eg = p.gated ? qexp16(f.gate) : wexp16(f.gate), eu = p.gated ? qexp16(f.up) : wexp16(f.up);
+  if (!p.gated) ART_TRY(launch_unpack(f.gate, f.up, false, eg, eu, p.w16, p.u16, f.Hp, f.F * f.Hp, pl, s));
   if (!p.direct) ART_TRY(launch_unpack(f.down, nullptr, false, wexp16(f.down), 0, p.d16, nullptr, f.Fp, f.H * f.Fp, pl, s));
   HGemm g{};
-  segments(g, {{p.x16, n * f.Hp, p.w16, f.F * f.Hp, p.u16}}, pl);
+  if (p.gated)
+    g.a[0] = p.x16, g.segs = 1;
+  else
+    segments(g, {{p.x16, n * f.Hp, p.w16, f.F * f.Hp, p.u16}}, pl);
   g.lda = g.ldb = g.K = f.Hp;
   g.M = n, g.N = f.F;
   g.epilogue = H_GLU;
-  g.row_e = p.xe, g.e = wexp16(f.gate), g.e2 = wexp16(f.up);
+  g.row_e = p.xe, g.e = eg, g.e2 = eu;
   g.act = f.act;
   g.out_e = p.he, g.h = p.h16, g.h_stride = f.Fp, g.h_plane = n * f.Fp, g.planes = pl;
   g.parts = p.parts;
-  ART_TRY(launch_hgemm(g, s));
+  ART_TRY(p.gated ? launch_qgemm(g, f.gate, f.up, s) : launch_hgemm(g, s));
   HGemm d{};
   if (p.direct)
     d.a[0] = p.h16, d.segs = 1;
@@ -424,7 +436,7 @@ int ffn_forward(const Ffn& f, const void* x, int dtype, int64_t n, int64_t x_str
   d.row_e = p.he, d.e = p.direct ? qexp16(f.down) : wexp16(f.down);
   d.y = y, d.y_stride = y_stride, d.dtype = dtype;
   d.parts = p.parts;
-  return p.direct ? launch_qgemm(d, f.down, s) : launch_hgemm(d, s);
+  return p.direct ? launch_qgemm(d, f.down, nullptr, s) : launch_hgemm(d, s);
 }
 
 // Rows up to which the gradients' products run from the blocks (dx alone, 2048 x 8192 Q4_K: 192 rows 122 us against 121 by
@@ -436,7 +448,7 @@ constexpr int FEW_ROWS_GRAD = 192;
 // Q4_0, 1 row 187 and 161, fp32 332 and 251, 256 rows 1136 and 1065; 2048 x 8192 Q4_K, 256 rows of bf16, 187 and 189)
 constexpr int64_t SHORT_SUMS = 256;
 struct GradPlan {
-  bool few;
+  bool few, gated;  // (gated: g and u from the blocks, k_qgemm)
   uint16_t* planes = nullptr;                    // few rows: x as planes, where it is not read as it is
   uint16_t *x16, *dy16, *a16, *b16, *c16;        // x, dy; gate and up, later their transposes; down's transpose
   uint16_t *h16, *dh16, *dg16, *du16;
@@ -449,6 +461,8 @@ GradPlan grad_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool weights) {
   const size_t pl = dtype == ARTLITE_X_BF16 ? 1 : 2;
   const size_t w = pl * size_t(f.F * f.Hp > f.H * f.Fp ? f.F * f.Hp : f.H * f.Fp);
   p.few = n <= FEW_ROWS_GRAD;
+  const bool fits = !p.few && pl == 1 && qgemm_fits(n, f.gate, true);
+  p.gated = fits && f.gate->direct && f.up->direct;
   p.x16 = c.take<uint16_t>(pl * n * f.Hp);
   p.dy16 = c.take<uint16_t>(pl * n * f.Hp);
   if (!p.few) {
@@ -486,6 +500,7 @@ GradPlan grad_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool weights) {
                            hgemm_parts_bytes(n, f.H, f.Fp, 2 * sg, false)});
   if (weights)
     parts = std::max({parts, hgemm_parts_bytes(f.F, f.H, pad64(n), sg, false), hgemm_parts_bytes(f.H, f.F, pad64(n), sg, false)});
+  if (fits) parts = std::max(parts, qgemm_parts_bytes(n, f.gate, true));
   p.parts = c.take<float>(parts / 4);
   return p;
 }
@@ -508,7 +523,7 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
   // (gate and up share a scale: dx sums over both)
   const int e = wexp16(f.gate) > wexp16(f.up) ? wexp16(f.gate) : wexp16(f.up), ed = wexp16(f.down);
   if (!p.few) {
-    ART_TRY(launch_unpack(f.gate, f.up, false, e, e, p.a16, p.b16, f.Hp, f.F * f.Hp, pl, s));
+    if (!p.gated) ART_TRY(launch_unpack(f.gate, f.up, false, e, e, p.a16, p.b16, f.Hp, f.F * f.Hp, pl, s));
     ART_TRY(launch_unpack(f.down, nullptr, true, ed, 0, p.c16, nullptr, f.Hp, f.F * f.Hp, pl, s));
   }
   HGemm d{};
@@ -526,7 +541,7 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
     ART_TRY(launch_hgemm(d, s));
   }
   HGemm g{};
-  if (!p.few) segments(g, {{p.x16, n * f.Hp, p.a16, f.F * f.Hp, p.b16}}, pl);
+  if (!p.few && !p.gated) segments(g, {{p.x16, n * f.Hp, p.a16, f.F * f.Hp, p.b16}}, pl);
   g.lda = g.ldb = g.K = f.Hp;
   g.M = n, g.N = f.F;
   g.epilogue = H_DGLU;
@@ -547,6 +562,10 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
     ART_TRY(launch_few(a, s));
     g.row_e = nullptr, g.e = g.e2 = 0;  // (sums of the values themselves)
     ART_TRY(launch_join(g, a.raw, s));
+  } else if (p.gated) {
+    g.a[0] = p.x16, g.segs = 1;
+    g.e = qexp16(f.gate), g.e2 = qexp16(f.up);
+    ART_TRY(launch_qgemm(g, f.gate, f.up, s));
   } else {
     ART_TRY(launch_hgemm(g, s));
   }

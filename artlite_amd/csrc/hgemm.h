@@ -47,10 +47,11 @@ size_t hgemm_parts_bytes(int64_t M, int64_t N, int64_t K, int segs, bool gated);
 int launch_hgemm(const HGemm& g, hipStream_t s);
 // up to three H_STORE products of as many 128 x 128 tiles each, in one launch without parts: short sums of many outputs
 int launch_hgemms(const HGemm* g, int count, hipStream_t s);
-// y = x W^T (H_STORE) with W in its blocks, values times 2^-g.e: a as one segment, no b
-bool qgemm_fits(int64_t M, const artlite_matrix* w);  // (by its shape; w has to be `direct` besides)
-size_t qgemm_parts_bytes(int64_t M, const artlite_matrix* w);
-int launch_qgemm(const HGemm& g, const artlite_matrix* w, hipStream_t s);
+// out = x W^T with W (gated, H_GLU and H_DGLU: and W2, alike) in its blocks, values times 2^-g.e (2^-g.e2): a as one segment of
+// one plane, no b
+bool qgemm_fits(int64_t M, const artlite_matrix* w, bool gated);  // (by its shape; the matrices have to be `direct` besides)
+size_t qgemm_parts_bytes(int64_t M, const artlite_matrix* w, bool gated);
+int launch_qgemm(HGemm g, const artlite_matrix* w, const artlite_matrix* w2, hipStream_t s);
 // what becomes of sums that are there already, in parts of M rows of pad64(N) values (gated: both matrices' side by side)
 int launch_join(const HGemm& g, int parts, hipStream_t s);
 

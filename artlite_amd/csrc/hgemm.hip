@@ -571,16 +571,19 @@ __device__ __forceinline__ u32x4 q_values(uint32_t w, uint32_t s, uint32_t o, ui
   return r;
 }
 
-template <int QT, bool PART>
-__global__ __launch_bounds__(256, 1) void k_qgemm(const HGemm g, const uint8_t* __restrict__ w, int64_t tiles, int units, int e,
-                                                  int gm, int gn) {
-  constexpr int UB = unit_bytes<QT>(), HB = hdr_bytes<QT>(), HD = HB == 32 ? 2 : 1;  // (header DMAs a unit)
+// gated: a wave's 64 rows are 32 of W and the same 32 of the second matrix
+template <int QT, int EPI, bool PART>
+__global__ __launch_bounds__(256, 1) void k_qgemm(const HGemm g, const uint8_t* __restrict__ w, const uint8_t* __restrict__ w2,
+                                                  int64_t tiles, int units, int gm, int gn) {
+  constexpr bool GATED = gated<EPI>;
+  constexpr int TN = GATED ? Q_TN / 2 : Q_TN, WT = TN / 4 / TROWS;  // (output columns; a wave's tiles of a matrix)
+  constexpr int UB = unit_bytes<QT>(), HB = hdr_bytes<QT>(), HD = GATED || HB == 32 ? 2 : 1;  // (header DMAs a unit)
   constexpr int CODES = Q_RING * Q_SLOT, HDRS = CODES + 4 * 8192, LDS = HDRS + 4 * 2048;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lg = lane >> 4, lr = lane & 15;
   int mt, nt;
   deal_tile(gm, gn, mt, nt);
-  const int64_t m0 = int64_t(mt) * Q_TM, n0 = int64_t(nt) * Q_TN;
+  const int64_t m0 = int64_t(mt) * Q_TM, n0 = int64_t(nt) * TN;
   const int mv = int(min(int64_t(Q_TM), g.M - m0));
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(hg_lds_addr(lds));
   uint32_t mask = 0x000F000Fu, top = 0x64006400u;
@@ -593,20 +596,21 @@ __global__ __launch_bounds__(256, 1) void k_qgemm(const HGemm g, const uint8_t* 
     offa[i] = uint32_t(min(r, mv - 1)) * uint32_t(g.lda) * 2 + 16 * c;
   }
   // (tiles past the last: the last again, their columns are not stored)
-  const int64_t tw = n0 / TROWS + 4 * wv, t0 = min(tw, tiles - 1);
+  const int64_t tw = n0 / TROWS + WT * wv, t0 = min(tw, tiles - 1);
   uint32_t tile_at[4], offh[HD];
 #pragma unroll
   for (int j = 0; j < 4; j++)
-    tile_at[j] = __builtin_amdgcn_readfirstlane(uint32_t(min(tw + j, tiles - 1) - t0) * uint32_t(units) * UB);
+    tile_at[j] = __builtin_amdgcn_readfirstlane(uint32_t(min(tw + j % WT, tiles - 1) - t0) * uint32_t(units) * UB);
   {
     constexpr int LT = TROWS * HB / 16;  // lanes of a tile's headers
 #pragma unroll
     for (int d = 0; d < HD; d++) {
-      const int j = LT >= 64 ? 0 : (lane / LT + d * (64 / LT)) & 3;
+      const int j = GATED ? (lane / LT) & 1 : (lane / LT + d * (64 / LT)) & 3;  // (gated: a DMA a matrix)
       offh[d] = uint32_t(min(tw + j, tiles - 1) - t0) * uint32_t(units) * UB + 16 * (lane % LT);
     }
   }
   const uint8_t* const wbase = w + t0 * units * UB;
+  const uint8_t* const wbase2 = GATED ? w2 + t0 * units * UB : nullptr;
   const int steps_all = int(g.K / BK);
   const int u0 = PART ? int(int64_t(units) * blockIdx.y / gridDim.y) : 0;
   const int u1 = PART ? int(int64_t(units) * (blockIdx.y + 1) / gridDim.y) : units;
@@ -618,11 +622,11 @@ __global__ __launch_bounds__(256, 1) void k_qgemm(const HGemm g, const uint8_t* 
   };
   auto dma_code = [&](int j, int h, int u) __attribute__((always_inline)) {
     const uint32_t d = __builtin_amdgcn_readfirstlane(lds0 + CODES + wv * 8192 + (h * 4 + j) * 1024);
-    const uint8_t* p = wbase + int64_t(min(u, u1 - 1)) * UB + tile_at[j] + 1024 * h;
+    const uint8_t* p = (j < WT ? wbase : wbase2) + int64_t(min(u, u1 - 1)) * UB + tile_at[j] + 1024 * h;
     hg_dma(hg_uniform(reinterpret_cast<const uint16_t*>(p)), 16 * lane, d);
   };
   auto dma_hdr = [&](int d, int u) __attribute__((always_inline)) {
-    const uint8_t* p = wbase + int64_t(min(u, u1 - 1)) * UB + 2048;
+    const uint8_t* p = (GATED && d ? wbase2 : wbase) + int64_t(min(u, u1 - 1)) * UB + 2048;
     hg_dma(hg_uniform(reinterpret_cast<const uint16_t*>(p)), offh[d],
            __builtin_amdgcn_readfirstlane(lds0 + HDRS + wv * 2048 + d * 1024));
   };
@@ -639,7 +643,7 @@ __global__ __launch_bounds__(256, 1) void k_qgemm(const HGemm g, const uint8_t* 
   const uint8_t* const mycodes = lds + CODES + wv * 8192 + 16 * lane;
   const uint8_t* const myhdrs = lds + HDRS + wv * 2048 + HB * lr;
   auto read_hdrs = [&]() __attribute__((always_inline)) {
-    hg_for<4>([&](auto j) { hd[j].load(myhdrs + decltype(j)::value * TROWS * HB); });
+    hg_for<4>([&](auto j) { hd[j].load(myhdrs + (GATED ? (j / 2) * 1024 + (j % 2) * TROWS * HB : j * TROWS * HB)); });
   };
   auto read_codes = [&](int h) __attribute__((always_inline)) {
     hg_for<4>([&](auto j) { code2[j] = ld(mycodes + (4 * h + decltype(j)::value) * 1024); });
@@ -649,6 +653,7 @@ __global__ __launch_bounds__(256, 1) void k_qgemm(const HGemm g, const uint8_t* 
     constexpr int j = decltype(jc)::value, H = decltype(hc)::value;
     float s[4], o[4] = {0, 0, 0, 0};
     hd[j].template fields<H>(s, o);
+    const int e = j < WT ? g.e : g.e2;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       const _Float16 a = _Float16(__builtin_amdgcn_ldexpf(s[k], -e)), b = _Float16(-__builtin_amdgcn_ldexpf(o[k], -e));
@@ -728,16 +733,16 @@ __global__ __launch_bounds__(256, 1) void k_qgemm(const HGemm g, const uint8_t* 
   // ---- outputs, as above
   RowExp* const rows_e = reinterpret_cast<RowExp*>(lds + LDS - Q_TM * sizeof(RowExp));
   if constexpr (!PART) {
-    for (int r = threadIdx.x; r < Q_TM; r += 256) rows_e[r] = row_exp<H_STORE>(g, m0 + min(r, mv - 1));
+    for (int r = threadIdx.x; r < Q_TM; r += 256) rows_e[r] = row_exp<EPI>(g, m0 + min(r, mv - 1));
     __syncthreads();
   }
-  constexpr int LROW = 64 + 4;
+  constexpr int LROW = 64 + 4, LPR = TN / 4 / 8, RPI = 64 / LPR;  // (lanes a row, rows an iteration)
   float* const buf = reinterpret_cast<float*>(lds) + wv * 32 * LROW;
   static_assert(4 * 32 * LROW * 4 + Q_TM * sizeof(RowExp) <= LDS, "LDS");
-  const int64_t n = n0 + 64 * wv + 8 * (lane & 7);
-  const float* const from = buf + (lane >> 3) * LROW + 8 * (lane & 7);
+  const int64_t n = n0 + TN / 4 * wv + 8 * (lane % LPR);
+  const float* const from = buf + (lane / LPR) * LROW + 8 * (lane % LPR);
   float bias[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (!PART && g.bias)
+  if (EPI == H_STORE && !PART && g.bias)
 #pragma unroll
     for (int k = 0; k < 8; k++)
       if (n + k < g.N) bias[k] = g.bias[n + k];
@@ -749,43 +754,60 @@ __global__ __launch_bounds__(256, 1) void k_qgemm(const HGemm g, const uint8_t* 
       });
     });
 #pragma unroll 1
-    for (int r = 0; r < 32; r += 8) {
-      const int row = 32 * P + r + (lane >> 3);
+    for (int r = 0; r < 32; r += RPI) {
+      const int row = 32 * P + r + lane / LPR;
       const int64_t m = m0 + row;
       if (m >= g.M) continue;
-      const f32x4 a = *reinterpret_cast<const f32x4*>(from + r * LROW), b = *reinterpret_cast<const f32x4*>(from + r * LROW + 4);
+      f32x4 a[GATED ? 4 : 2];
+#pragma unroll
+      for (int k = 0; k < (GATED ? 4 : 2); k++)
+        a[k] = *reinterpret_cast<const f32x4*>(from + r * LROW + (k / 2) * 32 + (k % 2) * 4);
       if constexpr (PART) {
-        const int64_t pr = part_row<H_STORE>(g);
+        const int64_t pr = part_row<EPI>(g);
         float* o = g.parts + (int64_t(blockIdx.y) * g.M + m) * pr + n;
-        if (n < pr) {
-          *reinterpret_cast<f32x4*>(o) = a;
-          *reinterpret_cast<f32x4*>(o + 4) = b;
+        if (n < pad64(g.N)) {
+#pragma unroll
+          for (int k = 0; k < (GATED ? 4 : 2); k++) *reinterpret_cast<f32x4*>(o + (k / 2) * (pr / 2) + (k % 2) * 4) = a[k];
         }
       } else {
-        float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}, none[8];
-        finish<H_STORE>(g, g.e, rows_e[row], m, n, v, none, bias);
+        float v[8] = {a[0][0], a[0][1], a[0][2], a[0][3], a[1][0], a[1][1], a[1][2], a[1][3]}, u[8];
+        if constexpr (GATED)
+#pragma unroll
+          for (int k = 0; k < 4; k++) u[k] = a[2][k], u[4 + k] = a[3][k];
+        finish<EPI>(g, g.e, rows_e[row], m, n, v, u, bias);
       }
     }
   });
 }
 
-template <int QT>
-int launch_q(const HGemm& g, const artlite_matrix* w, int parts, hipStream_t s) {
+int64_t q_groups(int64_t M, const artlite_matrix* w, bool gate) {
+  const int tn = gate ? Q_TN / 2 : Q_TN;
+  return (M + Q_TM - 1) / Q_TM * ((w->N + tn - 1) / tn);
+}
+template <int QT, int EPI>
+int launch_q(const HGemm& g, const artlite_matrix* w, const artlite_matrix* w2, int parts, hipStream_t s) {
   constexpr int LDS = Q_RING * Q_SLOT + 4 * 8192 + 4 * 2048;
-  const int64_t gm = (g.M + Q_TM - 1) / Q_TM, gn = (g.N + Q_TN - 1) / Q_TN;
+  const int64_t gm = (g.M + Q_TM - 1) / Q_TM, gn = q_groups(g.M, w, gated<EPI>) / gm;
   static DeviceOnce set, set_part;
-  if (!set.lds(reinterpret_cast<const void*>(k_qgemm<QT, false>), LDS) ||
-      !set_part.lds(reinterpret_cast<const void*>(k_qgemm<QT, true>), LDS))
+  if (!set.lds(reinterpret_cast<const void*>(k_qgemm<QT, EPI, false>), LDS) ||
+      !set_part.lds(reinterpret_cast<const void*>(k_qgemm<QT, EPI, true>), LDS))
     return fail(ARTLITE_EHIP, "dense tiles: kernel set-up failed");
   const dim3 grid(unsigned(gm * gn), unsigned(parts));
+  const uint8_t *a = w->w.as<uint8_t>(), *b = w2 ? w2->w.as<uint8_t>() : nullptr;
   if (parts == 1) {
-    k_qgemm<QT, false><<<grid, 256, LDS, s>>>(g, w->w.as<uint8_t>(), w->tiles, w->units, g.e, int(gm), int(gn));
+    k_qgemm<QT, EPI, false><<<grid, 256, LDS, s>>>(g, a, b, w->tiles, w->units, int(gm), int(gn));
     ART_HIP(hipGetLastError());
     return ARTLITE_OK;
   }
-  k_qgemm<QT, true><<<grid, 256, LDS, s>>>(g, w->w.as<uint8_t>(), w->tiles, w->units, g.e, int(gm), int(gn));
+  k_qgemm<QT, EPI, true><<<grid, 256, LDS, s>>>(g, a, b, w->tiles, w->units, int(gm), int(gn));
   ART_HIP(hipGetLastError());
-  return join<H_STORE>(g, parts, s);
+  return join<EPI>(g, parts, s);
+}
+template <int QT>
+int launch_q_e(const HGemm& g, const artlite_matrix* w, const artlite_matrix* w2, int parts, hipStream_t s) {
+  return g.epilogue == H_STORE ? launch_q<QT, H_STORE>(g, w, w2, parts, s)
+         : g.epilogue == H_GLU ? launch_q<QT, H_GLU>(g, w, w2, parts, s)
+                               : launch_q<QT, H_DGLU>(g, w, w2, parts, s);
 }
 
 }  // namespace
@@ -856,29 +878,31 @@ int launch_join(const HGemm& g, int parts, hipStream_t s) {
 // 257 rows 36 us against 42, 2048 rows, 256 workgroups, 80 against 95, 3000 rows, 384, 125 against 115; 4096 x 12288 Q4_0, 512
 // rows 75 against 105, 2048 rows 198 against 225; 12288 x 4096 IQ4_XS, 512 rows 88 against 101, 700 rows, 288, 137 against
 // 118), and where the unpacking is most of the work (32768 x 2048 Q4_K, 512 rows, 512 workgroups, 77 against 98).
-bool qgemm_fits(int64_t M, const artlite_matrix* w) {
-  return int64_t(4) * w->units * w->ub < (int64_t(1) << 32) &&
-         (M <= 512 || (M + Q_TM - 1) / Q_TM * ((w->N + Q_TN - 1) / Q_TN) <= CUS);
+bool qgemm_fits(int64_t M, const artlite_matrix* w, bool gate) {
+  return int64_t(4) * w->units * w->ub < (int64_t(1) << 32) && (M <= 512 || q_groups(M, w, gate) <= CUS);
 }
 // the parts of K: as long as they fill CUs and a part has two units
-int qgemm_parts(int64_t M, const artlite_matrix* w) {
-  const int64_t wgs = (M + Q_TM - 1) / Q_TM * ((w->N + Q_TN - 1) / Q_TN);
+int qgemm_parts(int64_t M, const artlite_matrix* w, bool gate) {
+  const int64_t wgs = q_groups(M, w, gate);
   int parts = 1;
   while (wgs * parts * 2 <= CUS && w->units / (2 * parts) >= 2) parts *= 2;
   return parts;
 }
-size_t qgemm_parts_bytes(int64_t M, const artlite_matrix* w) {
-  const int parts = qgemm_parts(M, w);
-  return parts > 1 ? size_t(parts) * M * pad64(w->N) * 4 : 0;
+size_t qgemm_parts_bytes(int64_t M, const artlite_matrix* w, bool gate) {
+  const int parts = qgemm_parts(M, w, gate);
+  return parts > 1 ? size_t(parts) * M * (gate ? 2 : 1) * pad64(w->N) * 4 : 0;
 }
 
-int launch_qgemm(const HGemm& g, const artlite_matrix* w, hipStream_t s) {
+int launch_qgemm(HGemm g, const artlite_matrix* w, const artlite_matrix* w2, hipStream_t s) {
   if (g.M <= 0) return ARTLITE_OK;
-  const int parts = qgemm_parts(g.M, w);
+  const bool gate = g.epilogue != H_STORE;
+  const int parts = qgemm_parts(g.M, w, gate);
+  g.h_cols = g.h_stride;
   if (g.K != pad64(w->K) || g.lda < g.K || g.lda % 8 || g.lda > (int64_t(1) << 22) || g.N != w->N || g.segs != 1 ||
-      !w->direct || !qgemm_fits(g.M, w) || (parts > 1 && !g.parts))
+      !w->direct || !qgemm_fits(g.M, w, gate) || g.epilogue == H_ROWS || (gate && g.planes != 1) || gate != (w2 != nullptr) ||
+      (w2 && (!w2->direct || w2->t != w->t || w2->N != w->N || w2->K != w->K)) || (parts > 1 && !g.parts))
     return fail(ARTLITE_EINVAL, "dense tiles: K %lld of rows of %lld", (long long)g.K, (long long)g.lda);
-#define ART_Q(QT) return launch_q<QT>(g, w, parts, s)
+#define ART_Q(QT) return launch_q_e<QT>(g, w, w2, parts, s)
   ART_TILE_QTYPES(w->t->id, ART_Q)
 #undef ART_Q
 }
