@@ -209,7 +209,8 @@ LinearPlan linear_layout(Carve& c, const artlite_matrix* w, int dtype, int64_t n
   LinearPlan p;
   const int few_pl = dtype == ARTLITE_X_BF16 ? 1 : 3;
   const bool apart = few_apart(w, few_pl, false, n);
-  p.few = apart || n <= (dtype == ARTLITE_X_BF16 ? FEW_ROWS : FEW_ROWS_F32);
+  const bool large = direct && w->tiles * w->units > FEW_LARGE && qgemm_fits(n, w, false);
+  p.few = apart || n <= (dtype != ARTLITE_X_BF16 ? FEW_ROWS_F32 : large ? FEW_ROWS_LARGE : FEW_ROWS);
   if (p.few) {
     const int pl = few_pl;
     if (pl == 3 && !apart) p.planes = c.take<uint16_t>(3 * size_t(n) * w->K);
@@ -343,7 +344,8 @@ struct FfnPlan {
 FfnPlan ffn_layout(Carve& c, const Ffn& f, int dtype, int64_t n, bool direct, bool gated) {
   FfnPlan p{};
   const bool b = dtype == ARTLITE_X_BF16, apart = few_apart(f.gate, b ? 1 : 3, true, n);
-  p.few = n <= FEW_ROWS_FFN || (apart && few_apart(f.down, b ? 2 : 3, false, n));
+  const bool made = b && direct && gated && qgemm_fits(n, f.gate, true) && qgemm_fits(n, f.down, false);
+  p.few = n <= (made ? FEW_ROWS_FFN_DIRECT : FEW_ROWS_FFN) || (apart && few_apart(f.down, b ? 2 : 3, false, n));
   if (p.few) {
     if (!b && !apart) p.planes = c.take<uint16_t>(3 * size_t(n) * f.H);
     p.hp = c.take<uint16_t>(size_t(b ? 2 : 3) * n * f.F);

@@ -327,11 +327,15 @@ struct FewTArgs {
 int few_t_parts(const artlite_matrix* w, int pairs, int planes, int64_t M);
 size_t few_t_bytes(const artlite_matrix* w, int pairs, int planes, int64_t M);
 int launch_few_t(const FewTArgs& a, hipStream_t s);
-// Rows past which the dense products go by way of 16-bit weights and the large tiles. One matrix's of bf16 rows: 4096 x 4096
-// Q4_K, 256 rows, 27 us against 40, 384 rows 40 against 45; 12288 x 2048 IQ4_XS, 256 rows, 37 against 46, 384 rows 54 against
-// 58, 512 rows 73 against 60. Of fp32 rows: 4096 x 4096, 128 rows, 45 against 55, 192 rows 68 against 62. The gated block's:
-// 2048 x 8192 Q4_K, 144 rows, 72 against 77, 192 rows 76 against 75, 256 rows 95 against 76; fp32 143, 150 and 217 against 153,
-// 149 and 155; 4096 x 11008 Q4_0, 192 rows, 182 against 220. And any number of rows that are few_apart.
+// Rows past which the dense products go by way of 16-bit operands and large tiles: one matrix's of bf16 rows (4096 x 4096 Q4_K,
+// 256 rows, 27 us against 35, 257 rows 36 against the few rows' 40), of more than FEW_LARGE units where its values can be made
+// from its blocks (4096 x 12288 Q4_0, 128 rows 33 against 49, 129 rows 56 against 49; 32768 x 2048 Q4_K, 128 rows 58 against
+// 53, 256 rows 100 against 48; 4096 units above: 27 against 35); of fp32 rows (4096 x 4096, 128 rows, 45 against 55, 192 rows 68
+// against 62). The gated block's: of bf16 rows where its matrices' values can be made so (2048 x 8192 Q4_K, 64 rows 41 against
+// 53, 96 rows 57 against 55, 192 rows 81 against 65; 4096 x 11008 Q4_0, 64 rows 72 against 72, 96 rows 109 against 75), else
+// (fp32, 2048 x 8192, 144, 192 and 256 rows, 143, 150 and 217 against 153, 149 and 155). And any number of rows that are
+// few_apart.
+constexpr int FEW_ROWS_LARGE = 128, FEW_LARGE = 8192, FEW_ROWS_FFN_DIRECT = 64;
 constexpr int FEW_ROWS = 256, FEW_ROWS_F32 = 128, FEW_ROWS_FFN = 192;
 // x (M rows of K values of dtype, stride apart) as planes of bf16 (1: bf16 as it is; 3: fp32), rows of Kp values (zeros past K)
 int launch_planes(const void* x, int dtype, int64_t M, int64_t K, int64_t stride, uint16_t* out, int64_t Kp, int64_t plane,

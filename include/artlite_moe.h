@@ -200,8 +200,8 @@ int artlite_stream_capturing(void* stream, int* out);
 int artlite_workspace_destroy(artlite_workspace* work); /* its calls have come to their end */
 
 /* y (n x rows) = x (n x cols) W^T (+ bias). x's products with the blocks' values are summed in fp32 and rounded once to y's
- * type (up to 256 bf16 rows or 128 fp32 ones, more of a small matrix, without rounding a weight; past that weights are fp16 of
- * 11 bits for bf16 x, of 22 for fp32 x).
+ * type (up to 128 rows, 256 bf16 ones of a matrix that is not large, more of a small one, without rounding a weight; past that
+ * weights are fp16 of 11 bits for bf16 x, of 22 for fp32 x).
  * artlite_linear_workspace: the bytes of workspace that a call of n rows needs (0 for up to 16 rows); work may be null where
  * that is 0. */
 int artlite_linear_workspace(const artlite_matrix* w, int dtype, int64_t n, size_t* nbytes);

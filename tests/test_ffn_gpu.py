@@ -58,7 +58,7 @@ def grads(f: GatedFFN, x: np.ndarray, dy: np.ndarray, names: tuple[str, ...] = G
 def test_forward(H: int, F: int, q: str, down: str, act: str, dtype: str) -> None:
     f, w = make(H, F, q, down, act)
     past = min(past_small(F, H, 1 if dtype == "bf16" else 3, True), past_small(H, F, 2))
-    for n in (1, 3, 6, 16, 17, 40, 65, 128, 129, 192, 193, 240, past):
+    for n in (1, 3, 6, 16, 17, 40, 65, 128, 129, 192, 193, 240, 300, past):
         x = rows(n, H, dtype, n, 3.0)
         check(f(x), dense.ffn(act, values(x), *w), FORWARD[dtype])
     assert f(np.empty((0, H), DTYPE[dtype])).shape == (0, H)
@@ -93,6 +93,25 @@ def test_large_tiles(dtype: str) -> None:
     want = dense.ffn_grad("silu", values(x), values(dy), *w)
     for k, g in grads(f, x, dy).items():
         check(g, want[k], BACKWARD[dtype])
+
+
+def test_scales_beyond_their_values() -> None:
+    """Matrices with groups whose values are small differences of their scales and offsets take the unpacked way."""
+    H, F = 288, 416
+    f, w = GatedFFN(hidden=H, ffn=F, gate_type="Q4_1", down_type="Q4_1"), []
+    for i, (name, r, c) in enumerate((("gate", F, H), ("up", F, H), ("down", H, F))):
+        raw, _ = dense.matrix("Q4_1", r, c, i)
+        raw = raw.reshape(r, c // 32, 20).copy()
+        raw[7, 2, :2], raw[7, 2, 2:4] = (np.array([v], np.float16).view(np.uint8) for v in (1.0, -15.0))
+        raw[7, 2, 4:] = 0xFF  # (15 d + m = 0)
+        f.upload("ffn_" + name, raw.reshape(r, -1))
+        w.append(dense.gguf_ref.dequantize("Q4_1", raw.reshape(r, -1), c).astype(np.float64))
+    for n in (9, 100, 240, 1500):
+        x, dy = rows(n, H, "bf16", n, 3.0), rows(n, H, "bf16", n + 1)
+        check(f(x), dense.ffn("silu", values(x), *w), FORWARD["bf16"])
+        want = dense.ffn_grad("silu", values(x), values(dy), *w)
+        for k, g in grads(f, x, dy).items():
+            check(g, want[k], BACKWARD["bf16"])
 
 
 def test_some_gradients() -> None:
