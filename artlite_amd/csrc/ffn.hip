@@ -2,8 +2,8 @@
 // (the C entry points artlite_linear*, artlite_ffn*), and the passes over activations that the large tiles need.
 //
 // Up to FEW_ROWS rows go through k_few (linear.hip; backward also k_few_t), straight from the blocks. More rows go through the
-// large tiles (hgemm.hip), over fp16 operands made for the call in its workspace, or, one matrix's of some hundreds of bf16
-// rows, through tiles that make W's from the blocks (k_qgemm):
+// large tiles (hgemm.hip), over fp16 operands made for the call in its workspace, or, some hundreds of bf16 rows, through tiles
+// that make the weights' operands from the blocks (k_qgemm):
 //   x, dy: each row times the power of two that brings its largest value into [2^14, 2^15): bf16 values convert exactly
 //     (those above 2^-29 of their row's largest; smaller ones keep 2^-39 of it), fp32 ones as two planes (hi + lo, 2^-22);
 //   weights: each value times the matrix's power of two, rounded once to fp16 (2^-11; fp32 calls: two planes, 2^-22), an

@@ -877,9 +877,12 @@ int launch_join(const HGemm& g, int parts, hipStream_t s) {
 // Where it is the faster way (against unpacking W and the tiles above): for what is one workgroup a CU at most (4096 x 4096 Q4_K,
 // 257 rows 36 us against 42, 2048 rows, 256 workgroups, 80 against 95, 3000 rows, 384, 125 against 115; 4096 x 12288 Q4_0, 512
 // rows 75 against 105, 2048 rows 198 against 225; 12288 x 4096 IQ4_XS, 512 rows 88 against 101, 700 rows, 288, 137 against
-// 118), and where the unpacking is most of the work (32768 x 2048 Q4_K, 512 rows, 512 workgroups, 77 against 98).
+// 118), and where the unpacking is most of the work (32768 x 2048 Q4_K, 512 rows, 512 workgroups, 77 against 98). A gated pair,
+// two matrices to unpack, to four a CU (a block's forward, 4096 x 11008 Q4_0: 1000 rows, 688 workgroups, 266 against 326, 1300
+// rows, 946, 359 against 445; 2048 x 8192 Q4_K, 2048 rows, 1024, 213 against 231; 3584 x 9472 IQ4_XS, 1000 rows, 592, 282
+// against 278).
 bool qgemm_fits(int64_t M, const artlite_matrix* w, bool gate) {
-  return int64_t(4) * w->units * w->ub < (int64_t(1) << 32) && (M <= 512 || q_groups(M, w, gate) <= CUS);
+  return int64_t(4) * w->units * w->ub < (int64_t(1) << 32) && (M <= 512 || q_groups(M, w, gate) <= (gate ? 4 : 1) * CUS);
 }
 // the parts of K: as long as they fill CUs and a part has two units
 int qgemm_parts(int64_t M, const artlite_matrix* w, bool gate) {
