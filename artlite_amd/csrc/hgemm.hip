@@ -116,12 +116,14 @@ __device__ __forceinline__ void finish16(const HGemm& g, int es, const RowExp& r
     } else if constexpr (EPI == H_GLU) {
       v[k] = gate_act<TWO>(g.act, __builtin_amdgcn_ldexpf(v[k], ev)) * __builtin_amdgcn_ldexpf(u[k], eu - r.out);
     } else {
-      const float uv = __builtin_amdgcn_ldexpf(u[k], eu), dh = __builtin_amdgcn_ldexpf(d[k], r.dh - r.out);
+      // (act(g) and u over 2^ga, which is above both: no factor passes fp32's range, however small or large the row)
+      const int ga = r.out - r.dh;
       float a, da;
       gate_act_grad<TWO>(g.act, __builtin_amdgcn_ldexpf(v[k], ev), a, da);
-      h[k] = a * __builtin_amdgcn_ldexpf(u[k], eu - r.h);
-      v[k] = dh * uv * da;
-      u[k] = dh * a;
+      a = __builtin_amdgcn_ldexpf(a, -ga);
+      h[k] = a * __builtin_amdgcn_ldexpf(u[k], eu + ga - r.h);
+      v[k] = d[k] * __builtin_amdgcn_ldexpf(u[k], eu - ga) * da;
+      u[k] = d[k] * a;
     }
   }
   if (there < 8) {
