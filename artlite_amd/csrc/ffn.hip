@@ -34,7 +34,7 @@ struct Rows16 {
   int arrays;
   int64_t K, Kp, plane;
   int32_t *he, *dhe, *de;   // (those that are wanted)
-  int lh, ld, lw;           // gate's and up's bounds together; down's; the larger of gate's and up's and 1 for the derivative
+  int lg, lu, ld;           // gate's, up's and down's bounds
 };
 
 // a row a workgroup -> fp16 planes of Kp values
@@ -95,9 +95,10 @@ __global__ __launch_bounds__(256) void k_rows16(const Rows16 a) {
     if (threadIdx.x == 0) a.e[i][m] = e - 15;
   }
   if (threadIdx.x == 0) {
-    if (a.he) a.he[m] = 2 * norm[0] + a.lh - 15;
+    // (h is act(g) times u over 2^he, which is below 2^127 that way: where g is below 2^-112, h has no value but 0 in fp32)
+    if (a.he) a.he[m] = max(norm[0] + a.lg, -112) + norm[0] + a.lu - 15;
     if (a.dhe) a.dhe[m] = norm[1] + a.ld - 15;
-    if (a.de) a.de[m] = norm[1] + a.ld + norm[0] + a.lw - 15;
+    if (a.de) a.de[m] = norm[1] + a.ld + norm[0] + max(a.lg, a.lu) + 1 - 15;  // (1 for the derivative)
   }
 }
 
@@ -410,7 +411,7 @@ int ffn_forward(const Ffn& f, const void* x, int dtype, int64_t n, int64_t x_str
   Rows16 r{};
   r.x[0] = x, r.stride[0] = x_stride, r.out[0] = p.x16, r.e[0] = p.xe;
   r.arrays = 1, r.K = f.H, r.Kp = f.Hp, r.plane = n * f.Hp;
-  r.he = p.he, r.lh = f.gate->row_exp + f.up->row_exp;
+  r.he = p.he, r.lg = f.gate->row_exp, r.lu = f.up->row_exp;
   ART_TRY(rows16(r, dtype, n, s));
   const int eg = p.gated ? qexp16(f.gate) : wexp16(f.gate), eu = p.gated ? qexp16(f.up) : wexp16(f.up);
   if (!p.gated) ART_TRY(launch_unpack(f.gate, f.up, false, eg, eu, p.w16, p.u16, f.Hp, f.F * f.Hp, pl, s));
@@ -513,13 +514,12 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
   Carve c(base);
   const GradPlan p = grad_plan(c, f, dtype, n, weights);
   const int pl = dtype == ARTLITE_X_BF16 ? 1 : 2;
-  const int lg = f.gate->row_exp, lu = f.up->row_exp;
   Rows16 r{};
   r.x[0] = x, r.stride[0] = x_stride, r.out[0] = p.x16, r.e[0] = p.xe;
   r.x[1] = dy, r.stride[1] = dy_stride, r.out[1] = p.dy16, r.e[1] = p.ye;
   r.arrays = 2, r.K = f.H, r.Kp = f.Hp, r.plane = n * f.Hp;
   r.he = p.he, r.dhe = p.dhe, r.de = p.de;
-  r.lh = lg + lu, r.lw = (lg > lu ? lg : lu) + 1;
+  r.lg = f.gate->row_exp, r.lu = f.up->row_exp;
   r.ld = f.down->max_exp + int(std::ceil(0.5 * std::log2(double(f.H))));
   ART_TRY(rows16(r, dtype, n, s));
   // (gate and up share a scale: dx sums over both)

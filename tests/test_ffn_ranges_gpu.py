@@ -8,7 +8,7 @@ import pytest
 from oracle import dense
 
 from .dense_helpers import check, encode, values
-from .test_ffn_gpu import BACKWARD, GRADS, grads, make, rows
+from .test_ffn_gpu import BACKWARD, FORWARD, GRADS, grads, make, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +46,19 @@ def test_small_rows_backward(dtype: str) -> None:
         for r in range(min(n, 40)):
             planes = 2.0 ** -134 / size[r, 0] if dtype == "f32" else 0.0
             check(got["dx"][r:r + 1], want["dx"][r:r + 1], 1.5 * BACKWARD[dtype] + planes)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_small_rows_forward(dtype: str) -> None:
+    """Rows whose h has no value but 0 in fp32, and rows that are small."""
+    f, w = make(H, F, "Q4_0", "Q4_1")
+    for n in (*ROWS, 18000):
+        size = np.resize([1e-37, 1.0, 1e-15, 3e-36, 0.0, 1e-33], n)[:, None]
+        x = encode(size * np.random.default_rng(n).standard_normal((n, H)), dtype)
+        got, want = values(f(x)), dense.ffn("silu", values(x), *w)
+        assert np.isfinite(got).all(), n
+        nothing = size[:, 0] < 1e-30
+        assert not got[nothing].any(), n
+        for r in range(min(n, 40)):
+            if not nothing[r]:
+                check(got[r:r + 1], want[r:r + 1], 1.5 * FORWARD[dtype])
