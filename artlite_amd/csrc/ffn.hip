@@ -37,7 +37,10 @@ struct Rows16 {
   int lg, lu, ld;           // gate's, up's and down's bounds
 };
 
-// a row a workgroup -> fp16 planes of Kp values
+__device__ __forceinline__ float finite(float v) { return fabsf(v) < __builtin_inff() ? v : 0.0f; }
+
+// a row a workgroup -> fp16 planes of Kp values. The exponents are those of its finite values: a row with an infinite one
+// keeps the others' bits, which a gradient of the weights sums apart from it.
 template <bool BF16>
 __global__ __launch_bounds__(256) void k_rows16(const Rows16 a) {
   __shared__ float red[4];
@@ -68,7 +71,7 @@ __global__ __launch_bounds__(256) void k_rows16(const Rows16 a) {
     for (int64_t k = threadIdx.x * 8; k < a.K; k += 2048) {
       float v[8];
       load(k, v);
-      for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(v[j]));
+      for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(finite(v[j])));
     }
     mx = all(mx, false);
     const int e = exp_above(mx);
@@ -80,7 +83,7 @@ __global__ __launch_bounds__(256) void k_rows16(const Rows16 a) {
       uint16_t hi[8], lo[8];
       for (int j = 0; j < 8; j++) {
         const float r = __builtin_amdgcn_ldexpf(v[j], -e), s = __builtin_amdgcn_ldexpf(r, 15);
-        ss = __builtin_fmaf(r, r, ss);
+        ss = __builtin_fmaf(finite(r), finite(r), ss);
         const _Float16 h = _Float16(s);
         hi[j] = __builtin_bit_cast(uint16_t, h);
         // (an infinite value is its first plane)

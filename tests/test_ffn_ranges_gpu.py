@@ -62,3 +62,20 @@ def test_small_rows_forward(dtype: str) -> None:
         for r in range(min(n, 40)):
             if not nothing[r]:
                 check(got[r:r + 1], want[r:r + 1], 1.5 * FORWARD[dtype])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_infinite_gradients(dtype: str) -> None:
+    """An infinite value of dy reaches its row's dx, the gate's and up's gradients (sums over that row too) and its own row
+    of ddown alone."""
+    f, w = make(H, F, "Q4_0", "Q4_1")
+    for n in ROWS[1:]:
+        x, dy = rows(n, H, dtype, n, 3.0), rows(n, H, dtype, n + 1)
+        clean = grads(f, x, dy, ("dx",))["dx"]
+        want = dense.ffn_grad("silu", values(x), values(dy), *w)["ddown"]
+        dy[1, 3] = encode(np.array([np.inf]), dtype)[0]
+        got = grads(f, x, dy)
+        assert not np.isfinite(values(got["dx"])[1]).any() and not np.isfinite(values(got["ddown"])[3]).any()
+        assert not np.isfinite(values(got["dgate"])).any() and not np.isfinite(values(got["dup"])).any()
+        assert np.array_equal(np.delete(got["dx"], 1, 0), np.delete(clean, 1, 0))
+        check(np.delete(got["ddown"], 3, 0), np.delete(want, 3, 0), BACKWARD[dtype])
