@@ -148,7 +148,7 @@ __global__ __launch_bounds__(256) void k_bounds(const uint8_t* __restrict__ w, i
           float gx = 0.0f;
 #pragma unroll
           for (int p = 0; p < 8; p++) {
-            gx = fmaxf(gx, fabsf(v[p]));
+            gx = fmaxf(gx, fabsf(v[p]) < __builtin_inff() ? fabsf(v[p]) : 0.0f);
             ss = __builtin_fmaf(v[p], v[p], ss);
           }
           mx = fmaxf(mx, gx);
@@ -359,7 +359,7 @@ int matrix_upload(artlite_matrix* m, const void* data) {
   ART_HIP(hipStreamSynchronize(c->stream));
   float f[2];
   std::memcpy(f, b, 8);
-  // (a matrix of zeros, or with scales that are no numbers: any bound will do)
+  // (of finite values; a matrix without any, or of zeros: any bound will do)
   m->max_exp = f[0] > 0.0f ? exp_above(f[0]) : 0;
   m->row_exp = f[1] > 0.0f ? exp_above(f[1]) : 0;
   m->direct = b[2] == 0;
