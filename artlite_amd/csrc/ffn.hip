@@ -12,7 +12,9 @@
 //     |g| <= |x| max |gate row| in the 2-norm, |act(g)| <= |g|, |act'| < 2, |dh| <= |dy| max |down| sqrt(H); typical values lie
 //     some 2^14 below their bound, fp16 holds 2^29 below it in full.
 // Products of two planes are three sums (hi hi + hi lo + lo hi). The weights' gradients sum over rows, so their operands are
-// turned and take one power of two for all rows (the largest; a value keeps 2^-39 of the largest).
+// turned, and the rows' powers of two go into one of the two: each of its turned rows, a row of the output, takes the power that
+// brings its own largest term's factor into [2^14, 2^15), so that what a row of x and of dy adds counts by what the two come to
+// together (k_top reads dg, du and dy once more for that: 37 us of the 2110 that all gradients of 4096 rows of 4096 x 8192 take).
 #include "hgemm.h"
 #include "matrix.h"
 
@@ -23,6 +25,9 @@
 namespace artlite {
 
 namespace {
+
+// the exponent of nothing but zeros, below those of all rows
+constexpr int NO_TOP = -(1 << 24);
 
 // A launch of k_rows16: x, or x and dy, and the exponents of their rows (and of h, dh, dg and du, from the rows' 2-norms and
 // the matrices' bounds)
@@ -35,6 +40,8 @@ struct Rows16 {
   int64_t K, Kp, plane;
   int32_t *he, *dhe, *de;   // (those that are wanted)
   int lg, lu, ld;           // gate's, up's and down's bounds
+  int32_t* top;             // (wanted) `tops` exponents to set to NO_TOP
+  int64_t tops;
 };
 
 __device__ __forceinline__ float finite(float v) { return fabsf(v) < __builtin_inff() ? v : 0.0f; }
@@ -46,6 +53,7 @@ __global__ __launch_bounds__(256) void k_rows16(const Rows16 a) {
   __shared__ float red[4];
   const int64_t m = blockIdx.x;
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  for (int64_t i = m * 256 + threadIdx.x; i < a.tops; i += int64_t(gridDim.x) * 256) a.top[i] = NO_TOP;
   auto all = [&](float v, bool add) {
     for (int o = 32; o; o >>= 1) {
       const float u = __shfl_xor(v, o);
@@ -105,29 +113,75 @@ __global__ __launch_bounds__(256) void k_rows16(const Rows16 a) {
   }
 }
 
-// the largest of each of up to 4 arrays
-struct MaxE {
-  const int32_t* a[4];
+// An fp16 value's place among those worth 2^e: its bits with the exponent put in, in the order of sizes (an infinite one comes
+// last: all of its output row is no number), nothing for 0; and the exponent that brings it into [2^14, 2^15) (or less: a
+// subnormal one counts as 2^-14)
+__device__ __forceinline__ int top_key(uint32_t h, int e) {
+  const int b = int(h & 0x7FFFu);
+  return b ? b + e * 1024 : NO_TOP;
+}
+__device__ __forceinline__ int top_exp(int key) { return key == NO_TOP ? NO_TOP : (key >> 10) - 29; }
+
+// Tops of a launch: of each of C columns of T rows of fp16 values (ld apart, row t worth 2^(e[t] + e2[t])), the exponent that
+// brings its largest value into [2^14, 2^15) (out: set to NO_TOP before; integer maxima, so any order is the same).
+// 128 rows of 512 columns a workgroup, read once.
+constexpr int TOP_ROWS = 128, TOP_COLS = 512;
+struct Top {
+  const uint16_t* in;
+  int64_t ld, C;
+  const int32_t *e, *e2;
+  int32_t* out;
 };
-__global__ __launch_bounds__(1024) void k_max_e(const MaxE in, int64_t M, int32_t* __restrict__ out) {
-  __shared__ int red[16];
-  const int32_t* a = in.a[blockIdx.x];
-  int v = INT32_MIN;
-  for (int64_t m = threadIdx.x; m < M; m += 1024) v = max(v, a[m]);
-  for (int o = 32; o; o >>= 1) v = max(v, __shfl_xor(v, o));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+struct Tops {
+  Top t[3];
+  int64_t T;
+};
+__global__ __launch_bounds__(256) void k_top(const Tops a) {
+  __shared__ __attribute__((aligned(16))) int red[4][TOP_COLS];
+  const Top& j = a.t[blockIdx.z];
+  const int64_t c0 = int64_t(blockIdx.x) * TOP_COLS, t0 = int64_t(blockIdx.y) * TOP_ROWS;
+  if (c0 >= j.C) return;
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  int top[8];
+#pragma unroll
+  for (int k = 0; k < 8; k++) top[k] = NO_TOP;
+  if (c0 + 8 * lane < j.ld) {  // (ld is a multiple of 64)
+    constexpr int AT_ONCE = 8;  // (rows of a wave in flight)
+    const int64_t end = min(t0 + TOP_ROWS, a.T);
+    for (int64_t t = t0 + wv; t < end; t += 4 * AT_ONCE) {
+      uint4 v[AT_ONCE];
+      int e[AT_ONCE];
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; i++) {  // (past the last row the last again: the largest stays)
+        const int64_t r = min(t + 4 * i, end - 1);
+        v[i] = *reinterpret_cast<const uint4*>(j.in + r * j.ld + c0 + 8 * lane);
+        e[i] = j.e[r] + j.e2[r];
+      }
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; i++) {
+        const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+        for (int k = 0; k < 8; k++) top[k] = max(top[k], top_key(w[k >> 1] >> (16 * (k & 1)), e[i]));
+      }
+    }
+  }
+  for (int k = 0; k < 8; k++) red[wv][8 * lane + k] = top[k];
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 0; w < 16; w++) v = max(v, red[w]);
-    out[blockIdx.x] = v;
+  for (int c = threadIdx.x; c < TOP_COLS; c += 256) {
+    const int v = max(max(red[0][c], red[1][c]), max(red[2][c], red[3][c]));
+    if (c0 + c < j.C && v > NO_TOP) atomicMax(j.out + c0 + c, top_exp(v));
   }
 }
 
-// Turns of a launch: rows of C fp16 values (ld apart, row t worth 2^e[t]) into C rows of Tp values worth 2^*top, zeros past T
+// Turns of a launch: rows of C fp16 values (ld apart) into C rows of Tp values, zeros past T; as they are, or (top) those of
+// row t worth 2^(e[t] + e2[t]) into those of row c worth 2^top[c]. Up to TURN_ROWS rows are a workgroup's (ONE): it finds `top`
+// by itself, a launch less (45 rows of 1024 x 2816, fp32, all gradients: 81 us, 86 with k_top)
+constexpr int TURN_ROWS = 64;
 struct Turn {
   const uint16_t* in;
   int64_t ld, C;
-  const int32_t *e, *top;
+  const int32_t *e, *e2;
+  int32_t* top;
   uint16_t* out;
 };
 struct Turns {
@@ -135,6 +189,7 @@ struct Turns {
   int64_t T, Tp;
   int planes;
 };
+template <bool ONE>
 __global__ __launch_bounds__(256) void k_turn(const Turns a) {
   __shared__ __attribute__((aligned(16))) uint16_t t[64][72];
   const Turn& j = a.t[blockIdx.z / a.planes];
@@ -143,19 +198,42 @@ __global__ __launch_bounds__(256) void k_turn(const Turns a) {
   const int64_t pl = blockIdx.z % a.planes;
   const uint16_t* in = j.in + pl * a.T * j.ld;
   uint16_t* out = j.out + pl * j.C * a.Tp;
-  const int E = *j.top;
-  for (int i = threadIdx.x; i < 64 * 8; i += 256) {
-    const int r = i >> 3, c = 8 * (i & 7);
-    uint16_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (t0 + r < a.T && c0 + c < j.ld) {  // (ld is a multiple of 64: the row's padding is read at most)
-      __builtin_memcpy(v, __builtin_assume_aligned(in + (t0 + r) * j.ld + c0 + c, 16), 16);
-      const int sh = j.e[t0 + r] - E;
-      for (int k = 0; k < 8; k++)
-        v[k] = __builtin_bit_cast(uint16_t,
-                                  _Float16(__builtin_amdgcn_ldexpf(float(__builtin_bit_cast(_Float16, v[k])), sh)));
+  const int c = 8 * (threadIdx.x & 7);
+  int top[8] = {0, 0, 0, 0, 0, 0, 0, 0}, e[2] = {0, 0};
+  uint16_t v[2][8] = {};
+#pragma unroll
+  for (int q = 0; q < 2; q++) {
+    const int64_t r = t0 + (threadIdx.x >> 3) + 32 * q;
+    if (r < a.T && c0 + c < j.ld) {  // (ld is a multiple of 64: the row's padding is read at most)
+      __builtin_memcpy(v[q], __builtin_assume_aligned(in + r * j.ld + c0 + c, 16), 16);
+      if (j.top) e[q] = j.e[r] + j.e2[r];
     }
-    for (int k = 0; k < 8; k++) t[c + k][r] = v[k];
   }
+  if (ONE && j.top) {
+    __shared__ int most[64];
+    if (threadIdx.x < 64) most[threadIdx.x] = NO_TOP;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+      uint16_t h[8] = {0, 0, 0, 0, 0, 0, 0, 0};  // (the first plane's: the second's come with its exponents)
+      const int64_t r = (threadIdx.x >> 3) + 32 * q;
+      if (r < a.T && c0 + c < j.ld) __builtin_memcpy(h, __builtin_assume_aligned(j.in + r * j.ld + c0 + c, 16), 16);
+#pragma unroll
+      for (int k = 0; k < 8; k++) atomicMax(&most[c + k], top_key(h[k], e[q]));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8; k++) top[k] = top_exp(most[c + k]);
+    if (pl == 0 && threadIdx.x < 64 && c0 + threadIdx.x < j.C) j.top[c0 + threadIdx.x] = top_exp(most[threadIdx.x]);
+  } else if (j.top && c0 + c < j.C) {  // (C is a multiple of 32)
+    __builtin_memcpy(top, __builtin_assume_aligned(j.top + c0 + c, 16), 32);
+  }
+#pragma unroll
+  for (int q = 0; q < 2; q++)
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      t[c + k][(threadIdx.x >> 3) + 32 * q] = __builtin_bit_cast(
+          uint16_t, _Float16(__builtin_amdgcn_ldexpf(float(__builtin_bit_cast(_Float16, v[q][k])), e[q] - top[k])));
   __syncthreads();
   for (int i = threadIdx.x; i < 64 * 8; i += 256) {
     const int c = i >> 3, r = 8 * (i & 7);
@@ -459,7 +537,8 @@ struct GradPlan {
   uint16_t *x16, *dy16, *a16, *b16, *c16;        // x, dy; gate and up, later their transposes; down's transpose
   uint16_t *h16, *dh16, *dg16, *du16;
   uint16_t *xt, *dyt, *ht, *dgt, *dut;           // (weights' gradients) turned
-  int32_t *xe, *ye, *he, *dhe, *de, *top;
+  int32_t *xe, *ye, *he, *dhe, *de;
+  int32_t* top;                                  // (weights' gradients) the exponents of rows of dgate, dup and ddown
   float* parts;
 };
 GradPlan grad_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool weights) {
@@ -494,7 +573,7 @@ GradPlan grad_plan(Carve& c, const Ffn& f, int dtype, int64_t n, bool weights) {
     p.ht = c.take<uint16_t>(pl * f.F * Tp);
     p.dgt = c.take<uint16_t>(pl * f.F * Tp);
     p.dut = c.take<uint16_t>(pl * f.F * Tp);
-    p.top = c.take<int32_t>(4);
+    p.top = c.take<int32_t>(2 * f.F + f.H);
   }
   const int sg = pl == 2 ? 3 : 1;
   size_t parts = 0;
@@ -524,6 +603,7 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
   r.he = p.he, r.dhe = p.dhe, r.de = p.de;
   r.lg = f.gate->row_exp, r.lu = f.up->row_exp;
   r.ld = f.down->max_exp + int(std::ceil(0.5 * std::log2(double(f.H))));
+  if (weights && n > TURN_ROWS) r.top = p.top, r.tops = 2 * f.F + f.H;
   ART_TRY(rows16(r, dtype, n, s));
   // (gate and up share a scale: dx sums over both)
   const int e = wexp16(f.gate) > wexp16(f.up) ? wexp16(f.gate) : wexp16(f.up), ed = wexp16(f.down);
@@ -591,36 +671,43 @@ int ffn_backward(const Ffn& f, const void* x, int64_t x_stride, const void* dy, 
     }
   }
   if (!weights) return ARTLITE_OK;
+  // Sums over rows t of a[t][m] b[t][k]: a (dg, du, dy) takes both rows' powers of two, and an output row one of its own, from
+  // what its terms come to; b (x, h) stays as it is.
   const int64_t Tp = pad64(n);
-  k_max_e<<<4, 1024, 0, s>>>(MaxE{{p.xe, p.ye, p.he, p.de}}, n, p.top);
+  int32_t *const ge = p.top, *const ue = ge + f.F, *const ddowne = ue + f.F;
+  Tops o{};
+  o.T = n;
   Turns t{};
   t.T = n, t.Tp = Tp, t.planes = pl;
-  int turns = 0;
-  if (dgate || dup) t.t[turns++] = Turn{p.x16, f.Hp, f.H, p.xe, p.top, p.xt};
-  if (dgate) t.t[turns++] = Turn{p.dg16, f.Fp, f.F, p.de, p.top + 3, p.dgt};
-  if (dup) t.t[turns++] = Turn{p.du16, f.Fp, f.F, p.de, p.top + 3, p.dut};
-  if (ddown) {
-    t.t[turns++] = Turn{p.dy16, f.Hp, f.H, p.ye, p.top + 1, p.dyt};
-    t.t[turns++] = Turn{p.h16, f.Fp, f.F, p.he, p.top + 2, p.ht};
-  }
-  k_turn<<<dim3(unsigned((std::max(f.H, f.F) + 63) / 64), unsigned(Tp / 64), unsigned(turns * pl)), 256, 0, s>>>(t);
-  ART_HIP(hipGetLastError());
   HGemm w[3] = {};
-  int count = 0;
-  const auto grad = [&](const uint16_t* a, int64_t M, const int32_t* ea, const uint16_t* b, int64_t N, const int32_t* eb,
-                        void* out) {
+  int turns = 0, count = 0;
+  const auto grad = [&](const uint16_t* a, uint16_t* at, int64_t M, int64_t Mp, const int32_t* ea, const uint16_t* bt, int64_t N,
+                        const int32_t* eb, int32_t* top, void* out) {
     if (!out) return;
+    o.t[count] = Top{a, Mp, M, ea, eb, top};
+    t.t[turns++] = Turn{a, Mp, M, ea, eb, top, at};
     HGemm& g = w[count++];
-    segments(g, {{a, M * Tp, b, N * Tp}}, pl);
+    segments(g, {{at, M * Tp, bt, N * Tp}}, pl);
     g.lda = g.ldb = g.K = Tp;
     g.M = M, g.N = N;
-    g.e0 = ea, g.e1 = eb;
+    g.row_e = top;
     g.y = out, g.y_stride = N, g.dtype = dtype;
     g.parts = p.parts;
   };
-  grad(p.dgt, f.F, p.top + 3, p.xt, f.H, p.top, dgate);
-  grad(p.dut, f.F, p.top + 3, p.xt, f.H, p.top, dup);
-  grad(p.dyt, f.H, p.top + 1, p.ht, f.F, p.top + 2, ddown);
+  grad(p.dg16, p.dgt, f.F, f.Fp, p.de, p.xt, f.H, p.xe, ge, dgate);
+  grad(p.du16, p.dut, f.F, f.Fp, p.de, p.xt, f.H, p.xe, ue, dup);
+  grad(p.dy16, p.dyt, f.H, f.Hp, p.ye, p.ht, f.F, p.he, ddowne, ddown);
+  if (dgate || dup) t.t[turns++] = Turn{p.x16, f.Hp, f.H, nullptr, nullptr, nullptr, p.xt};
+  if (ddown) t.t[turns++] = Turn{p.h16, f.Fp, f.F, nullptr, nullptr, nullptr, p.ht};
+  const int64_t widest = std::max(f.H, f.F);
+  if (n > TURN_ROWS) {
+    const dim3 grid(unsigned((widest + TOP_COLS - 1) / TOP_COLS), unsigned((n + TOP_ROWS - 1) / TOP_ROWS), unsigned(count));
+    k_top<<<grid, 256, 0, s>>>(o);
+    ART_HIP(hipGetLastError());
+  }
+  (n > TURN_ROWS ? k_turn<false> : k_turn<true>)<<<dim3(unsigned((widest + 63) / 64), unsigned(Tp / 64), unsigned(turns * pl)),
+                                                   256, 0, s>>>(t);
+  ART_HIP(hipGetLastError());
   if (Tp <= SHORT_SUMS) return launch_hgemms(w, count, s);
   for (int i = 0; i < count; i++) ART_TRY(launch_hgemm(w[i], s));
   return ARTLITE_OK;

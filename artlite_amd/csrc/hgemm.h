@@ -21,9 +21,8 @@ struct HGemm {
   int64_t lda, ldb;
   int64_t M, N, K;
   int epilogue;
-  // scales: the sums of row m are worth 2^(e + row_e[m] + *e0 + *e1) (row_e, e0, e1 may be null); gated: e2 the second's
+  // scales: the sums of row m are worth 2^(e + row_e[m]) (row_e may be null); gated: e2 the second's
   const int32_t* row_e;
-  const int32_t *e0, *e1;
   int e, e2;
   // H_STORE: y[m][n] = the sum + bias[n], bf16 or fp32
   const float* bias;

@@ -102,10 +102,9 @@ struct RowExp {
 // columns n .. n + 8 of row m of the planes from their sums v (gated: and the second matrix's u); the exponents of what is
 // written go into its factors, so that each value takes one scaling
 template <int EPI, bool TWO>
-__device__ __forceinline__ void finish16(const HGemm& g, int es, const RowExp& r, int64_t m, int64_t n, float (&v)[8],
-                                         float (&u)[8]) {
+__device__ __forceinline__ void finish16(const HGemm& g, const RowExp& r, int64_t m, int64_t n, float (&v)[8], float (&u)[8]) {
   const int64_t at = m * g.h_stride + n;
-  const int ev = es + r.sum, eu = es - g.e + g.e2 + r.sum;
+  const int ev = g.e + r.sum, eu = g.e2 + r.sum;
   const int there = int(max(int64_t(0), min(int64_t(8), g.N - n)));  // (columns that there are)
   float d[8], h[8];
   if constexpr (EPI == H_DGLU) load16<TWO>(g.dh + at, g.h_plane, d);
@@ -142,13 +141,13 @@ __device__ __forceinline__ void finish16(const HGemm& g, int es, const RowExp& r
 
 // columns n .. n + 8 of row m from their sums v (gated: and the second matrix's u)
 template <int EPI>
-__device__ __forceinline__ void finish(const HGemm& g, int es, const RowExp& r, int64_t m, int64_t n, float (&v)[8],
+__device__ __forceinline__ void finish(const HGemm& g, const RowExp& r, int64_t m, int64_t n, float (&v)[8],
                                        float (&u)[8], const float (&bias)[8]) {
   if constexpr (EPI == H_STORE) {
     const int there = int(max(int64_t(0), min(int64_t(8), g.N - n)));  // (columns that there are)
     if (there == 0) return;
 #pragma unroll
-    for (int k = 0; k < 8; k++) v[k] = __builtin_amdgcn_ldexpf(v[k], es + r.sum);
+    for (int k = 0; k < 8; k++) v[k] = __builtin_amdgcn_ldexpf(v[k], g.e + r.sum);
     if (g.bias)
 #pragma unroll
       for (int k = 0; k < 8; k++) v[k] += bias[k];
@@ -179,9 +178,9 @@ __device__ __forceinline__ void finish(const HGemm& g, int es, const RowExp& r, 
   } else {
     if (n >= g.h_cols) return;
     if (g.planes == 2)
-      finish16<EPI, true>(g, es, r, m, n, v, u);
+      finish16<EPI, true>(g, r, m, n, v, u);
     else
-      finish16<EPI, false>(g, es, r, m, n, v, u);
+      finish16<EPI, false>(g, r, m, n, v, u);
   }
 }
 
@@ -334,7 +333,6 @@ __device__ __forceinline__ void hgemm_tile(const HGemm& g, int gm, int gn) {
   constexpr int LPR = COLS / 8, RPI = 64 / LPR;        // lanes a row, rows an iteration
   float* const buf = reinterpret_cast<float*>(lds) + wv * 32 * LROW;
   static_assert(4 * 32 * LROW * 4 + TM * sizeof(RowExp) <= T::LDS, "LDS");
-  const int es = PART ? 0 : g.e + (g.e0 ? *g.e0 : 0) + (g.e1 ? *g.e1 : 0);
   const int64_t n = n0 + wn * COLS + 8 * (lane % LPR);
   const float* const from = buf + (lane / LPR) * LROW + 8 * (lane % LPR);
   const auto get = [](const float* p, float(&v)[8]) __attribute__((always_inline)) {
@@ -387,7 +385,7 @@ __device__ __forceinline__ void hgemm_tile(const HGemm& g, int gm, int gn) {
           }
         }
       } else {
-        finish<EPI>(g, es, rows_e[row], m, n, v, u, bias);
+        finish<EPI>(g, rows_e[row], m, n, v, u, bias);
       }
     }
   }
@@ -431,7 +429,7 @@ __global__ __launch_bounds__(256) void k_join(const HGemm g, int parts) {
   if (EPI == H_STORE && g.bias)
     for (int k = 0; k < 8; k++)
       if (n + k < g.N) bias[k] = g.bias[n + k];
-  finish<EPI>(g, g.e + (g.e0 ? *g.e0 : 0) + (g.e1 ? *g.e1 : 0), row_exp<EPI>(g, m), m, n, v, u, bias);
+  finish<EPI>(g, row_exp<EPI>(g, m), m, n, v, u, bias);
 }
 
 // How a product is cut: `gn` columns of tiles, big (256 x 256) or small (128 x 128), K in `parts`; columns past them are cut
@@ -776,7 +774,7 @@ __global__ __launch_bounds__(256, 1) void k_qgemm(const HGemm g, const uint8_t* 
         if constexpr (GATED)
 #pragma unroll
           for (int k = 0; k < 4; k++) u[k] = a[2][k], u[4 + k] = a[3][k];
-        finish<EPI>(g, g.e, rows_e[row], m, n, v, u, bias);
+        finish<EPI>(g, rows_e[row], m, n, v, u, bias);
       }
     }
   });
