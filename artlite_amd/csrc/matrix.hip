@@ -319,7 +319,8 @@ int WorkScope::begin(Work* work, size_t need, hipStream_t stream, const char* wh
   ART_HIP(hipStreamIsCapturing(stream, &st));
   if (st != hipStreamCaptureStatusNone)
     return w->eager ? fail(ARTLITE_EINVAL, "%s: a captured call takes a workspace of its own", what) : ARTLITE_OK;
-  if (w->used && w->last != stream) ART_HIP(hipStreamWaitEvent(stream, w->done, 0));
+  // (the per-thread default stream is one handle, and each thread's own stream behind it)
+  if (w->used && (w->last != stream || stream == hipStreamPerThread)) ART_HIP(hipStreamWaitEvent(stream, w->done, 0));
   note = true;
   return ARTLITE_OK;
 }
