@@ -78,13 +78,15 @@ class GatedFFN:
             return None
         return shared_workspace(self._m["ffn_gate"].device, self._need(code, n, backward), stream).handle
 
-    def _views(self, what: str, shapes: dict[str, tuple[object, int, int]]) -> dict[str, View]:
-        """The views of the arrays (array, rows, cols) that are given: all of one dtype, none of the written ones (all but
-        x and dy) over another."""
-        v = {k: View(a, f"{what}: {k}") for k, (a, _, _) in shapes.items() if a is not None}
-        code = v["x"].code
+    def _views(self, what: str, x: object, shapes: dict[str, tuple[object, int | None, int]]) -> dict[str, View]:
+        """The views of x and of the arrays (array, rows, or none: x's, cols) that are given: all of one dtype, none of the
+        written ones (all but x and dy) over another."""
+        shapes = {"x": (x, None, self.hidden), **shapes}
+        v = {k: View(a, f"{what}: {k}") for k, (a, _, _) in shapes.items() if a is not None or k == "x"}
+        code, n = v["x"].code, v["x"].rows
         for k, w in v.items():
             _, rows, cols = shapes[k]
+            rows = n if rows is None else rows
             if (w.rows, w.cols) != (rows, cols) or w.code != code:
                 raise _hip.Error(f"{what}: {k} is ({w.rows}, {w.cols}) of dtype {w.code}, x of {code}; expected ({rows}, {cols})")
         names = list(v)
@@ -104,11 +106,11 @@ class GatedFFN:
                 raise _hip.Error("ffn: out goes with device arrays")
             d = DeviceArray.of(x, self._m["ffn_gate"].device)
             return self(d, DeviceArray(d.shape, x.dtype, d.device), stream=stream, work=work).numpy()
-        n = x.shape[0]
-        v = self._views("ffn", {"x": (x, n, self.hidden), "out": (out, n, self.hidden)})
+        v = self._views("ffn", x, {"out": (out, None, self.hidden)})
         if "out" not in v:
             raise _hip.Error("ffn: device arrays need out")
         a, y = v["x"], v["out"]
+        n = a.rows
         _hip.check(_hip.lib().artlite_ffn_forward(ctypes.byref(self._open()), a.at, a.code, n, a.row, y.at, y.row,
                                                   self._work(work, a.code, n, 0, stream), stream))
         return out
@@ -118,8 +120,8 @@ class GatedFFN:
         """From x and the output's gradient dy (n, hidden): the gradients that are asked for, into dx (n, hidden), dgate, dup
         (ffn, hidden) and ddown (hidden, ffn; rows without gaps): those of the blocks' values. Device arrays, or numpy arrays
         throughout (written in place)."""
-        H, F, n = self.hidden, self.ffn, x.shape[0]
-        outs = {"dx": (dx, n, H), "dgate": (dgate, F, H), "dup": (dup, F, H), "ddown": (ddown, H, F)}
+        H, F = self.hidden, self.ffn
+        outs = {"dx": (dx, None, H), "dgate": (dgate, F, H), "dup": (dup, F, H), "ddown": (ddown, H, F)}
         if isinstance(x, np.ndarray):
             host = {k: a for k, (a, _, _) in outs.items() if a is not None}
             on = self._m["ffn_gate"].device
@@ -128,13 +130,14 @@ class GatedFFN:
             for k, a in host.items():
                 a[...] = dev[k].numpy()
             return
-        v = self._views("ffn backward", {"x": (x, n, H), "dy": (dy, n, H), **outs})
+        v = self._views("ffn backward", x, {"dy": (dy, None, H), **outs})
         for k in ("dgate", "dup", "ddown"):
             if k in v and v[k].row != v[k].cols:
                 raise _hip.Error(f"ffn backward: {k}'s rows are {v[k].row} values apart")
         if "dy" not in v:
             raise _hip.Error("ffn backward: no dy")
         a, d, o = v["x"], v["dy"], v.get("dx")
+        n = a.rows
         weights = any(k in v for k in ("dgate", "dup", "ddown"))
         at = [v[k].at if k in v else None for k in ("dgate", "dup", "ddown")]
         _hip.check(_hip.lib().artlite_ffn_backward(

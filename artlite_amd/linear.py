@@ -103,7 +103,7 @@ class QLinear:
         a, y = View(x, "linear: x"), View(out, "linear: out")
         n = a.rows
         if a.cols != self.cols or y.rows != n or y.cols != self.rows or y.code != a.code:
-            raise _hip.Error(f"linear: x {tuple(x.shape)} {x.dtype}, out {tuple(out.shape)} {out.dtype} for "
+            raise _hip.Error(f"linear: x ({a.rows}, {a.cols}) of dtype {a.code}, out ({y.rows}, {y.cols}) of dtype {y.code} for "
                              f"{self.rows} rows of {self.cols} values")
         if overlap(a, y):
             raise _hip.Error("linear: out overlaps x")
