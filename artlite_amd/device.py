@@ -161,8 +161,23 @@ class View:
 
 
 def overlap(a: View, b: View) -> bool:
-    """Whether the memory that two views span meets."""
-    def end(v: View) -> int:
-        return v.at + ((v.rows - 1) * v.row + v.cols) * (4 if v.code == F32 else 2)
+    """Whether two views have memory in common. (Views whose rows are different strides apart, or overlap themselves: whether the
+    memory that they span meets.)"""
+    def span(v: View) -> tuple[int, int, int]:  # (rows apart from each other, bytes of a row, bytes from one to the next)
+        size = 4 if v.code == F32 else 2
+        n = min(v.rows, 1) if v.row == 0 else v.rows
+        return n, v.cols * size, v.row * size
 
-    return bool(a.rows and b.rows) and a.at < end(b) and b.at < end(a)
+    (na, wa, sa), (nb, wb, sb) = span(a), span(b)
+    if not (na and nb) or a.at >= b.at + (nb - 1) * sb + wb or b.at >= a.at + (na - 1) * sa + wa:
+        return False
+    s = sa if nb == 1 else sb
+    if (na > 1 and nb > 1 and sa != sb) or s < max(wa, wb):
+        return True
+    # b's row j begins r bytes into a's row j + k
+    k, r = divmod(b.at - a.at, s)
+
+    def pair(k: int) -> bool:
+        return max(0, -k) < min(nb, na - k)
+
+    return (r < wa and pair(k)) or (r + wb > s and pair(k + 1))

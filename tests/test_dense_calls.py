@@ -2,6 +2,10 @@
 
 from pathlib import Path
 
+import numpy as np
+
+from artlite_amd.device import overlap
+
 from .fake_runtime import run_fake
 from .test_dense import PRELUDE
 
@@ -52,4 +56,53 @@ refused("dy is (4, 64)", lambda: f.backward(Cai(x), Cai(w, rows=4), dx=Cai(z)))
 refused("x: NoneType is no array", lambda: f(None, z))
 refused("x: list is no array", lambda: f.backward([1.0], w, dx=z))
 assert hip.launches == at
+""")
+
+
+class Span:
+    """A view's fields, of bf16 values."""
+
+    code = 1
+
+    def __init__(self, at: int, rows: int, cols: int, row: int):
+        self.at, self.rows, self.cols, self.row = at, rows, cols, row
+
+    def bytes(self) -> set[int]:
+        return {self.at + 2 * (i * self.row + j) + k for i in range(self.rows) for j in range(self.cols) for k in range(2)}
+
+
+def test_overlap() -> None:
+    """Against the bytes themselves: views of one buffer's columns share none, whatever they span. Where rows are different
+    strides apart the answer may be yes without any."""
+    rng = np.random.default_rng(1)
+    apart = 0
+    for _ in range(6000):
+        s = int(rng.integers(1, 9))
+        a, b = (Span(2 * int(rng.integers(0, 30)), int(rng.integers(0, 5)), int(rng.integers(1, 6)), s) for _ in range(2))
+        exact = s >= max(a.cols, b.cols) or min(a.rows, b.rows) == 0 or max(a.rows, b.rows) == 1
+        if rng.random() < 0.2:
+            b.row = int(rng.integers(0, 9))
+            exact = exact and (min(a.rows, b.rows) < 1 or a.row == b.row)
+        met = bool(a.bytes() & b.bytes())
+        assert overlap(a, b) == overlap(b, a)
+        assert overlap(a, b) == met if exact else overlap(a, b) or not met, (vars(a), vars(b))
+        ends = max(a.bytes(), default=0), max(b.bytes(), default=0)
+        apart += exact and not met and a.at <= ends[1] and b.at <= ends[0]
+    assert apart > 100  # (interleaved)
+
+
+def test_columns_of_one_buffer(tmp_path: Path) -> None:
+    run_fake(tmp_path, PRELUDE + """
+l, f = linear(96, 64), block(64, 96)
+whole = arr(300, 256)
+class Columns:
+    def __init__(self, first, cols): self.first, self.shape, self.dtype = first, (300, cols), whole.dtype
+    def data_ptr(self): return whole.data_ptr() + 2 * self.first
+    def stride(self): return 256, 1
+x, y, z = Columns(0, 64), Columns(64, 96), Columns(192, 64)
+assert l(x, y) is y and f(x, z) is z
+f.backward(x, z, dx=Columns(128, 64))
+refused("out overlaps x", lambda: l(x, Columns(63, 96)))
+refused("out overlaps x", lambda: f(x, Columns(1, 64)))
+refused("dx overlaps dy", lambda: f.backward(x, z, dx=Columns(190, 64)))
 """)

@@ -3,10 +3,11 @@
 import numpy as np
 import pytest
 
+from artlite_amd.device import DeviceArray
 from artlite_amd.linear import QLinear
 from oracle import dense
 
-from .dense_helpers import check, values
+from .dense_helpers import check, encode, values
 from .test_linear_gpu import TOL, few, x_rows
 
 pytestmark = pytest.mark.gpu
@@ -27,3 +28,30 @@ def test_infinite_scales(q: str, at: int, dtype: str) -> None:
         got, want = lin(x), values(x) @ w.T
         assert not np.isfinite(values(got)[:, 7]).any()
         check(np.delete(got, 7, 1), np.delete(want, 7, 1), TOL[dtype, few(N, K, M, dtype)])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_columns_of_one_buffer(dtype: str) -> None:
+    """x and the output as columns of one device array: what is beside them stays."""
+    K, N = 256, 100
+    raw, w = dense.matrix("Q4_K", N, K, 3)
+    lin = QLinear("Q4_K", N, K)
+    lin.upload(raw)
+    for M in (1, 20, 300, 20000):
+        whole = encode(np.random.default_rng(M).standard_normal((M, 420)), dtype)
+        dev = DeviceArray.of(whole)
+
+        class Columns:
+            def __init__(self, first: int, cols: int):
+                self.first, self.shape, self.dtype = first, (M, cols), dev.dtype
+
+            def data_ptr(self) -> int:
+                return dev.data_ptr() + self.first * dev.dtype.itemsize
+
+            def stride(self) -> tuple[int, int]:
+                return 420, 1
+
+        lin(Columns(3, K), Columns(3 + K, N))
+        got = dev.numpy()
+        check(got[:, 3 + K:3 + K + N], values(whole[:, 3:3 + K]) @ w.T, TOL[dtype, few(N, K, M, dtype)])
+        assert np.array_equal(np.delete(got, np.s_[3 + K:3 + K + N], 1), np.delete(whole, np.s_[3 + K:3 + K + N], 1))
