@@ -7,9 +7,13 @@
   of another runtime is refused),
 - or a host numpy array: copied to the GPU, computed there, and its result copied back before the call returns.
 
+Calls record no graph for torch's autograd: as with torch's own ``out=``, a tensor that requires grad is not written while it
+records one.
+
 Arrays are (rows, values) of fp32 or bf16 (numpy has no bf16: uint16 bit patterns), each row's values consecutive."""
 
 import ctypes
+import sys
 import threading
 
 import numpy as np
@@ -137,8 +141,11 @@ class View:
 
     __slots__ = ("at", "code", "rows", "cols", "row")
 
-    def __init__(self, a: object, what: str):
+    def __init__(self, a: object, what: str, *, written: bool = False):
         if hasattr(a, "data_ptr"):
+            torch = sys.modules.get("torch") if written and getattr(a, "requires_grad", False) else None
+            if torch is not None and torch.is_grad_enabled():
+                raise _hip.Error(f"{what}: requires grad, and a call records no graph (torch.no_grad(), or a tensor without)")
             shape, strides, self.code = a.shape, a.stride(), _code(a.dtype)
             if len(shape) != 2:
                 raise _hip.Error(f"{what}: {tuple(shape)}, not (rows, values)")

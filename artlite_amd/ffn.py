@@ -82,7 +82,8 @@ class GatedFFN:
         """The views of x and of the arrays (array, rows, or none: x's, cols) that are given: all of one dtype, none of the
         written ones (all but x and dy) over another."""
         shapes = {"x": (x, None, self.hidden), **shapes}
-        v = {k: View(a, f"{what}: {k}") for k, (a, _, _) in shapes.items() if a is not None or k == "x"}
+        v = {k: View(a, f"{what}: {k}", written=k not in ("x", "dy")) for k, (a, _, _) in shapes.items()
+             if a is not None or k == "x"}
         code, n = v["x"].code, v["x"].rows
         for k, w in v.items():
             _, rows, cols = shapes[k]

@@ -100,7 +100,7 @@ class QLinear:
                 raise _hip.Error("linear: out goes with device arrays")
             d = DeviceArray.of(x, self._m.device)
             return self(d, DeviceArray((d.shape[0], self.rows), x.dtype, d.device), stream=stream, work=work).numpy()
-        a, y = View(x, "linear: x"), View(out, "linear: out")
+        a, y = View(x, "linear: x"), View(out, "linear: out", written=True)
         n = a.rows
         if a.cols != self.cols or y.rows != n or y.cols != self.rows or y.code != a.code:
             raise _hip.Error(f"linear: x ({a.rows}, {a.cols}) of dtype {a.code}, out ({y.rows}, {y.cols}) of dtype {y.code} for "

@@ -106,3 +106,30 @@ refused("out overlaps x", lambda: l(x, Columns(63, 96)))
 refused("out overlaps x", lambda: f(x, Columns(1, 64)))
 refused("dx overlaps dy", lambda: f.backward(x, z, dx=Columns(190, 64)))
 """)
+
+
+def test_outputs_that_require_grad(tmp_path: Path) -> None:
+    """A tensor that requires grad is not written while torch records a graph; it may be read, and written under no_grad."""
+    run_fake(tmp_path, PRELUDE + """
+import types
+torch = types.ModuleType("torch")
+torch.is_grad_enabled = lambda: RECORDS
+sys.modules["torch"] = torch
+class Tensor:
+    requires_grad = True
+    def __init__(self, n, c):
+        self.a, self.shape, self.dtype = arr(n, c), (n, c), np.dtype(np.uint16)
+        self.data_ptr, self.stride = self.a.data_ptr, self.a.stride
+l, f = linear(96, 64), block(64, 96)
+t64, t96, s64, w = Tensor(5, 64), Tensor(5, 96), Tensor(5, 64), Tensor(96, 64)
+RECORDS = True
+before = hip.launches
+refused("linear: out: requires grad", lambda: l(t64, t96))
+refused("ffn: out: requires grad", lambda: f(t64, s64))
+refused("ffn backward: dx: requires grad", lambda: f.backward(t64, s64, dx=Tensor(5, 64)))
+refused("ffn backward: dgate: requires grad", lambda: f.backward(t64, s64, dgate=w))
+assert hip.launches == before
+l(t64, arr(5, 96)); f.backward(t64, s64, dx=arr(5, 64))
+RECORDS = False
+l(t64, t96); f(t64, s64); f.backward(t64, s64, dgate=w)
+""")
