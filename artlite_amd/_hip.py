@@ -83,6 +83,7 @@ SIGNATURES = {
     "artlite_workspace_create": (_I, [_I, _Z, _I, ctypes.POINTER(_P)]),
     "artlite_workspace_destroy": (_I, [_P]),
     "artlite_stream_capturing": (_I, [_P, ctypes.POINTER(_I)]),
+    "artlite_stream_wait": (_I, [_I, _P, _P]),
     "artlite_linear_workspace": (_I, [_P, _I, _I64, ctypes.POINTER(_Z)]),
     "artlite_linear": (_I, [_P, _P, _I, _I64, _I64, _P, _I64, _P, _P]),
     "artlite_ffn_workspace": (_I, [ctypes.POINTER(Ffn), _I, _I64, _I, ctypes.POINTER(_Z)]),

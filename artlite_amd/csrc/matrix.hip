@@ -8,6 +8,7 @@
 #include <type_traits>
 
 #include <cmath>
+#include <initializer_list>
 #include <new>
 
 namespace artlite {
@@ -471,6 +472,23 @@ extern "C" int artlite_stream_capturing(void* stream, int* out) {
   hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
   ART_HIP(hipStreamIsCapturing(static_cast<hipStream_t>(stream), &st));
   *out = st != hipStreamCaptureStatusNone;
+  return ARTLITE_OK;
+}
+
+extern "C" int artlite_stream_wait(int device, void* stream, void* other) {
+  OnDevice on;
+  ART_TRY(on.set(device));
+  for (void* s : {stream, other}) {
+    int capturing = 0;
+    ART_TRY(artlite_stream_capturing(s, &capturing));
+    if (capturing) return fail(ARTLITE_EINVAL, "stream wait: a stream that is being captured");
+  }
+  hipEvent_t e;
+  ART_HIP(hipEventCreateWithFlags(&e, hipEventDisableTiming));
+  hipError_t rc = hipEventRecord(e, static_cast<hipStream_t>(other));
+  if (rc == hipSuccess) rc = hipStreamWaitEvent(static_cast<hipStream_t>(stream), e, 0);
+  (void)hipEventDestroy(e);  // (once it has come, if it is still to come)
+  ART_HIP(rc);
   return ARTLITE_OK;
 }
 

@@ -15,6 +15,7 @@ Arrays are (rows, values) of fp32 or bf16 (numpy has no bf16: uint16 bit pattern
 import ctypes
 import sys
 import threading
+from collections.abc import Iterable
 
 import numpy as np
 
@@ -137,11 +138,13 @@ def shared_workspace(device: int, nbytes: int, stream: object) -> Workspace:
 
 
 class View:
-    """An argument as a call takes it: address, dtype code, rows, values a row, row stride in values."""
+    """An argument as a call takes it: address, dtype code, rows, values a row, row stride in values; the stream that its
+    interface names (none: nothing to wait for)."""
 
-    __slots__ = ("at", "code", "rows", "cols", "row")
+    __slots__ = ("at", "code", "rows", "cols", "row", "stream")
 
     def __init__(self, a: object, what: str, *, written: bool = False):
+        self.stream = None
         if hasattr(a, "data_ptr"):
             torch = sys.modules.get("torch") if written and getattr(a, "requires_grad", False) else None
             if torch is not None and torch.is_grad_enabled():
@@ -155,6 +158,9 @@ class View:
             shape, self.at, self.code = d["shape"], d["data"][0], _code(d["typestr"])
             if len(shape) != 2:
                 raise _hip.Error(f"{what}: {tuple(shape)}, not (rows, values)")
+            self.stream = d.get("stream")
+            if self.stream == 0:
+                raise _hip.Error(f"{what}: an interface whose stream is 0 (1: the null stream, 2: the per-thread one)")
             size = 4 if self.code == F32 else 2
             strides = [s / size for s in d["strides"]] if d.get("strides") else (shape[1], 1)
         else:
@@ -165,6 +171,12 @@ class View:
             raise _hip.Error(f"{what}: rows {strides[0]} values apart")
         if strides[1] != 1 and self.cols > 1:
             raise _hip.Error(f"{what}: a row's values are {strides[1]} apart")
+
+
+def after(device: int, stream: int | None, views: Iterable[View]) -> None:
+    """A call on ``stream`` comes after what the streams named by its arrays' interfaces (1: the null stream) have by now."""
+    for s in {0 if v.stream == 1 else v.stream for v in views if v.stream is not None} - {stream or 0}:
+        _hip.check(_hip.lib().artlite_stream_wait(device, stream, s))
 
 
 def overlap(a: View, b: View) -> bool:

@@ -7,7 +7,7 @@ import ctypes
 import numpy as np
 
 from . import _hip
-from .device import DeviceArray, View, Workspace, overlap, shared_workspace
+from .device import DeviceArray, View, Workspace, after, overlap, shared_workspace
 from .gguf_model import GGUFFile
 from .linear import FORMATS, Matrix
 
@@ -71,7 +71,10 @@ class GatedFFN:
             m.handle  # (raises when closed)
         return self._d
 
-    def _work(self, work: Workspace | None, code: int, n: int, backward: int, stream: object) -> object:
+    def _work(self, work: Workspace | None, v: dict[str, View], backward: int, stream: object) -> object:
+        """The workspace's handle, and the call ordered behind its arrays' streams."""
+        code, n = v["x"].code, v["x"].rows
+        after(self._m["ffn_gate"].device, stream, v.values())
         if work is not None:
             return work.handle
         if not n:
@@ -113,7 +116,7 @@ class GatedFFN:
         a, y = v["x"], v["out"]
         n = a.rows
         _hip.check(_hip.lib().artlite_ffn_forward(ctypes.byref(self._open()), a.at, a.code, n, a.row, y.at, y.row,
-                                                  self._work(work, a.code, n, 0, stream), stream))
+                                                  self._work(work, v, 0, stream), stream))
         return out
 
     def backward(self, x: object, dy: object, *, dx: object = None, dgate: object = None, dup: object = None,
@@ -143,4 +146,4 @@ class GatedFFN:
         at = [v[k].at if k in v else None for k in ("dgate", "dup", "ddown")]
         _hip.check(_hip.lib().artlite_ffn_backward(
             ctypes.byref(self._open()), a.at, a.row, d.at, d.row, a.code, n, o.at if o else None, o.row if o else 0, *at,
-            self._work(work, a.code, n, 2 if weights else 1, stream), stream))
+            self._work(work, v, 2 if weights else 1, stream), stream))

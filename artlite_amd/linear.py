@@ -7,7 +7,7 @@ import ctypes
 import numpy as np
 
 from . import _hip
-from .device import DeviceArray, View, Workspace, overlap, shared_workspace
+from .device import DeviceArray, View, Workspace, after, overlap, shared_workspace
 from .gguf_model import TYPE_ID, GGUFFile
 
 FORMATS = ("Q4_0", "Q4_1", "Q4_K", "IQ4_NL", "IQ4_XS")
@@ -112,5 +112,7 @@ class QLinear:
         if work is None and n > 16:
             need = self._need(a.code, n)
             w = shared_workspace(self._m.device, need, stream).handle if need else None
+        if a.stream is not None or y.stream is not None:
+            after(self._m.device, stream, (a, y))
         _hip.check(_hip.lib().artlite_linear(handle, a.at, a.code, n, a.row, y.at, y.row, w, stream))
         return out

@@ -193,10 +193,12 @@ int artlite_matrix_device(const artlite_matrix* m, int* device);
 
 /* Scratch memory of calls, of a fixed size, on a device (-1: the current one). eager_only: a call under stream capture that
  * would use it is refused (for one that many callers share). A stream's calls have come to their end before it is destroyed.
- * artlite_stream_capturing: whether a stream is being captured (memory is then not to be allocated). */
+ * artlite_stream_capturing: whether a stream is being captured (memory is then not to be allocated). artlite_stream_wait: what
+ * is queued on `stream` from now on waits for what is on `other` by now (streams of `device`, neither being captured). */
 typedef struct artlite_workspace artlite_workspace;
 int artlite_workspace_create(int device, size_t nbytes, int eager_only, artlite_workspace** out);
 int artlite_stream_capturing(void* stream, int* out);
+int artlite_stream_wait(int device, void* stream, void* other);
 int artlite_workspace_destroy(artlite_workspace* work); /* its calls have come to their end */
 
 /* y (n x rows) = x (n x cols) W^T (+ bias). x's products with the blocks' values are summed in fp32 and rounded once to y's

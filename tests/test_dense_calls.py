@@ -4,7 +4,10 @@ from pathlib import Path
 
 import numpy as np
 
+from artlite_amd import _hip
 from artlite_amd.device import overlap
+from artlite_amd.gguf_model import TYPE_ID
+from artlite_amd.linear import FORMATS
 
 from .fake_runtime import run_fake
 from .test_dense import PRELUDE
@@ -133,3 +136,39 @@ l(t64, arr(5, 96)); f.backward(t64, s64, dx=arr(5, 64))
 RECORDS = False
 l(t64, t96); f(t64, s64); f.backward(t64, s64, dgate=w)
 """)
+
+
+def test_streams_of_the_interface(tmp_path: Path) -> None:
+    """A call waits for the stream that an array's ``__cuda_array_interface__`` names, where that is another than its own."""
+    run_fake(tmp_path, PRELUDE + CAI + """
+def on(stream, a):
+    c = Cai(a)
+    c.__cuda_array_interface__["stream"] = stream
+    return c
+l, f = linear(96, 64), block(64, 96)
+x, y, z, w = arr(5, 64), arr(5, 96), arr(5, 64), arr(5, 64)
+f(x, z)  # (its workspace)
+def waits(call):
+    before = hip.waits
+    call()
+    return hip.waits - before
+assert waits(lambda: l(on(None, x), on(None, y))) == 0
+assert waits(lambda: l(on(7, x), on(7, y))) == 1 == waits(lambda: l(x, on(7, y)))
+assert waits(lambda: l(on(7, x), on(8, y))) == 2
+assert waits(lambda: l(on(7, x), on(7, y), stream=7)) == 0 == waits(lambda: l(on(1, x), y)) == waits(lambda: l(on(1, x), y, stream=None))
+assert waits(lambda: l(on(1, x), y, stream=7)) == 1 == waits(lambda: l(on(2, x), y))
+assert waits(lambda: f(on(7, x), z)) == 1 == waits(lambda: f.backward(x, on(7, w), dx=z))
+refused("stream is 0", lambda: l(on(0, x), y))
+at = hip.launches
+hip.capturing = 1
+refused("being captured", lambda: l(on(7, x), y))
+assert hip.launches == at
+l(on(None, x), y)
+hip.capturing = 0
+""")
+
+
+def test_formats() -> None:
+    """What ``artlite_matrix_supported`` says is what the classes take."""
+    assert {q for q, i in TYPE_ID.items() if _hip.lib().artlite_matrix_supported(i)} == set(FORMATS)
+    assert not _hip.lib().artlite_matrix_supported(-1) and not _hip.lib().artlite_matrix_supported(1 << 20)
