@@ -496,8 +496,9 @@ extern "C" int artlite_workspace_destroy(artlite_workspace* w) {
   if (!w) return ARTLITE_OK;
   OnDevice on;
   const int rc = on.set(w->w.device);
+  if (w->w.used) (void)hipEventSynchronize(w->w.done);  // (its calls outside captures)
   if (w->w.done) (void)hipEventDestroy(w->w.done);
-  if (w->w.p) (void)hipFree(w->w.p);  // (waits for the device)
+  if (w->w.p) (void)hipFree(w->w.p);
   delete w;
   return rc;
 }

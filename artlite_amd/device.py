@@ -118,23 +118,26 @@ class Workspace:
         self.close()
 
 
-_shared: dict[int, list[Workspace]] = {}
+_shared: dict[int, Workspace] = {}
 _shared_lock = threading.Lock()
 
 
 def shared_workspace(device: int, nbytes: int, stream: object) -> Workspace:
     """The workspace of a device's calls that are given none, grown as they need more (not while ``stream`` is captured: such
-    a call is refused). One that is outgrown stays until the process ends (a thread may be about to use it); each is at least
-    twice the one before."""
+    a call is refused), by a quarter at least. The caller keeps it until its call has returned; one that is outgrown is freed
+    with the last that does, behind its calls."""
     with _shared_lock:
-        all_ = _shared.setdefault(device, [])
-        if not all_ or all_[-1].nbytes < nbytes:
+        w = _shared.get(device)
+        if w is None or w.nbytes < nbytes:
             capturing = ctypes.c_int(0)
             _hip.check(_hip.lib().artlite_stream_capturing(stream, ctypes.byref(capturing)))
             if capturing.value:
                 raise _hip.Error("a captured call takes a workspace of its own")
-            all_.append(Workspace(max(nbytes, 2 * all_[-1].nbytes if all_ else 0), device, eager_only=True))
-        return all_[-1]
+            nbytes = max(nbytes, w.nbytes * 5 // 4 if w else 0)
+            _shared.pop(device, None)
+            w = None  # (freed before the new one is allocated)
+            w = _shared[device] = Workspace(nbytes, device, eager_only=True)
+        return w
 
 
 class View:

@@ -71,15 +71,13 @@ class GatedFFN:
             m.handle  # (raises when closed)
         return self._d
 
-    def _work(self, work: Workspace | None, v: dict[str, View], backward: int, stream: object) -> object:
-        """The workspace's handle, and the call ordered behind its arrays' streams."""
+    def _work(self, work: Workspace | None, v: dict[str, View], backward: int, stream: object) -> Workspace | None:
+        """The call's workspace (to be kept until it has returned), and the call ordered behind its arrays' streams."""
         code, n = v["x"].code, v["x"].rows
         after(self._m["ffn_gate"].device, stream, v.values())
-        if work is not None:
-            return work.handle
-        if not n:
-            return None
-        return shared_workspace(self._m["ffn_gate"].device, self._need(code, n, backward), stream).handle
+        if work is not None or not n:
+            return work
+        return shared_workspace(self._m["ffn_gate"].device, self._need(code, n, backward), stream)
 
     def _views(self, what: str, x: object, shapes: dict[str, tuple[object, int | None, int]]) -> dict[str, View]:
         """The views of x and of the arrays (array, rows, or none: x's, cols) that are given: all of one dtype, none of the
@@ -115,8 +113,10 @@ class GatedFFN:
             raise _hip.Error("ffn: device arrays need out")
         a, y = v["x"], v["out"]
         n = a.rows
-        _hip.check(_hip.lib().artlite_ffn_forward(ctypes.byref(self._open()), a.at, a.code, n, a.row, y.at, y.row,
-                                                  self._work(work, v, 0, stream), stream))
+        d = ctypes.byref(self._open())
+        work = self._work(work, v, 0, stream)
+        _hip.check(_hip.lib().artlite_ffn_forward(d, a.at, a.code, n, a.row, y.at, y.row,
+                                                  work.handle if work is not None else None, stream))
         return out
 
     def backward(self, x: object, dy: object, *, dx: object = None, dgate: object = None, dup: object = None,
@@ -144,6 +144,8 @@ class GatedFFN:
         n = a.rows
         weights = any(k in v for k in ("dgate", "dup", "ddown"))
         at = [v[k].at if k in v else None for k in ("dgate", "dup", "ddown")]
+        f = ctypes.byref(self._open())
+        work = self._work(work, v, 2 if weights else 1, stream)
         _hip.check(_hip.lib().artlite_ffn_backward(
-            ctypes.byref(self._open()), a.at, a.row, d.at, d.row, a.code, n, o.at if o else None, o.row if o else 0, *at,
-            self._work(work, v, 2 if weights else 1, stream), stream))
+            f, a.at, a.row, d.at, d.row, a.code, n, o.at if o else None, o.row if o else 0, *at,
+            work.handle if work is not None else None, stream))

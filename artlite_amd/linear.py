@@ -108,11 +108,11 @@ class QLinear:
         if overlap(a, y):
             raise _hip.Error("linear: out overlaps x")
         handle = self._m.handle
-        w = work.handle if work is not None else None
         if work is None and n > 16:
             need = self._need(a.code, n)
-            w = shared_workspace(self._m.device, need, stream).handle if need else None
+            work = shared_workspace(self._m.device, need, stream) if need else None
         if a.stream is not None or y.stream is not None:
             after(self._m.device, stream, (a, y))
-        _hip.check(_hip.lib().artlite_linear(handle, a.at, a.code, n, a.row, y.at, y.row, w, stream))
+        _hip.check(_hip.lib().artlite_linear(handle, a.at, a.code, n, a.row, y.at, y.row,
+                                             work.handle if work is not None else None, stream))
         return out

@@ -172,3 +172,30 @@ def test_formats() -> None:
     """What ``artlite_matrix_supported`` says is what the classes take."""
     assert {q for q, i in TYPE_ID.items() if _hip.lib().artlite_matrix_supported(i)} == set(FORMATS)
     assert not _hip.lib().artlite_matrix_supported(-1) and not _hip.lib().artlite_matrix_supported(1 << 20)
+
+
+def test_shared_workspace_is_one(tmp_path: Path) -> None:
+    """Growing frees what was outgrown (once no call uses it), and what is held is at most a quarter
+    more than a call has needed."""
+    run_fake(tmp_path, PRELUDE + """
+import weakref
+from artlite_amd import device as D
+l = linear(4096, 1024)
+x, y = arr(9000, 1024), arr(9000, 4096)
+class Rows:
+    def __init__(self, a, n): self.shape, self.dtype, self.data_ptr, self.stride = (n, a.shape[1]), a.dtype, a.data_ptr, a.stride
+def run(n): l(Rows(x, n), Rows(y, n))
+sizes = [300, 2000, 2100, 4000, 600, 610, 9000, 1000]
+assert sorted(sizes, key=l.workspace_bytes) == sizes
+old = None
+for n in sizes:
+    run(n)
+    w = D._shared[0]
+    assert l.workspace_bytes(n) <= w.nbytes <= 1.25 * l.workspace_bytes(n)
+    assert old is None or old() is None or old() is w
+    old = weakref.ref(w)
+    del w
+kept = shared_workspace(0, 1, 0)
+run(5); shared_workspace(0, 2 * kept.nbytes, 0)
+assert D._shared[0] is not kept and kept.handle and D._shared[0].nbytes == 2 * kept.nbytes
+""")
