@@ -353,7 +353,7 @@ int few_x(FewArgs& a, const void* x, int dtype, int64_t n, int64_t K, int64_t st
   a.x = x, a.x_stride = stride;
   if (!planes) return ARTLITE_OK;
   a.x = planes, a.x_stride = K, a.x_plane = n * K;
-  return launch_planes(x, dtype, n, K, stride, planes, K, n * K, 3, s);
+  return launch_planes(static_cast<const float*>(x), n, K, stride, planes, s);
 }
 
 int linear(const artlite_matrix* w, const void* x, int dtype, int64_t n, int64_t x_stride, void* y, int64_t y_stride,

@@ -336,14 +336,10 @@ __global__ __launch_bounds__(256) void k_few_join(const FewK a, int parts) {
   few_out<GLU>(a, m, n, s, u);
 }
 
-__global__ __launch_bounds__(256) void k_planes(const void* __restrict__ x, int bf16, int64_t K, int64_t stride,
-                                                uint16_t* __restrict__ out, int64_t Kp, int64_t plane, int planes) {
+__global__ __launch_bounds__(256) void k_planes(const float* __restrict__ x, int64_t K, int64_t stride,
+                                                uint16_t* __restrict__ out, int64_t plane) {
   const int64_t m = blockIdx.y, k = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (k >= Kp) return;
-  float v = 0.0f;
-  if (k < K)
-    v = bf16 ? bf16_to_f32(static_cast<const uint16_t*>(x)[m * stride + k]) : static_cast<const float*>(x)[m * stride + k];
-  store_planes(out + m * Kp + k, plane, planes, v);
+  if (k < K) store_planes(out + m * K + k, plane, 3, x[m * stride + k]);
 }
 
 // Tall matrices, up to 16 rows of x: a workgroup a CU; the tiles shared out among workgroups, a workgroup's units, tile after
@@ -850,14 +846,10 @@ int launch_few_t(const FewTArgs& a, hipStream_t s) {
 #undef ART_T
 }
 
-int launch_planes(const void* x, int dtype, int64_t M, int64_t K, int64_t stride, uint16_t* out, int64_t Kp, int64_t plane,
-                  int planes, hipStream_t s) {
-  if (M <= 0) return ARTLITE_OK;
+int launch_planes(const float* x, int64_t M, int64_t K, int64_t stride, uint16_t* out, hipStream_t s) {
   for (int64_t m = 0; m < M; m += 65535) {
     const int64_t rows = M - m < 65535 ? M - m : 65535;
-    const int es = dtype == ARTLITE_X_BF16 ? 2 : 4;
-    k_planes<<<dim3(unsigned((Kp + 255) / 256), unsigned(rows)), 256, 0, s>>>(
-        static_cast<const char*>(x) + m * stride * es, dtype == ARTLITE_X_BF16, K, stride, out + m * Kp, Kp, plane, planes);
+    k_planes<<<dim3(unsigned((K + 255) / 256), unsigned(rows)), 256, 0, s>>>(x + m * stride, K, stride, out + m * K, M * K);
     ART_HIP(hipGetLastError());
   }
   return ARTLITE_OK;

@@ -337,9 +337,8 @@ int launch_few_t(const FewTArgs& a, hipStream_t s);
 // few_apart.
 constexpr int FEW_ROWS_LARGE = 128, FEW_LARGE = 8192, FEW_ROWS_FFN_DIRECT = 64;
 constexpr int FEW_ROWS = 256, FEW_ROWS_F32 = 128, FEW_ROWS_FFN = 192;
-// x (M rows of K values of dtype, stride apart) as planes of bf16 (1: bf16 as it is; 3: fp32), rows of Kp values (zeros past K)
-int launch_planes(const void* x, int dtype, int64_t M, int64_t K, int64_t stride, uint16_t* out, int64_t Kp, int64_t plane,
-                  int planes, hipStream_t s);
+// x (M rows of K fp32 values, stride apart) as three planes of bf16, M rows of K values each
+int launch_planes(const float* x, int64_t M, int64_t K, int64_t stride, uint16_t* out, hipStream_t s);
 
 // ---- 16-bit operands of the large tiles (matrix.hip)
 
