@@ -3,6 +3,7 @@
 experts (an MoE model's leading dense blocks)."""
 
 import ctypes
+import itertools
 
 import numpy as np
 
@@ -128,6 +129,12 @@ class GatedFFN:
         outs = {"dx": (dx, None, H), "dgate": (dgate, F, H), "dup": (dup, F, H), "ddown": (ddown, H, F)}
         if isinstance(x, np.ndarray):
             host = {k: a for k, (a, _, _) in outs.items() if a is not None}
+            for k, a in {"dy": dy, **host}.items():
+                if not isinstance(a, np.ndarray) or a.ndim != 2:
+                    raise _hip.Error(f"ffn backward: {k} is no host array of (rows, values), as x is")
+            for i, j in itertools.combinations(host, 2):
+                if np.shares_memory(host[i], host[j]):
+                    raise _hip.Error(f"ffn backward: {j} overlaps {i}")
             on = self._m["ffn_gate"].device
             dev = {k: DeviceArray(a.shape, a.dtype, on) for k, a in host.items()}
             self.backward(DeviceArray.of(x, on), DeviceArray.of(dy, on), **dev, stream=stream, work=work)

@@ -199,3 +199,23 @@ kept = shared_workspace(0, 1, 0)
 run(5); shared_workspace(0, 2 * kept.nbytes, 0)
 assert D._shared[0] is not kept and kept.handle and D._shared[0].nbytes == 2 * kept.nbytes
 """)
+
+
+def test_host_arrays_refused(tmp_path: Path) -> None:
+    """A backward call on host arrays takes host arrays throughout, and no memory for two of its outputs."""
+    run_fake(tmp_path, PRELUDE + """
+f = block(64, 96)
+x, dy, dx, g, u = (np.zeros(s, np.uint16) for s in ((5, 64), (5, 64), (5, 64), (96, 64), (96, 64)))
+f.backward(x, dy, dx=dx, dgate=g, dup=u)
+f.backward(x, dy, dx=x)  # (x is copied before)
+both = np.zeros((96, 128), np.uint16)
+f.backward(x, dy, dgate=both[:, :64], dup=both[:, 64:])
+at = hip.launches
+refused("dy is no host array", lambda: f.backward(x, None, dx=dx))
+refused("dy is no host array", lambda: f.backward(x, arr(5, 64), dx=dx))
+refused("dx is no host array", lambda: f.backward(x, dy, dx=arr(5, 64)))
+refused("dgate is no host array", lambda: f.backward(x, dy, dgate=g.reshape(-1)))
+refused("dup overlaps dgate", lambda: f.backward(x, dy, dgate=g, dup=g))
+refused("dup overlaps dgate", lambda: f.backward(x, dy, dgate=both[:, 10:74], dup=both[:, 64:]))
+assert hip.launches == at
+""")
