@@ -41,6 +41,8 @@ def _code(dtype: object) -> int:
 class DeviceArray:
     """(rows, values) in GPU memory, on a device (-1: the current one). dtype: ``float32``, or ``uint16`` for bf16 bits."""
 
+    requires_grad = False
+
     def __init__(self, shape: tuple[int, int], dtype: object = np.float32, device: int = -1):
         self.dtype = np.dtype(dtype)
         _code(self.dtype)
@@ -140,17 +142,21 @@ def shared_workspace(device: int, nbytes: int, stream: object) -> Workspace:
         return w
 
 
+def _records() -> bool:
+    torch = sys.modules.get("torch")
+    return torch is not None and torch.is_grad_enabled()
+
+
 class View:
     """An argument as a call takes it: address, dtype code, rows, values a row, row stride in values; the stream that its
     interface names (none: nothing to wait for)."""
 
     __slots__ = ("at", "code", "rows", "cols", "row", "stream")
 
-    def __init__(self, a: object, what: str, *, written: bool = False):
+    def __init__(self, a: object, what: str, written: bool = False):
         self.stream = None
         if hasattr(a, "data_ptr"):
-            torch = sys.modules.get("torch") if written and getattr(a, "requires_grad", False) else None
-            if torch is not None and torch.is_grad_enabled():
+            if written and getattr(a, "requires_grad", False) and _records():
                 raise _hip.Error(f"{what}: requires grad, and a call records no graph (torch.no_grad(), or a tensor without)")
             shape, strides, self.code = a.shape, a.stride(), _code(a.dtype)
             if len(shape) != 2:
@@ -185,16 +191,14 @@ def after(device: int, stream: int | None, views: Iterable[View]) -> None:
 def overlap(a: View, b: View) -> bool:
     """Whether two views have memory in common. (Views whose rows are different strides apart, or overlap themselves: whether the
     memory that they span meets.)"""
-    def span(v: View) -> tuple[int, int, int]:  # (rows apart from each other, bytes of a row, bytes from one to the next)
-        size = 4 if v.code == F32 else 2
-        n = min(v.rows, 1) if v.row == 0 else v.rows
-        return n, v.cols * size, v.row * size
-
-    (na, wa, sa), (nb, wb, sb) = span(a), span(b)
-    if not (na and nb) or a.at >= b.at + (nb - 1) * sb + wb or b.at >= a.at + (na - 1) * sa + wa:
+    size, other = 4 if a.code == F32 else 2, 4 if b.code == F32 else 2
+    if not (a.rows and b.rows and a.at < b.at + ((b.rows - 1) * b.row + b.cols) * other
+            and b.at < a.at + ((a.rows - 1) * a.row + a.cols) * size):
         return False
-    s = sa if nb == 1 else sb
-    if (na > 1 and nb > 1 and sa != sb) or s < max(wa, wb):
+    na, nb = (1 if v.row == 0 else v.rows for v in (a, b))
+    wa, wb = a.cols * size, b.cols * other
+    s = a.row * size if nb == 1 else b.row * other
+    if (na > 1 and nb > 1 and a.row * size != s) or s < max(wa, wb):
         return True
     # b's row j begins r bytes into a's row j + k
     k, r = divmod(b.at - a.at, s)

@@ -75,7 +75,10 @@ class GatedFFN:
     def _work(self, work: Workspace | None, v: dict[str, View], backward: int, stream: object) -> Workspace | None:
         """The call's workspace (to be kept until it has returned), and the call ordered behind its arrays' streams."""
         code, n = v["x"].code, v["x"].rows
-        after(self._m["ffn_gate"].device, stream, v.values())
+        for w in v.values():
+            if w.stream is not None:
+                after(self._m["ffn_gate"].device, stream, v.values())
+                break
         if work is not None or not n:
             return work
         return shared_workspace(self._m["ffn_gate"].device, self._need(code, n, backward), stream)
@@ -83,14 +86,16 @@ class GatedFFN:
     def _views(self, what: str, x: object, shapes: dict[str, tuple[object, int | None, int]]) -> dict[str, View]:
         """The views of x and of the arrays (array, rows, or none: x's, cols) that are given: all of one dtype, none of the
         written ones (all but x and dy) over another."""
-        shapes = {"x": (x, None, self.hidden), **shapes}
-        v = {k: View(a, f"{what}: {k}", written=k not in ("x", "dy")) for k, (a, _, _) in shapes.items()
-             if a is not None or k == "x"}
-        code, n = v["x"].code, v["x"].rows
-        for k, w in v.items():
-            _, rows, cols = shapes[k]
+        w = View(x, f"{what}: x")
+        v, n, code = {"x": w}, w.rows, w.code
+        if w.cols != self.hidden:
+            raise _hip.Error(f"{what}: x is ({n}, {w.cols}), not of {self.hidden} columns")
+        for k, (a, rows, cols) in shapes.items():
+            if a is None:
+                continue
+            w = v[k] = View(a, f"{what}: {k}", k != "dy")
             rows = n if rows is None else rows
-            if (w.rows, w.cols) != (rows, cols) or w.code != code:
+            if w.rows != rows or w.cols != cols or w.code != code:
                 raise _hip.Error(f"{what}: {k} is ({w.rows}, {w.cols}) of dtype {w.code}, x of {code}; expected ({rows}, {cols})")
         names = list(v)
         for i, a in enumerate(names):

@@ -100,7 +100,7 @@ class QLinear:
                 raise _hip.Error("linear: out goes with device arrays")
             d = DeviceArray.of(x, self._m.device)
             return self(d, DeviceArray((d.shape[0], self.rows), x.dtype, d.device), stream=stream, work=work).numpy()
-        a, y = View(x, "linear: x"), View(out, "linear: out", written=True)
+        a, y = View(x, "linear: x"), View(out, "linear: out", True)
         n = a.rows
         if a.cols != self.cols or y.rows != n or y.cols != self.rows or y.code != a.code:
             raise _hip.Error(f"linear: x ({a.rows}, {a.cols}) of dtype {a.code}, out ({y.rows}, {y.cols}) of dtype {y.code} for "
@@ -108,11 +108,15 @@ class QLinear:
         if overlap(a, y):
             raise _hip.Error("linear: out overlaps x")
         handle = self._m.handle
-        if work is None and n > 16:
+        w = None
+        if work is not None:
+            w = work.handle
+        elif n > 16:
             need = self._need(a.code, n)
-            work = shared_workspace(self._m.device, need, stream) if need else None
+            if need:
+                work = shared_workspace(self._m.device, need, stream)
+                w = work.handle
         if a.stream is not None or y.stream is not None:
             after(self._m.device, stream, (a, y))
-        _hip.check(_hip.lib().artlite_linear(handle, a.at, a.code, n, a.row, y.at, y.row,
-                                             work.handle if work is not None else None, stream))
+        _hip.check(_hip.lib().artlite_linear(handle, a.at, a.code, n, a.row, y.at, y.row, w, stream))
         return out
