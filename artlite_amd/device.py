@@ -167,6 +167,8 @@ class View:
             shape, self.at, self.code = d["shape"], d["data"][0], _code(d["typestr"])
             if len(shape) != 2:
                 raise _hip.Error(f"{what}: {tuple(shape)}, not (rows, values)")
+            if written and d["data"][1]:
+                raise _hip.Error(f"{what}: read-only")
             self.stream = d.get("stream")
             if self.stream == 0:
                 raise _hip.Error(f"{what}: an interface whose stream is 0 (1: the null stream, 2: the per-thread one)")

@@ -155,7 +155,8 @@ def waits(call):
 assert waits(lambda: l(on(None, x), on(None, y))) == 0
 assert waits(lambda: l(on(7, x), on(7, y))) == 1 == waits(lambda: l(x, on(7, y)))
 assert waits(lambda: l(on(7, x), on(8, y))) == 2
-assert waits(lambda: l(on(7, x), on(7, y), stream=7)) == 0 == waits(lambda: l(on(1, x), y)) == waits(lambda: l(on(1, x), y, stream=None))
+assert waits(lambda: l(on(7, x), on(7, y), stream=7)) == 0
+assert waits(lambda: l(on(1, x), y)) == 0 == waits(lambda: l(on(1, x), y, stream=None))
 assert waits(lambda: l(on(1, x), y, stream=7)) == 1 == waits(lambda: l(on(2, x), y))
 assert waits(lambda: f(on(7, x), z)) == 1 == waits(lambda: f.backward(x, on(7, w), dx=z))
 refused("stream is 0", lambda: l(on(0, x), y))
@@ -165,6 +166,24 @@ refused("being captured", lambda: l(on(7, x), y))
 assert hip.launches == at
 l(on(None, x), y)
 hip.capturing = 0
+""")
+
+
+def test_read_only_outputs(tmp_path: Path) -> None:
+    """Memory whose interface says that it is read-only is read, not written."""
+    run_fake(tmp_path, PRELUDE + CAI + """
+def fixed(a):
+    c = Cai(a)
+    c.__cuda_array_interface__["data"] = (a.data_ptr(), True)
+    return c
+l, f = linear(96, 64), block(64, 96)
+x, y, z, w = arr(5, 64), arr(5, 96), arr(5, 64), arr(5, 64)
+l(fixed(x), y); f.backward(fixed(x), fixed(w), dx=z)
+at = hip.launches
+refused("linear: out: read-only", lambda: l(x, fixed(y)))
+refused("ffn: out: read-only", lambda: f(x, fixed(z)))
+refused("dup: read-only", lambda: f.backward(x, w, dup=fixed(arr(96, 64))))
+assert hip.launches == at
 """)
 
 
