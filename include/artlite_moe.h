@@ -172,13 +172,17 @@ int artlite_hbm_copy(size_t nbytes, int iters, double* ms_per_copy);
  * x, y and the gradients below are DEVICE memory of that device (anything else is refused), bf16 or fp32 (artlite_dtype;
  * y and gradients in x's type), rows of consecutive values `stride` values apart: x's at least 0 (0: one row for all),
  * those of what is written at least the row's values; what is written overlaps nothing else of the call's. Calls are
- * enqueued on `stream` (a hipStream_t; null: the null stream) and return at once; 0 rows write nothing. They may be
- * captured into a graph: its replays use the workspace that was given, and whatever else uses that workspace has to be
- * ordered with them by the caller's streams (a workspace for each graph that runs beside others). Outside captures, calls
- * on one workspace order themselves, whichever streams and threads they come from. The same call gives the same bits. A
- * value of x that is infinite or no number reaches its own row alone; values beyond 2^100 in size may overflow the sums of
- * few rows. Those are of codes, a group's times its scale: exact to about 2^-15 of the group's scale and offset, also where
- * its values themselves come out far smaller than both. */
+ * enqueued on `stream` (a hipStream_t; null: the null stream) and return at once; 0 rows write nothing (a backward call: zeros
+ * to the weights' gradients that are asked for). They may be captured into a graph: its replays use the workspace that was
+ * given, and whatever else uses that workspace has to be ordered with them by the caller's streams (a workspace for each graph
+ * that runs beside others). Outside captures, calls on one workspace order themselves, whichever streams and threads they come
+ * from (hipStreamPerThread among them). The same call gives the same bits.
+ * A value of x that is infinite or no number reaches its own row alone, one of a matrix its own row's outputs. Few rows' sums
+ * are of codes, a group's times its scale: exact to about 2^-15 of the group's scale and offset, also where its values
+ * themselves come out far smaller than both; values beyond 2^100 in size may overflow them, and fp32 ones are held to 2^-134.
+ * Past few rows (see artlite_linear) a row of x and a matrix's values are fp16, of fp32 calls two of them, each row times a
+ * power of two from its largest finite value and the matrix from its own: what is below 2^-29 (fp32: 2^-17) of that loses
+ * bits, what is below 2^-40 of it is 0. */
 typedef struct artlite_matrix artlite_matrix;
 int artlite_matrix_supported(int qtype);
 int artlite_matrix_create(int qtype, int64_t rows, int64_t cols, artlite_matrix** out);
@@ -215,7 +219,15 @@ int artlite_linear(const artlite_matrix* w, const void* x, int dtype, int64_t n,
  * dx = dg gate + du up, dgate = dg^T x, dup = du^T x, ddown = dy^T h, where g = x gate^T, u = x up^T, h = act(g) u,
  * dh = dy down, dg = dh u act'(g), du = dh act(g); dgate, dup (F x H) and ddown (H x F) are the gradients of the blocks'
  * values. The forward keeps nothing; the backward computes g and u again. Outputs that are null are not computed (dx too);
- * dgate, dup, ddown: rows without gaps. */
+ * dgate, dup, ddown: rows without gaps.
+ * Sums, activations and their derivatives are fp32. Between the products a forward's h goes as two planes of bf16 (2^-17; fp32
+ * calls three, 2^-24) on the few rows' way, up to 64 bf16 or 192 rows, more of a small block. Past that h, and in
+ * every backward the weights, x, dy, h, dh, dg and du, go as fp16 (2^-11; fp32 calls two of them, 2^-22), a row of h, dh, dg
+ * and du times a power of two from bounds: |x|^2 |gate| |up|, |dy| max |down| sqrt(H), and the latter times 2 |x| and the
+ * larger of |gate| and |up| (2-norms of rows, a matrix's largest one), each factor up to twice as large. What is below 2^-29
+ * (fp32: 2^-17) of a bound loses bits, what is below 2^-40 of it is 0.
+ * A value of x or dy that is infinite or no number reaches its own row of dx, all of dgate and dup, and, of x, all of ddown,
+ * of dy, its own row of ddown. */
 enum artlite_act { ARTLITE_ACT_SILU = 0, ARTLITE_ACT_GELU_TANH = 1 };
 typedef struct artlite_ffn {
   const artlite_matrix *gate, *up, *down;
