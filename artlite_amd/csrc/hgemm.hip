@@ -41,7 +41,7 @@ __device__ __forceinline__ const uint16_t* hg_uniform(const uint16_t* p) {
 // one DMA of 16 bytes a lane from base (uniform) + off (the lane's) into LDS at lds (uniform) + 16 lane
 __device__ __forceinline__ void hg_dma(const void* base, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
-               : "memory");
+               : "memory", "m0");
 }
 __device__ __forceinline__ f32x4 hg_mfma(const u32x4& a, const u32x4& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
