@@ -128,8 +128,8 @@ class GatedFFN:
     def backward(self, x: object, dy: object, *, dx: object = None, dgate: object = None, dup: object = None,
                  ddown: object = None, stream: int = 0, work: Workspace | None = None) -> None:
         """From x and the output's gradient dy (n, hidden): the gradients that are asked for, into dx (n, hidden), dgate, dup
-        (ffn, hidden) and ddown (hidden, ffn; rows without gaps): those of the blocks' values. Device arrays, or numpy arrays
-        throughout (written in place)."""
+        (ffn, hidden) and ddown (hidden, ffn; rows without gaps): those of the blocks' values, zeros where n is 0. Device
+        arrays, or numpy arrays throughout (written in place)."""
         H, F = self.hidden, self.ffn
         outs = {"dx": (dx, None, H), "dgate": (dgate, F, H), "dup": (dup, F, H), "ddown": (ddown, H, F)}
         if isinstance(x, np.ndarray):

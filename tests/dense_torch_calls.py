@@ -1,5 +1,5 @@
 """The dense operators beside torch: streams that arrays name, threads on their default streams, tensors that require grad,
-columns of one tensor. A program of its own, which imports torch before the library loads. Run by test_dense_torch_calls_gpu.py.
+columns of one tensor, gradients in graphs. A program of its own, which imports torch before the library loads. Run by test_dense_torch_calls_gpu.py.
 
 TOL: a bf16 output's half step (2^-8) and the inner roundings' eighths of it (at most 8)."""
 
@@ -12,6 +12,7 @@ import torch
 sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 
 from artlite_amd import _hip  # noqa: E402
+from artlite_amd.device import Workspace  # noqa: E402
 from artlite_amd.ffn import GatedFFN  # noqa: E402
 from artlite_amd.linear import QLinear  # noqa: E402
 from oracle import dense  # noqa: E402
@@ -141,7 +142,37 @@ def columns_of_one_tensor() -> None:
         assert torch.equal(whole, before)
 
 
+def gradients_in_graphs() -> None:
+    """Every gradient captured, replayed with inputs of other sizes and eager calls between: the eager call's bits each time
+    (nothing of a replay's powers of two is left for the next)."""
+    H, F = 256, 608
+    f = GatedFFN(hidden=H, ffn=F, gate_type="Q4_0", down_type="IQ4_NL")
+    for i, (name, q, r, c) in enumerate((("gate", "Q4_0", F, H), ("up", "Q4_0", F, H), ("down", "IQ4_NL", H, F))):
+        f.upload("ffn_" + name, dense.matrix(q, r, c, i)[0])
+    for n in (1, 30, 64, 65, 300, 1500):
+        for dtype in (torch.bfloat16, torch.float32):
+            x, dy = (torch.randn(n, H, device="cuda").to(dtype) for _ in range(2))
+            shapes = {"dx": (n, H), "dgate": (F, H), "dup": (F, H), "ddown": (H, F)}
+            out, eager = ({k: torch.empty(s, device="cuda", dtype=dtype) for k, s in shapes.items()} for _ in range(2))
+            work = Workspace(f.workspace_bytes(n, "bf16" if dtype == torch.bfloat16 else "f32", weights=True))
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                f.backward(x, dy, **out, stream=torch.cuda.current_stream().cuda_stream, work=work)
+            for size, grad in ((1.0, 1.0), (1e6, 1e-3), (1e-12, 1e4), (0.0, 1.0), (1.0, 1e-20), (1.0, 1.0)):
+                x.copy_(size * torch.randn(n, H, device="cuda"))
+                dy.copy_(grad * torch.randn(n, H, device="cuda"))
+                for t in out.values():
+                    t.fill_(7)
+                g.replay()
+                f.backward(x, dy, **eager)
+                torch.cuda.synchronize()
+                for k, t in out.items():
+                    assert torch.equal(t, eager[k]), (n, dtype, size, k)
+                assert all(t.isfinite().all() for t in out.values())
+
+
 if __name__ == "__main__":
-    for case in (streams_of_interfaces, per_thread_streams, tensors_that_require_grad, columns_of_one_tensor):
+    for case in (streams_of_interfaces, per_thread_streams, tensors_that_require_grad, columns_of_one_tensor, gradients_in_graphs):
         case()
         print(case.__name__, "passed", flush=True)

@@ -55,3 +55,24 @@ def test_columns_of_one_buffer(dtype: str) -> None:
         got = dev.numpy()
         check(got[:, 3 + K:3 + K + N], values(whole[:, 3:3 + K]) @ w.T, TOL[dtype, few(N, K, M, dtype)])
         assert np.array_equal(np.delete(got, np.s_[3 + K:3 + K + N], 1), np.delete(whole, np.s_[3 + K:3 + K + N], 1))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("q", dense.FORMATS)
+def test_smallest_rows(q: str, dtype: str) -> None:
+    """Rows of x about the smallest normal values beside ordinary ones, each row as exact as its own values are. On top of the
+    tolerance: a bf16 output's smallest half step (2^-134; fp32's 2^-150 is nothing beside the next), and of fp32 rows half the
+    smallest step of the planes that few of them go as (2^-134 a value; each of the output's K terms has one, times a weight)."""
+    N, K = 400, 512
+    raw, w = dense.matrix(q, N, K, 3)
+    lin = QLinear(q, N, K)
+    lin.upload(raw)
+    for M in (3, 16, 90, 300, 1300):
+        size = np.resize([1e-37, 1.0, 3e-36, 1e-33], M)[:, None]
+        x = encode(size * np.random.default_rng(M).standard_normal((M, K)), dtype)
+        got, want = lin(x), values(x) @ w.T
+        step = 2.0 ** -134 * (1.0 if dtype == "bf16" else np.sqrt((w ** 2).sum(1)).max())
+        for r in range(min(M, 24)):
+            top = step * np.sqrt(N) / np.linalg.norm(want[r])
+            check(got[r:r + 1], want[r:r + 1], 1.5 * TOL[dtype, few(N, K, M, dtype)] + top,
+                  np.sqrt(values(x[r:r + 1]) ** 2 @ (w ** 2).T))
