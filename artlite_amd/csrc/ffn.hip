@@ -529,7 +529,8 @@ int ffn_forward(const Ffn& f, const void* x, int dtype, int64_t n, int64_t x_str
 constexpr int FEW_ROWS_GRAD = 192;
 // Rows (a multiple of 64) up to which the weights' gradients are one launch of small tiles: what they write bounds them, and a
 // launch's start (all gradients of 1024 x 2816 IQ4_NL, 45 rows of fp32: 85 us in three launches, 82 in one; 4096 x 11008
-// Q4_0, 1 row 187 and 161, fp32 332 and 251, 256 rows 1136 and 1065; 2048 x 8192 Q4_K, 256 rows of bf16, 187 and 189)
+// Q4_0, 1 row 187 and 161, fp32 332 and 251, 256 rows 1136 and 1065; 2048 x 8192 Q4_K, 256 rows of bf16, 187 and 189; all
+// before k_top, which is as much for both: the last is 195 with it)
 constexpr int64_t SHORT_SUMS = 256;
 struct GradPlan {
   bool few, gated;  // (gated: g and u from the blocks, k_qgemm)
